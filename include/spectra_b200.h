@@ -247,6 +247,106 @@ SPECTRA_API int spectra_kv_dequantize(const uint8_t* packed, const uint16_t* sca
                                       void* out, int out_dtype, int64_t rows, int64_t D, void* stream);
 
 /*
+ * Paged INT4 KV cache (the reference keeps its INT4 cache as one dense tensor
+ * per layer and hands it dequantised to the model's attention,
+ * spectra/engine.py:614-727; these entry points keep it in pages, write it
+ * with the position rotation applied, and attend over its codes).
+ *
+ * The pool: u8 [num_pages][kv_heads][page_size / 16][tile], a tile = 16 tokens
+ * of one head, D = 32 G features, 608 G bytes (offsets in bytes):
+ *   0      key codes    [2 blocks of 8 tokens][8 tokens][4 words c][G]: word c
+ *                       of group g holds features 8c..8c+7 of the group, the
+ *                       first in the lowest nibble
+ *   256 G  value codes  [2 blocks][8 l][4 token pairs][G]: features 4l..4l+3
+ *                       of the even token in the low half, of the odd token in
+ *                       the high half of the word
+ *   512 G  key scales   fp16 [16][G]      544 G  value scales fp16 [8 pairs][G][2]
+ *   576 G  key zeros    u8   [16][G]      592 G  value zeros  u8   [8 pairs][G][2]
+ * A code q stands for (q - z) s.  Zeroed before its first use and written by
+ * spectra_paged_kv_append alone: no value scale in it passes 4364 (15 of them fit fp16).
+ * page_stride: bytes from page to page (a multiple of 16); heads and tiles of
+ * a page are contiguous.  head_dim 32, 64, 96, 128 or 256; page_size a power
+ * of two, 16..65536; the pool on a 16-byte boundary.
+ *
+ * The batch: sequence b holds seq_lens[b] tokens, its new ones included, in
+ * pages block_tables[b * table_stride + position / page_size]; its new tokens
+ * are rows cu_q[b] .. cu_q[b + 1] of the token tensors (cu_q NULL: q_len rows
+ * each) and have its last positions.  `total` rows in all, at most max_q of one sequence.
+ * max_len bounds seq_lens: positions from min(max_len, width * page_size) on
+ * are not touched.  A new token of negative position is padding (a slot of the
+ * batch that holds no sequence has seq_lens 0).  A page number outside
+ * [0, num_pages) names no page: nothing is written, its keys are not seen.
+ * All three arrays are device memory, read by the kernels only.
+ */
+typedef struct {
+  void* pool;
+  int64_t page_stride;
+  int64_t num_pages;
+  int32_t kv_heads, head_dim, page_size;
+} SpectraPagedCache;
+
+typedef struct {
+  const int32_t* block_tables;
+  int64_t table_stride;
+  int64_t width;            /* pages named per sequence */
+  const int32_t* seq_lens;
+  const int32_t* cu_q;      /* [batch + 1] or NULL */
+  int64_t batch, q_len, total, max_q, max_len;
+} SpectraTokenBatch;
+
+/*
+ * Rotate and append.  The first `rotary` features of every query and key head
+ * are turned by the angles of the token's position (row `position` of cos and
+ * sin, fp32 [>= min(max_len, width * page_size)][rotary / 2]): pairs (i, i + rotary / 2), or (2i, 2i + 1)
+ * with `interleaved`; fp32, one rounding for the queries.  Keys (not rounded in
+ * between) and values are quantised in groups of 32 and stored:
+ *   lo = min(0, x), hi = max(0, x), s = fp16((hi - lo) / 15),
+ *   z = min(rint(-lo / s), 15), q = clamp(rint(x / s) + z, 0, 15)
+ * (1 / s rounded once, then multiplied).  A group of key or value that holds a
+ * NaN or infinity or spans more than 65472: its key group reads NaN, its value
+ * group 0.  Padding: nothing is stored, the query row becomes 0.
+ *   q [total][q_heads][D] or NULL, q_out the same shape, not overlapping q;
+ *   k, v [total][kv_heads][D]; element (t, h, d) at t*_ts + h*_hs + d; dtype
+ *   F16 or BF16 for all four.  rotary 0: cos, sin NULL.  rotary a multiple of
+ *   16 (8 if interleaved), <= D.
+ */
+SPECTRA_API int spectra_paged_kv_append(
+    const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
+    const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int64_t qo_ts, int64_t qo_hs,
+    const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
+    const float* cos, const float* sin, int64_t cs_rows, int64_t cs_row_stride, int64_t rotary, int interleaved,
+    void* stream);
+
+/*
+ * What the cache holds of the batch's new tokens: k, v [total][kv_heads][D]
+ * contiguous on 16-byte boundaries, (q - z) s rounded once to out_dtype (F16, BF16, F32);
+ * 0 for padding and for tokens that no page holds.
+ */
+SPECTRA_API int spectra_paged_kv_read(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, void* k, void* v,
+                                      int out_dtype, void* stream);
+
+/*
+ * Attention of the batch's new tokens over the cache (append them first).  Row
+ * (token at position p, head h), head h / (q_heads / kv_heads) of the cache:
+ *   t_n = scale q . k_n;  softcap > 0: t = softcap tanh(t / softcap);
+ *   slopes: t += slopes[h] (n - p);  out = sum e^t_n v_n / sum e^t_n
+ * over n < seq_lens[b], with `causal` n <= p, with window > 0 n > p - window.
+ * A row that sees no key is 0; rows >= cu_q[batch] are 0.
+ *   q, out [total][q_heads][D], element strides, dtype F16 or BF16;
+ *   slopes fp32 [q_heads] or NULL; scale > 0.
+ *   workspace: spectra_paged_attention_workspace_bytes(head_dim) bytes, zeroed
+ *          once before its first use, 16-byte aligned; calls that share one
+ *          must not overlap in time.
+ */
+SPECTRA_API int spectra_paged_attention(
+    const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
+    const void* q, int64_t q_ts, int64_t q_hs, void* out, int64_t o_ts, int64_t o_hs,
+    float scale, float softcap, const float* slopes, int causal, int64_t window,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+SPECTRA_API size_t spectra_paged_attention_workspace_bytes(int64_t head_dim);
+
+/*
  * Quantised token-embedding gather (replaces SpectraFusedEmbedding.forward,
  * spectra/engine.py:167-212): out[t, :] = dequantised row ids[t] of the
  * [V, K] vocabulary matrix ((q - z) * s in fp32, rounded once to out_dtype),

@@ -6,7 +6,7 @@ fallback: if it is missing, every kernel call raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("libspectra_b200.so")
@@ -19,6 +19,19 @@ ERR_NULL_POINTER, ERR_SHAPE, ERR_STRIDE, ERR_ALIGNMENT, ERR_DTYPE, ERR_WORKSPACE
 ABI_VERSION = 1
 P2P_STATE_INTS = 128  # SPECTRA_P2P_STATE_INTS
 P2P_SIGNAL_BYTES = 8 * 128 * 4  # epoch flags [rank][cta] at the start of an exchange buffer
+
+
+
+class PagedCache(ctypes.Structure):  # SpectraPagedCache
+    _fields_ = [("pool", c_void_p), ("page_stride", c_int64), ("num_pages", c_int64),
+                ("kv_heads", c_int32), ("head_dim", c_int32), ("page_size", c_int32)]
+
+
+class TokenBatch(ctypes.Structure):  # SpectraTokenBatch
+    _fields_ = [("block_tables", c_void_p), ("table_stride", c_int64), ("width", c_int64),
+                ("seq_lens", c_void_p), ("cu_q", c_void_p), ("batch", c_int64), ("q_len", c_int64),
+                ("total", c_int64), ("max_q", c_int64), ("max_len", c_int64)]
+
 
 # name -> (restype, argtypes)
 PROTOTYPES = {
@@ -70,6 +83,22 @@ PROTOTYPES = {
     "spectra_unpack_zeros": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p]),
     "spectra_kv_quantize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
     "spectra_kv_dequantize": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p]),
+    "spectra_paged_kv_append": (c_int, [
+        c_void_p, c_void_p, c_int, c_int64,            # cache, batch, dtype, q_heads
+        c_void_p, c_int64, c_int64,                    # q, token stride, head stride
+        c_void_p, c_int64, c_int64,                    # q_out
+        c_void_p, c_int64, c_int64,                    # k
+        c_void_p, c_int64, c_int64,                    # v
+        c_void_p, c_void_p, c_int64, c_int64,          # cos, sin, rows, row stride
+        c_int64, c_int, c_void_p]),                    # rotary, interleaved, stream
+    "spectra_paged_kv_read": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "spectra_paged_attention": (c_int, [
+        c_void_p, c_void_p, c_int, c_int64,            # cache, batch, dtype, q_heads
+        c_void_p, c_int64, c_int64,                    # q
+        c_void_p, c_int64, c_int64,                    # out
+        c_float, c_float, c_void_p, c_int, c_int64,    # scale, softcap, slopes, causal, window
+        c_void_p, c_size_t, c_void_p]),                # workspace, workspace_bytes, stream
+    "spectra_paged_attention_workspace_bytes": (c_size_t, [c_int64]),
     "spectra_w4a16_embedding": (c_int, [
         c_void_p, c_int, c_int64,                      # ids, ids_dtype, T
         c_void_p, c_int64, c_void_p, c_int64,          # packed, scales

@@ -3,6 +3,7 @@
 // CUDA call, so an invalid call returns a status code and launches nothing.
 #include <cuda.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <cstdint>
@@ -13,6 +14,7 @@
 #include "gemm.h"
 #include "gemv.h"
 #include "p2p.h"
+#include "paged.h"
 
 namespace spectra {
 
@@ -255,14 +257,15 @@ int spectra_w4a16_gemm_noalloc(
 
 int spectra_device_timeouts(int64_t* count, int reset) {
   if (!count) return SPECTRA_ERR_NULL_POINTER;
-  long long a = 0, b = 0, c = 0, d = 0, e = 0;
+  long long a = 0, b = 0, c = 0, d = 0, e = 0, f = 0;
   int st = gemv_timeouts(&a, reset != 0);
   if (st == SPECTRA_OK) st = gemv_pf_timeouts(&b, reset != 0);
   if (st == SPECTRA_OK) st = gemm_timeouts(&c, reset != 0);
   if (st == SPECTRA_OK) st = p2p_timeouts(&d, reset != 0);
   if (st == SPECTRA_OK) st = gemv_mt_timeouts(&e, reset != 0);
+  if (st == SPECTRA_OK) st = paged_attn_timeouts(&f, reset != 0);
   if (st != SPECTRA_OK) return st;
-  *count = int64_t(a + b + c + d + e);
+  *count = int64_t(a + b + c + d + e + f);
   return SPECTRA_OK;
 }
 
@@ -413,6 +416,131 @@ int spectra_kv_dequantize(const uint8_t* packed, const uint16_t* scales, const u
   a.packed = packed; a.scales = scales; a.zeros = zeros;
   a.out = out; a.out_dtype = out_dtype; a.rows = rows; a.D = int(D);
   return launch_kv_dequantize(a, static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+// Checks of a cache and a batch, and the kernels' view of them.  `empty`: no
+// tokens, nothing to launch.
+int paged_view(const SpectraPagedCache* c, const SpectraTokenBatch* b, PagedView& v, bool& empty) {
+  if (!c || !b) return SPECTRA_ERR_NULL_POINTER;
+  const int64_t D = c->head_dim, P = c->page_size;
+  if (D != 32 && D != 64 && D != 96 && D != 128 && D != 256) return SPECTRA_ERR_UNSUPPORTED;
+  if (P < kTileTokens || P > 65536 || (P & (P - 1)) != 0) return SPECTRA_ERR_UNSUPPORTED;
+  if (c->kv_heads <= 0 || c->kv_heads > 65535 || c->num_pages < 0 || !fits_i32(c->num_pages)) return SPECTRA_ERR_SHAPE;
+  if (b->batch < 0 || !fits_i32(b->batch) || b->total < 0 || !fits_i32(b->total) || b->width < 0 ||
+      b->max_q < 0 || b->max_len < 0 || !fits_i32(b->max_len))
+    return SPECTRA_ERR_SHAPE;
+  if (!b->cu_q && (b->q_len < 0 || (b->total > 0 && b->q_len == 0) || (b->q_len > 0 && b->total > b->batch * b->q_len)))
+    return SPECTRA_ERR_SHAPE;
+  empty = b->total == 0;
+  if (empty) return SPECTRA_OK;
+  if (b->batch == 0 || b->max_q == 0) return SPECTRA_ERR_SHAPE;
+  const TileLayout L{int(D / 32)};
+  const int64_t page_bytes = int64_t(c->kv_heads) * (P / kTileTokens) * L.bytes();
+  if (!b->block_tables || !b->seq_lens || (!c->pool && c->num_pages > 0)) return SPECTRA_ERR_NULL_POINTER;
+  if (!aligned(c->pool, 16) || c->page_stride % 16 != 0) return SPECTRA_ERR_ALIGNMENT;
+  if (c->page_stride < page_bytes || (b->batch > 1 && b->table_stride < b->width)) return SPECTRA_ERR_STRIDE;
+  if (!aligned(b->block_tables, 4) || !aligned(b->seq_lens, 4) || (b->cu_q && !aligned(b->cu_q, 4)))
+    return SPECTRA_ERR_ALIGNMENT;
+  v.pool = static_cast<uint8_t*>(c->pool);
+  v.page_stride = c->page_stride;
+  v.num_pages = int(c->num_pages);
+  v.kv_heads = c->kv_heads;
+  v.head_dim = int(D);
+  v.page_log2 = 0;
+  while ((int64_t(1) << v.page_log2) < P) ++v.page_log2;
+  v.tables = b->block_tables;
+  v.table_stride = b->table_stride;
+  v.seq_lens = b->seq_lens;
+  v.cu_q = b->cu_q;
+  v.batch = int(b->batch);
+  v.total = b->total;
+  v.q_len = b->cu_q ? 0 : int(std::min<int64_t>(b->q_len, b->total));
+  v.max_q = int(std::min<int64_t>(b->max_q, b->total));
+  v.limit = int(std::min<int64_t>(b->max_len, std::min<int64_t>(b->width, INT32_MAX / P) * P));
+  return SPECTRA_OK;
+}
+
+// Rows of D elements at t * ts + h * hs: strides that can be addressed, and whether every row is 16-byte aligned.
+bool head_rows_ok(int64_t ts, int64_t hs) { return ts >= 0 && hs >= 0; }
+bool head_rows_vec(const void* p, int64_t ts, int64_t hs) { return aligned(p, 16) && ts % 8 == 0 && hs % 8 == 0; }
+bool is_half_dt(int dt) { return dt == SPECTRA_DT_F16 || dt == SPECTRA_DT_BF16; }
+}  // namespace
+
+int spectra_paged_kv_append(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
+                            const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int64_t qo_ts, int64_t qo_hs,
+                            const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
+                            const float* cos, const float* sin, int64_t cs_rows, int64_t cs_row_stride, int64_t rotary,
+                            int interleaved, void* stream) {
+  PagedAppendArgs a = {};
+  bool empty = false;
+  const int st = paged_view(cache, batch, a.c, empty);
+  if (st != SPECTRA_OK) return st;
+  if (!is_half_dt(dtype)) return SPECTRA_ERR_DTYPE;
+  if (rotary < 0 || rotary > cache->head_dim || rotary % (interleaved ? 8 : 16) != 0) return SPECTRA_ERR_SHAPE;
+  if (q && (q_heads <= 0 || q_heads > 65535)) return SPECTRA_ERR_SHAPE;
+  if (empty) return SPECTRA_OK;
+  if (!k || !v || (q && !q_out) || (rotary > 0 && (!cos || !sin))) return SPECTRA_ERR_NULL_POINTER;
+  if (rotary > 0 && (cs_rows < a.c.limit || cs_row_stride < rotary / 2)) return SPECTRA_ERR_SHAPE;
+  if (!head_rows_ok(k_ts, k_hs) || !head_rows_ok(v_ts, v_hs) || (q && (!head_rows_ok(q_ts, q_hs) || !head_rows_ok(qo_ts, qo_hs))))
+    return SPECTRA_ERR_STRIDE;
+  if (!aligned(k, 2) || !aligned(v, 2) || (q && (!aligned(q, 2) || !aligned(q_out, 2))) ||
+      (rotary > 0 && (!aligned(cos, 4) || !aligned(sin, 4))))
+    return SPECTRA_ERR_ALIGNMENT;
+  a.q = q; a.q_ts = q_ts; a.q_hs = q_hs;
+  a.q_out = q_out; a.qo_ts = qo_ts; a.qo_hs = qo_hs;
+  a.k = k; a.k_ts = k_ts; a.k_hs = k_hs;
+  a.v = v; a.v_ts = v_ts; a.v_hs = v_hs;
+  a.dtype = dtype; a.q_heads = q ? int(q_heads) : 0;
+  a.cos = cos; a.sin = sin; a.cs_rs = cs_row_stride; a.rotary = int(rotary); a.interleaved = interleaved != 0;
+  a.vec = head_rows_vec(k, k_ts, k_hs) && head_rows_vec(v, v_ts, v_hs) &&
+          (!q || (head_rows_vec(q, q_ts, q_hs) && head_rows_vec(q_out, qo_ts, qo_hs)));
+  return launch_paged_append(a, static_cast<cudaStream_t>(stream));
+}
+
+int spectra_paged_kv_read(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, void* k, void* v, int out_dtype,
+                          void* stream) {
+  PagedReadArgs a = {};
+  bool empty = false;
+  const int st = paged_view(cache, batch, a.c, empty);
+  if (st != SPECTRA_OK) return st;
+  if (!is_float_dt(out_dtype)) return SPECTRA_ERR_DTYPE;
+  if (empty) return SPECTRA_OK;
+  if (!k || !v) return SPECTRA_ERR_NULL_POINTER;
+  if (!aligned(k, 16) || !aligned(v, 16)) return SPECTRA_ERR_ALIGNMENT;
+  a.k = k; a.v = v; a.out_dtype = out_dtype;
+  return launch_paged_read(a, static_cast<cudaStream_t>(stream));
+}
+
+int spectra_paged_attention(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
+                            const void* q, int64_t q_ts, int64_t q_hs, void* out, int64_t o_ts, int64_t o_hs, float scale,
+                            float softcap, const float* slopes, int causal, int64_t window, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  PagedAttnArgs a = {};
+  bool empty = false;
+  const int st = paged_view(cache, batch, a.c, empty);
+  if (st != SPECTRA_OK) return st;
+  if (!is_half_dt(dtype)) return SPECTRA_ERR_DTYPE;
+  if (q_heads <= 0 || q_heads > 65535 || q_heads % cache->kv_heads != 0 || window < 0) return SPECTRA_ERR_SHAPE;
+  if (!(scale > 0.f) || !std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap)) return SPECTRA_ERR_UNSUPPORTED;
+  if (empty) return SPECTRA_OK;
+  if (!q || !out || !workspace) return SPECTRA_ERR_NULL_POINTER;
+  if (!head_rows_ok(q_ts, q_hs) || !head_rows_ok(o_ts, o_hs)) return SPECTRA_ERR_STRIDE;
+  if (!aligned(q, 2) || !aligned(out, 2) || (slopes && !aligned(slopes, 4)) || !aligned(workspace, 16))
+    return SPECTRA_ERR_ALIGNMENT;
+  if (workspace_bytes < paged_attn_workspace_bytes(cache->head_dim)) return SPECTRA_ERR_WORKSPACE;
+  a.q = q; a.q_ts = q_ts; a.q_hs = q_hs;
+  a.out = out; a.o_ts = o_ts; a.o_hs = o_hs;
+  a.dtype = dtype; a.q_heads = int(q_heads); a.group = int(q_heads / cache->kv_heads);
+  a.scale = scale; a.softcap = softcap; a.slopes = slopes; a.causal = causal != 0;
+  a.window = int(std::min<int64_t>(window, INT32_MAX));
+  a.vec = head_rows_vec(q, q_ts, q_hs) && head_rows_vec(out, o_ts, o_hs);
+  a.workspace = workspace; a.workspace_bytes = workspace_bytes;
+  return launch_paged_attn(a, static_cast<cudaStream_t>(stream));
+}
+
+size_t spectra_paged_attention_workspace_bytes(int64_t head_dim) {
+  return head_dim > 0 && head_dim <= 256 ? paged_attn_workspace_bytes(int(head_dim)) : 0;
 }
 
 int spectra_w4a16_embedding(
