@@ -257,15 +257,16 @@ int spectra_w4a16_gemm_noalloc(
 
 int spectra_device_timeouts(int64_t* count, int reset) {
   if (!count) return SPECTRA_ERR_NULL_POINTER;
-  long long a = 0, b = 0, c = 0, d = 0, e = 0, f = 0;
+  long long a = 0, b = 0, c = 0, d = 0, e = 0, f = 0, g = 0;
   int st = gemv_timeouts(&a, reset != 0);
   if (st == SPECTRA_OK) st = gemv_pf_timeouts(&b, reset != 0);
   if (st == SPECTRA_OK) st = gemm_timeouts(&c, reset != 0);
   if (st == SPECTRA_OK) st = p2p_timeouts(&d, reset != 0);
   if (st == SPECTRA_OK) st = gemv_mt_timeouts(&e, reset != 0);
   if (st == SPECTRA_OK) st = paged_attn_timeouts(&f, reset != 0);
+  if (st == SPECTRA_OK) st = paged_prompt_timeouts(&g, reset != 0);
   if (st != SPECTRA_OK) return st;
-  *count = int64_t(a + b + c + d + e + f);
+  *count = int64_t(a + b + c + d + e + f + g);
   return SPECTRA_OK;
 }
 
@@ -528,7 +529,7 @@ int spectra_paged_attention(const SpectraPagedCache* cache, const SpectraTokenBa
   if (!head_rows_ok(q_ts, q_hs) || !head_rows_ok(o_ts, o_hs)) return SPECTRA_ERR_STRIDE;
   if (!aligned(q, 2) || !aligned(out, 2) || (slopes && !aligned(slopes, 4)) || !aligned(workspace, 16))
     return SPECTRA_ERR_ALIGNMENT;
-  if (workspace_bytes < paged_attn_workspace_bytes(cache->head_dim)) return SPECTRA_ERR_WORKSPACE;
+  if (workspace_bytes < spectra_paged_attention_workspace_bytes(cache->head_dim)) return SPECTRA_ERR_WORKSPACE;
   a.q = q; a.q_ts = q_ts; a.q_hs = q_hs;
   a.out = out; a.o_ts = o_ts; a.o_hs = o_hs;
   a.dtype = dtype; a.q_heads = int(q_heads); a.group = int(q_heads / cache->kv_heads);
@@ -536,11 +537,21 @@ int spectra_paged_attention(const SpectraPagedCache* cache, const SpectraTokenBa
   a.window = int(std::min<int64_t>(window, INT32_MAX));
   a.vec = head_rows_vec(q, q_ts, q_hs) && head_rows_vec(out, o_ts, o_hs);
   a.workspace = workspace; a.workspace_bytes = workspace_bytes;
-  return launch_paged_attn(a, static_cast<cudaStream_t>(stream));
+  // Rows of one key/value head (new tokens times the query heads that share it): up to kFewRows a sequence is
+  // the few-token kernel's, above it the prompt kernel's.  A batch of equal sequences takes one launch; a ragged
+  // one with long sequences both, as either kind may be in it.
+  constexpr int kFewRows = 64;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t rows = int64_t(a.c.max_q) * a.group;
+  if (rows <= kFewRows || cache->head_dim > 128) return launch_paged_attn(a, INT32_MAX, s);
+  if (!a.c.cu_q) return launch_paged_prompt(a, 0, s);
+  const int few = launch_paged_attn(a, kFewRows, s);
+  return few != SPECTRA_OK ? few : launch_paged_prompt(a, kFewRows, s);
 }
 
 size_t spectra_paged_attention_workspace_bytes(int64_t head_dim) {
-  return head_dim > 0 && head_dim <= 256 ? paged_attn_workspace_bytes(int(head_dim)) : 0;
+  if (head_dim <= 0 || head_dim > 256) return 0;
+  return std::max(paged_attn_workspace_bytes(int(head_dim)), paged_prompt_workspace_bytes(int(head_dim)));
 }
 
 int spectra_w4a16_embedding(

@@ -71,8 +71,16 @@ struct PagedAttnArgs {
   int vec;                                 // rows of q and out on 16-byte boundaries
   void* workspace; size_t workspace_bytes;
 };
+// A workspace: kPagedCounterBytes of counters (zero between calls), then partial results.
+constexpr size_t kPagedCounterBytes = 4096;
+// One or a few tokens per sequence (paged_attn.cu); many (paged_prompt.cu).
+// Sequences with more than max_rows (the first) or at most min_rows (the
+// second) rows per key/value head are left to the other.
 size_t paged_attn_workspace_bytes(int head_dim);
-int launch_paged_attn(const PagedAttnArgs& a, cudaStream_t st);
+size_t paged_prompt_workspace_bytes(int head_dim);
+int launch_paged_attn(const PagedAttnArgs& a, int max_rows, cudaStream_t st);
+int launch_paged_prompt(const PagedAttnArgs& a, int min_rows, cudaStream_t st);
 int paged_attn_timeouts(long long* out, bool reset);
+int paged_prompt_timeouts(long long* out, bool reset);
 
 }  // namespace spectra

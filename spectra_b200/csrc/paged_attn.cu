@@ -47,82 +47,15 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kUnit = 32;          // tokens of a unit: two tiles
 constexpr int kStages = 2;         // units in flight per warp
-constexpr int kMaxCtas = 1024;     // counters of the workspace
-constexpr float kLazy = 8.f;
-constexpr float kNone = -1e30f;    // below every score that is seen
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxCtas = int(kPagedCounterBytes / sizeof(int));
 
 struct AttnParams {
   PagedAttnArgs a;
   int* counters;
   float* partials;
   int min_share;                   // units a CTA takes at least
+  int max_rows;                    // a sequence with more rows per head is the other kernel's
 };
-
-// ------------------------------------------------------------ small helpers
-template <int BYTES>
-__device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[(BYTES + 3) / 4]) {
-  if constexpr (BYTES % 16 == 0) {
-#pragma unroll
-    for (int i = 0; i < BYTES / 16; ++i) {
-      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
-      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-    }
-  } else if constexpr (BYTES % 8 == 0) {
-#pragma unroll
-    for (int i = 0; i < BYTES / 8; ++i) {
-      const uint2 v = reinterpret_cast<const uint2*>(p)[i];
-      w[2 * i] = v.x; w[2 * i + 1] = v.y;
-    }
-  } else if constexpr (BYTES % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < BYTES / 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
-  } else if constexpr (BYTES % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < (BYTES + 3) / 4; ++i) w[i] = 0;
-#pragma unroll
-    for (int i = 0; i < BYTES / 2; ++i) w[i >> 1] |= uint32_t(reinterpret_cast<const uint16_t*>(p)[i]) << (16 * (i & 1));
-  } else {
-#pragma unroll
-    for (int i = 0; i < (BYTES + 3) / 4; ++i) w[i] = 0;
-#pragma unroll
-    for (int i = 0; i < BYTES; ++i) w[i >> 2] |= uint32_t(p[i]) << (8 * (i & 3));
-  }
-}
-
-// Nibble J of both halves of a code word on top of `magic`.
-template <int J>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t magic) {
-  return ((w >> (4 * J)) & 0x000F000Fu) | magic;
-}
-
-__device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
-  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t h2_pack(float lo, float hi) {
-  const __half2 r = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
-  uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-__device__ __forceinline__ float half_of(uint32_t w, int hi) {
-  return __half2float(__ushort_as_half(uint16_t(hi ? w >> 16 : w & 0xFFFFu)));
-}
-__device__ __forceinline__ float byte_of(uint32_t w, int i) {  // 2^23 + byte, less 2^23
-  return __uint_as_float(__byte_perm(w, kMagic, 0x7650u | i)) - 8388608.f;
-}
-// tanh by its exponential: absolute error a few 2^-24 over the whole range.
-__device__ __forceinline__ float tanh_exp(float x) {
-  return 1.f - __fdividef(2.f, 1.f + exp2f(2.f * kLog2e * x));
-}
 
 // ------------------------------------------------------------ the batch
 struct Span {  // a sequence's rows and the keys its rows look at
@@ -136,13 +69,14 @@ struct Span {  // a sequence's rows and the keys its rows look at
 };
 
 template <int ROWS>
-__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int b) {
+__device__ __forceinline__ Span span_of(const AttnParams& p, int b) {
+  const PagedAttnArgs& a = p.a;
   Span s;
   new_tokens(a.c, b, s.first, s.count);
   const int len = a.c.seq_lens[b];
   s.pos0 = len - s.count;
   s.len = len < 0 ? 0 : (len < a.c.limit ? len : a.c.limit);
-  s.tiles = (s.count * a.group + ROWS - 1) / ROWS;
+  s.tiles = s.count * a.group > p.max_rows ? 0 : (s.count * a.group + ROWS - 1) / ROWS;
   const int lo = a.window > 0 ? max(0, s.pos0 - a.window + 1) : 0;
   s.unit0 = lo / kUnit;
   s.units = max(1, (s.len + kUnit - 1) / kUnit - s.unit0);
@@ -205,7 +139,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
   long long total = 0;
   for (int b0 = 0; b0 < c.batch; b0 += kThreads) {
     if (b0 + tid < c.batch) {
-      const Span s = span_of<ROWS>(a, b0 + tid);
+      const Span s = span_of<ROWS>(p, b0 + tid);
       total += (long long)(s.units) * s.tiles * c.kv_heads;
     }
   }
@@ -236,7 +170,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
   for (int b0 = 0; b0 < c.batch; b0 += kThreads) {
     long long mine = 0;
     if (b0 + tid < c.batch) {
-      const Span s = span_of<ROWS>(a, b0 + tid);
+      const Span s = span_of<ROWS>(p, b0 + tid);
       mine = (long long)(s.units) * s.tiles * c.kv_heads;
     }
     long long sum = mine;
@@ -272,12 +206,12 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
 
   while (at < end) {
     // ---- the segment that holds unit `at`
-    Span s = span_of<ROWS>(a, b);
+    Span s = span_of<ROWS>(p, b);
     long long seq_units = (long long)(s.units) * s.tiles * c.kv_heads;
     while (at >= seq_base + seq_units) {
       seq_base += seq_units;
       ++b;
-      s = span_of<ROWS>(a, b);
+      s = span_of<ROWS>(p, b);
       seq_units = (long long)(s.units) * s.tiles * c.kv_heads;
     }
     const int seg = int((at - seq_base) / s.units);
@@ -622,7 +556,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
 }
 
 template <bool BF16, int G, int NT, bool MOD>
-int launch_one(const PagedAttnArgs& a, cudaStream_t st) {
+int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   using C = Cfg<G, NT>;
   static PerContextOnce once;
   static int ctas_per_sm[kMaxDevices];
@@ -639,13 +573,14 @@ int launch_one(const PagedAttnArgs& a, cudaStream_t st) {
   AttnParams p;
   p.a = a;
   p.min_share = kWarps;
-  const int64_t tiles = (int64_t(a.c.max_q) * a.group + C::ROWS - 1) / C::ROWS;
+  p.max_rows = max_rows;
+  const int64_t tiles = (std::min<int64_t>(int64_t(a.c.max_q) * a.group, max_rows) + C::ROWS - 1) / C::ROWS;
   const int64_t most = int64_t(a.c.batch) * a.c.kv_heads * tiles * ((a.c.limit + kUnit - 1) / kUnit + 1);
   const int64_t room = std::min<int64_t>(int64_t(device_sms(dev)) * std::max(1, ctas_per_sm[dev]), kMaxCtas);
   const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(room, (most + p.min_share - 1) / p.min_share));
   p.counters = static_cast<int*>(a.workspace);
-  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + kMaxCtas * sizeof(int));
-  if (a.workspace_bytes < kMaxCtas * sizeof(int) + size_t(grid) * 2 * C::kPartial * sizeof(float)) return SPECTRA_ERR_WORKSPACE;
+  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + kPagedCounterBytes);
+  if (a.workspace_bytes < kPagedCounterBytes + size_t(grid) * 2 * C::kPartial * sizeof(float)) return SPECTRA_ERR_WORKSPACE;
 
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(grid));
@@ -661,24 +596,24 @@ int launch_one(const PagedAttnArgs& a, cudaStream_t st) {
 }
 
 template <bool BF16, int G>
-int launch_rows(const PagedAttnArgs& a, cudaStream_t st) {
+int launch_rows(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   const bool mod = a.softcap > 0.f || a.slopes;
   // up to 8 rows per key/value head: one column tile (fewer registers, more CTAs per SM); heads of 256 have
   // no registers for two
   if (G == 8 || int64_t(a.c.max_q) * a.group <= 8)
-    return mod ? launch_one<BF16, G, 1, true>(a, st) : launch_one<BF16, G, 1, false>(a, st);
+    return mod ? launch_one<BF16, G, 1, true>(a, max_rows, st) : launch_one<BF16, G, 1, false>(a, max_rows, st);
   constexpr int NT = G == 8 ? 1 : 2;
-  return mod ? launch_one<BF16, G, NT, true>(a, st) : launch_one<BF16, G, NT, false>(a, st);
+  return mod ? launch_one<BF16, G, NT, true>(a, max_rows, st) : launch_one<BF16, G, NT, false>(a, max_rows, st);
 }
 
 template <bool BF16>
-int launch_dim(const PagedAttnArgs& a, cudaStream_t st) {
+int launch_dim(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   switch (a.c.head_dim) {
-    case 32: return launch_rows<BF16, 1>(a, st);
-    case 64: return launch_rows<BF16, 2>(a, st);
-    case 96: return launch_rows<BF16, 3>(a, st);
-    case 128: return launch_rows<BF16, 4>(a, st);
-    case 256: return launch_rows<BF16, 8>(a, st);
+    case 32: return launch_rows<BF16, 1>(a, max_rows, st);
+    case 64: return launch_rows<BF16, 2>(a, max_rows, st);
+    case 96: return launch_rows<BF16, 3>(a, max_rows, st);
+    case 128: return launch_rows<BF16, 4>(a, max_rows, st);
+    case 256: return launch_rows<BF16, 8>(a, max_rows, st);
   }
   return SPECTRA_ERR_UNSUPPORTED;
 }
@@ -686,11 +621,11 @@ int launch_dim(const PagedAttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 size_t paged_attn_workspace_bytes(int head_dim) {
-  return kMaxCtas * sizeof(int) + size_t(kMaxCtas) * 2 * 16 * (head_dim + 2) * sizeof(float);
+  return kPagedCounterBytes + size_t(kMaxCtas) * 2 * 16 * (head_dim + 2) * sizeof(float);
 }
 
-int launch_paged_attn(const PagedAttnArgs& a, cudaStream_t st) {
-  return a.dtype == SPECTRA_DT_BF16 ? launch_dim<true>(a, st) : launch_dim<false>(a, st);
+int launch_paged_attn(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
+  return a.dtype == SPECTRA_DT_BF16 ? launch_dim<true>(a, max_rows, st) : launch_dim<false>(a, max_rows, st);
 }
 
 int paged_attn_timeouts(long long* out, bool reset) { return read_timeout_counter(g_paged_attn_timeouts, out, reset); }

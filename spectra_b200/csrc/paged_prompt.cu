@@ -1,0 +1,677 @@
+// Attention over the paged INT4 KV cache for sm_100a: many new tokens of a
+// sequence (prompts, chunks of prompts), on the tcgen05 tensor cores.
+//
+// The definition is paged_attn.cu's.  With hundreds of rows per key/value head
+// the work is products, so a CTA takes 256 rows (tokens x the query heads that
+// share the head; two M = 128 tiles) of one sequence and walks the keys 128 at
+// a time:
+//   warps 8-11  bring the raw tiles in by bulk copies and write them to shared
+//               memory as fp16 operands: K [token][feature] and V^T
+//               [feature][token], K-major, 128-byte swizzle.  (q - z) s is an
+//               exact difference and one rounding (11 bits).
+//   warp 12     S_t = Q_t K^T (Q in shared memory) and O_t += P_t V (P in
+//               TMEM), t = 0, 1: while one tile's softmax runs, the other
+//               tile's products do.
+//   warps 0-7   one row per thread: scores from TMEM, P back to TMEM over
+//               them as fp16, running maximum and sum in registers.  The
+//               maximum is raised only when a score passes it by 2^kLazy; then
+//               (rarely after the first tile) O is rescaled in TMEM.
+// The features of Q and K, and the tokens of P and V, are contracted in the
+// order in which the codes unpack.  bf16 queries are scaled by a power of two
+// per row to fit fp16, so only differences below 2^-28 of a row's largest
+// entry are lost.
+// TMEM (512 columns): S_0 | S_1 | O_0 | O_1.
+//
+// With fewer CTAs than SMs the keys are split over `splits` CTAs per tile,
+// whose partial results a second small kernel puts together.
+#include <math.h>
+
+#include <algorithm>
+
+#include "gemv_mma.cuh"
+#include "paged_view.cuh"
+#include "sm100_ptx.cuh"
+
+namespace spectra {
+
+__device__ int g_paged_prompt_timeouts = 0;
+
+namespace {
+
+using namespace sm100;
+
+constexpr int kRows = 256;   // rows of a CTA
+constexpr int kKeys = 128;   // keys of a step
+constexpr int kThreads = 13 * 32;
+constexpr int kStages = 2;   // operand stages
+
+struct PromptParams {
+  PagedAttnArgs a;
+  int row_tiles;   // per sequence and head, at most
+  int splits;
+  int min_rows;    // a sequence with at most this many rows per head is the other kernel's
+  float* partials; // [item][split][kRows][D + 2]
+};
+
+template <int G>
+struct Cfg {
+  static constexpr int D = 32 * G;
+  static constexpr int kAtoms = (D + 63) / 64;                 // 128-byte column blocks of Q and K
+  static constexpr int kTile = TileLayout{G}.bytes();
+  static constexpr int kAtomBytes = 128 * 128;
+  static constexpr int kQ = 2 * kAtoms * kAtomBytes;
+  static constexpr int kK = kAtoms * kAtomBytes;               // one stage
+  static constexpr int kV = 2 * D * 128;                       // one stage
+  static constexpr int kRaw = 4 * 2 * kTile;
+  static constexpr int kSmem = 1024 + kQ + kStages * (kK + kV) + kRaw;
+};
+
+// The rows of one item: row R of a (sequence, head) is token R / group, query head R % group.
+struct Item {
+  int b, head, row0, rows;
+  int64_t first;
+  int pos0, len;
+  int step0, steps;  // of this CTA's share of the keys, kKeys each
+};
+
+__device__ __forceinline__ bool item_of(const PromptParams& p, int index, int split, Item& it) {
+  const PagedView& c = p.a.c;
+  const int per = c.batch * c.kv_heads;
+  const int tile = p.row_tiles - 1 - index / per;  // the longest first
+  const int bh = index % per;
+  it.head = bh % c.kv_heads;
+  it.b = bh / c.kv_heads;
+  int count;
+  new_tokens(c, it.b, it.first, count);
+  const int all = count * p.a.group;
+  it.row0 = tile * kRows;
+  if (all <= p.min_rows || it.row0 >= all) return false;
+  it.rows = min(kRows, all - it.row0);
+  const int len = c.seq_lens[it.b];
+  it.pos0 = len - count;
+  it.len = len < 0 ? 0 : (len < c.limit ? len : c.limit);
+  const int p0 = it.pos0 + it.row0 / p.a.group, p1 = it.pos0 + (it.row0 + it.rows - 1) / p.a.group;
+  const int hi = p1 < 0 ? 0 : (p.a.causal ? min(it.len, p1 + 1) : it.len);
+  const int lo = p.a.window > 0 ? max(0, p0 - p.a.window + 1) : 0;
+  const int s0 = lo / kKeys, s1 = (hi + kKeys - 1) / kKeys;
+  const int n = hi > lo ? s1 - s0 : 0;
+  it.step0 = s0 + int((int64_t(n) * split) / p.splits);
+  it.steps = s0 + int((int64_t(n) * (split + 1)) / p.splits) - it.step0;
+  return true;
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  tmem_ld_x32_nowait(taddr, r);
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+template <bool BF16, int G, bool MOD>
+__global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams p) {
+  using C = Cfg<G>;
+  constexpr int D = C::D;
+  constexpr TileLayout L{G};
+  const PagedAttnArgs& a = p.a;
+  const PagedView& c = a.c;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sq = smem;
+  uint8_t* sk = sq + C::kQ;
+  uint8_t* sv = sk + kStages * C::kK;
+  uint8_t* raw = sv + kStages * C::kV;
+  __shared__ uint64_t q_full, k_full[kStages], v_full[kStages], k_empty[kStages], v_empty[kStages];
+  __shared__ uint64_t s_full[2], p_full[2], o_done[2], raw_full[4], drain;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_held[4][4];  // [step % 4][warp]: which of the warp's two tiles a page holds
+  __shared__ volatile int s_abort, s_never;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int split = blockIdx.y;
+  if (tid == 0) {
+    mbar_init(&q_full, 8);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(k_full + i, 4);
+      mbar_init(v_full + i, 4);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 4);
+      mbar_init(o_done + i, 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(raw_full + i, 1);
+    mbar_init(&drain, 1);
+    s_abort = s_never = 0;
+    fence_mbar_init();
+  }
+  pdl_wait();
+  Item it;
+  if (!item_of(p, blockIdx.x, split, it)) return;
+  if (warp == 12) {
+    tmem_alloc(&s_tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const int tiles = it.rows > 128 ? 2 : 1;
+  const int n = it.steps;
+
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    if (mbar_wait(bar, parity, &s_abort)) return true;
+    if (!s_abort) {
+      s_abort = 1;
+      if (lane == 0) atomicAdd(&g_paged_prompt_timeouts, 1);
+    }
+    return false;
+  };
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ rows
+    const int t = warp >> 2, row = tid & 127, r = t * 128 + row;
+    const bool real = r < it.rows;
+    const int R = it.row0 + r, tok = real ? R / a.group : 0;
+    const int h = it.head * a.group + (real ? R - tok * a.group : 0);
+    const int pos = it.pos0 + tok;
+    float c_row = a.scale;
+    if (t < tiles) {
+      // this row's query into the operand: 8 features at a time in the order (0,4)(1,5)(2,6)(3,7)
+      uint32_t w[D / 2];
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (it.first + tok) * a.q_ts + h * a.q_hs;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (real) {
+          if (a.vec) {
+            v = *reinterpret_cast<const uint4*>(src + 8 * i);
+          } else {
+            uint32_t u[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = uint32_t(src[8 * i + 2 * j]) | (uint32_t(src[8 * i + 2 * j + 1]) << 16);
+            v = make_uint4(u[0], u[1], u[2], u[3]);
+          }
+        }
+        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+      }
+      float f = 1.f;  // power of two that the row is multiplied by
+      if constexpr (BF16) {
+        uint32_t top = 0;  // largest exponent (an infinity or NaN: 255, left as it is)
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i) {
+          top = max(top, (w[i] >> 7) & 0xFFu);
+          top = max(top, (w[i] >> 23) & 0xFFu);
+        }
+        // largest entry to [2^14, 2^15); both factors stay normal numbers
+        int e = top == 255u ? 0 : 141 - int(top);
+        e = min(e, 100);
+        f = __uint_as_float(uint32_t(127 + e) << 23);
+        c_row *= __uint_as_float(uint32_t(127 - e) << 23);
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i)
+          w[i] = h2_pack(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xFFFF0000u) * f);
+      }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const uint4 v = make_uint4(__byte_perm(w[4 * i], w[4 * i + 2], 0x5410), __byte_perm(w[4 * i], w[4 * i + 2], 0x7632),
+                                   __byte_perm(w[4 * i + 1], w[4 * i + 3], 0x5410),
+                                   __byte_perm(w[4 * i + 1], w[4 * i + 3], 0x7632));
+        *reinterpret_cast<uint4*>(sq + (t * C::kAtoms + i / 8) * C::kAtomBytes + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = v;
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&q_full);
+
+    if (t < tiles) {
+      int hi = 0x7FFFFFFF, lo = 0;  // keys this row sees
+      if (real) {
+        hi = pos < 0 ? 0 : (a.causal ? min(it.len, pos + 1) : it.len);
+        if (a.window > 0) lo = max(0, pos - a.window + 1);
+      }
+      const float slope = MOD && a.slopes ? a.slopes[h] * kLog2e : 0.f;
+      const float inv = MOD && a.softcap > 0.f ? c_row / a.softcap : 0.f;
+      const float k_exp = MOD ? 1.f : c_row * kLog2e;
+      const uint32_t quarter = uint32_t((warp & 3) * 32) << 16;
+      const uint32_t ts = tmem + quarter + t * 128, to = tmem + quarter + 256 + t * 128;
+      float m = kNone, l = 0.f;
+      bool ok = true;
+
+      for (int i = 0; i < n; ++i) {
+        ok = wait(s_full + t, i & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const int n0 = (it.step0 + i) * kKeys;
+        const int* hp = s_held[i & 3];
+        const int held = hp[0] | (hp[1] << 2) | (hp[2] << 4) | (hp[3] << 6);  // one bit per 16 keys
+        const bool masked = __any_sync(0xffffffffu, n0 < lo || n0 + kKeys > hi) || held != 0xFF;
+
+        // 32 scores from column 32 q on, in powers of two once multiplied by k_exp
+        auto scores = [&](int q, float (&v)[32]) {
+          tmem_ld32(ts + 32 * q, v);
+          if constexpr (MOD) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float x = a.softcap > 0.f ? a.softcap * tanh_exp(v[k] * inv) : v[k] * c_row;
+              v[k] = fmaf(slope, float(n0 + 32 * q + k - pos), x * kLog2e);
+            }
+          }
+          if (masked) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const int key = n0 + 32 * q + k;
+              if (key >= hi || key < lo || !((held >> (2 * q + k / 16)) & 1)) v[k] = -INFINITY;
+            }
+          }
+        };
+        uint32_t pk[64];
+        float sum = 0.f, top = -INFINITY;
+        bool redo = i == 0;
+        if (!redo) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float v[32];
+            scores(q, v);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) top = fmaxf(top, v[k]);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v[k]) : "f"(fmaf(v[k], k_exp, -m)));
+              sum += v[k];
+            }
+            // pairs in the order of the value operand's tokens
+#pragma unroll
+            for (int k = 0; k < 16; ++k) pk[16 * q + 4 * (k & 3) + (k >> 2)] = h2_pack(v[2 * k], v[2 * k + 1]);
+          }
+          redo = __any_sync(0xffffffffu, top * k_exp > m + kLazy);
+        }
+        if (redo) {
+          if (i == 0) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float v[32];
+              scores(q, v);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) top = fmaxf(top, v[k]);
+            }
+          }
+          const float up = fmaxf(m, top * k_exp), f = exp2f(m - up);
+          m = up;
+          l *= f;
+          if (i > 0) {
+            // (this step's scores come after the last step's product: O is complete)
+#pragma unroll
+            for (int d = 0; d < D; d += 32) {
+              float v[32];
+              tmem_ld32(to + d, v);
+              uint32_t u[16];
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(v[16 * hh + k] * f);
+                tmem_st_x16(to + d + 16 * hh, u);
+              }
+            }
+          }
+          sum = 0.f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float v[32];
+            scores(q, v);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v[k]) : "f"(fmaf(v[k], k_exp, -m)));
+              sum += v[k];
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) pk[16 * q + 4 * (k & 3) + (k >> 2)] = h2_pack(v[2 * k], v[2 * k + 1]);
+          }
+        }
+        l += sum;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t u[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) u[k] = pk[16 * q + k];
+          tmem_st_x16(ts + 16 * q, u);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + t);
+      }
+
+      // ---- result
+      if (n > 0 && ok) ok = wait(o_done + t, 0);
+      tc_fence_after();
+      if (p.splits > 1) {
+        float* part = p.partials + ((int64_t(blockIdx.x) * p.splits + split) * kRows + r) * (D + 2);
+#pragma unroll
+        for (int d = 0; d < D; d += 32) {
+          float v[32];
+          if (n > 0) tmem_ld32(to + d, v);
+          if (real) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 2)
+              *reinterpret_cast<float2*>(part + d + k) = n > 0 ? make_float2(v[k], v[k + 1]) : make_float2(0.f, 0.f);
+          }
+        }
+        if (real) *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
+      } else {
+        const float f = l == 0.f ? 0.f : 1.f / l;
+        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + (it.first + tok) * a.o_ts + h * a.o_hs;
+#pragma unroll
+        for (int d = 0; d < D; d += 32) {
+          float v[32];
+          if (n > 0) tmem_ld32(to + d, v);
+          if (real) {
+            uint32_t u[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const float x = l == 0.f ? 0.f : v[2 * k] * f, y = l == 0.f ? 0.f : v[2 * k + 1] * f;
+              if constexpr (BF16) {
+                const __nv_bfloat162 b2 = __floats2bfloat162_rn(x, y);
+                u[k] = *reinterpret_cast<const uint32_t*>(&b2);
+              } else {
+                u[k] = h2_pack(x, y);
+              }
+            }
+            if (a.vec) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<uint4*>(dst + d + 8 * k) = make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) dst[d + k] = uint16_t(u[k >> 1] >> (16 * (k & 1)));
+            }
+          }
+        }
+      }
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------ operands
+    const int dw = warp - 8, g = lane >> 2, cc = lane & 3;  // keys 32 dw .. 32 dw + 31 of each step
+    uint8_t* buf = raw + dw * 2 * C::kTile;
+    int mine = 0;            // lanes 0, 1: page of the tile to load next
+    auto look = [&](int i) {
+      const int at = (it.step0 + i) * kKeys + 32 * dw + 16 * lane;
+      mine = lane < 2 && i < n && at < it.len ? c.tables[it.b * c.table_stride + (at >> c.page_log2)] : -1;
+    };
+    unsigned held_next = 0;  // lanes 0, 1: of the tiles in flight
+    auto issue = [&](int i) {
+      if (lane < 2) {
+        const bool hold = unsigned(mine) < unsigned(c.num_pages);
+        held_next = __ballot_sync(0x3u, hold);
+        if (lane == 0) mbar_arrive_expect_tx(raw_full + dw, __popc(held_next) * C::kTile);
+        __syncwarp(0x3u);
+        if (hold) {
+          const int at = (it.step0 + i) * kKeys + 32 * dw + 16 * lane;
+          const int per = 1 << (c.page_log2 - 4);
+          bulk_g2s(buf + lane * C::kTile, c.pool + mine * c.page_stride + (int64_t(it.head) * per + ((at >> 4) & (per - 1))) * C::kTile,
+                   C::kTile, raw_full + dw);
+        }
+      }
+    };
+    if (n > 0) {
+      look(0);
+      issue(0);
+      look(1);
+    }
+    bool ok = true, flying = false;  // a copy that nothing has waited for, and its phase
+    uint32_t phase = 0;
+    for (int i = 0; i < n; ++i) {
+      const int st = i & 1;
+      const uint32_t par = (i >> 1) & 1;
+      const unsigned held = __shfl_sync(0xffffffffu, held_next, 0);
+      if (!mbar_wait(raw_full + dw, i & 1, &s_never)) {  // (its own copy: waited for whatever the others saw)
+        if (lane == 0) atomicAdd(&g_paged_prompt_timeouts, 1);
+        s_abort = 1;
+        flying = false;
+        break;
+      }
+      uint32_t kw[2][2][G], vw[2][2][G], ks[2][2][(2 * G + 3) / 4], kz[2][2][(G + 3) / 4], vs[2][2][G], vz[2][2][(2 * G + 3) / 4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint8_t* tp = buf + x * C::kTile;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          lds<4 * G>(tp + L.k_codes() + y * L.block() + lane * 4 * G, kw[x][y]);
+          lds<4 * G>(tp + L.v_codes() + y * L.block() + lane * 4 * G, vw[x][y]);
+          lds<2 * G>(tp + L.k_scales() + (g + 8 * y) * 2 * G, ks[x][y]);
+          lds<G>(tp + L.k_zeros() + (g + 8 * y) * G, kz[x][y]);
+          lds<4 * G>(tp + L.v_scales() + (cc + 4 * y) * 4 * G, vs[x][y]);
+          lds<2 * G>(tp + L.v_zeros() + (cc + 4 * y) * 2 * G, vz[x][y]);
+        }
+        if (!((held >> x) & 1u)) {  // no page: keys are masked, values have to be finite
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int q = 0; q < G; ++q) vs[x][y][q] = 0;
+        }
+      }
+      __syncwarp();
+      flying = i + 1 < n;
+      phase = (i + 1) & 1;
+      if (flying) {
+        issue(i + 1);
+        look(i + 2);
+      }
+
+      // ---- keys: [token][feature]
+      if (i >= kStages) ok = wait(k_empty + st, par ^ 1);
+      if (!ok) break;
+      if (lane == 0) s_held[i & 3][dw] = int(held);
+      uint8_t* kd = sk + st * C::kK;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int q = 0; q < G; ++q) {
+            const uint32_t s2 = __byte_perm(ks[x][y][q >> 1], 0, q & 1 ? 0x3232 : 0x1010);
+            const uint32_t b = q & 3, z2 = __byte_perm(kz[x][y][q >> 2], 0x64646464u, b | 0x40u | (b << 8) | 0x4000u);
+            const uint32_t w = kw[x][y][q];
+            uint4 o;
+            o.x = h2_mul(h2_sub(code_pair<0>(w, 0x64006400u), z2), s2);
+            o.y = h2_mul(h2_sub(code_pair<1>(w, 0x64006400u), z2), s2);
+            o.z = h2_mul(h2_sub(code_pair<2>(w, 0x64006400u), z2), s2);
+            o.w = h2_mul(h2_sub(code_pair<3>(w, 0x64006400u), z2), s2);
+            const int row = 32 * dw + 16 * x + 8 * y + g;
+            *reinterpret_cast<uint4*>(kd + (q >> 1) * C::kAtomBytes + row * 128 + ((((q & 1) * 4 + cc) ^ g) << 4)) = o;
+          }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(k_full + st);
+
+      // ---- values: [feature][token], tokens {2c, 2c+1, 2c+8, 2c+9, 2c+16, ...} of the 32 as chunk c
+      if (i >= kStages) ok = wait(v_empty + st, par ^ 1);
+      if (!ok) break;
+      uint8_t* vd = sv + st * C::kV + (dw >> 1) * (D * 128);
+#pragma unroll
+      for (int q = 0; q < G; ++q) {
+        uint32_t o[4][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t z2 = __byte_perm(vz[x][y][q >> 1], 0x64646464u, q & 1 ? 0x4342u : 0x4140u);
+            const uint32_t w = vw[x][y][q], s2 = vs[x][y][q];
+            o[0][2 * x + y] = h2_mul(h2_sub(code_pair<0>(w, 0x64006400u), z2), s2);
+            o[1][2 * x + y] = h2_mul(h2_sub(code_pair<1>(w, 0x64006400u), z2), s2);
+            o[2][2 * x + y] = h2_mul(h2_sub(code_pair<2>(w, 0x64006400u), z2), s2);
+            o[3][2 * x + y] = h2_mul(h2_sub(code_pair<3>(w, 0x64006400u), z2), s2);
+          }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = 32 * q + 4 * g + j;
+          *reinterpret_cast<uint4*>(vd + row * 128 + ((((dw & 1) * 4 + cc) ^ (row & 7)) << 4)) =
+              make_uint4(o[j][0], o[j][1], o[j][2], o[j][3]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(v_full + st);
+    }
+    if (flying && !ok) mbar_wait(raw_full + dw, phase, &s_never);
+  } else if (lane == 0 && n > 0) {
+    // ------------------------------------------------------------ products
+    constexpr uint32_t id_s = idesc_f16(false, 128, kKeys), id_o = idesc_f16(false, 128, D);
+    auto scores = [&](int t, int st) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t off = (k / 4) * C::kAtomBytes + (k % 4) * 32;
+        mma_ss(tmem + t * 128, smem_desc_k_sw128(smem_u32(sq) + t * C::kAtoms * C::kAtomBytes + off),
+               smem_desc_k_sw128(smem_u32(sk) + st * C::kK + off), id_s, k > 0);
+      }
+      mma_commit(s_full + t);
+    };
+    bool ok = wait(&q_full, 0) && wait(k_full, 0);
+    if (ok) {
+      tc_fence_after();
+      for (int t = 0; t < tiles; ++t) scores(t, 0);
+      mma_commit(k_empty);
+      for (int i = 0; i < n && ok; ++i) {
+        const int st = i & 1, sn = (i + 1) & 1;
+        for (int t = 0; t < tiles && ok; ++t) {
+          if (t == 0) ok = wait(v_full + st, (i >> 1) & 1);
+          ok = ok && wait(p_full + t, i & 1);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8,
+                   smem_desc_k_sw128(smem_u32(sv) + st * C::kV + (k / 4) * (D * 128) + (k % 4) * 32), id_o, i > 0 || k > 0);
+          if (t == tiles - 1) mma_commit(v_empty + st);
+          if (i + 1 < n) {
+            if (t == 0) ok = wait(k_full + sn, ((i + 1) >> 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            scores(t, sn);
+            if (t == tiles - 1) mma_commit(k_empty + sn);
+          } else {
+            mma_commit(o_done + t);
+          }
+        }
+      }
+    }
+    if (!ok) {  // products that are still running read shared memory and TMEM
+      mma_commit(&drain);
+      mbar_wait(&drain, 0, &s_never);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// One warp per row: the partial results of its splits.
+template <bool BF16, int G>
+__global__ void __launch_bounds__(256) paged_prompt_join_kernel(PromptParams p) {
+  constexpr int D = 32 * G;
+  pdl_wait();
+  const PagedAttnArgs& a = p.a;
+  const int lane = threadIdx.x & 31;
+  Item it;
+  if (!item_of(p, blockIdx.x, 0, it)) return;
+  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < it.rows; r += gridDim.y * 8) {
+    const float* part = p.partials + (int64_t(blockIdx.x) * p.splits * kRows + r) * (D + 2);
+    const int64_t step = int64_t(kRows) * (D + 2);
+    float top = kNone, sum = 0.f, acc[G];
+#pragma unroll
+    for (int q = 0; q < G; ++q) acc[q] = 0.f;
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, part[s * step + D]);
+    for (int s = 0; s < p.splits; ++s) {
+      const float f = exp2f(part[s * step + D] - top);
+      sum = fmaf(f, part[s * step + D + 1], sum);
+#pragma unroll
+      for (int q = 0; q < G; ++q) acc[q] = fmaf(f, part[s * step + 32 * q + lane], acc[q]);
+    }
+    const int R = it.row0 + r, tok = R / a.group, h = it.head * a.group + R - tok * a.group;
+#pragma unroll
+    for (int q = 0; q < G; ++q)
+      store_from_float(a.out, (it.first + tok) * a.o_ts + h * a.o_hs + 32 * q + lane, a.dtype,
+                       sum == 0.f ? 0.f : acc[q] / sum);
+  }
+}
+
+template <class K>
+int launch_dep(K kernel, dim3 grid, int threads, int smem, const PromptParams& p, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p));
+}
+
+template <bool BF16, int G, bool MOD>
+int launch_one(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
+  using C = Cfg<G>;
+  static PerContextOnce once;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e);
+  auto kern = paged_prompt_kernel<BF16, G, MOD>;
+  e = once.run(dev, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem); });
+  if (e != cudaSuccess) return cuda_status(e);
+  PromptParams p;
+  p.a = a;
+  p.min_rows = min_rows;
+  p.row_tiles = int((int64_t(a.c.max_q) * a.group + kRows - 1) / kRows);
+  const int64_t items = int64_t(p.row_tiles) * a.c.batch * a.c.kv_heads;
+  if (items > INT32_MAX) return SPECTRA_ERR_SHAPE;
+  // two steps of keys a split at least
+  const int64_t most = std::max<int64_t>(1, a.c.limit / (2 * kKeys));
+  p.splits = int(std::max<int64_t>(1, std::min<int64_t>(most, device_sms(dev) / items)));
+  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + kPagedCounterBytes);
+  if (p.splits > 1 &&
+      a.workspace_bytes < kPagedCounterBytes + size_t(items) * p.splits * kRows * (C::D + 2) * sizeof(float))
+    return SPECTRA_ERR_WORKSPACE;
+  const int status = launch_dep(kern, dim3(unsigned(items), unsigned(p.splits)), kThreads, C::kSmem, p, st);
+  if (status != SPECTRA_OK || p.splits == 1) return status;
+  return launch_dep(paged_prompt_join_kernel<BF16, G>, dim3(unsigned(items), 8), 256, 0, p, st);
+}
+
+template <bool BF16, int G>
+int launch_mod(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
+  return a.softcap > 0.f || a.slopes ? launch_one<BF16, G, true>(a, min_rows, st) : launch_one<BF16, G, false>(a, min_rows, st);
+}
+
+template <bool BF16>
+int launch_dim(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
+  switch (a.c.head_dim) {
+    case 32: return launch_mod<BF16, 1>(a, min_rows, st);
+    case 64: return launch_mod<BF16, 2>(a, min_rows, st);
+    case 96: return launch_mod<BF16, 3>(a, min_rows, st);
+    case 128: return launch_mod<BF16, 4>(a, min_rows, st);
+  }
+  return SPECTRA_ERR_UNSUPPORTED;
+}
+
+}  // namespace
+
+size_t paged_prompt_workspace_bytes(int head_dim) {
+  // (splits only while items * splits <= SMs; 160 covers every sm_100a part)
+  return kPagedCounterBytes + size_t(160) * kRows * (head_dim + 2) * sizeof(float);
+}
+
+int launch_paged_prompt(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
+  return a.dtype == SPECTRA_DT_BF16 ? launch_dim<true>(a, min_rows, st) : launch_dim<false>(a, min_rows, st);
+}
+
+int paged_prompt_timeouts(long long* out, bool reset) { return read_timeout_counter(g_paged_prompt_timeouts, out, reset); }
+
+}  // namespace spectra

@@ -45,4 +45,75 @@ __device__ __forceinline__ uint8_t* tile_of(const PagedView& c, int b, int h, in
   return c.pool + page * c.page_stride + (int64_t(h) * tiles + tile) * L.bytes();
 }
 
+// Scores are kept in powers of two.  A running maximum is raised when a score
+// passes it by more than kLazy.
+constexpr float kLazy = 8.f;
+constexpr float kNone = -1e30f;  // below every score that is seen
+constexpr float kLog2e = 1.4426950408889634f;
+
+// BYTES of shared memory into registers, as wide as their alignment allows.
+template <int BYTES>
+__device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[(BYTES + 3) / 4]) {
+  if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (BYTES % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 8; ++i) {
+      const uint2 v = reinterpret_cast<const uint2*>(p)[i];
+      w[2 * i] = v.x; w[2 * i + 1] = v.y;
+    }
+  } else if constexpr (BYTES % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+  } else if constexpr (BYTES % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < (BYTES + 3) / 4; ++i) w[i] = 0;
+#pragma unroll
+    for (int i = 0; i < BYTES / 2; ++i) w[i >> 1] |= uint32_t(reinterpret_cast<const uint16_t*>(p)[i]) << (16 * (i & 1));
+  } else {
+#pragma unroll
+    for (int i = 0; i < (BYTES + 3) / 4; ++i) w[i] = 0;
+#pragma unroll
+    for (int i = 0; i < BYTES; ++i) w[i >> 2] |= uint32_t(p[i]) << (8 * (i & 3));
+  }
+}
+
+// Nibble J of both halves of a code word on top of `magic`.
+template <int J>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t magic) {
+  return ((w >> (4 * J)) & 0x000F000Fu) | magic;
+}
+
+__device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t h2_pack(float lo, float hi) {
+  const __half2 r = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float half_of(uint32_t w, int hi) {
+  return __half2float(__ushort_as_half(uint16_t(hi ? w >> 16 : w & 0xFFFFu)));
+}
+__device__ __forceinline__ float byte_of(uint32_t w, int i) {  // 2^23 + byte, less 2^23
+  return __uint_as_float(__byte_perm(w, kMagic, 0x7650u | i)) - 8388608.f;
+}
+// tanh by its exponential: absolute error a few 2^-24 over the whole range.
+__device__ __forceinline__ float tanh_exp(float x) {
+  return 1.f - __fdividef(2.f, 1.f + exp2f(2.f * kLog2e * x));
+}
+
 }  // namespace spectra

@@ -5,7 +5,7 @@ The reference keeps its INT4 cache as one dense tensor per layer
 all of it at every step for the model's own attention.  Here the cache stays
 in pages of 4-bit codes that sequences share out among themselves, the keys
 enter it with the position rotation applied, and the attention reads the codes
-(csrc/paged_kv.cu, csrc/paged_attn.cu):
+(csrc/paged_kv.cu, csrc/paged_attn.cu, csrc/paged_prompt.cu):
 
     cache = PagedKVCache(num_pages, kv_heads, head_dim, page_size=64)
     batch = TokenBatch(block_tables, seq_lens)              # one new token per sequence
