@@ -458,7 +458,7 @@ int paged_view(const SpectraPagedCache* c, const SpectraTokenBatch* b, PagedView
   v.total = b->total;
   v.q_len = b->cu_q ? 0 : int(std::min<int64_t>(b->q_len, b->total));
   v.max_q = int(std::min<int64_t>(b->max_q, b->total));
-  v.limit = int(std::min<int64_t>(b->max_len, std::min<int64_t>(b->width, INT32_MAX / P) * P));
+  v.limit = c->num_pages == 0 ? 0 : int(std::min<int64_t>(b->max_len, std::min<int64_t>(b->width, INT32_MAX / P) * P));
   return SPECTRA_OK;
 }
 

@@ -9,17 +9,22 @@
 // heads times the new tokens) are the columns of the tensor-core products, so
 // the codes are unpacked once for all of them.
 //
-// Products (mma.sync m16n8k16, fp32 accumulation; with 1-16 rows per head the
+// Products (mma.sync m16n8k16, fp16 in, fp32 out; with 1-16 rows per head the
 // tcgen05 shapes would be mostly padding, and the kernel is bound by bytes
 // and by unpacking instructions, not by the tensor pipe):
-//   S^T = K Q^T: A = raw key codes offset + q (128 + q in bf16, 1024 + q in
-//     fp16: one mask-and-or per pair), 16 tokens x 16 features; per group of
-//     32 features the accumulator starts at -offset * X, X = sum of q over the
-//     group, and t = s (D - z X) in fp32: the keys are never rounded.
+//   S^T = K Q^T: A = raw key codes, 16 tokens x 16 features.  A nibble under
+//     fp16's 0x6400 is 1024 + q where it lies in bits 0-3 and 1024 + 16 q in
+//     bits 4-7 (no shift; those queries are divided by 16 and see 64 + q).  Per
+//     group of 32 features, X = sum of q over the group, the accumulator starts
+//     at the offsets' share of the sum less 1024 X, and t = s (D - (1024 + z)
+//     X) + 1024 X s in fp32, with 1024 + z again a nibble under 0x6400: the keys
+//     are never rounded.
 //   O^T = V^T P^T: A = values (q - z) s in fp16 (exact difference, one
 //     rounding of the product, 11 bits), B = P in fp16, transposed in
 //     registers (movmatrix).  P <= 2^kLazy, so fp16 holds it; its rounding
 //     (2^-12) averages over the keys.
+// Queries of both types are scaled per row by a power of two to fp16's upper
+// range (exact down to 2^-24 of the row's largest entry).
 // The running maximum is only raised when a score passes it by more than
 // kLazy (in powers of two): most tiles need no cross-lane reduction and no
 // rescaling of O.
@@ -94,19 +99,18 @@ struct Cfg {
   static constexpr int kMerge = kWarps * kSlab * 4;           // shares the ring's memory
   static constexpr int kBig = kRing > kMerge ? kRing : kMerge;
   static constexpr int kQ = G * NT * 32 * 16;                 // query fragments
-  static constexpr int kX = G * NT * 4 * 16;                  // {-offset X, X} of a lane's two rows
+  static constexpr int kX = G * NT * 4 * 32;                  // {C, C', C, C'} and {X, X'} of a lane's two rows
   static constexpr int kMeta = ROWS * 16;                     // hi, lo, slope, position of a row
-  static constexpr int kSmem = kBig + kQ + kX + kMeta + kWarps * kStages * 8 + 64;
+  static constexpr int kCtas = G * NT <= 4 ? 4 : 2;  // per SM: what the registers allow
+  static constexpr int kSmem = kBig + kQ + kX + kMeta + ROWS * 4 + kWarps * kStages * 8;
   static constexpr int kPartial = ROWS * (D + 2);             // floats of one CTA's partial result
 };
 
 // ------------------------------------------------------------ the kernel
-template <bool BF16, int G, int NT, bool MOD>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
+template <int G, int NT, bool MOD>
+__global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel(AttnParams p) {
   using C = Cfg<G, NT>;
   constexpr int D = C::D, ROWS = C::ROWS;
-  constexpr uint32_t kKeyMagic = BF16 ? 0x43004300u : 0x64006400u;
-  constexpr float kKeyOffset = BF16 ? 128.f : 1024.f;
   constexpr TileLayout L{G};
   const PagedAttnArgs& a = p.a;
   const PagedView& c = a.c;
@@ -117,7 +121,8 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
   uint4* qfrag = reinterpret_cast<uint4*>(smem + C::kBig);
   float4* xs = reinterpret_cast<float4*>(smem + C::kBig + C::kQ);
   int4* meta = reinterpret_cast<int4*>(smem + C::kBig + C::kQ + C::kX);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBig + C::kQ + C::kX + C::kMeta);
+  float* factor = reinterpret_cast<float*>(smem + C::kBig + C::kQ + C::kX + C::kMeta);  // of a row's scores
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBig + C::kQ + C::kX + C::kMeta + ROWS * 4);
   __shared__ long long s_scan[kWarps];
   __shared__ long long s_base;
   __shared__ int s_seq, s_last;
@@ -200,7 +205,8 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
   long long seq_base = s_base;
   if (b < 0) return;
 
-  const float c_exp = MOD ? 1.f : a.scale * kLog2e;
+  const bool bf16 = a.dtype == SPECTRA_DT_BF16;
+  const int per_page = 1 << (c.page_log2 - 4);  // tiles
   uint32_t phase = 0;  // a bit for each stage
   long long at = begin;
 
@@ -214,70 +220,124 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
       s = span_of<ROWS>(p, b);
       seq_units = (long long)(s.units) * s.tiles * c.kv_heads;
     }
-    const int seg = int((at - seq_base) / s.units);
+    const int seg = int(unsigned(at - seq_base) / unsigned(s.units));  // (the launch checks that a sequence's fit)
     const long long seg_begin = seq_base + (long long)(seg) * s.units, seg_end = seg_begin + s.units;
     const int head = seg / s.tiles, row0 = (seg - head * s.tiles) * ROWS;
     const int u_begin = s.unit0 + int(at - seg_begin);
-    const int u_end = s.unit0 + int((seg_end < end ? seg_end : end) - seg_begin);
+    const int u_stop = s.unit0 + int((seg_end < end ? seg_end : end) - seg_begin);
+    const int u_end = s.len > 0 ? u_stop : u_begin;  // (nothing held: nothing to load)
     const int rows = min(ROWS, s.count * a.group - row0);
 
-    // ---- units to load: warp w takes u_begin + w, + kWarps, ...
-    auto issue = [&](int u, int stage) {
-      if (lane < 2) {
-        const int pos = u * kUnit + lane * kTileTokens;
-        const uint8_t* src = pos < s.len ? tile_of(c, b, head, pos) : nullptr;
-        uint64_t* bar = bars + warp * kStages + stage;
-        uint8_t* dst = ring + (warp * kStages + stage) * C::kStage + lane * C::kTile;
-        const unsigned held = __ballot_sync(0x3u, src != nullptr);
-        if (lane == 0) {
-          s_held[warp * kStages + stage] = int(held);
-          sm100::mbar_arrive_expect_tx(bar, __popc(held) * C::kTile);
-        }
-        __syncwarp(0x3u);
-        if (src) {
-          bulk_g2s(dst, src, C::kTile, bar);
-        } else {  // its keys are masked; its values have to be finite
-          for (int i = L.v_codes(); i < C::kTile; i += 4) *reinterpret_cast<uint32_t*>(dst + i) = 0;
-          sm100::fence_proxy_async_smem();
-        }
+    // ---- units to load: warp w takes u_begin + w, + kWarps, ...  Lane j knows where
+    // the j-th of the next 32 of them lies, and in the address's low bits which of its
+    // tiles a page holds; where none does, page 0's tile takes its place (the keys are
+    // masked, the values finite).
+    const int next = u_begin + warp;
+    const uint8_t* head_pool = c.pool + int64_t(head) * per_page * C::kTile;
+    const int* table = c.tables + b * c.table_stride;
+    const bool small = c.page_log2 == 4;  // a page is one tile
+    uint64_t here = 0, here1 = 0, ahead = 0, ahead1 = 0;
+    auto look = [&](int from, uint64_t& w0, uint64_t& w1) {  // of the warp's units from `from` on
+      const int u = next + (from + lane) * kWarps, pos = u * kUnit;
+      const bool in = u < u_end && pos < s.len;
+      const int p0 = in ? table[pos >> c.page_log2] : -1;
+      const bool h0 = unsigned(p0) < unsigned(c.num_pages);
+      w0 = reinterpret_cast<uint64_t>(head_pool + (h0 ? p0 : 0) * c.page_stride + (u * 2 & (per_page - 1)) * C::kTile) + (h0 ? 3 : 0);
+      if (small) {
+        const int p1 = in && pos + kTileTokens < s.len ? table[(pos >> 4) + 1] : -1;
+        const bool h1 = unsigned(p1) < unsigned(c.num_pages);
+        w0 -= h0 && !h1 ? 2 : 0;
+        w0 += h1 && !h0 ? 2 : 0;
+        w1 = reinterpret_cast<uint64_t>(head_pool + (h1 ? p1 : 0) * c.page_stride);
       }
     };
-    int next = u_begin + warp;
+    auto issue = [&](int k, int stage) {  // the warp's k-th unit
+      const uint64_t w0 = __shfl_sync(0xffffffffu, here, k & 31);
+      const uint64_t w1 = small ? __shfl_sync(0xffffffffu, here1, k & 31) : 0;
+      if (lane == 0) {
+        uint64_t* bar = bars + warp * kStages + stage;
+        uint8_t* dst = ring + (warp * kStages + stage) * C::kStage;
+        s_held[warp * kStages + stage] = int(w0) & 3;
+        sm100::mbar_arrive_expect_tx(bar, C::kStage);
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(w0 & ~uint64_t(15));
+        bulk_g2s(dst, src, small ? C::kTile : C::kStage, bar);
+        if (small) bulk_g2s(dst + C::kTile, reinterpret_cast<const uint8_t*>(w1), C::kTile, bar);
+      }
+      if ((k & 31) == 31) {
+        here = ahead;
+        here1 = ahead1;
+        look(k + 33, ahead, ahead1);
+      }
+    };
+    look(0, here, here1);
+    if (next + 32 * kWarps < u_end) look(32, ahead, ahead1);
 #pragma unroll
     for (int st = 0; st < kStages; ++st) {
-      if (next + st * kWarps < u_end) issue(next + st * kWarps, st);
+      if (next + st * kWarps < u_end) issue(st, st);
     }
 
-    // ---- query fragments: X and the two products' B registers
-    for (int i = tid; i < G * NT * 32; i += kThreads) {
-      const int grp = i / (NT * 32), nt = (i / 32) % NT, row = row0 + nt * 8 + g;
-      float x[8] = {};
-      uint32_t raw[4] = {};
-      if (nt * 8 + g < rows) {
-        const int tok = row / a.group, h = head * a.group + row - tok * a.group;
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (s.first + tok) * a.q_ts + h * a.q_hs + grp * 32 + cc * 8;
-        if (a.vec) {
-          const uint4 v = *reinterpret_cast<const uint4*>(src);
-          raw[0] = v.x; raw[1] = v.y; raw[2] = v.z; raw[3] = v.w;
-        } else {
+    // ---- query fragments: the products' B registers, the groups' sums; four lanes a row
+    if (warp < NT) {
+      const int row = warp * 8 + g;
+      uint32_t raw[G][4];
+      if (row < rows) {
+        const int tok = (row0 + row) / a.group, h = head * a.group + (row0 + row) - tok * a.group;
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (s.first + tok) * a.q_ts + h * a.q_hs + cc * 8;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) raw[j >> 1] |= uint32_t(src[j]) << (16 * (j & 1));
+        for (int grp = 0; grp < G; ++grp) {
+          if (a.vec) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src + grp * 32);
+            raw[grp][0] = v.x; raw[grp][1] = v.y; raw[grp][2] = v.z; raw[grp][3] = v.w;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              raw[grp][j] = uint32_t(src[grp * 32 + 2 * j]) | (uint32_t(src[grp * 32 + 2 * j + 1]) << 16);
+          }
         }
+      } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t bits = (raw[j >> 1] >> (16 * (j & 1))) & 0xFFFFu;
-          x[j] = BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(uint16_t(bits)));
+        for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) raw[grp][j] = 0;
+      }
+      auto value = [&](int grp, int j) {
+        const uint32_t w = raw[grp][j >> 1], bits = j & 1 ? w >> 16 : w & 0xFFFFu;
+        return bf16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(uint16_t(bits)));
+      };
+      uint32_t top = 0;  // the row's largest exponent, in fp32's terms
+#pragma unroll
+      for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, (__float_as_uint(value(grp, j)) >> 23) & 0xFFu);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // largest entry to [2^11, 2^12) (an infinity or NaN: left as it is); both factors are normal numbers
+      const int e = min(top == 255u ? 0 : 138 - int(top), 100);
+      const float f = __uint_as_float(uint32_t(127 + e) << 23);
+      if (cc == 0) factor[row] = a.scale * __uint_as_float(uint32_t(127 - e) << 23);
+#pragma unroll
+      for (int grp = 0; grp < G; ++grp) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = value(grp, j) * f;
+        // pairs (0,4) (1,5) (2,6) (3,7): the order in which the code pairs come
+        qfrag[(grp * NT + warp) * 32 + lane] = make_uint4(h2_pack(x[0], x[4]), h2_pack(x[1] * 0.0625f, x[5] * 0.0625f),
+                                                          h2_pack(x[2], x[6]), h2_pack(x[3] * 0.0625f, x[7] * 0.0625f));
+        float even = (x[0] + x[4]) + (x[2] + x[6]), odd = (x[1] + x[5]) + (x[3] + x[7]);
+#pragma unroll
+        for (int k = 1; k <= 2; k <<= 1) {
+          even += __shfl_xor_sync(0xffffffffu, even, k);
+          odd += __shfl_xor_sync(0xffffffffu, odd, k);
+        }
+        // (1024 + q) even + (64 + q) odd - (1024 + z) X, X = even + odd: the constant is 960 odd
+        const float start = 960.f * odd, sum = even + odd;
+        const float start1 = __shfl_xor_sync(0xffffffffu, start, 4), sum1 = __shfl_xor_sync(0xffffffffu, sum, 4);
+        if (cc == 0 && (g & 1) == 0) {
+          float4* x4 = xs + ((grp * NT + warp) * 4 + g / 2) * 2;
+          x4[0] = make_float4(start, start1, start, start1);
+          x4[1] = make_float4(sum, sum1, 0.f, 0.f);
         }
       }
-      // pairs (0,4) (1,5) (2,6) (3,7): the order in which the code pairs come
-      qfrag[i] = make_uint4(__byte_perm(raw[0], raw[2], 0x5410), __byte_perm(raw[0], raw[2], 0x7632),
-                            __byte_perm(raw[1], raw[3], 0x5410), __byte_perm(raw[1], raw[3], 0x7632));
-      float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const float other = __shfl_xor_sync(0xffffffffu, sum, 4);  // row g ^ 1
-      if (cc == 0 && (g & 1) == 0)
-        xs[(grp * NT + nt) * 4 + g / 2] = make_float4(-kKeyOffset * sum, -kKeyOffset * other, sum, other);
     }
     if (tid < ROWS) {
       int hi = 0, lo = 0, pos = 0;
@@ -309,8 +369,14 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
       for (int i = 0; i < G * 2 * 4; ++i) o[i / 8][(i / 4) & 1][nt][i & 3] = 0.f;
     }
 
-    int stage = 0;
-    for (int u = next; u < u_end; u += kWarps) {
+    float c_exp[NT][2];  // from a product to a score in powers of two (MOD: done before)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) c_exp[nt][j] = MOD ? 1.f : factor[nt * 8 + 2 * cc + j] * kLog2e;
+
+    int stage = 0, unit = 0;
+    for (int u = next; u < u_end; u += kWarps, ++unit) {
       if (!sm100::mbar_wait(bars + warp * kStages + stage, (phase >> stage) & 1u, &s_never)) {
         s_stop = 1;
         if (lane == 0) atomicAdd(&g_paged_attn_timeouts, 1);
@@ -318,41 +384,47 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
       const int held = s_held[warp * kStages + stage];
       const uint8_t* buf = ring + (warp * kStages + stage) * C::kStage;
 
-      // ---- scores of 32 tokens: s[tile][nt][4], tokens g, g + 8, rows 2cc, 2cc + 1
+      // ---- scores of 32 tokens: sc[tile][nt][4], tokens g, g + 8, rows 2cc, 2cc + 1
       float sc[2][NT][4];
+      {
+        uint32_t w0[2][G], w1[2][G], ks0[2][(2 * G + 3) / 4], ks1[2][(2 * G + 3) / 4], kz0[2][(G + 3) / 4], kz1[2][(G + 3) / 4];
 #pragma unroll
-      for (int tile = 0; tile < 2; ++tile) {
-        const uint8_t* t = buf + tile * C::kTile;
-        uint32_t w0[G], w1[G], ks0[(2 * G + 3) / 4], ks1[(2 * G + 3) / 4], kz0[(G + 3) / 4], kz1[(G + 3) / 4];
-        lds<4 * G>(t + L.k_codes() + lane * 4 * G, w0);
-        lds<4 * G>(t + L.k_codes() + L.block() + lane * 4 * G, w1);
-        lds<2 * G>(t + L.k_scales() + g * 2 * G, ks0);
-        lds<2 * G>(t + L.k_scales() + (g + 8) * 2 * G, ks1);
-        lds<G>(t + L.k_zeros() + g * G, kz0);
-        lds<G>(t + L.k_zeros() + (g + 8) * G, kz1);
+        for (int tile = 0; tile < 2; ++tile) {
+          const uint8_t* t = buf + tile * C::kTile;
+          lds<4 * G>(t + L.k_codes() + lane * 4 * G, w0[tile]);
+          lds<4 * G>(t + L.k_codes() + L.block() + lane * 4 * G, w1[tile]);
+          lds<2 * G>(t + L.k_scales() + g * 2 * G, ks0[tile]);
+          lds<2 * G>(t + L.k_scales() + (g + 8) * 2 * G, ks1[tile]);
+          lds<G>(t + L.k_zeros() + g * G, kz0[tile]);
+          lds<G>(t + L.k_zeros() + (g + 8) * G, kz1[tile]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[tile][nt][i] = 0.f;
+            for (int i = 0; i < 4; ++i) sc[tile][nt][i] = 0.f;
+        }
 #pragma unroll
         for (int grp = 0; grp < G; ++grp) {
-          const uint32_t a0 = code_pair<0>(w0[grp], kKeyMagic), a1 = code_pair<0>(w1[grp], kKeyMagic);
-          const uint32_t a2 = code_pair<1>(w0[grp], kKeyMagic), a3 = code_pair<1>(w1[grp], kKeyMagic);
-          const uint32_t a4 = code_pair<2>(w0[grp], kKeyMagic), a5 = code_pair<2>(w1[grp], kKeyMagic);
-          const uint32_t a6 = code_pair<3>(w0[grp], kKeyMagic), a7 = code_pair<3>(w1[grp], kKeyMagic);
-          const float s0 = half_of(ks0[grp >> 1], grp & 1), s1 = half_of(ks1[grp >> 1], grp & 1);
-          const float z0 = byte_of(kz0[grp >> 2], grp & 3), z1 = byte_of(kz1[grp >> 2], grp & 3);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const uint4 q = qfrag[(grp * NT + nt) * 32 + lane];
-            const float4 x = xs[(grp * NT + nt) * 4 + cc];
-            float d[4] = {x.x, x.y, x.x, x.y};
-            mma16816<BF16>(d, a0, a1, a2, a3, q.x, q.y);
-            mma16816<BF16>(d, a4, a5, a6, a7, q.z, q.w);
-            sc[tile][nt][0] = fmaf(s0, fmaf(-z0, x.z, d[0]), sc[tile][nt][0]);
-            sc[tile][nt][1] = fmaf(s0, fmaf(-z0, x.w, d[1]), sc[tile][nt][1]);
-            sc[tile][nt][2] = fmaf(s1, fmaf(-z1, x.z, d[2]), sc[tile][nt][2]);
-            sc[tile][nt][3] = fmaf(s1, fmaf(-z1, x.w, d[3]), sc[tile][nt][3]);
+            const float4* x4 = xs + ((grp * NT + nt) * 4 + cc) * 2;
+            const float2 x = *reinterpret_cast<const float2*>(x4 + 1);
+#pragma unroll
+            for (int tile = 0; tile < 2; ++tile) {
+              const uint32_t a0 = w0[tile][grp], a1 = w1[tile][grp];
+              const float s0 = half_of(ks0[tile][grp >> 1], grp & 1), s1 = half_of(ks1[tile][grp >> 1], grp & 1);
+              // 1024 + zero point
+              const float z0 = half_of(__byte_perm(kz0[tile][grp >> 2], 0x64646464u, 0x4040u | (grp & 3)), 0);
+              const float z1 = half_of(__byte_perm(kz1[tile][grp >> 2], 0x64646464u, 0x4040u | (grp & 3)), 0);
+              const float4 start = x4[0];
+              float d[4] = {start.x, start.y, start.z, start.w};
+              mma16816<false>(d, code_low(a0), code_low(a1), code_high(a0), code_high(a1), q.x, q.y);
+              mma16816<false>(d, code_low(a0 >> 8), code_low(a1 >> 8), code_high(a0 >> 8), code_high(a1 >> 8), q.z, q.w);
+              sc[tile][nt][0] = fmaf(s0, fmaf(-z0, x.x, d[0]), sc[tile][nt][0]);
+              sc[tile][nt][1] = fmaf(s0, fmaf(-z0, x.y, d[1]), sc[tile][nt][1]);
+              sc[tile][nt][2] = fmaf(s1, fmaf(-z1, x.x, d[2]), sc[tile][nt][2]);
+              sc[tile][nt][3] = fmaf(s1, fmaf(-z1, x.y, d[3]), sc[tile][nt][3]);
+            }
           }
         }
       }
@@ -360,16 +432,16 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
       // ---- cap, bias, mask
       const int n0 = u * kUnit;
       if constexpr (MOD) {
-        const float inv = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int4 r = meta[nt * 8 + 2 * cc + j];
+            const float scale = factor[nt * 8 + 2 * cc + j], inv = a.softcap > 0.f ? scale / a.softcap : 0.f;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               float& v = sc[k >> 1][nt][2 * (k & 1) + j];
-              const float t = a.softcap > 0.f ? a.softcap * tanh_exp(v * inv) : v * a.scale;
+              const float t = a.softcap > 0.f ? a.softcap * tanh_exp(v * inv) : v * scale;
               v = fmaf(__int_as_float(r.z), float(n0 + 8 * k + g - r.w), t * kLog2e);
             }
           }
@@ -395,7 +467,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          top[nt][j] = fmaxf(fmaxf(sc[0][nt][j], sc[0][nt][2 + j]), fmaxf(sc[1][nt][j], sc[1][nt][2 + j])) * c_exp;
+          top[nt][j] = fmaxf(fmaxf(sc[0][nt][j], sc[0][nt][2 + j]), fmaxf(sc[1][nt][j], sc[1][nt][2 + j])) * c_exp[nt][j];
           raise = raise || top[nt][j] > m[nt][j] + kLazy;
         }
       if (__any_sync(0xffffffffu, raise)) {
@@ -427,7 +499,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
           float e[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i]) : "f"(fmaf(sc[tile][nt][i], c_exp, -m[nt][i & 1])));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i]) : "f"(fmaf(sc[tile][nt][i], c_exp[nt][i & 1], -m[nt][i & 1])));
             l[nt][i & 1] += e[i];
           }
           pb[tile][nt][0] = transpose8x8(h2_pack(e[0], e[1]));
@@ -449,15 +521,15 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
         for (int grp = 0; grp < G; ++grp) {
           const uint32_t pick = grp & 1 ? 0x4342u : 0x4140u;  // 1024 + zero point of both tokens
           const uint32_t z0 = __byte_perm(vz0[grp >> 1], 0x64646464u, pick), z1 = __byte_perm(vz1[grp >> 1], 0x64646464u, pick);
+          const uint32_t c0 = h2_sub(0x63806380u, z0), c1 = h2_sub(0x63806380u, z1);  // 960 - (1024 + z)
           uint32_t v0[4], v1[4];
-          v0[0] = code_pair<0>(w0[grp], 0x64006400u); v0[1] = code_pair<1>(w0[grp], 0x64006400u);
-          v0[2] = code_pair<2>(w0[grp], 0x64006400u); v0[3] = code_pair<3>(w0[grp], 0x64006400u);
-          v1[0] = code_pair<0>(w1[grp], 0x64006400u); v1[1] = code_pair<1>(w1[grp], 0x64006400u);
-          v1[2] = code_pair<2>(w1[grp], 0x64006400u); v1[3] = code_pair<3>(w1[grp], 0x64006400u);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            v0[j] = h2_mul(h2_sub(v0[j], z0), vs0[grp]);
-            v1[j] = h2_mul(h2_sub(v1[j], z1), vs1[grp]);
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t x0 = w0[grp] >> (8 * j), x1 = w1[grp] >> (8 * j);
+            v0[2 * j] = h2_mul(h2_sub(code_low(x0), z0), vs0[grp]);
+            v1[2 * j] = h2_mul(h2_sub(code_low(x1), z1), vs1[grp]);
+            v0[2 * j + 1] = h2_mul(h2_fma(code_high(x0), 0x2C002C00u, c0), vs0[grp]);  // (1024 + 16 q) / 16 - 64 - z
+            v1[2 * j + 1] = h2_mul(h2_fma(code_high(x1), 0x2C002C00u, c1), vs1[grp]);
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -468,7 +540,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
       }
       __syncwarp();
       phase ^= 1u << stage;
-      if (u + kStages * kWarps < u_end && !s_stop) issue(u + kStages * kWarps, stage);
+      if (u + kStages * kWarps < u_end && !s_stop) issue(unit + kStages, stage);
       stage = stage + 1 == kStages ? 0 : stage + 1;
     }
 
@@ -494,15 +566,40 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
     __syncthreads();
 
     const bool whole = seg_begin >= begin && seg_end <= end;
-    const int cta0 = int(seg_begin / share), cta1 = int((seg_end - 1) / share);
+    // the CTAs that share this segment
+    const unsigned step = unsigned(share < (1ll << 30) ? share : (1ll << 30));
+    const int cta0 = seg_begin < begin ? int(blockIdx.x - (unsigned(begin - seg_begin) + step - 1) / step) : int(blockIdx.x);
+    const int cta1 = int(blockIdx.x) + (seg_end > end ? int(unsigned(seg_end - 1 - begin) / step) : 0);
     float* mine = p.partials + int64_t(2 * blockIdx.x + (seg_begin < begin ? 0 : 1)) * C::kPartial;
-    auto put = [&](int row, int d, float v) {
+    auto put = [&](int row, int d, float4 v, float sum) {
       const int tok = (row0 + row) / a.group, h = head * a.group + (row0 + row) - tok * a.group;
-      store_from_float(a.out, (s.first + tok) * a.o_ts + h * a.o_hs + d, a.dtype, v);
+      const float f = sum == 0.f ? 0.f : 1.f / sum;
+      const int64_t at_out = (s.first + tok) * a.o_ts + h * a.o_hs + d;
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      if (a.vec) {
+        uint32_t w[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float lo = sum == 0.f ? 0.f : x[2 * j] * f, hi = sum == 0.f ? 0.f : x[2 * j + 1] * f;
+          const __nv_bfloat162 b2 = __floats2bfloat162_rn(lo, hi);
+          w[j] = bf16 ? *reinterpret_cast<const uint32_t*>(&b2) : h2_pack(lo, hi);
+        }
+        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + at_out) = make_uint2(w[0], w[1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) store_from_float(a.out, at_out + j, a.dtype, sum == 0.f ? 0.f : x[j] * f);
+      }
     };
-    for (int i = tid; i < rows * D; i += kThreads) {
-      const int row = i / D, d = i - row * D;
-      float top = kNone, sum = 0.f, acc = 0.f;
+    auto add = [](float4& acc, float f, const float4& v) {
+      acc.x = fmaf(f, v.x, acc.x);
+      acc.y = fmaf(f, v.y, acc.y);
+      acc.z = fmaf(f, v.z, acc.z);
+      acc.w = fmaf(f, v.w, acc.w);
+    };
+    for (int i = tid; i < rows * (D / 4); i += kThreads) {
+      const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
+      float top = kNone, sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, merge[w * C::kSlab + row * (D + 4) + D]);
 #pragma unroll
@@ -510,16 +607,13 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
         const float* slab = merge + w * C::kSlab + row * (D + 4);
         const float f = exp2f(slab[D] - top);
         sum = fmaf(f, slab[D + 1], sum);
-        acc = fmaf(f, slab[d], acc);
+        add(acc, f, *reinterpret_cast<const float4*>(slab + d));
       }
       if (whole) {
-        put(row, d, sum == 0.f ? 0.f : acc / sum);
+        put(row, d, acc, sum);
       } else {
-        mine[row * D + d] = acc;
-        if (d == 0) {
-          mine[ROWS * D + row] = top;
-          mine[ROWS * D + ROWS + row] = sum;
-        }
+        *reinterpret_cast<float4*>(mine + row * D + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(mine + ROWS * D + 2 * row) = make_float2(top, sum);
       }
     }
     if (!whole) {
@@ -533,29 +627,46 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
       __syncthreads();
       if (s_last) {
         __threadfence();
-        for (int i = tid; i < rows * D; i += kThreads) {
-          const int row = i / D, d = i - row * D;
-          float top = kNone, sum = 0.f, acc = 0.f;
-          for (int k = cta0; k <= cta1; ++k) {
-            const float* part = p.partials + int64_t(2 * k + (k == cta0 ? 1 : 0)) * C::kPartial;
-            const float mk = __ldcg(part + ROWS * D + row), lk = __ldcg(part + ROWS * D + ROWS + row);
-            const float ok = __ldcg(part + row * D + d), t = fmaxf(top, mk);
-            const float f0 = exp2f(top - t), f1 = exp2f(mk - t);
-            sum = sum * f0 + lk * f1;
-            acc = acc * f0 + ok * f1;
-            top = t;
-          }
-          put(row, d, sum == 0.f ? 0.f : acc / sum);
+        // the first CTA's part is its last segment's (slot 1), the others' their first's (slot 0)
+        const float* part0 = p.partials + int64_t(2 * cta0 + 1) * C::kPartial;
+        const float* parts = p.partials + int64_t(2 * cta0) * C::kPartial;
+        const int n = cta1 - cta0;
+        float* tops = merge;  // (every thread is past its reads of the slabs)
+        for (int row = warp; row < rows; row += kWarps) {
+          float top = lane == 0 ? __ldcg(part0 + ROWS * D + 2 * row) : kNone;
+          for (int k = 1 + lane; k <= n; k += 32)
+            top = fmaxf(top, __ldcg(parts + int64_t(2 * k) * C::kPartial + ROWS * D + 2 * row));
+#pragma unroll
+          for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+          if (lane == 0) tops[row] = top;
+        }
+        __syncthreads();
+        for (int i = tid; i < rows * (D / 4); i += kThreads) {
+          const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
+          const float top = tops[row];
+          float sum = 0.f;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          auto take = [&](const float* part) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + ROWS * D + 2 * row));
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + row * D + d));
+            const float f = exp2f(ml.x - top);
+            sum = fmaf(f, ml.y, sum);
+            add(acc, f, v);
+          };
+          take(part0);
+#pragma unroll 8
+          for (int k = 1; k <= n; ++k) take(parts + int64_t(2 * k) * C::kPartial);
+          put(row, d, acc, sum);
         }
       }
     }
     sm100::fence_proxy_async_smem();
     __syncthreads();  // before the ring, the fragments and the row table are written again
-    at = seg_begin + (u_end - s.unit0);
+    at = seg_begin + (u_stop - s.unit0);
   }
 }
 
-template <bool BF16, int G, int NT, bool MOD>
+template <int G, int NT, bool MOD>
 int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   using C = Cfg<G, NT>;
   static PerContextOnce once;
@@ -563,7 +674,7 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e);
-  auto kern = paged_attn_kernel<BF16, G, NT, MOD>;
+  auto kern = paged_attn_kernel<G, NT, MOD>;
   e = once.run(dev, [&] {
     cudaError_t r = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (r == cudaSuccess) r = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas_per_sm[dev], kern, kThreads, C::kSmem);
@@ -575,7 +686,9 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   p.min_share = kWarps;
   p.max_rows = max_rows;
   const int64_t tiles = (std::min<int64_t>(int64_t(a.c.max_q) * a.group, max_rows) + C::ROWS - 1) / C::ROWS;
-  const int64_t most = int64_t(a.c.batch) * a.c.kv_heads * tiles * ((a.c.limit + kUnit - 1) / kUnit + 1);
+  const int64_t of_one = int64_t(a.c.kv_heads) * tiles * ((a.c.limit + kUnit - 1) / kUnit + 1);
+  if (of_one >= (int64_t(1) << 30)) return SPECTRA_ERR_SHAPE;
+  const int64_t most = a.c.batch * of_one;
   const int64_t room = std::min<int64_t>(int64_t(device_sms(dev)) * std::max(1, ctas_per_sm[dev]), kMaxCtas);
   const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(room, (most + p.min_share - 1) / p.min_share));
   p.counters = static_cast<int*>(a.workspace);
@@ -595,37 +708,32 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
-template <bool BF16, int G>
+template <int G>
 int launch_rows(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   const bool mod = a.softcap > 0.f || a.slopes;
   // up to 8 rows per key/value head: one column tile (fewer registers, more CTAs per SM); heads of 256 have
   // no registers for two
   if (G == 8 || int64_t(a.c.max_q) * a.group <= 8)
-    return mod ? launch_one<BF16, G, 1, true>(a, max_rows, st) : launch_one<BF16, G, 1, false>(a, max_rows, st);
+    return mod ? launch_one<G, 1, true>(a, max_rows, st) : launch_one<G, 1, false>(a, max_rows, st);
   constexpr int NT = G == 8 ? 1 : 2;
-  return mod ? launch_one<BF16, G, NT, true>(a, max_rows, st) : launch_one<BF16, G, NT, false>(a, max_rows, st);
-}
-
-template <bool BF16>
-int launch_dim(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
-  switch (a.c.head_dim) {
-    case 32: return launch_rows<BF16, 1>(a, max_rows, st);
-    case 64: return launch_rows<BF16, 2>(a, max_rows, st);
-    case 96: return launch_rows<BF16, 3>(a, max_rows, st);
-    case 128: return launch_rows<BF16, 4>(a, max_rows, st);
-    case 256: return launch_rows<BF16, 8>(a, max_rows, st);
-  }
-  return SPECTRA_ERR_UNSUPPORTED;
+  return mod ? launch_one<G, NT, true>(a, max_rows, st) : launch_one<G, NT, false>(a, max_rows, st);
 }
 
 }  // namespace
 
-size_t paged_attn_workspace_bytes(int head_dim) {
-  return kPagedCounterBytes + size_t(kMaxCtas) * 2 * 16 * (head_dim + 2) * sizeof(float);
+int launch_paged_attn(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
+  switch (a.c.head_dim) {
+    case 32: return launch_rows<1>(a, max_rows, st);
+    case 64: return launch_rows<2>(a, max_rows, st);
+    case 96: return launch_rows<3>(a, max_rows, st);
+    case 128: return launch_rows<4>(a, max_rows, st);
+    case 256: return launch_rows<8>(a, max_rows, st);
+  }
+  return SPECTRA_ERR_UNSUPPORTED;
 }
 
-int launch_paged_attn(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
-  return a.dtype == SPECTRA_DT_BF16 ? launch_dim<true>(a, max_rows, st) : launch_dim<false>(a, max_rows, st);
+size_t paged_attn_workspace_bytes(int head_dim) {
+  return kPagedCounterBytes + size_t(kMaxCtas) * 2 * 16 * (head_dim + 2) * sizeof(float);
 }
 
 int paged_attn_timeouts(long long* out, bool reset) { return read_timeout_counter(g_paged_attn_timeouts, out, reset); }

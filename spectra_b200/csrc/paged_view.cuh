@@ -88,6 +88,15 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t magic) {
   return ((w >> (4 * J)) & 0x000F000Fu) | magic;
 }
 
+// 1024 + q of bits 0-3 of both halves; 1024 + 16 q of bits 4-7.
+__device__ __forceinline__ uint32_t code_low(uint32_t w) { return (w & 0x000F000Fu) | 0x64006400u; }
+__device__ __forceinline__ uint32_t code_high(uint32_t w) { return (w & 0x00F000F0u) | 0x64006400u; }
+
+__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                            *reinterpret_cast<const __half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 __device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
@@ -107,9 +116,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 }
 __device__ __forceinline__ float half_of(uint32_t w, int hi) {
   return __half2float(__ushort_as_half(uint16_t(hi ? w >> 16 : w & 0xFFFFu)));
-}
-__device__ __forceinline__ float byte_of(uint32_t w, int i) {  // 2^23 + byte, less 2^23
-  return __uint_as_float(__byte_perm(w, kMagic, 0x7650u | i)) - 8388608.f;
 }
 // tanh by its exponential: absolute error a few 2^-24 over the whole range.
 __device__ __forceinline__ float tanh_exp(float x) {
