@@ -208,6 +208,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
   const bool bf16 = a.dtype == SPECTRA_DT_BF16;
   const int per_page = 1 << (c.page_log2 - 4);  // tiles
   uint32_t phase = 0;  // a bit for each stage
+  const uint32_t magic = fp16_1024();
   long long at = begin;
 
   while (at < end) {
@@ -276,10 +277,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
       if (next + st * kWarps < u_end) issue(st, st);
     }
 
-    // ---- query fragments: the products' B registers, the groups' sums; four lanes a row
-    if (warp < NT) {
-      const int row = warp * 8 + g;
-      uint32_t raw[G][4];
+    // ---- query fragments: the products' B registers and the groups' sums.  Four
+    // lanes a row; every warp reads whole rows and prepares some of their groups.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = nt * 8 + g;
+      uint32_t raw[G][4], top2 = 0;
+#pragma unroll
+      for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) raw[grp][j] = 0;
       if (row < rows) {
         const int tok = (row0 + row) / a.group, h = head * a.group + (row0 + row) - tok * a.group;
         const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (s.first + tok) * a.q_ts + h * a.q_hs + cc * 8;
@@ -294,35 +301,33 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
               raw[grp][j] = uint32_t(src[grp * 32 + 2 * j]) | (uint32_t(src[grp * 32 + 2 * j + 1]) << 16);
           }
         }
-      } else {
-#pragma unroll
-        for (int grp = 0; grp < G; ++grp)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) raw[grp][j] = 0;
       }
-      auto value = [&](int grp, int j) {
-        const uint32_t w = raw[grp][j >> 1], bits = j & 1 ? w >> 16 : w & 0xFFFFu;
-        return bf16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(uint16_t(bits)));
-      };
-      uint32_t top = 0;  // the row's largest exponent, in fp32's terms
+      // the row's largest entry: of both types, the order of the bits is that of the numbers
 #pragma unroll
       for (int grp = 0; grp < G; ++grp)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, (__float_as_uint(value(grp, j)) >> 23) & 0xFFu);
+        for (int j = 0; j < 4; ++j) top2 = __vmaxu2(top2, raw[grp][j] & 0x7FFF7FFFu);
+      uint32_t top = max(top2 >> 16, top2 & 0xFFFFu);
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // largest entry to [2^11, 2^12) (an infinity or NaN: left as it is); both factors are normal numbers
-      const int e = min(top == 255u ? 0 : 138 - int(top), 100);
+      // to [2^11, 2^12) (an infinity or NaN: left as it is); both factors are normal numbers
+      const float most = bf16 ? __uint_as_float(top << 16) : __half2float(__ushort_as_half(uint16_t(top)));
+      const int top_e = int(__float_as_uint(most) >> 23);
+      const int e = min(top_e == 255 ? 0 : 138 - top_e, 100);
       const float f = __uint_as_float(uint32_t(127 + e) << 23);
-      if (cc == 0) factor[row] = a.scale * __uint_as_float(uint32_t(127 - e) << 23);
+      if (warp == 0 && cc == 0) factor[row] = a.scale * __uint_as_float(uint32_t(127 - e) << 23);
 #pragma unroll
       for (int grp = 0; grp < G; ++grp) {
+        if (grp % kWarps != warp) continue;
         float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = value(grp, j) * f;
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t w = raw[grp][j >> 1];
+          x[j] = f * (bf16 ? __uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16) : half_of(w, j & 1));
+        }
         // pairs (0,4) (1,5) (2,6) (3,7): the order in which the code pairs come
-        qfrag[(grp * NT + warp) * 32 + lane] = make_uint4(h2_pack(x[0], x[4]), h2_pack(x[1] * 0.0625f, x[5] * 0.0625f),
-                                                          h2_pack(x[2], x[6]), h2_pack(x[3] * 0.0625f, x[7] * 0.0625f));
+        qfrag[(grp * NT + nt) * 32 + lane] = make_uint4(h2_pack(x[0], x[4]), h2_pack(x[1] * 0.0625f, x[5] * 0.0625f),
+                                                        h2_pack(x[2], x[6]), h2_pack(x[3] * 0.0625f, x[7] * 0.0625f));
         float even = (x[0] + x[4]) + (x[2] + x[6]), odd = (x[1] + x[5]) + (x[3] + x[7]);
 #pragma unroll
         for (int k = 1; k <= 2; k <<= 1) {
@@ -333,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
         const float start = 960.f * odd, sum = even + odd;
         const float start1 = __shfl_xor_sync(0xffffffffu, start, 4), sum1 = __shfl_xor_sync(0xffffffffu, sum, 4);
         if (cc == 0 && (g & 1) == 0) {
-          float4* x4 = xs + ((grp * NT + warp) * 4 + g / 2) * 2;
+          float4* x4 = xs + ((grp * NT + nt) * 4 + g / 2) * 2;
           x4[0] = make_float4(start, start1, start, start1);
           x4[1] = make_float4(sum, sum1, 0.f, 0.f);
         }
@@ -413,13 +418,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
             for (int tile = 0; tile < 2; ++tile) {
               const uint32_t a0 = w0[tile][grp], a1 = w1[tile][grp];
               const float s0 = half_of(ks0[tile][grp >> 1], grp & 1), s1 = half_of(ks1[tile][grp >> 1], grp & 1);
-              // 1024 + zero point
-              const float z0 = half_of(__byte_perm(kz0[tile][grp >> 2], 0x64646464u, 0x4040u | (grp & 3)), 0);
-              const float z1 = half_of(__byte_perm(kz1[tile][grp >> 2], 0x64646464u, 0x4040u | (grp & 3)), 0);
-              const float4 start = x4[0];
-              float d[4] = {start.x, start.y, start.z, start.w};
-              mma16816<false>(d, code_low(a0), code_low(a1), code_high(a0), code_high(a1), q.x, q.y);
-              mma16816<false>(d, code_low(a0 >> 8), code_low(a1 >> 8), code_high(a0 >> 8), code_high(a1 >> 8), q.z, q.w);
+              const uint32_t zz0 = byte_pair(kz0[tile][grp >> 2], (grp >> 1) & 1), zz1 = byte_pair(kz1[tile][grp >> 2], (grp >> 1) & 1);
+              const float z0 = half_of(zz0, grp & 1), z1 = half_of(zz1, grp & 1);  // 1024 + zero point
+              float d[4];
+              mma_f16(d, code_low(a0, magic), code_low(a1, magic), code_high(a0, magic), code_high(a1, magic), q.x, q.y, x4[0]);
+              mma_f16(d, code_low(a0 >> 8, magic), code_low(a1 >> 8, magic), code_high(a0 >> 8, magic), code_high(a1 >> 8, magic), q.z, q.w);
               sc[tile][nt][0] = fmaf(s0, fmaf(-z0, x.x, d[0]), sc[tile][nt][0]);
               sc[tile][nt][1] = fmaf(s0, fmaf(-z0, x.y, d[1]), sc[tile][nt][1]);
               sc[tile][nt][2] = fmaf(s1, fmaf(-z1, x.x, d[2]), sc[tile][nt][2]);
@@ -519,22 +522,21 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
         lds<2 * G>(t + L.v_zeros() + (cc + 4) * 2 * G, vz1);
 #pragma unroll
         for (int grp = 0; grp < G; ++grp) {
-          const uint32_t pick = grp & 1 ? 0x4342u : 0x4140u;  // 1024 + zero point of both tokens
-          const uint32_t z0 = __byte_perm(vz0[grp >> 1], 0x64646464u, pick), z1 = __byte_perm(vz1[grp >> 1], 0x64646464u, pick);
+          const uint32_t z0 = byte_pair(vz0[grp >> 1], grp & 1), z1 = byte_pair(vz1[grp >> 1], grp & 1);  // 1024 + zero points
           const uint32_t c0 = h2_sub(0x63806380u, z0), c1 = h2_sub(0x63806380u, z1);  // 960 - (1024 + z)
           uint32_t v0[4], v1[4];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const uint32_t x0 = w0[grp] >> (8 * j), x1 = w1[grp] >> (8 * j);
-            v0[2 * j] = h2_mul(h2_sub(code_low(x0), z0), vs0[grp]);
-            v1[2 * j] = h2_mul(h2_sub(code_low(x1), z1), vs1[grp]);
-            v0[2 * j + 1] = h2_mul(h2_fma(code_high(x0), 0x2C002C00u, c0), vs0[grp]);  // (1024 + 16 q) / 16 - 64 - z
-            v1[2 * j + 1] = h2_mul(h2_fma(code_high(x1), 0x2C002C00u, c1), vs1[grp]);
+            v0[2 * j] = h2_mul(h2_sub(code_low(x0, magic), z0), vs0[grp]);
+            v1[2 * j] = h2_mul(h2_sub(code_low(x1, magic), z1), vs1[grp]);
+            v0[2 * j + 1] = h2_mul(h2_fma(code_high(x0, magic), 0x2C002C00u, c0), vs0[grp]);  // (1024 + 16 q) / 16 - 64 - z
+            v1[2 * j + 1] = h2_mul(h2_fma(code_high(x1, magic), 0x2C002C00u, c1), vs1[grp]);
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma16816<false>(o[grp][0][nt], v0[0], v0[1], v1[0], v1[1], pb[tile][nt][0], pb[tile][nt][1]);
-            mma16816<false>(o[grp][1][nt], v0[2], v0[3], v1[2], v1[3], pb[tile][nt][0], pb[tile][nt][1]);
+            mma_f16(o[grp][0][nt], v0[0], v0[1], v1[0], v1[1], pb[tile][nt][0], pb[tile][nt][1]);
+            mma_f16(o[grp][1][nt], v0[2], v0[3], v1[2], v1[3], pb[tile][nt][0], pb[tile][nt][1]);
           }
         }
       }

@@ -396,6 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
     // ------------------------------------------------------------ operands
     const int dw = warp - 8, g = lane >> 2, cc = lane & 3;  // keys 32 dw .. 32 dw + 31 of each step
     uint8_t* buf = raw + dw * 2 * C::kTile;
+    const uint32_t magic = fp16_1024();
     int mine = 0;            // lanes 0, 1: page of the tile to load next
     auto look = [&](int i) {
       const int at = (it.step0 + i) * kKeys + 32 * dw + 16 * lane;
@@ -474,12 +475,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           for (int q = 0; q < G; ++q) {
             const uint32_t s2 = __byte_perm(ks[x][y][q >> 1], 0, q & 1 ? 0x3232 : 0x1010);
             const uint32_t b = q & 3, z2 = __byte_perm(kz[x][y][q >> 2], 0x64646464u, b | 0x40u | (b << 8) | 0x4000u);
+            const uint32_t c2 = h2_sub(0x63806380u, z2);  // 960 - (1024 + z)
             const uint32_t w = kw[x][y][q];
             uint4 o;
-            o.x = h2_mul(h2_sub(code_pair<0>(w, 0x64006400u), z2), s2);
-            o.y = h2_mul(h2_sub(code_pair<1>(w, 0x64006400u), z2), s2);
-            o.z = h2_mul(h2_sub(code_pair<2>(w, 0x64006400u), z2), s2);
-            o.w = h2_mul(h2_sub(code_pair<3>(w, 0x64006400u), z2), s2);
+            o.x = h2_mul(h2_sub(code_low(w, magic), z2), s2);
+            o.y = h2_mul(h2_fma(code_high(w, magic), 0x2C002C00u, c2), s2);
+            o.z = h2_mul(h2_sub(code_low(w >> 8, magic), z2), s2);
+            o.w = h2_mul(h2_fma(code_high(w >> 8, magic), 0x2C002C00u, c2), s2);
             const int row = 32 * dw + 16 * x + 8 * y + g;
             *reinterpret_cast<uint4*>(kd + (q >> 1) * C::kAtomBytes + row * 128 + ((((q & 1) * 4 + cc) ^ g) << 4)) = o;
           }
@@ -498,12 +500,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const uint32_t z2 = __byte_perm(vz[x][y][q >> 1], 0x64646464u, q & 1 ? 0x4342u : 0x4140u);
+            const uint32_t z2 = byte_pair(vz[x][y][q >> 1], q & 1), c2 = h2_sub(0x63806380u, z2);
             const uint32_t w = vw[x][y][q], s2 = vs[x][y][q];
-            o[0][2 * x + y] = h2_mul(h2_sub(code_pair<0>(w, 0x64006400u), z2), s2);
-            o[1][2 * x + y] = h2_mul(h2_sub(code_pair<1>(w, 0x64006400u), z2), s2);
-            o[2][2 * x + y] = h2_mul(h2_sub(code_pair<2>(w, 0x64006400u), z2), s2);
-            o[3][2 * x + y] = h2_mul(h2_sub(code_pair<3>(w, 0x64006400u), z2), s2);
+            o[0][2 * x + y] = h2_mul(h2_sub(code_low(w, magic), z2), s2);
+            o[1][2 * x + y] = h2_mul(h2_fma(code_high(w, magic), 0x2C002C00u, c2), s2);
+            o[2][2 * x + y] = h2_mul(h2_sub(code_low(w >> 8, magic), z2), s2);
+            o[3][2 * x + y] = h2_mul(h2_fma(code_high(w >> 8, magic), 0x2C002C00u, c2), s2);
           }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {

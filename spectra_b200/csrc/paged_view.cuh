@@ -82,15 +82,24 @@ __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[(BYTES + 3) 
   }
 }
 
-// Nibble J of both halves of a code word on top of `magic`.
-template <int J>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t magic) {
-  return ((w >> (4 * J)) & 0x000F000Fu) | magic;
+// fp16's 1024.0 twice, as a register: with the mask as the immediate, mask-and-or
+// is one instruction (two constants would make it two).
+__device__ __forceinline__ uint32_t fp16_1024() {
+  uint32_t r;
+  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(r));
+  return r;
 }
-
 // 1024 + q of bits 0-3 of both halves; 1024 + 16 q of bits 4-7.
-__device__ __forceinline__ uint32_t code_low(uint32_t w) { return (w & 0x000F000Fu) | 0x64006400u; }
-__device__ __forceinline__ uint32_t code_high(uint32_t w) { return (w & 0x00F000F0u) | 0x64006400u; }
+__device__ __forceinline__ uint32_t code_low(uint32_t w, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(r) : "r"(w), "r"(magic));
+  return r;
+}
+__device__ __forceinline__ uint32_t code_high(uint32_t w, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(r) : "r"(w), "r"(magic));
+  return r;
+}
 
 __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
@@ -115,7 +124,25 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return r;
 }
 __device__ __forceinline__ float half_of(uint32_t w, int hi) {
-  return __half2float(__ushort_as_half(uint16_t(hi ? w >> 16 : w & 0xFFFFu)));
+  const __half2 h = *reinterpret_cast<const __half2*>(&w);
+  return hi ? __high2float(h) : __low2float(h);
+}
+// 1024 + byte, of bytes 2 i and 2 i + 1 of w.
+__device__ __forceinline__ uint32_t byte_pair(uint32_t w, int i) {
+  return __byte_perm(w, 0x64646464u, i ? 0x4342u : 0x4140u);
+}
+// D = A B + C of mma.sync m16n8k16, fp16 in, fp32 out.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1, const float4& c) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // tanh by its exponential: absolute error a few 2^-24 over the whole range.
 __device__ __forceinline__ float tanh_exp(float x) {
