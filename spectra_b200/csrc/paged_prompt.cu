@@ -42,7 +42,7 @@ using namespace sm100;
 
 constexpr int kRows = 256;   // rows of a CTA
 constexpr int kKeys = 128;   // keys of a step
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 512;  // warps 13-15 only give their registers away
 constexpr int kStages = 2;   // operand stages
 
 struct PromptParams {
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
   const int n = it.steps;
 
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    if (mbar_wait(bar, parity, &s_abort)) return true;
+    if (mbar_wait_inline(bar, parity, &s_abort)) return true;
     if (!s_abort) {
       s_abort = 1;
       if (lane == 0) atomicAdd(&g_paged_prompt_timeouts, 1);
@@ -171,8 +171,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
     return false;
   };
 
+  // Registers by role: 2 x 128 x 176 + 128 x 120 + 128 x 40 = the launch's 512 x 128.
   if (warp < 8) {
     // ------------------------------------------------------------ rows
+    reg_inc<176>();
     const int t = warp >> 2, row = tid & 127, r = t * 128 + row;
     const bool real = r < it.rows;
     const int R = it.row0 + r, tok = real ? R / a.group : 0;
@@ -236,6 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       const float slope = MOD && a.slopes ? a.slopes[h] * kLog2e : 0.f;
       const float inv = MOD && a.softcap > 0.f ? c_row / a.softcap : 0.f;
       const float k_exp = MOD ? 1.f : c_row * kLog2e;
+      const float cap2 = a.softcap * kLog2e;
       const uint32_t quarter = uint32_t((warp & 3) * 32) << 16;
       const uint32_t ts = tmem + quarter + t * 128, to = tmem + quarter + 256 + t * 128;
       float m = kNone, l = 0.f;
@@ -250,62 +253,105 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         const int held = hp[0] | (hp[1] << 2) | (hp[2] << 4) | (hp[3] << 6);  // one bit per 16 keys
         const bool masked = __any_sync(0xffffffffu, n0 < lo || n0 + kKeys > hi) || held != 0xFF;
 
-        // 32 scores from column 32 q on, in powers of two once multiplied by k_exp
-        auto scores = [&](int q, float (&v)[32]) {
-          tmem_ld32(ts + 32 * q, v);
-          if constexpr (MOD) {
+        // Most steps: no mask, no new maximum.  The weights are computed with the old maximum
+        // while the new one is looked for, and stored only if that was right.
+        bool slow = i == 0 || masked;
+        if (!slow) {
+          uint32_t buf[2][16], pk[64];
+          uint64_t sums[2] = {0, 0};
+          float top = -INFINITY, far = 0.f;
+          const uint64_t m2 = f2(-m, -m);
+          tmem_ld_x16_nowait(ts, buf[0]);
+          tmem_ld_wait16(buf[0]);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float x = a.softcap > 0.f ? a.softcap * tanh_exp(v[k] * inv) : v[k] * c_row;
-              v[k] = fmaf(slope, float(n0 + 32 * q + k - pos), x * kLog2e);
+          for (int q = 0; q < 8; ++q) {
+            if (q < 7) tmem_ld_x16_nowait(ts + 16 * (q + 1), buf[(q + 1) & 1]);
+            uint32_t(&v)[16] = buf[q & 1];
+            if constexpr (MOD) {
+              const float bias = slope * float(n0 + 16 * q - pos);
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) {
+                const float v0 = __uint_as_float(v[k]), v1 = __uint_as_float(v[k + 1]);
+                uint64_t y;
+                if (a.softcap > 0.f) {
+                  far = fmaxf(far, fmaxf(fabsf(v0), fabsf(v1)));
+                  const uint64_t x = f2_mul(f2(v0, v1), f2(inv, inv)), u = f2_mul(x, x);
+                  uint64_t r = f2(kTanhFit[6], kTanhFit[6]);
+#pragma unroll
+                  for (int d = 5; d >= 0; --d) r = f2_fma(r, u, f2(kTanhFit[d], kTanhFit[d]));
+                  y = f2_mul(f2_mul(x, f2(cap2, cap2)), r);
+                } else {
+                  y = f2_mul(f2(v0, v1), f2(c_row * kLog2e, c_row * kLog2e));
+                }
+                y = f2_fma(f2(slope, slope), f2(float(k), float(k + 1)), f2_add(y, f2(bias, bias)));
+                float y0, y1;
+                f2_split(y, y0, y1);
+                v[k] = __float_as_uint(y0);
+                v[k + 1] = __float_as_uint(y1);
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+              const float v0 = __uint_as_float(v[k]), v1 = __uint_as_float(v[k + 1]);
+              top = fmaxf(fmaxf(top, v0), v1);
+              float e0, e1;
+              f2_split(MOD ? f2_add(f2(v0, v1), m2) : f2_fma(f2(v0, v1), f2(k_exp, k_exp), m2), e0, e1);
+              e0 = ex2(e0);
+              e1 = ex2(e1);
+              sums[(k >> 1) & 1] = f2_add(sums[(k >> 1) & 1], f2(e0, e1));
+              // pairs in the order of the value operand's tokens
+              pk[16 * (q >> 1) + 4 * ((k >> 1) & 3) + 2 * (q & 1) + (k >> 3)] = h2_pack(e0, e1);
+            }
+            if (q < 7) tmem_ld_wait16(buf[(q + 1) & 1]);
+          }
+          slow = __any_sync(0xffffffffu, top * k_exp > m + kLazy || far * fabsf(inv) > kTanhRange);
+          if (!slow) {
+            float s0, s1;
+            f2_split(f2_add(sums[0], sums[1]), s0, s1);
+            l += s0 + s1;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t u[16];
+#pragma unroll
+              for (int k = 0; k < 16; ++k) u[k] = pk[16 * q + k];
+              tmem_st_x16(ts + 16 * q, u);
             }
           }
-          if (masked) {
+        }
+        if (slow) {
+          // 32 scores from column 32 q on, masked; in powers of two once multiplied by k_exp
+          auto scores = [&](int q, float (&v)[32]) {
+            tmem_ld32(ts + 32 * q, v);
+            if constexpr (MOD) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const int key = n0 + 32 * q + k;
-              if (key >= hi || key < lo || !((held >> (2 * q + k / 16)) & 1)) v[k] = -INFINITY;
+              for (int k = 0; k < 32; ++k) {
+                const float x = a.softcap > 0.f ? a.softcap * tanh_exp(v[k] * inv) : v[k] * c_row;
+                v[k] = fmaf(slope, float(n0 + 32 * q + k - pos), x * kLog2e);
+              }
             }
-          }
-        };
-        uint32_t pk[64];
-        float sum = 0.f, top = -INFINITY;
-        bool redo = i == 0;
-        if (!redo) {
+            if (masked) {
 #pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                const int key = n0 + 32 * q + k;
+                if (key >= hi || key < lo || !((held >> (2 * q + k / 16)) & 1)) v[k] = -INFINITY;
+              }
+            }
+          };
+          float top = -INFINITY;
+#pragma unroll 1
           for (int q = 0; q < 4; ++q) {
             float v[32];
             scores(q, v);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) top = fmaxf(top, v[k]);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v[k]) : "f"(fmaf(v[k], k_exp, -m)));
-              sum += v[k];
-            }
-            // pairs in the order of the value operand's tokens
-#pragma unroll
-            for (int k = 0; k < 16; ++k) pk[16 * q + 4 * (k & 3) + (k >> 2)] = h2_pack(v[2 * k], v[2 * k + 1]);
+            for (int k = 0; k < 32; k += 2) top = fmaxf(fmaxf(top, v[k]), v[k + 1]);
           }
-          redo = __any_sync(0xffffffffu, top * k_exp > m + kLazy);
-        }
-        if (redo) {
-          if (i == 0) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float v[32];
-              scores(q, v);
-#pragma unroll
-              for (int k = 0; k < 32; ++k) top = fmaxf(top, v[k]);
-            }
-          }
-          const float up = fmaxf(m, top * k_exp), f = exp2f(m - up);
-          m = up;
-          l *= f;
-          if (i > 0) {
-            // (this step's scores come after the last step's product: O is complete)
-#pragma unroll
-            for (int d = 0; d < D; d += 32) {
+          if (__any_sync(0xffffffffu, top * k_exp > m + kLazy)) {
+            const float up = fmaxf(m, top * k_exp), f = exp2f(m - up);
+            m = up;
+            l *= f;
+            // (a step's scores come after the product of the step before: O is complete)
+#pragma unroll 1
+            for (int d = 0; d < (i > 0 ? D : 0); d += 32) {
               float v[32];
               tmem_ld32(to + d, v);
               uint32_t u[16];
@@ -317,27 +363,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
               }
             }
           }
-          sum = 0.f;
-#pragma unroll
+          // (weights q take the place of scores that have been read: columns 16 q.. < 32 q + 32)
+#pragma unroll 1
           for (int q = 0; q < 4; ++q) {
             float v[32];
             scores(q, v);
+            uint32_t u[16];
+            float s[4] = {};
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
-              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v[k]) : "f"(fmaf(v[k], k_exp, -m)));
-              sum += v[k];
+              v[k] = ex2(fmaf(v[k], k_exp, -m));
+              s[k & 3] += v[k];
             }
+            l += (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) pk[16 * q + 4 * (k & 3) + (k >> 2)] = h2_pack(v[2 * k], v[2 * k + 1]);
+            for (int k = 0; k < 16; ++k) u[4 * (k & 3) + (k >> 2)] = h2_pack(v[2 * k], v[2 * k + 1]);
+            tmem_st_x16(ts + 16 * q, u);
           }
-        }
-        l += sum;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t u[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) u[k] = pk[16 * q + k];
-          tmem_st_x16(ts + 16 * q, u);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -394,6 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------ operands
+    reg_dec<120>();
     const int dw = warp - 8, g = lane >> 2, cc = lane & 3;  // keys 32 dw .. 32 dw + 31 of each step
     uint8_t* buf = raw + dw * 2 * C::kTile;
     const uint32_t magic = fp16_1024();
@@ -428,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       const int st = i & 1;
       const uint32_t par = (i >> 1) & 1;
       const unsigned held = __shfl_sync(0xffffffffu, held_next, 0);
-      if (!mbar_wait(raw_full + dw, i & 1, &s_never)) {  // (its own copy: waited for whatever the others saw)
+      if (!mbar_wait_inline(raw_full + dw, i & 1, &s_never)) {  // (its own copy: waited for whatever the others saw)
         if (lane == 0) atomicAdd(&g_paged_prompt_timeouts, 1);
         s_abort = 1;
         flying = false;
@@ -518,8 +561,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       __syncwarp();
       if (lane == 0) mbar_arrive(v_full + st);
     }
-    if (flying && !ok) mbar_wait(raw_full + dw, phase, &s_never);
-  } else if (lane == 0 && n > 0) {
+    if (flying && !ok) mbar_wait_inline(raw_full + dw, phase, &s_never);
+  } else {
+    reg_dec<40>();
+  }
+  if (warp == 12 && lane == 0 && n > 0) {
     // ------------------------------------------------------------ products
     constexpr uint32_t id_s = idesc_f16(false, 128, kKeys), id_o = idesc_f16(false, 128, D);
     auto scores = [&](int t, int st) {
@@ -562,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
     }
     if (!ok) {  // products that are still running read shared memory and TMEM
       mma_commit(&drain);
-      mbar_wait(&drain, 0, &s_never);
+      mbar_wait_inline(&drain, 0, &s_never);
     }
   }
   __syncwarp();

@@ -149,4 +149,17 @@ __device__ __forceinline__ float tanh_exp(float x) {
   return 1.f - __fdividef(2.f, 1.f + exp2f(2.f * kLog2e * x));
 }
 
+// tanh(x) = x P(x^2) for |x| <= kTanhRange, absolute error 2.4e-6: a least-maximum
+// fit of tanh(x) / x in powers of x^2 (own computation: iteratively reweighted least
+// squares on Chebyshev nodes).  On the FMA pipe, where tanh_exp takes two of the
+// special-function unit's turns.
+constexpr float kTanhRange = 1.5f;
+__device__ constexpr float kTanhFit[7] = {0.9999780058860779f,   -0.3329300582408905f,   0.13116055727005005f, -0.0486324205994606f,
+                                          0.01468246802687645f, -0.0029362221248447895f, 0.0002737895119935274f};
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 }  // namespace spectra
