@@ -565,49 +565,52 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
   } else {
     reg_dec<40>();
   }
-  if (warp == 12 && lane == 0 && n > 0) {
+  if (warp == 12 && n > 0) {
     // ------------------------------------------------------------ products
     constexpr uint32_t id_s = idesc_f16(false, 128, kKeys), id_o = idesc_f16(false, 128, D);
+    const uint32_t one = elect_one();
+    const uint64_t dq = smem_desc_k_sw128(smem_u32(sq)), dk = smem_desc_k_sw128(smem_u32(sk)), dv = smem_desc_k_sw128(smem_u32(sv));
     auto scores = [&](int t, int st) {
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        const uint32_t off = (k / 4) * C::kAtomBytes + (k % 4) * 32;
-        mma_ss(tmem + t * 128, smem_desc_k_sw128(smem_u32(sq) + t * C::kAtoms * C::kAtomBytes + off),
-               smem_desc_k_sw128(smem_u32(sk) + st * C::kK + off), id_s, k > 0);
+        const uint32_t off = ((k / 4) * C::kAtomBytes + (k % 4) * 32) >> 4;  // (descriptors count in 16 bytes)
+        mma_ss_one(tmem + t * 128, dq + t * (C::kAtoms * C::kAtomBytes >> 4) + off, dk + st * (C::kK >> 4) + off, id_s, k > 0, one);
       }
-      mma_commit(s_full + t);
+      mma_commit_one(s_full + t, one);
     };
-    bool ok = wait(&q_full, 0) && wait(k_full, 0);
+    // every lane waits; the vote makes them agree
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
+    bool ok = wait_all(&q_full, 0) && wait_all(k_full, 0);
     if (ok) {
       tc_fence_after();
       for (int t = 0; t < tiles; ++t) scores(t, 0);
-      mma_commit(k_empty);
+      mma_commit_one(k_empty, one);
       for (int i = 0; i < n && ok; ++i) {
         const int st = i & 1, sn = (i + 1) & 1;
         for (int t = 0; t < tiles && ok; ++t) {
-          if (t == 0) ok = wait(v_full + st, (i >> 1) & 1);
-          ok = ok && wait(p_full + t, i & 1);
+          if (t == 0) ok = wait_all(v_full + st, (i >> 1) & 1);
+          ok = ok && wait_all(p_full + t, i & 1);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k)
-            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8,
-                   smem_desc_k_sw128(smem_u32(sv) + st * C::kV + (k / 4) * (D * 128) + (k % 4) * 32), id_o, i > 0 || k > 0);
-          if (t == tiles - 1) mma_commit(v_empty + st);
+            mma_ts_one(tmem + 256 + t * 128, tmem + t * 128 + k * 8,
+                       dv + st * (C::kV >> 4) + (((k / 4) * (D * 128) + (k % 4) * 32) >> 4), id_o, i > 0 || k > 0, one);
+          if (t == tiles - 1) mma_commit_one(v_empty + st, one);
           if (i + 1 < n) {
-            if (t == 0) ok = wait(k_full + sn, ((i + 1) >> 1) & 1);
+            if (t == 0) ok = wait_all(k_full + sn, ((i + 1) >> 1) & 1);
             if (!ok) break;
             tc_fence_after();
             scores(t, sn);
-            if (t == tiles - 1) mma_commit(k_empty + sn);
+            if (t == tiles - 1) mma_commit_one(k_empty + sn, one);
           } else {
-            mma_commit(o_done + t);
+            mma_commit_one(o_done + t, one);
           }
         }
       }
     }
     if (!ok) {  // products that are still running read shared memory and TMEM
-      mma_commit(&drain);
+      mma_commit_one(&drain, one);
       mbar_wait_inline(&drain, 0, &s_never);
     }
   }
