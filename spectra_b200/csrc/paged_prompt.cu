@@ -3,24 +3,24 @@
 //
 // The definition is paged_attn.cu's.  With hundreds of rows per key/value head
 // the work is products, so a CTA takes 256 rows (tokens x the query heads that
-// share the head; two M = 128 tiles) of one sequence and walks the keys 128 at
+// share the head; two M = 128 tiles) of one sequence and walks the keys 64 at
 // a time:
 //   warps 8-11  bring the raw tiles in by bulk copies and write them to shared
 //               memory as fp16 operands: K [token][feature] and V^T
-//               [feature][token], K-major, 128-byte swizzle.  (q - z) s is an
-//               exact difference and one rounding (11 bits).
-//   warp 12     S_t = Q_t K^T (Q in shared memory) and O_t += P_t V (P in
-//               TMEM), t = 0, 1: while one tile's softmax runs, the other
-//               tile's products do.
+//               [feature][token], K-major, 128-byte swizzle; two warps a step,
+//               in turn.  (q - z) s is an exact difference and one rounding (11 bits).
+//   warps 12, 13  S_t = Q_t K^T (Q in shared memory) and O_t += P_t V (P in
+//               TMEM), t = 0, 1.  Each tile has two S buffers, so the scores of
+//               the next step are there when a softmax ends.
 //   warps 0-7   one row per thread: scores from TMEM, P back to TMEM over
 //               them as fp16, running maximum and sum in registers.  The
 //               maximum is raised only when a score passes it by 2^kLazy; then
-//               (rarely after the first tile) O is rescaled in TMEM.
+//               (rarely after the first step) O is rescaled in TMEM.
 // The features of Q and K, and the tokens of P and V, are contracted in the
 // order in which the codes unpack.  bf16 queries are scaled by a power of two
 // per row to fit fp16, so only differences below 2^-28 of a row's largest
 // entry are lost.
-// TMEM (512 columns): S_0 | S_1 | O_0 | O_1.
+// TMEM (512 columns): S_0 (two buffers) | S_1 (two) | O_0 | O_1.
 //
 // With fewer CTAs than SMs the keys are split over `splits` CTAs per tile,
 // whose partial results a second small kernel puts together.
@@ -41,9 +41,9 @@ namespace {
 using namespace sm100;
 
 constexpr int kRows = 256;   // rows of a CTA
-constexpr int kKeys = 128;   // keys of a step
-constexpr int kThreads = 512;  // warps 13-15 only give their registers away
-constexpr int kStages = 2;   // operand stages
+constexpr int kKeys = 64;    // keys of a step
+constexpr int kThreads = 512;  // warps 14 and 15 only give their registers away
+constexpr int kStages = 4;   // operand stages
 
 struct PromptParams {
   PagedAttnArgs a;
@@ -58,10 +58,11 @@ struct Cfg {
   static constexpr int D = 32 * G;
   static constexpr int kAtoms = (D + 63) / 64;                 // 128-byte column blocks of Q and K
   static constexpr int kTile = TileLayout{G}.bytes();
-  static constexpr int kAtomBytes = 128 * 128;
-  static constexpr int kQ = 2 * kAtoms * kAtomBytes;
-  static constexpr int kK = kAtoms * kAtomBytes;               // one stage
-  static constexpr int kV = 2 * D * 128;                       // one stage
+  static constexpr int kQAtom = 128 * 128;                     // 128 rows
+  static constexpr int kKAtom = kKeys * 128;                   // 64 rows
+  static constexpr int kQ = 2 * kAtoms * kQAtom;
+  static constexpr int kK = kAtoms * kKAtom;                   // one stage
+  static constexpr int kV = D * 128;                           // one stage
   static constexpr int kRaw = 4 * 2 * kTile;
   static constexpr int kSmem = 1024 + kQ + kStages * (kK + kV) + kRaw;
 };
@@ -103,12 +104,13 @@ __device__ __forceinline__ bool item_of(const PromptParams& p, int index, int sp
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   uint32_t r[32];
   tmem_ld_x32_nowait(taddr, r);
-  tmem_ld_wait();
+  tmem_ld_wait32(r);
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-template <bool BF16, int G, bool MOD>
+// MOD: 0 plain scores, 1 capped, 2 with a bias (and capped where softcap > 0)
+template <bool BF16, int G, int MOD>
 __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams p) {
   using C = Cfg<G>;
   constexpr int D = C::D;
@@ -123,34 +125,41 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
   uint8_t* sv = sk + kStages * C::kK;
   uint8_t* raw = sv + kStages * C::kV;
   __shared__ uint64_t q_full, k_full[kStages], v_full[kStages], k_empty[kStages], v_empty[kStages];
-  __shared__ uint64_t s_full[2], p_full[2], o_done[2], raw_full[4], drain;
+  __shared__ uint64_t s_full[2][2], p_full[2][2], o_full[2], o_done[2], raw_full[4], drain[2];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_held[4][4];  // [step % 4][warp]: which of the warp's two tiles a page holds
+  __shared__ int s_held[8][2];  // [step % 8][half]: which of the half's two tiles a page holds
   __shared__ volatile int s_abort, s_never;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // what a whole warp agrees on comes out of a shuffle, which tells the compiler so: the
+  // products' operands then stay in uniform registers
+  auto same = [](auto v) { return __shfl_sync(0xffffffffu, v, 0); };
+  const int tid = threadIdx.x, warp = same(tid >> 5), lane = tid & 31;
   const int split = blockIdx.y;
-  if (tid == 0) {
-    mbar_init(&q_full, 8);
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(k_full + i, 4);
-      mbar_init(v_full + i, 4);
-      mbar_init(k_empty + i, 1);
-      mbar_init(v_empty + i, 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 4);
-      mbar_init(o_done + i, 1);
-    }
-    for (int i = 0; i < 4; ++i) mbar_init(raw_full + i, 1);
-    mbar_init(&drain, 1);
-    s_abort = s_never = 0;
-    fence_mbar_init();
-  }
   pdl_wait();
   Item it;
   if (!item_of(p, blockIdx.x, split, it)) return;
+  const int tiles = same(it.rows > 128 ? 2 : 1);
+  if (tid == 0) {
+    mbar_init(&q_full, 8);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(k_full + i, 2);
+      mbar_init(v_full + i, 2);
+      mbar_init(k_empty + i, tiles);
+      mbar_init(v_empty + i, tiles);
+    }
+    for (int i = 0; i < 2; ++i) {
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(&s_full[i][j], 1);
+        mbar_init(&p_full[i][j], 4);
+      }
+      mbar_init(o_full + i, 1);
+      mbar_init(o_done + i, 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(raw_full + i, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(drain + i, 1);
+    s_abort = s_never = 0;
+    fence_mbar_init();
+  }
   if (warp == 12) {
     tmem_alloc(&s_tmem, 512);
     tmem_relinquish();
@@ -158,9 +167,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
-  const int tiles = it.rows > 128 ? 2 : 1;
-  const int n = it.steps;
+  const uint32_t tmem = same(s_tmem);
+  const int n = same(it.steps);
 
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     if (mbar_wait_inline(bar, parity, &s_abort)) return true;
@@ -171,10 +179,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
     return false;
   };
 
-  // Registers by role: 2 x 128 x 176 + 128 x 120 + 128 x 40 = the launch's 512 x 128.
+  // Registers by role: 2 x 128 x 152 + 128 x 128 (unchanged) + 128 x 80 = the launch's 512 x 128.
   if (warp < 8) {
     // ------------------------------------------------------------ rows
-    reg_inc<176>();
+    reg_inc<152>();
     const int t = warp >> 2, row = tid & 127, r = t * 128 + row;
     const bool real = r < it.rows;
     const int R = it.row0 + r, tok = real ? R / a.group : 0;
@@ -222,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         const uint4 v = make_uint4(__byte_perm(w[4 * i], w[4 * i + 2], 0x5410), __byte_perm(w[4 * i], w[4 * i + 2], 0x7632),
                                    __byte_perm(w[4 * i + 1], w[4 * i + 3], 0x5410),
                                    __byte_perm(w[4 * i + 1], w[4 * i + 3], 0x7632));
-        *reinterpret_cast<uint4*>(sq + (t * C::kAtoms + i / 8) * C::kAtomBytes + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = v;
+        *reinterpret_cast<uint4*>(sq + (t * C::kAtoms + i / 8) * C::kQAtom + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = v;
       }
     }
     fence_proxy_async_smem();
@@ -235,82 +243,90 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         hi = pos < 0 ? 0 : (a.causal ? min(it.len, pos + 1) : it.len);
         if (a.window > 0) lo = max(0, pos - a.window + 1);
       }
-      const float slope = MOD && a.slopes ? a.slopes[h] * kLog2e : 0.f;
-      const float inv = MOD && a.softcap > 0.f ? c_row / a.softcap : 0.f;
+      const float slope = MOD == 2 ? a.slopes[h] * kLog2e : 0.f;
+      const float inv = MOD != 0 && a.softcap > 0.f ? c_row / a.softcap : 0.f;
       const float k_exp = MOD ? 1.f : c_row * kLog2e;
-      const float cap2 = a.softcap * kLog2e;
+      // constants of the scores, twice each
+      const float first = MOD == 0 ? k_exp : inv;
+      uint64_t inv2 = f2(first, first), fit[6];
+      if constexpr (MOD != 0) {
+#pragma unroll
+        for (int d = 0; d < 6; ++d) {
+          const float x = a.softcap * kLog2e * kTanhFit[d];
+          fit[d] = f2(x, x);
+          asm volatile("" : "+l"(fit[d]));
+        }
+      }
+      asm volatile("" : "+l"(inv2));
       const uint32_t quarter = uint32_t((warp & 3) * 32) << 16;
-      const uint32_t ts = tmem + quarter + t * 128, to = tmem + quarter + 256 + t * 128;
+      const uint32_t to = tmem + quarter + 256 + t * 128;
       float m = kNone, l = 0.f;
       bool ok = true;
 
       for (int i = 0; i < n; ++i) {
-        ok = wait(s_full + t, i & 1);
+        const uint32_t ts = tmem + quarter + t * 128 + (i & 1) * 64;
+        ok = wait(&s_full[t][i & 1], (i >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
         const int n0 = (it.step0 + i) * kKeys;
-        const int* hp = s_held[i & 3];
-        const int held = hp[0] | (hp[1] << 2) | (hp[2] << 4) | (hp[3] << 6);  // one bit per 16 keys
-        const bool masked = __any_sync(0xffffffffu, n0 < lo || n0 + kKeys > hi) || held != 0xFF;
+        const int held = s_held[i & 7][0] | s_held[i & 7][1] << 2;  // one bit per 16 keys
+        const bool masked = __any_sync(0xffffffffu, n0 < lo || n0 + kKeys > hi) || held != 0xF;
 
         // Most steps: no mask, no new maximum.  The weights are computed with the old maximum
         // while the new one is looked for, and stored only if that was right.
         bool slow = i == 0 || masked;
         if (!slow) {
-          uint32_t buf[2][16], pk[64];
+          uint32_t buf[2][32], pk[32];
           uint64_t sums[2] = {0, 0};
-          float top = -INFINITY, far = 0.f;
+          float tops[2] = {-INFINITY, -INFINITY}, far = 0.f;
           const uint64_t m2 = f2(-m, -m);
-          tmem_ld_x16_nowait(ts, buf[0]);
-          tmem_ld_wait16(buf[0]);
+          tmem_ld_x32_nowait(ts, buf[0]);
+          tmem_ld_wait32(buf[0]);
+          tmem_ld_x32_nowait(ts + 32, buf[1]);
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            if (q < 7) tmem_ld_x16_nowait(ts + 16 * (q + 1), buf[(q + 1) & 1]);
-            uint32_t(&v)[16] = buf[q & 1];
-            if constexpr (MOD) {
-              const float bias = slope * float(n0 + 16 * q - pos);
+          for (int q = 0; q < 2; ++q) {
+            if (q == 1) tmem_ld_wait32(buf[1]);
+            const uint32_t(&v)[32] = buf[q];
+            const float bias = MOD == 2 ? slope * float(n0 + 32 * q - pos) - m : 0.f;
 #pragma unroll
-              for (int k = 0; k < 16; k += 2) {
-                const float v0 = __uint_as_float(v[k]), v1 = __uint_as_float(v[k + 1]);
-                uint64_t y;
-                if (a.softcap > 0.f) {
-                  far = fmaxf(far, fmaxf(fabsf(v0), fabsf(v1)));
-                  const uint64_t x = f2_mul(f2(v0, v1), f2(inv, inv)), u = f2_mul(x, x);
-                  uint64_t r = f2(kTanhFit[6], kTanhFit[6]);
+            for (int k = 0; k < 32; k += 2) {
+              const uint64_t raw2 = f2(__uint_as_float(v[k]), __uint_as_float(v[k + 1]));
+              uint64_t e2;  // exponents: scores in powers of two, less the maximum
+              if constexpr (MOD == 0) {
+                e2 = f2_fma(raw2, inv2, m2);
+              } else {
+                uint64_t y = m2;
+                if constexpr (MOD == 2) y = f2_fma(f2(slope, slope), f2(float(k), float(k + 1)), f2(bias, bias));
+                if (MOD == 1 || a.softcap > 0.f) {
+                  const uint64_t x = f2_mul(raw2, inv2), u = f2_mul(x, x);
+                  float u0, u1;
+                  f2_split(u, u0, u1);
+                  far = max3(far, u0, u1);
+                  uint64_t r = fit[5];
 #pragma unroll
-                  for (int d = 5; d >= 0; --d) r = f2_fma(r, u, f2(kTanhFit[d], kTanhFit[d]));
-                  y = f2_mul(f2_mul(x, f2(cap2, cap2)), r);
+                  for (int d = 4; d >= 0; --d) r = f2_fma(r, u, fit[d]);
+                  e2 = f2_fma(x, r, y);
                 } else {
-                  y = f2_mul(f2(v0, v1), f2(c_row * kLog2e, c_row * kLog2e));
+                  e2 = f2_fma(raw2, f2(c_row * kLog2e, c_row * kLog2e), y);
                 }
-                y = f2_fma(f2(slope, slope), f2(float(k), float(k + 1)), f2_add(y, f2(bias, bias)));
-                float y0, y1;
-                f2_split(y, y0, y1);
-                v[k] = __float_as_uint(y0);
-                v[k + 1] = __float_as_uint(y1);
               }
-            }
-#pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-              const float v0 = __uint_as_float(v[k]), v1 = __uint_as_float(v[k + 1]);
-              top = fmaxf(fmaxf(top, v0), v1);
               float e0, e1;
-              f2_split(MOD ? f2_add(f2(v0, v1), m2) : f2_fma(f2(v0, v1), f2(k_exp, k_exp), m2), e0, e1);
+              f2_split(e2, e0, e1);
+              tops[(k >> 1) & 1] = max3(tops[(k >> 1) & 1], e0, e1);
               e0 = ex2(e0);
               e1 = ex2(e1);
               sums[(k >> 1) & 1] = f2_add(sums[(k >> 1) & 1], f2(e0, e1));
               // pairs in the order of the value operand's tokens
-              pk[16 * (q >> 1) + 4 * ((k >> 1) & 3) + 2 * (q & 1) + (k >> 3)] = h2_pack(e0, e1);
+              pk[16 * q + 4 * ((k >> 1) & 3) + (k >> 3)] = h2_pack(e0, e1);
             }
-            if (q < 7) tmem_ld_wait16(buf[(q + 1) & 1]);
           }
-          slow = __any_sync(0xffffffffu, top * k_exp > m + kLazy || far * fabsf(inv) > kTanhRange);
+          slow = __any_sync(0xffffffffu, fmaxf(tops[0], tops[1]) > kLazy || far > kTanhRange2);
           if (!slow) {
             float s0, s1;
             f2_split(f2_add(sums[0], sums[1]), s0, s1);
             l += s0 + s1;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < 2; ++q) {
               uint32_t u[16];
 #pragma unroll
               for (int k = 0; k < 16; ++k) u[k] = pk[16 * q + k];
@@ -322,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           // 32 scores from column 32 q on, masked; in powers of two once multiplied by k_exp
           auto scores = [&](int q, float (&v)[32]) {
             tmem_ld32(ts + 32 * q, v);
-            if constexpr (MOD) {
+            if constexpr (MOD != 0) {
 #pragma unroll
               for (int k = 0; k < 32; ++k) {
                 const float x = a.softcap > 0.f ? a.softcap * tanh_exp(v[k] * inv) : v[k] * c_row;
@@ -339,33 +355,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           };
           float top = -INFINITY;
 #pragma unroll 1
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 2; ++q) {
             float v[32];
             scores(q, v);
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) top = fmaxf(fmaxf(top, v[k]), v[k + 1]);
+            for (int k = 0; k < 32; k += 2) top = max3(top, v[k], v[k + 1]);
           }
           if (__any_sync(0xffffffffu, top * k_exp > m + kLazy)) {
             const float up = fmaxf(m, top * k_exp), f = exp2f(m - up);
             m = up;
             l *= f;
-            // (a step's scores come after the product of the step before: O is complete)
+            if (i > 0) {  // O, once the last step's product has been added
+              ok = wait(o_full + t, (i - 1) & 1);
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll 1
-            for (int d = 0; d < (i > 0 ? D : 0); d += 32) {
-              float v[32];
-              tmem_ld32(to + d, v);
-              uint32_t u[16];
+              for (int d = 0; d < D; d += 32) {
+                float v[32];
+                tmem_ld32(to + d, v);
+                uint32_t u[16];
 #pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
+                for (int hh = 0; hh < 2; ++hh) {
 #pragma unroll
-                for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(v[16 * hh + k] * f);
-                tmem_st_x16(to + d + 16 * hh, u);
+                  for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(v[16 * hh + k] * f);
+                  tmem_st_x16(to + d + 16 * hh, u);
+                }
               }
             }
           }
           // (weights q take the place of scores that have been read: columns 16 q.. < 32 q + 32)
 #pragma unroll 1
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 2; ++q) {
             float v[32];
             scores(q, v);
             uint32_t u[16];
@@ -384,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + t);
+        if (lane == 0) mbar_arrive(&p_full[t][i & 1]);
       }
 
       // ---- result
@@ -436,13 +456,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------ operands
-    reg_dec<120>();
-    const int dw = warp - 8, g = lane >> 2, cc = lane & 3;  // keys 32 dw .. 32 dw + 31 of each step
+    // warps 8 and 9 take steps 0, 2, ..., warps 10 and 11 steps 1, 3, ...; each 32 of a step's keys
+    const int dw = warp - 8, g = lane >> 2, cc = lane & 3, half = dw & 1;
     uint8_t* buf = raw + dw * 2 * C::kTile;
     const uint32_t magic = fp16_1024();
     int mine = 0;            // lanes 0, 1: page of the tile to load next
     auto look = [&](int i) {
-      const int at = (it.step0 + i) * kKeys + 32 * dw + 16 * lane;
+      const int at = (it.step0 + i) * kKeys + 32 * half + 16 * lane;
       mine = lane < 2 && i < n && at < it.len ? c.tables[it.b * c.table_stride + (at >> c.page_log2)] : -1;
     };
     unsigned held_next = 0;  // lanes 0, 1: of the tiles in flight
@@ -453,30 +473,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         if (lane == 0) mbar_arrive_expect_tx(raw_full + dw, __popc(held_next) * C::kTile);
         __syncwarp(0x3u);
         if (hold) {
-          const int at = (it.step0 + i) * kKeys + 32 * dw + 16 * lane;
+          const int at = (it.step0 + i) * kKeys + 32 * half + 16 * lane;
           const int per = 1 << (c.page_log2 - 4);
           bulk_g2s(buf + lane * C::kTile, c.pool + mine * c.page_stride + (int64_t(it.head) * per + ((at >> 4) & (per - 1))) * C::kTile,
                    C::kTile, raw_full + dw);
         }
       }
     };
-    if (n > 0) {
-      look(0);
-      issue(0);
-      look(1);
+    const int first = dw >> 1;
+    if (first < n) {
+      look(first);
+      issue(first);
+      look(first + 2);
     }
     bool ok = true, flying = false;  // a copy that nothing has waited for, and its phase
     uint32_t phase = 0;
-    for (int i = 0; i < n; ++i) {
-      const int st = i & 1;
-      const uint32_t par = (i >> 1) & 1;
+    for (int i = first; i < n; i += 2) {
+      const int st = i & 3;
+      const uint32_t par = (i >> 2) & 1;
       const unsigned held = __shfl_sync(0xffffffffu, held_next, 0);
-      if (!mbar_wait_inline(raw_full + dw, i & 1, &s_never)) {  // (its own copy: waited for whatever the others saw)
+      if (!mbar_wait_inline(raw_full + dw, phase, &s_never)) {  // (its own copy: waited for whatever the others saw)
         if (lane == 0) atomicAdd(&g_paged_prompt_timeouts, 1);
         s_abort = 1;
         flying = false;
         break;
       }
+      phase ^= 1;
       uint32_t kw[2][2][G], vw[2][2][G], ks[2][2][(2 * G + 3) / 4], kz[2][2][(G + 3) / 4], vs[2][2][G], vz[2][2][(2 * G + 3) / 4];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -498,17 +520,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         }
       }
       __syncwarp();
-      flying = i + 1 < n;
-      phase = (i + 1) & 1;
+      flying = i + 2 < n;
       if (flying) {
-        issue(i + 1);
-        look(i + 2);
+        issue(i + 2);
+        look(i + 4);
       }
 
       // ---- keys: [token][feature]
       if (i >= kStages) ok = wait(k_empty + st, par ^ 1);
       if (!ok) break;
-      if (lane == 0) s_held[i & 3][dw] = int(held);
+      if (lane == 0) s_held[i & 7][half] = int(held);
       uint8_t* kd = sk + st * C::kK;
 #pragma unroll
       for (int x = 0; x < 2; ++x)
@@ -525,8 +546,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
             o.y = h2_mul(h2_fma(code_high(w, magic), 0x2C002C00u, c2), s2);
             o.z = h2_mul(h2_sub(code_low(w >> 8, magic), z2), s2);
             o.w = h2_mul(h2_fma(code_high(w >> 8, magic), 0x2C002C00u, c2), s2);
-            const int row = 32 * dw + 16 * x + 8 * y + g;
-            *reinterpret_cast<uint4*>(kd + (q >> 1) * C::kAtomBytes + row * 128 + ((((q & 1) * 4 + cc) ^ g) << 4)) = o;
+            const int row = 32 * half + 16 * x + 8 * y + g;
+            *reinterpret_cast<uint4*>(kd + (q >> 1) * C::kKAtom + row * 128 + ((((q & 1) * 4 + cc) ^ g) << 4)) = o;
           }
       fence_proxy_async_smem();
       __syncwarp();
@@ -535,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       // ---- values: [feature][token], tokens {2c, 2c+1, 2c+8, 2c+9, 2c+16, ...} of the 32 as chunk c
       if (i >= kStages) ok = wait(v_empty + st, par ^ 1);
       if (!ok) break;
-      uint8_t* vd = sv + st * C::kV + (dw >> 1) * (D * 128);
+      uint8_t* vd = sv + st * C::kV;
 #pragma unroll
       for (int q = 0; q < G; ++q) {
         uint32_t o[4][4];
@@ -553,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int row = 32 * q + 4 * g + j;
-          *reinterpret_cast<uint4*>(vd + row * 128 + ((((dw & 1) * 4 + cc) ^ (row & 7)) << 4)) =
+          *reinterpret_cast<uint4*>(vd + row * 128 + (((half * 4 + cc) ^ (row & 7)) << 4)) =
               make_uint4(o[j][0], o[j][1], o[j][2], o[j][3]);
         }
       }
@@ -563,55 +584,54 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
     }
     if (flying && !ok) mbar_wait_inline(raw_full + dw, phase, &s_never);
   } else {
-    reg_dec<40>();
+    reg_dec<80>();
   }
-  if (warp == 12 && n > 0) {
-    // ------------------------------------------------------------ products
+  if (warp >= 12 && warp < 12 + tiles && n > 0) {
+    // ------------------------------------------------------------ products, a warp for each tile
     constexpr uint32_t id_s = idesc_f16(false, 128, kKeys), id_o = idesc_f16(false, 128, D);
     const uint32_t one = elect_one();
-    const uint64_t dq = smem_desc_k_sw128(smem_u32(sq)), dk = smem_desc_k_sw128(smem_u32(sk)), dv = smem_desc_k_sw128(smem_u32(sv));
-    auto scores = [&](int t, int st) {
+    const int t = warp - 12;
+    const uint32_t ts = tmem + t * 128, to = tmem + 256 + t * 128;
+    const uint64_t dq = smem_desc_k_sw128(smem_u32(sq) + t * C::kAtoms * C::kQAtom), dk = smem_desc_k_sw128(smem_u32(sk)),
+                   dv = smem_desc_k_sw128(smem_u32(sv));
+    // (descriptors count in 16 bytes)
+    auto scores = [&](int i) {
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t off = ((k / 4) * C::kAtomBytes + (k % 4) * 32) >> 4;  // (descriptors count in 16 bytes)
-        mma_ss_one(tmem + t * 128, dq + t * (C::kAtoms * C::kAtomBytes >> 4) + off, dk + st * (C::kK >> 4) + off, id_s, k > 0, one);
-      }
-      mma_commit_one(s_full + t, one);
+      for (int k = 0; k < D / 16; ++k)
+        mma_ss_one(ts + (i & 1) * 64, dq + (((k / 4) * C::kQAtom + (k % 4) * 32) >> 4),
+                   dk + (((i & 3) * C::kK + (k / 4) * C::kKAtom + (k % 4) * 32) >> 4), id_s, k > 0, one);
+      mma_commit_one(&s_full[t][i & 1], one);
+      mma_commit_one(k_empty + (i & 3), one);
     };
     // every lane waits; the vote makes them agree
     auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
-    bool ok = wait_all(&q_full, 0) && wait_all(k_full, 0);
-    if (ok) {
+    bool ok = wait_all(&q_full, 0);
+    for (int i = 0; i < 2 && i < n && ok; ++i) {
+      ok = wait_all(k_full + i, 0);
       tc_fence_after();
-      for (int t = 0; t < tiles; ++t) scores(t, 0);
-      mma_commit_one(k_empty, one);
-      for (int i = 0; i < n && ok; ++i) {
-        const int st = i & 1, sn = (i + 1) & 1;
-        for (int t = 0; t < tiles && ok; ++t) {
-          if (t == 0) ok = wait_all(v_full + st, (i >> 1) & 1);
-          ok = ok && wait_all(p_full + t, i & 1);
-          if (!ok) break;
-          tc_fence_after();
+      if (ok) scores(i);
+    }
+    for (int i = 0; i < n && ok; ++i) {
+      ok = wait_all(v_full + (i & 3), (i >> 2) & 1) && wait_all(&p_full[t][i & 1], (i >> 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
 #pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            mma_ts_one(tmem + 256 + t * 128, tmem + t * 128 + k * 8,
-                       dv + st * (C::kV >> 4) + (((k / 4) * (D * 128) + (k % 4) * 32) >> 4), id_o, i > 0 || k > 0, one);
-          if (t == tiles - 1) mma_commit_one(v_empty + st, one);
-          if (i + 1 < n) {
-            if (t == 0) ok = wait_all(k_full + sn, ((i + 1) >> 1) & 1);
-            if (!ok) break;
-            tc_fence_after();
-            scores(t, sn);
-            if (t == tiles - 1) mma_commit_one(k_empty + sn, one);
-          } else {
-            mma_commit_one(o_done + t, one);
-          }
-        }
+      for (int k = 0; k < kKeys / 16; ++k)
+        mma_ts_one(to, ts + (i & 1) * 64 + k * 8, dv + (((i & 3) * C::kV + k * 32) >> 4), id_o, i > 0 || k > 0, one);
+      mma_commit_one(o_full + t, one);
+      mma_commit_one(v_empty + (i & 3), one);
+      if (i + 1 == n) mma_commit_one(o_done + t, one);
+      if (i + 2 < n) {
+        // its weights have been read: scores may take their place
+        ok = wait_all(k_full + ((i + 2) & 3), ((i + 2) >> 2) & 1) && wait_all(o_full + t, i & 1);
+        if (!ok) break;
+        tc_fence_after();
+        scores(i + 2);
       }
     }
     if (!ok) {  // products that are still running read shared memory and TMEM
-      mma_commit_one(&drain, one);
-      mbar_wait_inline(&drain, 0, &s_never);
+      mma_commit_one(drain + t, one);
+      mbar_wait_inline(drain + t, 0, &s_never);
     }
   }
   __syncwarp();
@@ -668,7 +688,7 @@ int launch_dep(K kernel, dim3 grid, int threads, int smem, const PromptParams& p
   return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p));
 }
 
-template <bool BF16, int G, bool MOD>
+template <bool BF16, int G, int MOD>
 int launch_one(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
   using C = Cfg<G>;
   static PerContextOnce once;
@@ -684,8 +704,8 @@ int launch_one(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
   p.row_tiles = int((int64_t(a.c.max_q) * a.group + kRows - 1) / kRows);
   const int64_t items = int64_t(p.row_tiles) * a.c.batch * a.c.kv_heads;
   if (items > INT32_MAX) return SPECTRA_ERR_SHAPE;
-  // two steps of keys a split at least
-  const int64_t most = std::max<int64_t>(1, a.c.limit / (2 * kKeys));
+  // four steps of keys a split at least
+  const int64_t most = std::max<int64_t>(1, a.c.limit / (4 * kKeys));
   p.splits = int(std::max<int64_t>(1, std::min<int64_t>(most, device_sms(dev) / items)));
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + kPagedCounterBytes);
   if (p.splits > 1 &&
@@ -698,7 +718,8 @@ int launch_one(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
 
 template <bool BF16, int G>
 int launch_mod(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
-  return a.softcap > 0.f || a.slopes ? launch_one<BF16, G, true>(a, min_rows, st) : launch_one<BF16, G, false>(a, min_rows, st);
+  if (a.slopes) return launch_one<BF16, G, 2>(a, min_rows, st);
+  return a.softcap > 0.f ? launch_one<BF16, G, 1>(a, min_rows, st) : launch_one<BF16, G, 0>(a, min_rows, st);
 }
 
 template <bool BF16>

@@ -149,13 +149,18 @@ __device__ __forceinline__ float tanh_exp(float x) {
   return 1.f - __fdividef(2.f, 1.f + exp2f(2.f * kLog2e * x));
 }
 
-// tanh(x) = x P(x^2) for |x| <= kTanhRange, absolute error 2.4e-6: a least-maximum
+// tanh(x) = x P(x^2) for x^2 <= kTanhRange2, absolute error 2.4e-6: a least-maximum
 // fit of tanh(x) / x in powers of x^2 (own computation: iteratively reweighted least
 // squares on Chebyshev nodes).  On the FMA pipe, where tanh_exp takes two of the
 // special-function unit's turns.
-constexpr float kTanhRange = 1.5f;
-__device__ constexpr float kTanhFit[7] = {0.9999780058860779f,   -0.3329300582408905f,   0.13116055727005005f, -0.0486324205994606f,
-                                          0.01468246802687645f, -0.0029362221248447895f, 0.0002737895119935274f};
+constexpr float kTanhRange2 = 1.25f * 1.25f;
+__device__ constexpr float kTanhFit[6] = {0.9999746680259705f,  -0.3328392803668976f, 0.13053609430789948f,
+                                          -0.04692651331424713f, 0.01253186073154211f, -0.001682034693658352f};
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
