@@ -14,8 +14,8 @@
 //               the next step are there when a softmax ends.
 //   warps 0-7   one row per thread: scores from TMEM, P back to TMEM over
 //               them as fp16, running maximum and sum in registers.  The
-//               maximum is raised only when a score passes it by 2^kLazy; then
-//               (rarely after the first step) O is rescaled in TMEM.
+//               maximum is raised only when the weights it gives grow large;
+//               then (rarely after the first step) O is rescaled in TMEM.
 // The features of Q and K, and the tokens of P and V, are contracted in the
 // order in which the codes unpack.  bf16 queries are scaled by a power of two
 // per row to fit fp16, so only differences below 2^-28 of a row's largest
@@ -27,6 +27,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "gemv_mma.cuh"
 #include "paged_view.cuh"
@@ -216,8 +217,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           top = max(top, (w[i] >> 7) & 0xFFu);
           top = max(top, (w[i] >> 23) & 0xFFu);
         }
-        // largest entry to [2^14, 2^15); both factors stay normal numbers
-        int e = top == 255u ? 0 : 141 - int(top);
+        // largest entry to [2^4, 2^5); both factors stay normal numbers
+        int e = top == 255u ? 0 : 131 - int(top);
         e = min(e, 100);
         f = __uint_as_float(uint32_t(127 + e) << 23);
         c_row *= __uint_as_float(uint32_t(127 - e) << 23);
@@ -246,18 +247,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       const float slope = MOD == 2 ? a.slopes[h] * kLog2e : 0.f;
       const float inv = MOD != 0 && a.softcap > 0.f ? c_row / a.softcap : 0.f;
       const float k_exp = MOD ? 1.f : c_row * kLog2e;
-      // constants of the scores, twice each
-      const float first = MOD == 0 ? k_exp : inv;
-      uint64_t inv2 = f2(first, first), fit[6];
-      if constexpr (MOD != 0) {
-#pragma unroll
-        for (int d = 0; d < 6; ++d) {
-          const float x = a.softcap * kLog2e * kTanhFit[d];
-          fit[d] = f2(x, x);
-          asm volatile("" : "+l"(fit[d]));
-        }
-      }
-      asm volatile("" : "+l"(inv2));
+      // how a capped score's tanh is computed: four terms unless one of the last steps has shown
+      // that six are needed (or the factors, powers of inv, would vanish)
+      const bool tiny = MOD == 1 && __any_sync(0xffffffffu, fabsf(inv) < 2e-5f);
+      int wide = tiny ? 1 : 0;  // steps to go with six
       const uint32_t quarter = uint32_t((warp & 3) * 32) << 16;
       const uint32_t to = tmem + quarter + 256 + t * 128;
       float m = kNone, l = 0.f;
@@ -272,14 +265,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         const int held = s_held[i & 7][0] | s_held[i & 7][1] << 2;  // one bit per 16 keys
         const bool masked = __any_sync(0xffffffffu, n0 < lo || n0 + kKeys > hi) || held != 0xF;
 
-        // Most steps: no mask, no new maximum.  The weights are computed with the old maximum
-        // while the new one is looked for, and stored only if that was right.
-        bool slow = i == 0 || masked;
-        if (!slow) {
+        // Most steps: no mask, no new maximum.  The weights are computed with the old maximum and
+        // stored if their sum is small enough to say that no score passed it by much (then each
+        // weight fits fp16 too); TERMS: of the cap's tanh, which may be out of their range as well.
+        auto fast = [&](auto terms) -> bool {
+          constexpr int TERMS = decltype(terms)::value;
+          constexpr float kMost = 1024.f;
           uint32_t buf[2][32], pk[32];
-          uint64_t sums[2] = {0, 0};
-          float tops[2] = {-INFINITY, -INFINITY}, far = 0.f;
+          uint64_t sums[2] = {0, 0}, fit[TERMS + 1];
+          float far = 0.f;
           const uint64_t m2 = f2(-m, -m);
+          const float c1 = TERMS == 0 ? (MOD == 0 ? k_exp : c_row * kLog2e) : inv, c2 = inv * inv;
+          const uint64_t first = f2(c1, c1);
+          if constexpr (TERMS == 4) {
+            float pw = a.softcap * kLog2e * inv;  // in the scores themselves: inv's powers go into the factors
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              fit[d] = f2(pw * kTanhFit4[d], pw * kTanhFit4[d]);
+              pw *= c2;
+            }
+          } else if constexpr (TERMS == 6) {
+#pragma unroll
+            for (int d = 0; d < 6; ++d) {
+              const float x = a.softcap * kLog2e * kTanhFit6[d];
+              fit[d] = f2(x, x);
+            }
+          }
           tmem_ld_x32_nowait(ts, buf[0]);
           tmem_ld_wait32(buf[0]);
           tmem_ld_x32_nowait(ts + 32, buf[1]);
@@ -287,32 +298,26 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           for (int q = 0; q < 2; ++q) {
             if (q == 1) tmem_ld_wait32(buf[1]);
             const uint32_t(&v)[32] = buf[q];
-            const float bias = MOD == 2 ? slope * float(n0 + 32 * q - pos) - m : 0.f;
+            [[maybe_unused]] const float bias = MOD == 2 ? slope * float(n0 + 32 * q - pos) - m : 0.f;
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
               const uint64_t raw2 = f2(__uint_as_float(v[k]), __uint_as_float(v[k + 1]));
-              uint64_t e2;  // exponents: scores in powers of two, less the maximum
-              if constexpr (MOD == 0) {
-                e2 = f2_fma(raw2, inv2, m2);
+              uint64_t y = m2;
+              if constexpr (MOD == 2) y = f2_fma(f2(slope, slope), f2(float(k), float(k + 1)), f2(bias, bias));
+              if constexpr (TERMS == 0) {
+                y = f2_fma(raw2, first, y);
               } else {
-                uint64_t y = m2;
-                if constexpr (MOD == 2) y = f2_fma(f2(slope, slope), f2(float(k), float(k + 1)), f2(bias, bias));
-                if (MOD == 1 || a.softcap > 0.f) {
-                  const uint64_t x = f2_mul(raw2, inv2), u = f2_mul(x, x);
-                  float u0, u1;
-                  f2_split(u, u0, u1);
-                  far = max3(far, u0, u1);
-                  uint64_t r = fit[5];
+                const uint64_t x = TERMS == 6 ? f2_mul(raw2, first) : raw2, u = f2_mul(x, x);
+                float u0, u1;
+                f2_split(u, u0, u1);
+                far = max3(far, u0, u1);
+                uint64_t r = fit[TERMS - 1];
 #pragma unroll
-                  for (int d = 4; d >= 0; --d) r = f2_fma(r, u, fit[d]);
-                  e2 = f2_fma(x, r, y);
-                } else {
-                  e2 = f2_fma(raw2, f2(c_row * kLog2e, c_row * kLog2e), y);
-                }
+                for (int d = TERMS - 2; d >= 0; --d) r = f2_fma(r, u, fit[d]);
+                y = f2_fma(x, r, y);
               }
-              float e0, e1;
-              f2_split(e2, e0, e1);
-              tops[(k >> 1) & 1] = max3(tops[(k >> 1) & 1], e0, e1);
+              float e0, e1;  // exponents: scores in powers of two, less the maximum
+              f2_split(y, e0, e1);
               e0 = ex2(e0);
               e1 = ex2(e1);
               sums[(k >> 1) & 1] = f2_add(sums[(k >> 1) & 1], f2(e0, e1));
@@ -320,48 +325,55 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
               pk[16 * q + 4 * ((k >> 1) & 3) + (k >> 3)] = h2_pack(e0, e1);
             }
           }
-          slow = __any_sync(0xffffffffu, fmaxf(tops[0], tops[1]) > kLazy || far > kTanhRange2);
-          if (!slow) {
-            float s0, s1;
-            f2_split(f2_add(sums[0], sums[1]), s0, s1);
-            l += s0 + s1;
+          float s0, s1;
+          f2_split(f2_add(sums[0], sums[1]), s0, s1);
+          s0 += s1;
+          if constexpr (TERMS == 4) far *= c2;
+          const bool out = __any_sync(0xffffffffu, s0 > kMost || (TERMS != 0 && far > (TERMS == 4 ? kTanhRange4 : kTanhRange6)));
+          if constexpr (MOD == 1) wide = __any_sync(0xffffffffu, far > kTanhRange4) ? 8 : max(wide - 1, int(tiny));
+          if (out) return false;
+          l += s0;
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t u[16];
+          for (int q = 0; q < 2; ++q) {
+            uint32_t u[16];
 #pragma unroll
-              for (int k = 0; k < 16; ++k) u[k] = pk[16 * q + k];
-              tmem_st_x16(ts + 16 * q, u);
-            }
+            for (int k = 0; k < 16; ++k) u[k] = pk[16 * q + k];
+            tmem_st_x16(ts + 16 * q, u);
+          }
+          return true;
+        };
+        bool done = false;
+        if (i > 0 && !masked) {
+          if constexpr (MOD == 0)
+            done = fast(std::integral_constant<int, 0>{});
+          else if (MOD == 2 && !(a.softcap > 0.f))
+            done = fast(std::integral_constant<int, 0>{});
+          else {
+            if (MOD == 1 && wide == 0) done = fast(std::integral_constant<int, 4>{});
+            if (!done && (MOD == 2 || wide > 0)) done = fast(std::integral_constant<int, 6>{});
           }
         }
-        if (slow) {
-          // 32 scores from column 32 q on, masked; in powers of two once multiplied by k_exp
-          auto scores = [&](int q, float (&v)[32]) {
-            tmem_ld32(ts + 32 * q, v);
-            if constexpr (MOD != 0) {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) {
-                const float x = a.softcap > 0.f ? a.softcap * tanh_exp(v[k] * inv) : v[k] * c_row;
-                v[k] = fmaf(slope, float(n0 + 32 * q + k - pos), x * kLog2e);
-              }
-            }
-            if (masked) {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) {
-                const int key = n0 + 32 * q + k;
-                if (key >= hi || key < lo || !((held >> (2 * q + k / 16)) & 1)) v[k] = -INFINITY;
-              }
-            }
-          };
+        if (!done) {
+          uint32_t buf[2][32];
+          tmem_ld_x32_nowait(ts, buf[0]);
+          tmem_ld_x32_nowait(ts + 32, buf[1]);
+          tmem_ld_wait32(buf[0]);
+          tmem_ld_wait32(buf[1]);
           float top = -INFINITY;
-#pragma unroll 1
-          for (int q = 0; q < 2; ++q) {
-            float v[32];
-            scores(q, v);
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) top = max3(top, v[k], v[k + 1]);
+          for (int k = 0; k < 64; ++k) {
+            uint32_t& w = buf[k >> 5][k & 31];
+            float x = __uint_as_float(w);
+            if constexpr (MOD != 0) {
+              x = a.softcap > 0.f ? a.softcap * tanh_exp(x * inv) : x * c_row;
+              x = fmaf(slope, float(n0 + k - pos), x * kLog2e);
+            }
+            if (masked) x = n0 + k >= hi || n0 + k < lo || !((held >> (k / 16)) & 1) ? -INFINITY : x;
+            w = __float_as_uint(x);
+            top = fmaxf(top, x);
           }
-          if (__any_sync(0xffffffffu, top * k_exp > m + kLazy)) {
+          // (after this no weight of this step passes 2^3: sums like it stay in fast's bound)
+          if (__any_sync(0xffffffffu, top * k_exp > m + 3.f)) {
             const float up = fmaxf(m, top * k_exp), f = exp2f(m - up);
             m = up;
             l *= f;
@@ -383,23 +395,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
               }
             }
           }
-          // (weights q take the place of scores that have been read: columns 16 q.. < 32 q + 32)
-#pragma unroll 1
+          float sum[4] = {};
+#pragma unroll
           for (int q = 0; q < 2; ++q) {
-            float v[32];
-            scores(q, v);
             uint32_t u[16];
-            float s[4] = {};
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              v[k] = ex2(fmaf(v[k], k_exp, -m));
-              s[k & 3] += v[k];
+            for (int k = 0; k < 32; k += 2) {
+              const float e0 = ex2(fmaf(__uint_as_float(buf[q][k]), k_exp, -m));
+              const float e1 = ex2(fmaf(__uint_as_float(buf[q][k + 1]), k_exp, -m));
+              sum[k & 2] += e0;
+              sum[(k & 2) + 1] += e1;
+              u[4 * ((k >> 1) & 3) + (k >> 3)] = h2_pack(e0, e1);
             }
-            l += (s[0] + s[1]) + (s[2] + s[3]);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) u[4 * (k & 3) + (k >> 2)] = h2_pack(v[2 * k], v[2 * k + 1]);
             tmem_st_x16(ts + 16 * q, u);
           }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
         tmem_st_wait();
         tc_fence_before();

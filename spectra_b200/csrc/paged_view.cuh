@@ -144,18 +144,15 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// tanh by its exponential: absolute error a few 2^-24 over the whole range.
-__device__ __forceinline__ float tanh_exp(float x) {
-  return 1.f - __fdividef(2.f, 1.f + exp2f(2.f * kLog2e * x));
-}
-
-// tanh(x) = x P(x^2) for x^2 <= kTanhRange2, absolute error 2.4e-6: a least-maximum
-// fit of tanh(x) / x in powers of x^2 (own computation: iteratively reweighted least
-// squares on Chebyshev nodes).  On the FMA pipe, where tanh_exp takes two of the
-// special-function unit's turns.
-constexpr float kTanhRange2 = 1.25f * 1.25f;
-__device__ constexpr float kTanhFit[6] = {0.9999746680259705f,  -0.3328392803668976f, 0.13053609430789948f,
-                                          -0.04692651331424713f, 0.01253186073154211f, -0.001682034693658352f};
+// tanh(x) = x P(x^2), on the FMA pipe where tanh_exp takes two of the special-function
+// unit's turns: fits of tanh(x) / x in powers of x^2 for the least maximum of the
+// absolute error (own computation: iteratively reweighted least squares on Chebyshev
+// nodes).  Six terms for |x| <= 1.25, error 2.4e-6; four for |x| <= 0.6, error 6.3e-7.
+constexpr float kTanhRange6 = 1.25f * 1.25f, kTanhRange4 = 0.6f * 0.6f;
+__device__ constexpr float kTanhFit6[6] = {0.9999746680259705f,  -0.3328392803668976f, 0.13053609430789948f,
+                                           -0.04692651331424713f, 0.01253186073154211f, -0.001682034693658352f};
+__device__ constexpr float kTanhFit4[4] = {0.9999909996986389f, -0.33298975229263306f, 0.1297455132007599f,
+                                           -0.03961124271154404f};
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -165,6 +162,12 @@ __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+// tanh by its exponential: absolute error a few 2^-24 over the whole range.
+__device__ __forceinline__ float tanh_exp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(2.f * kLog2e * x)));
+  return fmaf(-2.f, r, 1.f);
 }
 
 }  // namespace spectra
