@@ -302,11 +302,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
           }
         }
       }
-      // the row's largest entry: of both types, the order of the bits is that of the numbers
+      // the row's largest entry
 #pragma unroll
       for (int grp = 0; grp < G; ++grp)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top2 = __vmaxu2(top2, raw[grp][j] & 0x7FFF7FFFu);
+        for (int j = 0; j < 4; ++j) top2 = bf16 ? max_abs2<true>(top2, raw[grp][j]) : max_abs2<false>(top2, raw[grp][j]);
       uint32_t top = max(top2 >> 16, top2 & 0xFFFFu);
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));

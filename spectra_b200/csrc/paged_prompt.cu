@@ -190,48 +190,63 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
     const int h = it.head * a.group + (real ? R - tok * a.group : 0);
     const int pos = it.pos0 + tok;
     float c_row = a.scale;
+    // rows of 16-byte chunks, swizzled: the query operand, and later the result; kLanes lanes bring a row
+    constexpr int kChunks = D / 8, kLanes = G == 3 ? 16 : kChunks, kPer = 32 / kLanes;
+    const int w0 = (warp & 3) * 32;
+    uint8_t* q_tile = sq + t * C::kAtoms * C::kQAtom;
+    auto chunk_at = [&](int r, int ch) { return q_tile + (ch / 8) * C::kQAtom + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
+    const int ch = lane & (kLanes - 1);
     if (t < tiles) {
-      // this row's query into the operand: 8 features at a time in the order (0,4)(1,5)(2,6)(3,7)
-      uint32_t w[D / 2];
-      const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (it.first + tok) * a.q_ts + h * a.q_hs;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (real) {
+      // The warp's 32 queries to where their operand will be, whole rows at a time (a lane brings 16
+      // bytes of one; row by row per thread, each load would touch 32 lines) ...
+      const uint16_t* mine = reinterpret_cast<const uint16_t*>(a.q) + (it.first + tok) * a.q_ts + h * a.q_hs;
+#pragma unroll 4
+      for (int r0 = 0; r0 < 32; r0 += kPer) {
+        const int r = r0 + lane / kLanes;
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(mine), r)) + 8 * ch;
+        const bool have = t * 128 + w0 + r < it.rows;
+        if (ch < kChunks) {
+          uint8_t* dst = chunk_at(w0 + r, ch);
           if (a.vec) {
-            v = *reinterpret_cast<const uint4*>(src + 8 * i);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(have ? src : mine), "r"(have ? 16 : 0)
+                         : "memory");
           } else {
-            uint32_t u[4];
+            uint32_t u[4] = {};
+            if (have) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) u[j] = uint32_t(src[8 * i + 2 * j]) | (uint32_t(src[8 * i + 2 * j + 1]) << 16);
-            v = make_uint4(u[0], u[1], u[2], u[3]);
+              for (int j = 0; j < 4; ++j) u[j] = uint32_t(src[2 * j]) | (uint32_t(src[2 * j + 1]) << 16);
+            }
+            *reinterpret_cast<uint4*>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
           }
         }
-        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
       }
-      float f = 1.f;  // power of two that the row is multiplied by
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      // ... then each thread its row, in place: scaled to fp16, features in the order (0,4)(1,5)(2,6)(3,7)
+      float f = 1.f;
       if constexpr (BF16) {
-        uint32_t top = 0;  // largest exponent (an infinity or NaN: 255, left as it is)
-#pragma unroll
-        for (int i = 0; i < D / 2; ++i) {
-          top = max(top, (w[i] >> 7) & 0xFFu);
-          top = max(top, (w[i] >> 23) & 0xFFu);
+        uint32_t top2 = 0;
+#pragma unroll 4
+        for (int i = 0; i < kChunks; ++i) {
+          const uint4 v = *reinterpret_cast<const uint4*>(chunk_at(row, i));
+          top2 = max_abs2<true>(max_abs2<true>(max_abs2<true>(max_abs2<true>(top2, v.x), v.y), v.z), v.w);
         }
-        // largest entry to [2^4, 2^5); both factors stay normal numbers
-        int e = top == 255u ? 0 : 131 - int(top);
-        e = min(e, 100);
+        const uint32_t top = max(top2 >> 16, top2 & 0xFFFFu) >> 7;  // largest exponent
+        // largest entry to [2^4, 2^5) (an infinity or NaN: as it is); both factors stay normal numbers
+        const int e = min(top == 255u ? 0 : 131 - int(top), 100);
         f = __uint_as_float(uint32_t(127 + e) << 23);
         c_row *= __uint_as_float(uint32_t(127 - e) << 23);
-#pragma unroll
-        for (int i = 0; i < D / 2; ++i)
-          w[i] = h2_pack(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xFFFF0000u) * f);
       }
+#pragma unroll 4
+      for (int i = 0; i < kChunks; ++i) {
+        uint4* at = reinterpret_cast<uint4*>(chunk_at(row, i));
+        uint32_t w[4] = {at->x, at->y, at->z, at->w};
+        if constexpr (BF16) {
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        const uint4 v = make_uint4(__byte_perm(w[4 * i], w[4 * i + 2], 0x5410), __byte_perm(w[4 * i], w[4 * i + 2], 0x7632),
-                                   __byte_perm(w[4 * i + 1], w[4 * i + 3], 0x5410),
-                                   __byte_perm(w[4 * i + 1], w[4 * i + 3], 0x7632));
-        *reinterpret_cast<uint4*>(sq + (t * C::kAtoms + i / 8) * C::kQAtom + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = v;
+          for (int j = 0; j < 4; ++j) w[j] = h2_pack(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xFFFF0000u) * f);
+        }
+        *at = make_uint4(__byte_perm(w[0], w[2], 0x5410), __byte_perm(w[0], w[2], 0x7632), __byte_perm(w[1], w[3], 0x5410),
+                         __byte_perm(w[1], w[3], 0x7632));
       }
     }
     fence_proxy_async_smem();
@@ -434,31 +449,41 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         }
         if (real) *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
       } else {
+        // through shared memory (this tile's queries are no longer needed), so that whole rows are stored
         const float f = l == 0.f ? 0.f : 1.f / l;
-        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + (it.first + tok) * a.o_ts + h * a.o_hs;
-#pragma unroll
+#pragma unroll 1
         for (int d = 0; d < D; d += 32) {
           float v[32];
           if (n > 0) tmem_ld32(to + d, v);
-          if (real) {
-            uint32_t u[16];
+          uint32_t u[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const float x = l == 0.f ? 0.f : v[2 * k] * f, y = l == 0.f ? 0.f : v[2 * k + 1] * f;
-              if constexpr (BF16) {
-                const __nv_bfloat162 b2 = __floats2bfloat162_rn(x, y);
-                u[k] = *reinterpret_cast<const uint32_t*>(&b2);
-              } else {
-                u[k] = h2_pack(x, y);
-              }
-            }
-            if (a.vec) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                *reinterpret_cast<uint4*>(dst + d + 8 * k) = make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]);
+          for (int k = 0; k < 16; ++k) {
+            const float x = l == 0.f ? 0.f : v[2 * k] * f, y = l == 0.f ? 0.f : v[2 * k + 1] * f;
+            if constexpr (BF16) {
+              const __nv_bfloat162 b2 = __floats2bfloat162_rn(x, y);
+              u[k] = *reinterpret_cast<const uint32_t*>(&b2);
             } else {
+              u[k] = h2_pack(x, y);
+            }
+          }
 #pragma unroll
-              for (int k = 0; k < 32; ++k) dst[d + k] = uint16_t(u[k >> 1] >> (16 * (k & 1)));
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<uint4*>(chunk_at(row, d / 8 + k)) = make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]);
+        }
+        __syncwarp();
+        const uint64_t mine = reinterpret_cast<uint64_t>(reinterpret_cast<uint16_t*>(a.out) + (it.first + tok) * a.o_ts + h * a.o_hs);
+#pragma unroll 4
+        for (int r0 = 0; r0 < 32; r0 += kPer) {
+          const int rr = r0 + lane / kLanes;
+          uint16_t* dst = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, mine, rr)) + 8 * ch;
+          if (ch < kChunks && t * 128 + w0 + rr < it.rows) {
+            const uint4 v = *reinterpret_cast<const uint4*>(chunk_at(w0 + rr, ch));
+            if (a.vec) {
+              *reinterpret_cast<uint4*>(dst) = v;
+            } else {
+              const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int k = 0; k < 8; ++k) dst[k] = uint16_t(u[k >> 1] >> (16 * (k & 1)));
             }
           }
         }

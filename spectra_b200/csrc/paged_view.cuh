@@ -153,6 +153,17 @@ __device__ constexpr float kTanhFit6[6] = {0.9999746680259705f,  -0.332839280366
                                            -0.04692651331424713f, 0.01253186073154211f, -0.001682034693658352f};
 __device__ constexpr float kTanhFit4[4] = {0.9999909996986389f, -0.33298975229263306f, 0.1297455132007599f,
                                            -0.03961124271154404f};
+// Larger magnitude of both halves (bf16 or fp16; a NaN is passed over), as bits.
+template <bool BF16>
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+  b &= 0x7FFF7FFFu;
+  if constexpr (BF16) {
+    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
