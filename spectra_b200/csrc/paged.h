@@ -50,6 +50,7 @@ struct PagedAppendArgs {
   const float* cos; const float* sin; int64_t cs_rs;  // [limit, rotary / 2] or NULL
   int rotary, interleaved;
   int vec;                                 // every row starts on a 16-byte boundary
+  int tokens;                              // of a block (set by the launcher)
 };
 int launch_paged_append(const PagedAppendArgs& a, cudaStream_t st);
 
@@ -57,6 +58,7 @@ struct PagedReadArgs {
   PagedView c;
   void* k; void* v;                        // [total, kv_heads, D], contiguous
   int out_dtype;
+  int tokens;                              // of a block (set by the launcher)
 };
 int launch_paged_read(const PagedReadArgs& a, cudaStream_t st);
 

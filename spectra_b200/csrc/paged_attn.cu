@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
   sm100::fence_mbar_init();
   __syncthreads();
   sm100::pdl_wait();
+  sm100::pdl_trigger();
 
   // ---- this CTA's share of the units
   long long total = 0;

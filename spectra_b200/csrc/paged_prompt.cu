@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
   const int tid = threadIdx.x, warp = same(tid >> 5), lane = tid & 31;
   const int split = blockIdx.y;
   pdl_wait();
+  pdl_trigger();
   Item it;
   if (!item_of(p, blockIdx.x, split, it)) return;
   const int tiles = same(it.rows > 128 ? 2 : 1);
@@ -683,6 +684,7 @@ template <bool BF16, int G>
 __global__ void __launch_bounds__(256) paged_prompt_join_kernel(PromptParams p) {
   constexpr int D = 32 * G;
   pdl_wait();
+  pdl_trigger();
   const PagedAttnArgs& a = p.a;
   const int lane = threadIdx.x & 31;
   Item it;

@@ -20,18 +20,22 @@ __device__ __forceinline__ void new_tokens(const PagedView& c, int b, int64_t& f
   }
 }
 
-// Sequence of new token t, or -1 where none holds it.
+// Sequence of new token t, or -1 where none holds it; the whole warp asks for one
+// token.  (A 32-way search: two loads that wait for each other up to 1024 sequences.)
 __device__ __forceinline__ int sequence_of(const PagedView& c, int64_t t) {
   if (!c.cu_q) {
     const int64_t b = t / c.q_len;
     return b < c.batch ? int(b) : -1;
   }
-  int lo = 0, hi = c.batch;  // the last b with cu_q[b] <= t
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (c.cu_q[mid] <= t) lo = mid; else hi = mid;
+  const int lane = threadIdx.x & 31;
+  int at = -1, step = c.batch + 1;  // cu_q[at] <= t (or at = -1) < cu_q[at + step + 1]
+  while (step > 1) {
+    step = (step + 31) / 32;
+    const int64_t i = int64_t(at) + int64_t(lane + 1) * step;
+    const bool below = i <= c.batch && c.cu_q[i] <= t;
+    at += __popc(__ballot_sync(0xffffffffu, below)) * step;
   }
-  return t >= c.cu_q[lo] && t < c.cu_q[lo + 1] ? lo : -1;
+  return at >= 0 && at < c.batch ? at : -1;
 }
 
 // Tile that holds position `pos` (0 <= pos < limit) of head h, or NULL where

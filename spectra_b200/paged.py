@@ -133,6 +133,7 @@ class TokenBatch:
         self.block_tables, self.seq_lens, self.cu_q = block_tables, seq_lens, cu_q
         self.batch, self.q_len, self.total, self.max_q, self.max_len = B, q_len, total, max_q, max_len
         self._index = block_tables.get_device()
+        self._like: dict = {}
         self._c = L.TokenBatch(block_tables.data_ptr(), block_tables.stride(0) if B > 1 else width, width,
                                seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), B, q_len or 0, total,
                                max_q, 2**31 - 1 if max_len is None else int(max_len))
@@ -155,14 +156,29 @@ def _rows(name: str, t: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, he
     return t if t.stride(2) == 1 else t.contiguous()
 
 
-def _same_device(cache: PagedKVCache, batch: TokenBatch) -> None:
-    if batch._index != cache._index:
-        raise RuntimeError("spectra_b200.paged: the batch's arrays must be on the cache's device")
+def _strided(name: str, t: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, heads: Optional[int]):
+    """The tensor with its token and head strides; the common case in few steps
+    (a call's host time is what a single token waits for)."""
+    ts, hs, unit = t.stride() if t.dim() == 3 else (0, 0, 0)
+    if unit != 1 or t.get_device() != cache._index or t.dtype not in _DT or t.shape != (
+            batch.total, t.shape[1] if heads is None else heads, cache.head_dim):
+        t = _rows(name, t, cache, batch, heads)
+        ts, hs, _ = t.stride()
+    return t, ts, hs
+
+
+def _other_device():
+    raise RuntimeError("spectra_b200.paged: the batch's arrays must be on the cache's device")
+
+
+_FNS: dict = {}  # the library's functions, looked up once
 
 
 def _call(index: int, fn: str, *args) -> None:
-    f = getattr(L.lib(), fn)
-    if torch.cuda.current_device() == index:
+    f = _FNS.get(fn)
+    if f is None:
+        f = _FNS[fn] = getattr(L.lib(), fn)
+    if torch._C._cuda_getDevice() == index:
         st = f(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -185,38 +201,32 @@ def paged_kv_append(cache: PagedKVCache, batch: TokenBatch, k: torch.Tensor, v: 
     Groups that hold a NaN or infinity make their token's key NaN, so every row
     that looks at it is NaN and no other.  Token tensors may be views (any
     token and head strides), of a fused projection for example."""
-    _same_device(cache, batch)
-    k = _rows("k", k, cache, batch, cache.kv_heads)
-    v = _rows("v", v, cache, batch, cache.kv_heads)
+    index = cache._index
+    if batch._index != index:
+        _other_device()
+    k, k_ts, k_hs = _strided("k", k, cache, batch, cache.kv_heads)
+    v, v_ts, v_hs = _strided("v", v, cache, batch, cache.kv_heads)
     dt = k.dtype
     rotary = rows = cs = 0
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin come together")
-    if cos is not None:
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32:
-            raise TypeError("cos and sin must be float32")
-        if cos.get_device() != cache._index or sin.get_device() != cache._index:
-            raise RuntimeError("spectra_b200.paged: cos and sin must be on the cache's CUDA device")
-        if cos.dim() != 2 or cos.shape != sin.shape:
-            raise ValueError(f"cos and sin must be [positions, rotary / 2], got {tuple(cos.shape)} and {tuple(sin.shape)}")
-        if cos.stride(1) != 1 or sin.stride() != cos.stride():
-            cos, sin = cos.contiguous(), sin.contiguous()
-        rows, rotary, cs = cos.shape[0], 2 * cos.shape[1], cos.stride(0)
-        if rotary > cache.head_dim or rotary % (8 if interleaved else 16):
-            raise ValueError(f"the rotated part must be a multiple of {8 if interleaved else 16} and at most "
-                             f"{cache.head_dim}, got {rotary}")
-        if rows < batch._limit(cache):
-            raise ValueError(f"cos and sin have {rows} positions, the batch may hold {batch._limit(cache)}")
-    if q is None:
-        qp = op = None
-        heads = q_ts = q_hs = o_ts = o_hs = 0
-    else:
-        q = _rows("q", q, cache, batch, None)
+    cp = sp = None
+    if cos is not None or sin is not None:
+        cos, sin, rotary, rows, cs = _angles(cos, sin, cache, batch, interleaved)
+        if rotary:
+            cp, sp = cos.data_ptr(), sin.data_ptr()
+    qp = op = None
+    heads = q_ts = q_hs = o_ts = o_hs = 0
+    if q is not None:
+        q, q_ts, q_hs = _strided("q", q, cache, batch, None)
         heads = q.shape[1]
         if out is None:
-            out = torch.empty(q.shape, dtype=dt, device=q.device)
+            out = torch.empty_like(q)
+            o_ts, o_hs, unit = out.stride()
+            if unit != 1:
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                o_ts, o_hs, _ = out.stride()
         else:
-            if _rows("out", out, cache, batch, heads) is not out:
+            given, o_ts, o_hs = _strided("out", out, cache, batch, heads)
+            if given is not out:
                 raise ValueError("out must have unit stride along a head")
             lo, hi = _extent(q)
             olo, ohi = _extent(out)
@@ -224,15 +234,35 @@ def paged_kv_append(cache: PagedKVCache, batch: TokenBatch, k: torch.Tensor, v: 
                 raise ValueError("out must not overlap q")
         if q.dtype != dt or out.dtype != dt:
             raise TypeError("q, k, v and out must have one dtype")
-        qp, (q_ts, q_hs, _), op, (o_ts, o_hs, _) = q.data_ptr(), q.stride(), out.data_ptr(), out.stride()
+        qp, op = q.data_ptr(), out.data_ptr()
     if v.dtype != dt:
         raise TypeError("q, k, v and out must have one dtype")
-    k_ts, k_hs, _ = k.stride()
-    v_ts, v_hs, _ = v.stride()
-    _call(cache._index, "spectra_paged_kv_append", cache._at, batch._at, _DT[dt], heads, qp, q_ts, q_hs, op, o_ts, o_hs,
-          k.data_ptr(), k_ts, k_hs, v.data_ptr(), v_ts, v_hs, cos.data_ptr() if rotary else None,
-          sin.data_ptr() if rotary else None, rows, cs, rotary, interleaved)
+    _call(index, "spectra_paged_kv_append", cache._at, batch._at, _DT[dt], heads, qp, q_ts, q_hs, op, o_ts, o_hs,
+          k.data_ptr(), k_ts, k_hs, v.data_ptr(), v_ts, v_hs, cp, sp, rows, cs, rotary, interleaved)
     return out if q is not None else None
+
+
+def _angles(cos, sin, cache: PagedKVCache, batch: TokenBatch, interleaved: bool):
+    if cos is None or sin is None:
+        raise ValueError("cos and sin come together")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise TypeError("cos and sin must be float32")
+    if cos.get_device() != cache._index or sin.get_device() != cache._index:
+        raise RuntimeError("spectra_b200.paged: cos and sin must be on the cache's CUDA device")
+    if cos.dim() != 2 or cos.shape != sin.shape:
+        raise ValueError(f"cos and sin must be [positions, rotary / 2], got {tuple(cos.shape)} and {tuple(sin.shape)}")
+    strides = cos.stride()
+    if strides[1] != 1 or sin.stride() != strides:
+        cos, sin = cos.contiguous(), sin.contiguous()
+        strides = cos.stride()
+    rows, half = cos.shape
+    rotary = 2 * half
+    if rotary > cache.head_dim or rotary % (8 if interleaved else 16):
+        raise ValueError(f"the rotated part must be a multiple of {8 if interleaved else 16} and at most "
+                         f"{cache.head_dim}, got {rotary}")
+    if rows < batch._limit(cache):
+        raise ValueError(f"cos and sin have {rows} positions, the batch may hold {batch._limit(cache)}")
+    return cos, sin, rotary, rows, strides[0]
 
 
 def _extent(t: torch.Tensor) -> Tuple[int, int]:
@@ -244,12 +274,16 @@ def paged_kv_read(cache: PagedKVCache, batch: TokenBatch, dtype: torch.dtype = t
     """Keys and values [total, kv_heads, D] that the cache holds of the batch's
     new tokens: ``(q - z) * s`` rounded once to ``dtype`` (exact in fp32); 0 for
     padding.  ``cu_q`` of cumulated seq_lens reads whole sequences."""
-    _same_device(cache, batch)
+    if batch._index != cache._index:
+        _other_device()
     if dtype not in _OUT_DT:
         raise TypeError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
-    shape = (batch.total, cache.kv_heads, cache.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=cache.pool.device)
-    v = torch.empty(shape, dtype=dtype, device=cache.pool.device)
+    like = batch._like.get((dtype, cache.kv_heads, cache.head_dim))
+    if like is None:  # a shape to allocate by, without memory of its own
+        like = torch.empty(1, 1, 1, dtype=dtype, device=cache.pool.device).expand(batch.total, cache.kv_heads, cache.head_dim)
+        batch._like[dtype, cache.kv_heads, cache.head_dim] = like
+    k = torch.empty_like(like, memory_format=torch.contiguous_format)
+    v = torch.empty_like(like, memory_format=torch.contiguous_format)
     _call(cache._index, "spectra_paged_kv_read", cache._at, batch._at, k.data_ptr(), v.data_ptr(), _OUT_DT[dtype])
     return k, v
 
@@ -261,13 +295,14 @@ def paged_kv_read(cache: PagedKVCache, batch: TokenBatch, dtype: torch.dtype = t
 _WORKSPACES: dict = {}
 
 
-def _workspace(index: int, head_dim: int) -> torch.Tensor:
+def _workspace(index: int, head_dim: int) -> Tuple[int, int]:
     key = (index, torch._C._cuda_getCurrentRawStream(index), head_dim)
     ws = _WORKSPACES.get(key)
     if ws is None:
         nbytes = L.lib().spectra_paged_attention_workspace_bytes(head_dim)
-        ws = _WORKSPACES[key] = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
-    return ws
+        buf = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+        ws = _WORKSPACES[key] = (buf.data_ptr(), nbytes, buf)
+    return ws[0], ws[1]
 
 
 def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, *, scale: Optional[float] = None,
@@ -282,8 +317,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, *, 
     then plus ``alibi_slopes[h] * (n - p)`` (fp32 [q_heads]).  q_heads is a
     multiple of kv_heads; consecutive heads share one.  A row that sees no key
     is 0.  Scores, softmax statistics and sums are fp32."""
-    _same_device(cache, batch)
-    q = _rows("q", q, cache, batch, None)
+    index = cache._index
+    if batch._index != index:
+        _other_device()
+    q, q_ts, q_hs = _strided("q", q, cache, batch, None)
     heads = q.shape[1]
     if heads % cache.kv_heads or not heads:
         raise ValueError(f"q has {heads} heads, not a multiple of the cache's {cache.kv_heads}")
@@ -296,17 +333,21 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, *, 
     if alibi_slopes is not None:
         if alibi_slopes.dtype != torch.float32 or alibi_slopes.shape != (heads,):
             raise ValueError(f"alibi_slopes must be float32 [{heads}]")
-        if alibi_slopes.get_device() != cache._index:
+        if alibi_slopes.get_device() != index:
             raise RuntimeError("spectra_b200.paged: alibi_slopes must be on the cache's CUDA device")
         slopes = alibi_slopes if heads == 1 or alibi_slopes.stride(0) == 1 else alibi_slopes.contiguous()
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif _rows("out", out, cache, batch, heads) is not out or out.dtype != q.dtype:
-        raise ValueError("out must have q's dtype and unit stride along a head")
-    ws = _workspace(cache._index, cache.head_dim)
-    q_ts, q_hs, _ = q.stride()
-    o_ts, o_hs, _ = out.stride()
-    _call(cache._index, "spectra_paged_attention", cache._at, batch._at, _DT[q.dtype], heads, q.data_ptr(), q_ts, q_hs,
+        out = torch.empty_like(q)
+        o_ts, o_hs, unit = out.stride()
+        if unit != 1:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            o_ts, o_hs, _ = out.stride()
+    else:
+        given, o_ts, o_hs = _strided("out", out, cache, batch, heads)
+        if given is not out or out.dtype != q.dtype:
+            raise ValueError("out must have q's dtype and unit stride along a head")
+    ws, nbytes = _workspace(index, cache.head_dim)
+    _call(index, "spectra_paged_attention", cache._at, batch._at, _DT[q.dtype], heads, q.data_ptr(), q_ts, q_hs,
           out.data_ptr(), o_ts, o_hs, scale, softcap, None if slopes is None else slopes.data_ptr(), causal, window,
-          ws.data_ptr(), ws.numel())
+          ws, nbytes)
     return out
