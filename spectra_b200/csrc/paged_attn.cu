@@ -230,18 +230,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
     const int u_end = s.len > 0 ? u_stop : u_begin;  // (nothing held: nothing to load)
     const int rows = min(ROWS, s.count * a.group - row0);
 
-    // ---- units to load: warp w takes u_begin + w, + kWarps, ...  Lane j knows where
-    // the j-th of the next 32 of them lies, and in the address's low bits which of its
-    // tiles a page holds; where none does, page 0's tile takes its place (the keys are
-    // masked, the values finite).
-    const int next = u_begin + warp;
+    // ---- units to load: warp w takes u_end - 1 - w, - kWarps, ... (the last keys first: a
+    // bias on distance only falls on the way).  Lane j knows where the j-th of the next 32
+    // of them lies, and in the address's low bits which of its tiles a page holds; where
+    // none does, page 0's tile takes its place (the keys are masked, the values finite).
+    const int next = u_end - 1 - warp;
     const uint8_t* head_pool = c.pool + int64_t(head) * per_page * C::kTile;
     const int* table = c.tables + b * c.table_stride;
     const bool small = c.page_log2 == 4;  // a page is one tile
     uint64_t here = 0, here1 = 0, ahead = 0, ahead1 = 0;
     auto look = [&](int from, uint64_t& w0, uint64_t& w1) {  // of the warp's units from `from` on
-      const int u = next + (from + lane) * kWarps, pos = u * kUnit;
-      const bool in = u < u_end && pos < s.len;
+      const int u = next - (from + lane) * kWarps, pos = u * kUnit;
+      const bool in = u >= u_begin && pos < s.len;
       const int p0 = in ? table[pos >> c.page_log2] : -1;
       const bool h0 = unsigned(p0) < unsigned(c.num_pages);
       w0 = reinterpret_cast<uint64_t>(head_pool + (h0 ? p0 : 0) * c.page_stride + (u * 2 & (per_page - 1)) * C::kTile) + (h0 ? 3 : 0);
@@ -272,10 +272,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
       }
     };
     look(0, here, here1);
-    if (next + 32 * kWarps < u_end) look(32, ahead, ahead1);
+    if (next - 32 * kWarps >= u_begin) look(32, ahead, ahead1);
 #pragma unroll
     for (int st = 0; st < kStages; ++st) {
-      if (next + st * kWarps < u_end) issue(st, st);
+      if (next - st * kWarps >= u_begin) issue(st, st);
     }
 
     // ---- query fragments: the products' B registers and the groups' sums.  Four
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
       for (int j = 0; j < 2; ++j) c_exp[nt][j] = MOD ? 1.f : factor[nt * 8 + 2 * cc + j] * kLog2e;
 
     int stage = 0, unit = 0;
-    for (int u = next; u < u_end; u += kWarps, ++unit) {
+    for (int u = next; u >= u_begin; u -= kWarps, ++unit) {
       if (!sm100::mbar_wait(bars + warp * kStages + stage, (phase >> stage) & 1u, &s_never)) {
         s_stop = 1;
         if (lane == 0) atomicAdd(&g_paged_attn_timeouts, 1);
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
       }
       __syncwarp();
       phase ^= 1u << stage;
-      if (u + kStages * kWarps < u_end && !s_stop) issue(unit + kStages, stage);
+      if (u - kStages * kWarps >= u_begin && !s_stop) issue(unit + kStages, stage);
       stage = stage + 1 == kStages ? 0 : stage + 1;
     }
 

@@ -4,7 +4,8 @@
 // The definition is paged_attn.cu's.  With hundreds of rows per key/value head
 // the work is products, so a CTA takes 256 rows (tokens x the query heads that
 // share the head; two M = 128 tiles) of one sequence and walks the keys 64 at
-// a time:
+// a time, the last ones first: the step with the causal edge is then the one that
+// has to look for a maximum anyway, and a bias on distance only falls afterwards.
 //   warps 8-11  bring the raw tiles in by bulk copies and write them to shared
 //               memory as fp16 operands: K [token][feature] and V^T
 //               [feature][token], K-major, 128-byte swizzle; two warps a step,
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         ok = wait(&s_full[t][i & 1], (i >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
-        const int n0 = (it.step0 + i) * kKeys;
+        const int n0 = (it.step0 + n - 1 - i) * kKeys;
         const int held = s_held[i & 7][0] | s_held[i & 7][1] << 2;  // one bit per 16 keys
         const bool masked = __any_sync(0xffffffffu, n0 < lo || n0 + kKeys > hi) || held != 0xF;
 
@@ -498,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
     const uint32_t magic = fp16_1024();
     int mine = 0;            // lanes 0, 1: page of the tile to load next
     auto look = [&](int i) {
-      const int at = (it.step0 + i) * kKeys + 32 * half + 16 * lane;
+      const int at = (it.step0 + n - 1 - i) * kKeys + 32 * half + 16 * lane;
       mine = lane < 2 && i < n && at < it.len ? c.tables[it.b * c.table_stride + (at >> c.page_log2)] : -1;
     };
     unsigned held_next = 0;  // lanes 0, 1: of the tiles in flight
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         if (lane == 0) mbar_arrive_expect_tx(raw_full + dw, __popc(held_next) * C::kTile);
         __syncwarp(0x3u);
         if (hold) {
-          const int at = (it.step0 + i) * kKeys + 32 * half + 16 * lane;
+          const int at = (it.step0 + n - 1 - i) * kKeys + 32 * half + 16 * lane;
           const int per = 1 << (c.page_log2 - 4);
           bulk_g2s(buf + lane * C::kTile, c.pool + mine * c.page_stride + (int64_t(it.head) * per + ((at >> 4) & (per - 1))) * C::kTile,
                    C::kTile, raw_full + dw);
