@@ -97,7 +97,8 @@ struct Cfg {
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kSlab = ROWS * (D + 4);               // one warp's partial result, floats
   static constexpr int kMerge = kWarps * kSlab * 4;           // shares the ring's memory
-  static constexpr int kBig = kRing > kMerge ? kRing : kMerge;
+  static constexpr int kJoin = ROWS * 66 * 4;                 // weights of 64 parts
+  static constexpr int kBig = kRing > kMerge ? (kRing > kJoin ? kRing : kJoin) : (kMerge > kJoin ? kMerge : kJoin);
   static constexpr int kQ = G * NT * 32 * 16;                 // query fragments
   static constexpr int kX = G * NT * 4 * 32;                  // {C, C', C, C'} and {X, X'} of a lane's two rows
   static constexpr int kMeta = ROWS * 16;                     // hi, lo, slope, position of a row
@@ -142,13 +143,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
   sm100::pdl_trigger();
 
   // ---- this CTA's share of the units
-  long long total = 0;
-  for (int b0 = 0; b0 < c.batch; b0 += kThreads) {
-    if (b0 + tid < c.batch) {
-      const Span s = span_of<ROWS>(p, b0 + tid);
-      total += (long long)(s.units) * s.tiles * c.kv_heads;
-    }
-  }
+  auto units_of = [&](int i) -> long long {
+    if (i >= c.batch) return 0;
+    const Span s = span_of<ROWS>(p, i);
+    return (long long)(s.units) * s.tiles * c.kv_heads;
+  };
+  const long long first_units = units_of(tid);  // (the only ones of a batch of up to kThreads)
+  long long total = first_units;
+  for (int b0 = kThreads; b0 < c.batch; b0 += kThreads) total += units_of(b0 + tid);
 #pragma unroll
   for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) s_scan[warp] = total;
@@ -156,7 +158,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
   total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) total += s_scan[w];
-  long long share = (total + gridDim.x - 1) / gridDim.x;
+  const long long up = total + gridDim.x - 1;
+  long long share = up < (1ll << 32) ? (long long)(unsigned(up) / gridDim.x) : up / gridDim.x;
   if (share < p.min_share) share = p.min_share;
   const long long begin = share * blockIdx.x;
   const long long end = begin + share < total ? begin + share : total;
@@ -174,11 +177,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
   // ---- the sequence where the share begins
   long long base = 0;
   for (int b0 = 0; b0 < c.batch; b0 += kThreads) {
-    long long mine = 0;
-    if (b0 + tid < c.batch) {
-      const Span s = span_of<ROWS>(p, b0 + tid);
-      mine = (long long)(s.units) * s.tiles * c.kv_heads;
-    }
+    const long long mine = b0 == 0 ? first_units : units_of(b0 + tid);
     long long sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -630,36 +629,84 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
       __syncthreads();
       if (s_last) {
         __threadfence();
-        // the first CTA's part is its last segment's (slot 1), the others' their first's (slot 0)
-        const float* part0 = p.partials + int64_t(2 * cta0 + 1) * C::kPartial;
+        // 64 parts at a time: a warp per row finds their weights, then every thread adds its
+        // items up, 16 loads in flight (one after the other took 7 us of a 34 us call).  The first CTA's part is its last segment's (slot 1),
+        // the others' their first's (slot 0).
         const float* parts = p.partials + int64_t(2 * cta0) * C::kPartial;
-        const int n = cta1 - cta0;
-        float* tops = merge;  // (every thread is past its reads of the slabs)
-        for (int row = warp; row < rows; row += kWarps) {
-          float top = lane == 0 ? __ldcg(part0 + ROWS * D + 2 * row) : kNone;
-          for (int k = 1 + lane; k <= n; k += 32)
-            top = fmaxf(top, __ldcg(parts + int64_t(2 * k) * C::kPartial + ROWS * D + 2 * row));
+        const int n = cta1 - cta0 + 1;
+        auto part_of = [&](int k) { return parts + int64_t(k == 0 ? 1 : 2 * k) * C::kPartial; };
+        constexpr int kItems = (ROWS * D / 4 + kThreads - 1) / kThreads, kRowsOfWarp = ROWS / kWarps;
+        constexpr int kFlight = kItems >= 4 ? 4 : 16 / kItems;  // parts whose loads are in flight
+        float* weight = merge;                        // [ROWS][64] (every thread is past its reads of the slabs)
+        float* fade = merge + ROWS * 64;              // [ROWS] of what has been added up
+        float* whole_sum = merge + ROWS * 65;         // [ROWS]
+        float top[kRowsOfWarp], sum[kRowsOfWarp];
+        float4 acc[kItems];
 #pragma unroll
-          for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-          if (lane == 0) tops[row] = top;
+        for (int j = 0; j < kItems; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < kRowsOfWarp; ++j) {
+          top[j] = kNone;
+          sum[j] = 0.f;
         }
-        __syncthreads();
-        for (int i = tid; i < rows * (D / 4); i += kThreads) {
-          const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
-          const float top = tops[row];
-          float sum = 0.f;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          auto take = [&](const float* part) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + ROWS * D + 2 * row));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + row * D + d));
-            const float f = exp2f(ml.x - top);
-            sum = fmaf(f, ml.y, sum);
-            add(acc, f, v);
-          };
-          take(part0);
-#pragma unroll 8
-          for (int k = 1; k <= n; ++k) take(parts + int64_t(2 * k) * C::kPartial);
-          put(row, d, acc, sum);
+        for (int k0 = 0; k0 < n; k0 += 64) {
+          float2 ml[kRowsOfWarp][2];
+#pragma unroll
+          for (int j = 0; j < kRowsOfWarp; ++j)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int k = k0 + 32 * x + lane, row = warp + j * kWarps;
+              ml[j][x] = make_float2(kNone, 0.f);
+              if (k < n && row < rows) ml[j][x] = __ldcg(reinterpret_cast<const float2*>(part_of(k) + ROWS * D + 2 * row));
+            }
+#pragma unroll
+          for (int j = 0; j < kRowsOfWarp; ++j) {
+            const int row = warp + j * kWarps;
+            float up = fmaxf(top[j], fmaxf(ml[j][0].x, ml[j][1].x));
+#pragma unroll
+            for (int k = 16; k; k >>= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, k));
+            const float f = exp2f(top[j] - up), f0 = exp2f(ml[j][0].x - up), f1 = exp2f(ml[j][1].x - up);
+            float add_up = f0 * ml[j][0].y + f1 * ml[j][1].y;
+#pragma unroll
+            for (int k = 16; k; k >>= 1) add_up += __shfl_xor_sync(0xffffffffu, add_up, k);
+            top[j] = up;
+            sum[j] = fmaf(sum[j], f, add_up);
+            weight[row * 64 + lane] = f0;
+            weight[row * 64 + 32 + lane] = f1;
+            if (lane == 0) {
+              fade[row] = f;
+              whole_sum[row] = sum[j];
+            }
+          }
+          __syncthreads();
+          int row[kItems], d[kItems];
+#pragma unroll
+          for (int j = 0; j < kItems; ++j) {
+            const int i = min(tid + j * kThreads, rows * (D / 4) - 1);
+            row[j] = i / (D / 4);
+            d[j] = (i - row[j] * (D / 4)) * 4;
+            const float f = fade[row[j]];
+            acc[j] = make_float4(acc[j].x * f, acc[j].y * f, acc[j].z * f, acc[j].w * f);
+          }
+          const int most = min(64, n - k0);
+          for (int k = 0; k < most; k += kFlight) {  // (past the last part: the last again, with weight 0)
+            float4 v[kFlight][kItems];
+#pragma unroll
+            for (int x = 0; x < kFlight; ++x)
+#pragma unroll
+              for (int j = 0; j < kItems; ++j)
+                v[x][j] = __ldcg(reinterpret_cast<const float4*>(part_of(k0 + min(k + x, most - 1)) + row[j] * D + d[j]));
+#pragma unroll
+            for (int x = 0; x < kFlight; ++x)
+#pragma unroll
+              for (int j = 0; j < kItems; ++j) add(acc[j], k + x < most ? weight[row[j] * 64 + k + x] : 0.f, v[x][j]);
+          }
+          __syncthreads();
+        }
+#pragma unroll
+        for (int j = 0; j < kItems; ++j) {
+          const int i = tid + j * kThreads, row = i / (D / 4), d = (i - row * (D / 4)) * 4;
+          if (i < rows * (D / 4)) put(row, d, acc[j], whole_sum[row]);
         }
       }
     }
