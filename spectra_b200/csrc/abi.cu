@@ -537,16 +537,7 @@ int spectra_paged_attention(const SpectraPagedCache* cache, const SpectraTokenBa
   a.window = int(std::min<int64_t>(window, INT32_MAX));
   a.vec = head_rows_vec(q, q_ts, q_hs) && head_rows_vec(out, o_ts, o_hs);
   a.workspace = workspace; a.workspace_bytes = workspace_bytes;
-  // Rows of one key/value head (new tokens times the query heads that share it): up to kFewRows a sequence is
-  // the few-token kernel's, above it the prompt kernel's.  A batch of equal sequences takes one launch; a ragged
-  // one with long sequences both, as either kind may be in it.
-  constexpr int kFewRows = 64;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t rows = int64_t(a.c.max_q) * a.group;
-  if (rows <= kFewRows || cache->head_dim > 128) return launch_paged_attn(a, INT32_MAX, s);
-  if (!a.c.cu_q) return launch_paged_prompt(a, 0, s);
-  const int few = launch_paged_attn(a, kFewRows, s);
-  return few != SPECTRA_OK ? few : launch_paged_prompt(a, kFewRows, s);
+  return launch_paged_attention(a, static_cast<cudaStream_t>(stream));
 }
 
 size_t spectra_paged_attention_workspace_bytes(int64_t head_dim) {

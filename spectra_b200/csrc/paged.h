@@ -82,6 +82,7 @@ size_t paged_attn_workspace_bytes(int head_dim);
 size_t paged_prompt_workspace_bytes(int head_dim);
 int launch_paged_attn(const PagedAttnArgs& a, int max_rows, cudaStream_t st);
 int launch_paged_prompt(const PagedAttnArgs& a, int min_rows, cudaStream_t st);
+int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st);  // the one or the other, or both
 int paged_attn_timeouts(long long* out, bool reset);
 int paged_prompt_timeouts(long long* out, bool reset);
 

@@ -690,25 +690,46 @@ __global__ void __launch_bounds__(256) paged_prompt_join_kernel(PromptParams p) 
   const int lane = threadIdx.x & 31;
   Item it;
   if (!item_of(p, blockIdx.x, 0, it)) return;
-  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < it.rows; r += gridDim.y * 8) {
-    const float* part = p.partials + (int64_t(blockIdx.x) * p.splits * kRows + r) * (D + 2);
-    const int64_t step = int64_t(kRows) * (D + 2);
-    float top = kNone, sum = 0.f, acc[G];
+  const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (r >= it.rows) return;
+  const float* part = p.partials + (int64_t(blockIdx.x) * p.splits * kRows + r) * (D + 2);
+  const int64_t step = int64_t(kRows) * (D + 2);
+  float top = kNone, sum = 0.f, acc[G];
 #pragma unroll
-    for (int q = 0; q < G; ++q) acc[q] = 0.f;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, part[s * step + D]);
-    for (int s = 0; s < p.splits; ++s) {
-      const float f = exp2f(part[s * step + D] - top);
-      sum = fmaf(f, part[s * step + D + 1], sum);
+  for (int q = 0; q < G; ++q) acc[q] = 0.f;
+  for (int s0 = 0; s0 < p.splits; s0 += 32) {  // 32 splits' weights at once, then eight splits' loads in flight
+    const bool in = s0 + lane < p.splits;
+    const float2 ml = in ? *reinterpret_cast<const float2*>(part + (s0 + lane) * step + D) : make_float2(kNone, 0.f);
+    float up = fmaxf(top, ml.x);
 #pragma unroll
-      for (int q = 0; q < G; ++q) acc[q] = fmaf(f, part[s * step + 32 * q + lane], acc[q]);
+    for (int k = 16; k; k >>= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, k));
+    const float fade = exp2f(top - up), f = in ? exp2f(ml.x - up) : 0.f;
+    float more = f * ml.y;
+#pragma unroll
+    for (int k = 16; k; k >>= 1) more += __shfl_xor_sync(0xffffffffu, more, k);
+    top = up;
+    sum = fmaf(sum, fade, more);
+#pragma unroll
+    for (int q = 0; q < G; ++q) acc[q] *= fade;
+    const int n = min(32, p.splits - s0);
+    for (int s = 0; s < n; s += 8) {
+      float v[8][G];
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+#pragma unroll
+        for (int q = 0; q < G; ++q) v[x][q] = part[(s0 + min(s + x, n - 1)) * step + 32 * q + lane];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const float w = __shfl_sync(0xffffffffu, f, (s + x) & 31);
+#pragma unroll
+        for (int q = 0; q < G; ++q) acc[q] = s + x < n ? fmaf(w, v[x][q], acc[q]) : acc[q];
+      }
     }
-    const int R = it.row0 + r, tok = R / a.group, h = it.head * a.group + R - tok * a.group;
-#pragma unroll
-    for (int q = 0; q < G; ++q)
-      store_from_float(a.out, (it.first + tok) * a.o_ts + h * a.o_hs + 32 * q + lane, a.dtype,
-                       sum == 0.f ? 0.f : acc[q] / sum);
   }
+  const int R = it.row0 + r, tok = R / a.group, h = it.head * a.group + R - tok * a.group;
+#pragma unroll
+  for (int q = 0; q < G; ++q)
+    store_from_float(a.out, (it.first + tok) * a.o_ts + h * a.o_hs + 32 * q + lane, a.dtype, sum == 0.f ? 0.f : acc[q] / sum);
 }
 
 template <class K>
@@ -751,7 +772,7 @@ int launch_one(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
     return SPECTRA_ERR_WORKSPACE;
   const int status = launch_dep(kern, dim3(unsigned(items), unsigned(p.splits)), kThreads, C::kSmem, p, st);
   if (status != SPECTRA_OK || p.splits == 1) return status;
-  return launch_dep(paged_prompt_join_kernel<BF16, G>, dim3(unsigned(items), 8), 256, 0, p, st);
+  return launch_dep(paged_prompt_join_kernel<BF16, G>, dim3(unsigned(items), kRows / 8), 256, 0, p, st);
 }
 
 template <bool BF16, int G>
@@ -780,6 +801,27 @@ size_t paged_prompt_workspace_bytes(int head_dim) {
 
 int launch_paged_prompt(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
   return a.dtype == SPECTRA_DT_BF16 ? launch_dim<true>(a, min_rows, st) : launch_dim<false>(a, min_rows, st);
+}
+
+// Rows of one key/value head (new tokens times the query heads that share it): up to `few` a
+// sequence is paged_attn.cu's, above it this file's.  A batch of equal sequences takes one
+// launch; a ragged one with long sequences both, as either kind may be in it.  Measured with
+// heads of 128, 8 of them, 32 queries' heads, us (paged_attn / paged_prompt):
+//   keys   1 sequence, 64 rows   96 rows       16 sequences, 32 rows   64 rows
+//   1024   13.3 / 17.1           19.4 / 18.2   27.7 / 25.1             44.3 / 25.8
+//   8192   27.9 / 33.5           33.7 / 34.9   107 / 134               200 / 136
+// (few CTAs have to split the keys, which paged_attn does at a finer grain).  Heads of 256 have
+// no room in TMEM and shared memory here.
+int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e);
+  const bool many = int64_t(a.c.batch) * a.c.kv_heads * 2 >= device_sms(dev);
+  const int few = many ? 32 : 96;
+  if (int64_t(a.c.max_q) * a.group <= few || a.c.head_dim > 128) return launch_paged_attn(a, INT32_MAX, st);
+  if (!a.c.cu_q) return launch_paged_prompt(a, 0, st);
+  const int status = launch_paged_attn(a, few, st);
+  return status != SPECTRA_OK ? status : launch_paged_prompt(a, few, st);
 }
 
 int paged_prompt_timeouts(long long* out, bool reset) { return read_timeout_counter(g_paged_prompt_timeouts, out, reset); }
