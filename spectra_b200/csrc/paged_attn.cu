@@ -21,7 +21,7 @@
 //     are never rounded.
 //   O^T = V^T P^T: A = values (q - z) s in fp16 (exact difference, one
 //     rounding of the product, 11 bits), B = P in fp16, transposed in
-//     registers (movmatrix).  P <= 2^kLazy, so fp16 holds it; its rounding
+//     registers (movmatrix).  P <= 2^(kLazy + kShift), so fp16 holds it; its rounding
 //     (2^-12) averages over the keys.
 // Queries of both types are scaled per row by a power of two to fp16's upper
 // range (exact down to 2^-24 of the row's largest entry).
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
           float e[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i]) : "f"(fmaf(sc[tile][nt][i], c_exp[nt][i & 1], -m[nt][i & 1])));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i]) : "f"(fmaf(sc[tile][nt][i], c_exp[nt][i & 1], kShift - m[nt][i & 1])));
             l[nt][i & 1] += e[i];
           }
           pb[tile][nt][0] = transpose8x8(h2_pack(e[0], e[1]));

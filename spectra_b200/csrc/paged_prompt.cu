@@ -3,7 +3,7 @@
 //
 // The definition is paged_attn.cu's.  With hundreds of rows per key/value head
 // the work is products, so a CTA takes 256 rows (tokens x the query heads that
-// share the head; two M = 128 tiles) of one sequence and walks the keys 64 at
+// share the head; two M = 128 tiles, one for heads of 256) of one sequence and walks the keys 64 at
 // a time, the last ones first: the step with the causal edge is then the one that
 // has to look for a maximum anyway, and a bias on distance only falls afterwards.
 //   warps 8-11  bring the raw tiles in by bulk copies and write them to shared
@@ -42,17 +42,17 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kRows = 256;   // rows of a CTA
+constexpr int kRows = 256;   // rows of a CTA, at most
 constexpr int kKeys = 64;    // keys of a step
 constexpr int kThreads = 512;  // warps 14 and 15 only give their registers away
-constexpr int kStages = 4;   // operand stages
 
 struct PromptParams {
   PagedAttnArgs a;
   int row_tiles;   // per sequence and head, at most
   int splits;
+  int rows;        // of a CTA
   int min_rows;    // a sequence with at most this many rows per head is the other kernel's
-  float* partials; // [item][split][kRows][D + 2]
+  float* partials; // [item][split][rows][D + 2]
 };
 
 template <int G>
@@ -62,11 +62,15 @@ struct Cfg {
   static constexpr int kTile = TileLayout{G}.bytes();
   static constexpr int kQAtom = 128 * 128;                     // 128 rows
   static constexpr int kKAtom = kKeys * 128;                   // 64 rows
-  static constexpr int kQ = 2 * kAtoms * kQAtom;
+  // Heads of 256: O takes 256 columns of TMEM and a step's operands 64 KB, so one tile, two stages of
+  // keys and one of values.
+  static constexpr int kTiles = G == 8 ? 1 : 2;
+  static constexpr int kKStages = G == 8 ? 2 : 4, kVStages = G == 8 ? 1 : 4;
+  static constexpr int kQ = kTiles * kAtoms * kQAtom;
   static constexpr int kK = kAtoms * kKAtom;                   // one stage
   static constexpr int kV = D * 128;                           // one stage
   static constexpr int kRaw = 4 * 2 * kTile;
-  static constexpr int kSmem = 1024 + kQ + kStages * (kK + kV) + kRaw;
+  static constexpr int kSmem = 1024 + kQ + kKStages * kK + kVStages * kV + kRaw;
 };
 
 // The rows of one item: row R of a (sequence, head) is token R / group, query head R % group.
@@ -87,9 +91,9 @@ __device__ __forceinline__ bool item_of(const PromptParams& p, int index, int sp
   int count;
   new_tokens(c, it.b, it.first, count);
   const int all = count * p.a.group;
-  it.row0 = tile * kRows;
+  it.row0 = tile * p.rows;
   if (all <= p.min_rows || it.row0 >= all) return false;
-  it.rows = min(kRows, all - it.row0);
+  it.rows = min(p.rows, all - it.row0);
   const int len = c.seq_lens[it.b];
   it.pos0 = len - count;
   it.len = len < 0 ? 0 : (len < c.limit ? len : c.limit);
@@ -124,9 +128,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = smem;
   uint8_t* sk = sq + C::kQ;
-  uint8_t* sv = sk + kStages * C::kK;
-  uint8_t* raw = sv + kStages * C::kV;
-  __shared__ uint64_t q_full, k_full[kStages], v_full[kStages], k_empty[kStages], v_empty[kStages];
+  uint8_t* sv = sk + C::kKStages * C::kK;
+  uint8_t* raw = sv + C::kVStages * C::kV;
+  // (the values' stages are freed on two barriers at least: the warps of the odd and of the even steps
+  // each see every phase of the one they wait on)
+  constexpr int SK = C::kKStages, SV = C::kVStages, SE = SV == 1 ? 2 : SV;
+  __shared__ uint64_t q_full, k_full[SK], v_full[SV], k_empty[SK], v_empty[SE];
   __shared__ uint64_t s_full[2][2], p_full[2][2], o_full[2], o_done[2], raw_full[4], drain[2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_held[8][2];  // [step % 8][half]: which of the half's two tiles a page holds
@@ -144,12 +151,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
   const int tiles = same(it.rows > 128 ? 2 : 1);
   if (tid == 0) {
     mbar_init(&q_full, 8);
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < SK; ++i) {
       mbar_init(k_full + i, 2);
-      mbar_init(v_full + i, 2);
       mbar_init(k_empty + i, tiles);
-      mbar_init(v_empty + i, tiles);
     }
+    for (int i = 0; i < SV; ++i) mbar_init(v_full + i, 2);
+    for (int i = 0; i < SE; ++i) mbar_init(v_empty + i, tiles);
     for (int i = 0; i < 2; ++i) {
       for (int j = 0; j < 2; ++j) {
         mbar_init(&s_full[i][j], 1);
@@ -287,11 +294,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         // weight fits fp16 too); TERMS: of the cap's tanh, which may be out of their range as well.
         auto fast = [&](auto terms) -> bool {
           constexpr int TERMS = decltype(terms)::value;
-          constexpr float kMost = 1024.f;
+          constexpr float kMost = 32768.f;  // 2^10, times 2^kShift
           uint32_t buf[2][32], pk[32];
           uint64_t sums[2] = {0, 0}, fit[TERMS + 1];
           float far = 0.f;
-          const uint64_t m2 = f2(-m, -m);
+          const uint64_t m2 = f2(kShift - m, kShift - m);
           const float c1 = TERMS == 0 ? (MOD == 0 ? k_exp : c_row * kLog2e) : inv, c2 = inv * inv;
           const uint64_t first = f2(c1, c1);
           if constexpr (TERMS == 4) {
@@ -315,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           for (int q = 0; q < 2; ++q) {
             if (q == 1) tmem_ld_wait32(buf[1]);
             const uint32_t(&v)[32] = buf[q];
-            [[maybe_unused]] const float bias = MOD == 2 ? slope * float(n0 + 32 * q - pos) - m : 0.f;
+            [[maybe_unused]] const float bias = MOD == 2 ? slope * float(n0 + 32 * q - pos) + (kShift - m) : 0.f;
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
               const uint64_t raw2 = f2(__uint_as_float(v[k]), __uint_as_float(v[k + 1]));
@@ -418,8 +425,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
             uint32_t u[16];
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
-              const float e0 = ex2(fmaf(__uint_as_float(buf[q][k]), k_exp, -m));
-              const float e1 = ex2(fmaf(__uint_as_float(buf[q][k + 1]), k_exp, -m));
+              const float e0 = ex2(fmaf(__uint_as_float(buf[q][k]), k_exp, kShift - m));
+              const float e1 = ex2(fmaf(__uint_as_float(buf[q][k + 1]), k_exp, kShift - m));
               sum[k & 2] += e0;
               sum[(k & 2) + 1] += e1;
               u[4 * ((k >> 1) & 3) + (k >> 3)] = h2_pack(e0, e1);
@@ -438,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       if (n > 0 && ok) ok = wait(o_done + t, 0);
       tc_fence_after();
       if (p.splits > 1) {
-        float* part = p.partials + ((int64_t(blockIdx.x) * p.splits + split) * kRows + r) * (D + 2);
+        float* part = p.partials + ((int64_t(blockIdx.x) * p.splits + split) * p.rows + r) * (D + 2);
 #pragma unroll
         for (int d = 0; d < D; d += 32) {
           float v[32];
@@ -525,49 +532,61 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
     }
     bool ok = true, flying = false;  // a copy that nothing has waited for, and its phase
     uint32_t phase = 0;
+    // Heads of 256 have no registers for a whole step: their values are read after the keys are done,
+    // and the next copy waits for that.
+    constexpr bool kLate = G == 8;
     for (int i = first; i < n; i += 2) {
-      const int st = i & 3;
-      const uint32_t par = (i >> 2) & 1;
+      const int sk_at = i % SK, sv_at = i % SV;
       const unsigned held = __shfl_sync(0xffffffffu, held_next, 0);
+      flying = false;
       if (!mbar_wait_inline(raw_full + dw, phase, &s_never)) {  // (its own copy: waited for whatever the others saw)
         if (lane == 0) atomicAdd(&g_paged_prompt_timeouts, 1);
         s_abort = 1;
-        flying = false;
         break;
       }
       phase ^= 1;
       uint32_t kw[2][2][G], vw[2][2][G], ks[2][2][(2 * G + 3) / 4], kz[2][2][(G + 3) / 4], vs[2][2][G], vz[2][2][(2 * G + 3) / 4];
+      auto values = [&]() {  // and the next step's copy
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint8_t* tp = buf + x * C::kTile;
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            lds<4 * G>(tp + L.v_codes() + y * L.block() + lane * 4 * G, vw[x][y]);
+            lds<4 * G>(tp + L.v_scales() + (cc + 4 * y) * 4 * G, vs[x][y]);
+            lds<2 * G>(tp + L.v_zeros() + (cc + 4 * y) * 2 * G, vz[x][y]);
+          }
+          if (!((held >> x) & 1u)) {  // no page: keys are masked, values have to be finite
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+              for (int q = 0; q < G; ++q) vs[x][y][q] = 0;
+          }
+        }
+        __syncwarp();
+        flying = i + 2 < n;
+        if (flying) {
+          issue(i + 2);
+          look(i + 4);
+        }
+      };
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const uint8_t* tp = buf + x * C::kTile;
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           lds<4 * G>(tp + L.k_codes() + y * L.block() + lane * 4 * G, kw[x][y]);
-          lds<4 * G>(tp + L.v_codes() + y * L.block() + lane * 4 * G, vw[x][y]);
           lds<2 * G>(tp + L.k_scales() + (g + 8 * y) * 2 * G, ks[x][y]);
           lds<G>(tp + L.k_zeros() + (g + 8 * y) * G, kz[x][y]);
-          lds<4 * G>(tp + L.v_scales() + (cc + 4 * y) * 4 * G, vs[x][y]);
-          lds<2 * G>(tp + L.v_zeros() + (cc + 4 * y) * 2 * G, vz[x][y]);
-        }
-        if (!((held >> x) & 1u)) {  // no page: keys are masked, values have to be finite
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int q = 0; q < G; ++q) vs[x][y][q] = 0;
         }
       }
-      __syncwarp();
-      flying = i + 2 < n;
-      if (flying) {
-        issue(i + 2);
-        look(i + 4);
-      }
+      if constexpr (!kLate) values();
 
       // ---- keys: [token][feature]
-      if (i >= kStages) ok = wait(k_empty + st, par ^ 1);
+      if (i >= SK) ok = wait(k_empty + sk_at, (i / SK - 1) & 1);
       if (!ok) break;
       if (lane == 0) s_held[i & 7][half] = int(held);
-      uint8_t* kd = sk + st * C::kK;
+      uint8_t* kd = sk + sk_at * C::kK;
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -588,12 +607,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(k_full + st);
+      if (lane == 0) mbar_arrive(k_full + sk_at);
+      if constexpr (kLate) values();
 
       // ---- values: [feature][token], tokens {2c, 2c+1, 2c+8, 2c+9, 2c+16, ...} of the 32 as chunk c
-      if (i >= kStages) ok = wait(v_empty + st, par ^ 1);
+      if (i >= SV) ok = wait(v_empty + (i - SV) % SE, ((i - SV) / SE) & 1);
       if (!ok) break;
-      uint8_t* vd = sv + st * C::kV;
+      uint8_t* vd = sv + sv_at * C::kV;
 #pragma unroll
       for (int q = 0; q < G; ++q) {
         uint32_t o[4][4];
@@ -617,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(v_full + st);
+      if (lane == 0) mbar_arrive(v_full + sv_at);
     }
     if (flying && !ok) mbar_wait_inline(raw_full + dw, phase, &s_never);
   } else {
@@ -636,31 +656,31 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
 #pragma unroll
       for (int k = 0; k < D / 16; ++k)
         mma_ss_one(ts + (i & 1) * 64, dq + (((k / 4) * C::kQAtom + (k % 4) * 32) >> 4),
-                   dk + (((i & 3) * C::kK + (k / 4) * C::kKAtom + (k % 4) * 32) >> 4), id_s, k > 0, one);
+                   dk + (((i % SK) * C::kK + (k / 4) * C::kKAtom + (k % 4) * 32) >> 4), id_s, k > 0, one);
       mma_commit_one(&s_full[t][i & 1], one);
-      mma_commit_one(k_empty + (i & 3), one);
+      mma_commit_one(k_empty + i % SK, one);
     };
     // every lane waits; the vote makes them agree
     auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
     bool ok = wait_all(&q_full, 0);
     for (int i = 0; i < 2 && i < n && ok; ++i) {
-      ok = wait_all(k_full + i, 0);
+      ok = wait_all(k_full + i, 0);  // (two stages at least)
       tc_fence_after();
       if (ok) scores(i);
     }
     for (int i = 0; i < n && ok; ++i) {
-      ok = wait_all(v_full + (i & 3), (i >> 2) & 1) && wait_all(&p_full[t][i & 1], (i >> 1) & 1);
+      ok = wait_all(v_full + i % SV, (i / SV) & 1) && wait_all(&p_full[t][i & 1], (i >> 1) & 1);
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
       for (int k = 0; k < kKeys / 16; ++k)
-        mma_ts_one(to, ts + (i & 1) * 64 + k * 8, dv + (((i & 3) * C::kV + k * 32) >> 4), id_o, i > 0 || k > 0, one);
+        mma_ts_one(to, ts + (i & 1) * 64 + k * 8, dv + (((i % SV) * C::kV + k * 32) >> 4), id_o, i > 0 || k > 0, one);
       mma_commit_one(o_full + t, one);
-      mma_commit_one(v_empty + (i & 3), one);
+      mma_commit_one(v_empty + i % SE, one);
       if (i + 1 == n) mma_commit_one(o_done + t, one);
       if (i + 2 < n) {
         // its weights have been read: scores may take their place
-        ok = wait_all(k_full + ((i + 2) & 3), ((i + 2) >> 2) & 1) && wait_all(o_full + t, i & 1);
+        ok = wait_all(k_full + (i + 2) % SK, ((i + 2) / SK) & 1) && wait_all(o_full + t, i & 1);
         if (!ok) break;
         tc_fence_after();
         scores(i + 2);
@@ -692,8 +712,8 @@ __global__ void __launch_bounds__(256) paged_prompt_join_kernel(PromptParams p) 
   if (!item_of(p, blockIdx.x, 0, it)) return;
   const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
   if (r >= it.rows) return;
-  const float* part = p.partials + (int64_t(blockIdx.x) * p.splits * kRows + r) * (D + 2);
-  const int64_t step = int64_t(kRows) * (D + 2);
+  const float* part = p.partials + (int64_t(blockIdx.x) * p.splits * p.rows + r) * (D + 2);
+  const int64_t step = int64_t(p.rows) * (D + 2);
   float top = kNone, sum = 0.f, acc[G];
 #pragma unroll
   for (int q = 0; q < G; ++q) acc[q] = 0.f;
@@ -760,7 +780,8 @@ int launch_one(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
   PromptParams p;
   p.a = a;
   p.min_rows = min_rows;
-  p.row_tiles = int((int64_t(a.c.max_q) * a.group + kRows - 1) / kRows);
+  p.rows = 128 * C::kTiles;
+  p.row_tiles = int((int64_t(a.c.max_q) * a.group + p.rows - 1) / p.rows);
   const int64_t items = int64_t(p.row_tiles) * a.c.batch * a.c.kv_heads;
   if (items > INT32_MAX) return SPECTRA_ERR_SHAPE;
   // four steps of keys a split at least
@@ -768,11 +789,11 @@ int launch_one(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
   p.splits = int(std::max<int64_t>(1, std::min<int64_t>(most, device_sms(dev) / items)));
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + kPagedCounterBytes);
   if (p.splits > 1 &&
-      a.workspace_bytes < kPagedCounterBytes + size_t(items) * p.splits * kRows * (C::D + 2) * sizeof(float))
+      a.workspace_bytes < kPagedCounterBytes + size_t(items) * p.splits * p.rows * (C::D + 2) * sizeof(float))
     return SPECTRA_ERR_WORKSPACE;
   const int status = launch_dep(kern, dim3(unsigned(items), unsigned(p.splits)), kThreads, C::kSmem, p, st);
   if (status != SPECTRA_OK || p.splits == 1) return status;
-  return launch_dep(paged_prompt_join_kernel<BF16, G>, dim3(unsigned(items), kRows / 8), 256, 0, p, st);
+  return launch_dep(paged_prompt_join_kernel<BF16, G>, dim3(unsigned(items), unsigned(p.rows / 8)), 256, 0, p, st);
 }
 
 template <bool BF16, int G>
@@ -788,6 +809,7 @@ int launch_dim(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
     case 64: return launch_mod<BF16, 2>(a, min_rows, st);
     case 96: return launch_mod<BF16, 3>(a, min_rows, st);
     case 128: return launch_mod<BF16, 4>(a, min_rows, st);
+    case 256: return launch_mod<BF16, 8>(a, min_rows, st);
   }
   return SPECTRA_ERR_UNSUPPORTED;
 }
@@ -810,15 +832,14 @@ int launch_paged_prompt(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
 //   keys   1 sequence, 64 rows   96 rows       16 sequences, 32 rows   64 rows
 //   1024   13.3 / 17.1           19.4 / 18.2   27.7 / 25.1             44.3 / 25.8
 //   8192   27.9 / 33.5           33.7 / 34.9   107 / 134               200 / 136
-// (few CTAs have to split the keys, which paged_attn does at a finer grain).  Heads of 256 have
-// no room in TMEM and shared memory here.
+// (few CTAs have to split the keys, which paged_attn does at a finer grain).
 int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
   int dev = 0;
   const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e);
   const bool many = int64_t(a.c.batch) * a.c.kv_heads * 2 >= device_sms(dev);
   const int few = many ? 32 : 96;
-  if (int64_t(a.c.max_q) * a.group <= few || a.c.head_dim > 128) return launch_paged_attn(a, INT32_MAX, st);
+  if (int64_t(a.c.max_q) * a.group <= few) return launch_paged_attn(a, INT32_MAX, st);
   if (!a.c.cu_q) return launch_paged_prompt(a, 0, st);
   const int status = launch_paged_attn(a, few, st);
   return status != SPECTRA_OK ? status : launch_paged_prompt(a, few, st);

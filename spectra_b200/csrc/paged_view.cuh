@@ -52,6 +52,10 @@ __device__ __forceinline__ uint8_t* tile_of(const PagedView& c, int b, int h, in
 // Scores are kept in powers of two.  A running maximum is raised when a score
 // passes it by more than kLazy.
 constexpr float kLazy = 8.f;
+// Weights are kept times 2^kShift (their sums too, so nothing else changes): the
+// largest still fit fp16, and the smallest that fp16 holds as normal numbers lie
+// 2^-19 below the maximum's.
+constexpr float kShift = 5.f;
 constexpr float kNone = -1e30f;  // below every score that is seen
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -314,6 +314,29 @@ def test_attention_one_prompt(n, heads, kv_heads, dim):
     run_masked(st, q, "plain")
 
 
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 4), (128, 8, 4), (256, 4, 4), (256, 8, 2)])
+@pytest.mark.parametrize("mask", ["plain", "all"])
+def test_attention_prompts_of_many_sequences(dim, heads, kv_heads, mask):
+    """Enough (sequence, head) pairs that no keys are split; chunks that look back, odd lengths, long sequences
+    beside single tokens."""
+    lens = [200, 129, 65, 331, 97, 128, 193, 64, 250, 130, 77, 160, 140, 99, 201, 127, 180, 1, 300, 150]
+    news = [n if i % 3 else max(1, n // 2) for i, n in enumerate(lens)]
+    news[5], news[8] = 1, 3
+    st = Step(lens, news, heads, kv_heads, dim, 32, "bf16", seed=12)
+    st.fill()
+    q = draw((st.total, heads, dim), 91, "bf16").to(DEV)
+    run_masked(st, q, mask)
+
+
+def test_attention_wide_heads_prompt_and_repeatable_bits():
+    st = Step([901], [700], 6, 2, 256, 64, "f16", seed=13)
+    st.fill()
+    q = draw((700, 6, 256), 92, "f16").to(DEV)
+    out = run_masked(st, q, "cap")
+    for _ in range(3):
+        assert torch.equal(out, PG.paged_attention(q, st.cache, st.batch, softcap=5.0))
+
+
 def test_attention_long_sequence_is_split_and_repeatable():
     st = Step([20011, 3, 7000], [1] * 3, 8, 2, 128, 64, "bf16", seed=1)
     st.fill()
