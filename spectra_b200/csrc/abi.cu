@@ -523,6 +523,7 @@ int spectra_paged_attention(const SpectraPagedCache* cache, const SpectraTokenBa
   if (st != SPECTRA_OK) return st;
   if (!is_half_dt(dtype)) return SPECTRA_ERR_DTYPE;
   if (q_heads <= 0 || q_heads > 65535 || q_heads % cache->kv_heads != 0 || window < 0) return SPECTRA_ERR_SHAPE;
+  if (batch->max_q > (INT32_MAX - 4096) / q_heads) return SPECTRA_ERR_SHAPE;  // rows of a sequence are counted in 32 bits
   if (!(scale > 0.f) || !std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap)) return SPECTRA_ERR_UNSUPPORTED;
   if (empty) return SPECTRA_OK;
   if (!q || !out || !workspace) return SPECTRA_ERR_NULL_POINTER;

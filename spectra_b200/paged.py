@@ -291,7 +291,9 @@ def paged_kv_read(cache: PagedKVCache, batch: TokenBatch, dtype: torch.dtype = t
 # Partial results of split sequences, one buffer per (device, stream, head_dim):
 # calls on one stream never overlap.  Zeroed once; every call leaves its
 # counters zero.  The size does not depend on the batch, so a buffer is never
-# replaced and a captured graph's address stays good.
+# replaced and a captured graph's address stays good (a graph holds the buffer
+# of the stream it was captured on: its replays must not overlap other calls of
+# that stream).
 _WORKSPACES: dict = {}
 
 

@@ -130,6 +130,12 @@ def test_attention_refuses(kw, code):
     assert attend(cache(), batch(), **kw) == code
 
 
+def test_attention_refuses_rows_that_32_bits_do_not_count():
+    b = batch(cu_q=P, total=1 << 30, max_q=1 << 30)
+    assert attend(cache(), b) == L.ERR_SHAPE
+    assert attend(cache(kv_heads=1, page_stride=4 * 1216), b, q_heads=2) == L.ERR_SHAPE
+
+
 def test_read_refuses():
     assert read(cache(), batch(), dt=L.DT_I32) == L.ERR_DTYPE
     assert read(cache(), batch(), k=None) == L.ERR_NULL_POINTER
