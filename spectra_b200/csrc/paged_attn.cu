@@ -34,6 +34,12 @@
 // end, are dealt to the CTAs in equal contiguous shares, whatever the lengths
 // of the sequences; a segment that several CTAs share is put together by the
 // last of them to finish, always in the same order.
+//
+// Measured: one token over 131072, 32 query heads on 8, heads of 128, 48.6
+// us (3.3 TB/s); one token of 64 ragged sequences up to 8192, 64 on 8, 97.6 us
+// (3.8 TB/s); one over 1024 9 us, nearly all of it launch and latency.  Long
+// caches are bound by the unpacking instructions (about 390 a tile of 16 tokens,
+// a third of them for scales and zero points).
 #include <math.h>
 
 #include <algorithm>

@@ -1,4 +1,4 @@
-"""The paged INT4 KV cache (csrc/paged_kv.cu, csrc/paged_attn.cu)
+"""The paged INT4 KV cache (csrc/paged_kv.cu, paged_attn.cu, paged_prompt.cu)
 against the oracle (oracle/paged.py): appended bytes and rotated queries bit
 for bit, attention within a bound derived from its roundings."""
 import numpy as np
