@@ -44,6 +44,7 @@
 
 #include <algorithm>
 
+#include "copy_ring.h"
 #include "gemv_mma.cuh"
 #include "paged_view.cuh"
 #include "sm100_ptx.cuh"
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
   __shared__ long long s_scan[kWarps];
   __shared__ long long s_base;
   __shared__ int s_seq, s_last;
-  __shared__ volatile int s_stop;     // a copy did not arrive: no further ones
+  __shared__ volatile int s_stop;     // a copy did not arrive: the segments after this one load nothing
   __shared__ int s_held[kWarps * kStages];  // tiles of a stage that a page holds
   __shared__ volatile int s_never;    // 0: each warp waits for its own copies, whatever the others saw
 
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
 
   const bool bf16 = a.dtype == SPECTRA_DT_BF16;
   const int per_page = 1 << (c.page_log2 - 4);  // tiles
-  uint32_t phase = 0;  // a bit for each stage
+  CopyRing<kStages> ring_order;
   const uint32_t magic = fp16_1024();
   long long at = begin;
 
@@ -232,7 +233,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
     const int head = seg / s.tiles, row0 = (seg - head * s.tiles) * ROWS;
     const int u_begin = s.unit0 + int(at - seg_begin);
     const int u_stop = s.unit0 + int((seg_end < end ? seg_end : end) - seg_begin);
-    const int u_end = s.len > 0 ? u_stop : u_begin;  // (nothing held: nothing to load)
+    // nothing held, or a copy that did not arrive in an earlier segment: nothing to load.  (After a
+    // loss the results are undefined, but every segment is counted, so that the counters end at zero.)
+    const int u_end = s.len > 0 && !s_stop ? u_stop : u_begin;
     const int rows = min(ROWS, s.count * a.group - row0);
 
     // ---- units to load: warp w takes u_end - 1 - w, - kWarps, ... (the last keys first: a
@@ -278,10 +281,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
     };
     look(0, here, here1);
     if (next - 32 * kWarps >= u_begin) look(32, ahead, ahead1);
-#pragma unroll
-    for (int st = 0; st < kStages; ++st) {
-      if (next - st * kWarps >= u_begin) issue(st, st);
-    }
+    ring_order.start(next >= u_begin ? (next - u_begin) / kWarps + 1 : 0, issue);
 
     // ---- query fragments: the products' B registers and the groups' sums.  Four
     // lanes a row; every warp reads whole rows and prepares some of their groups.
@@ -386,12 +386,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
 #pragma unroll
       for (int j = 0; j < 2; ++j) c_exp[nt][j] = MOD ? 1.f : factor[nt * 8 + 2 * cc + j] * kLog2e;
 
-    int stage = 0, unit = 0;
-    for (int u = next; u >= u_begin; u -= kWarps, ++unit) {
-      if (!sm100::mbar_wait(bars + warp * kStages + stage, (phase >> stage) & 1u, &s_never)) {
+    auto arrived = [&](int stage, uint32_t parity) {  // (the vote makes the lanes agree)
+      const bool ok = __all_sync(0xffffffffu, sm100::mbar_wait(bars + warp * kStages + stage, parity, &s_never));
+      if (!ok && lane == 0) atomicAdd(&g_paged_attn_timeouts, 1);
+      return ok;
+    };
+    for (int u = next; ring_order.more(); u -= kWarps) {
+      if (!ring_order.take(arrived)) {
         s_stop = 1;
-        if (lane == 0) atomicAdd(&g_paged_attn_timeouts, 1);
+        break;
       }
+      const int stage = ring_order.stage;
       const int held = s_held[warp * kStages + stage];
       const uint8_t* buf = ring + (warp * kStages + stage) * C::kStage;
 
@@ -547,9 +552,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
         }
       }
       __syncwarp();
-      phase ^= 1u << stage;
-      if (u - kStages * kWarps >= u_begin && !s_stop) issue(unit + kStages, stage);
-      stage = stage + 1 == kStages ? 0 : stage + 1;
+      ring_order.next(issue);
     }
 
     // ---- the warps' results become one
