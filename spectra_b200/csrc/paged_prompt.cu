@@ -192,8 +192,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
   const uint32_t tmem = same(s_tmem);
   const int n = same(it.steps);
 
+  // A whole warp waits, and the vote makes its lanes agree: one may see a phase complete, or the
+  // abort, a poll later than the next, and lanes that part here would miss each other at the votes
+  // and the warp-wide TMEM accesses that follow.
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    if (mbar_wait_inline(bar, parity, &s_abort)) return true;
+    if (__all_sync(0xffffffffu, mbar_wait_inline(bar, parity, &s_abort))) return true;
     if (!s_abort) {
       s_abort = 1;
       if (lane == 0) atomicAdd(&g_paged_prompt_timeouts, 1);
@@ -551,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       const int sk_at = i % SK, sv_at = i % SV;
       const unsigned held = __shfl_sync(0xffffffffu, held_next, 0);
       flying = false;
-      if (!mbar_wait_inline(raw_full + dw, phase, &s_never)) {  // (its own copy: waited for whatever the others saw)
+      if (!__all_sync(0xffffffffu, mbar_wait_inline(raw_full + dw, phase, &s_never))) {  // (its own copy: waited for whatever the others saw)
         if (lane == 0) atomicAdd(&g_paged_prompt_timeouts, 1);
         s_abort = 1;
         break;
@@ -672,16 +675,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       mma_commit_one(&s_full[t][i & 1], one);
       mma_commit_one(k_empty + i % SK, one);
     };
-    // every lane waits; the vote makes them agree
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
-    bool ok = wait_all(&q_full, 0);
+    bool ok = wait(&q_full, 0);
     for (int i = 0; i < 2 && i < n && ok; ++i) {
-      ok = wait_all(k_full + i, 0);  // (two stages at least)
+      ok = wait(k_full + i, 0);  // (two stages at least)
       tc_fence_after();
       if (ok) scores(i);
     }
     for (int i = 0; i < n && ok; ++i) {
-      ok = wait_all(v_full + i % SV, (i / SV) & 1) && wait_all(&p_full[t][i & 1], (i >> 1) & 1);
+      ok = wait(v_full + i % SV, (i / SV) & 1) && wait(&p_full[t][i & 1], (i >> 1) & 1);
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
@@ -692,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       if (i + 1 == n) mma_commit_one(o_done + t, one);
       if (i + 2 < n) {
         // its weights have been read: scores may take their place
-        ok = wait_all(k_full + (i + 2) % SK, ((i + 2) / SK) & 1) && wait_all(o_full + t, i & 1);
+        ok = wait(k_full + (i + 2) % SK, ((i + 2) / SK) & 1) && wait(o_full + t, i & 1);
         if (!ok) break;
         tc_fence_after();
         scores(i + 2);
