@@ -89,8 +89,7 @@ __device__ __forceinline__ Span span_of(const AttnParams& p, int b) {
   s.pos0 = len - s.count;
   s.len = len < 0 ? 0 : (len < a.c.limit ? len : a.c.limit);
   s.tiles = s.count * a.group > p.max_rows ? 0 : (s.count * a.group + ROWS - 1) / ROWS;
-  const int lo = a.window > 0 ? max(0, s.pos0 - a.window + 1) : 0;
-  s.unit0 = lo / kUnit;
+  s.unit0 = first_key(s.pos0, a.window) / kUnit;
   s.units = max(1, (s.len + kUnit - 1) / kUnit - s.unit0);
   return s;
 }
@@ -357,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
         const int tok = (row0 + tid) / a.group, h = head * a.group + (row0 + tid) - tok * a.group;
         pos = s.pos0 + tok;
         if (pos >= 0) hi = a.causal ? min(s.len, pos + 1) : s.len;
-        if (a.window > 0) lo = max(0, pos - a.window + 1);
+        lo = first_key(pos, a.window);
         if (a.slopes) slope = a.slopes[h] * kLog2e;
       }
       meta[tid] = make_int4(hi, lo, __float_as_int(slope), pos);

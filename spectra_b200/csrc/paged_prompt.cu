@@ -111,7 +111,7 @@ __device__ __forceinline__ bool item_of(const PromptParams& p, int index, int sp
   it.len = len < 0 ? 0 : (len < c.limit ? len : c.limit);
   const int p0 = it.pos0 + it.row0 / p.a.group, p1 = it.pos0 + (it.row0 + it.rows - 1) / p.a.group;
   const int hi = p1 < 0 ? 0 : (p.a.causal ? min(it.len, p1 + 1) : it.len);
-  const int lo = p.a.window > 0 ? max(0, p0 - p.a.window + 1) : 0;
+  const int lo = first_key(p0, p.a.window);
   const int s0 = lo / kKeys, s1 = (hi + kKeys - 1) / kKeys;
   const int n = hi > lo ? s1 - s0 : 0;
   it.step0 = s0 + int((int64_t(n) * split) / p.splits);
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       int hi = 0x7FFFFFFF, lo = 0;  // keys this row sees
       if (real) {
         hi = pos < 0 ? 0 : (a.causal ? min(it.len, pos + 1) : it.len);
-        if (a.window > 0) lo = max(0, pos - a.window + 1);
+        lo = first_key(pos, a.window);
       }
       const float slope = MOD == 2 ? a.slopes[h] * kLog2e : 0.f;
       const float inv = MOD != 0 && a.softcap > 0.f ? c_row / a.softcap : 0.f;

@@ -49,6 +49,10 @@ __device__ __forceinline__ uint8_t* tile_of(const PagedView& c, int b, int h, in
   return c.pool + page * c.page_stride + (int64_t(h) * tiles + tile) * L.bytes();
 }
 
+// First key that a row at `pos` may see (window 0: none; pos negative: padding).  Any window up to
+// INT32_MAX: nothing is computed that 32 bits do not hold.
+__device__ __forceinline__ int first_key(int pos, int window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
+
 // Scores are kept in powers of two.  A running maximum is raised when a score
 // passes it by more than kLazy.
 constexpr float kLazy = 8.f;

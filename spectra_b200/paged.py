@@ -350,6 +350,6 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, *, 
             raise ValueError("out must have q's dtype and unit stride along a head")
     ws, nbytes = _workspace(index, cache.head_dim)
     _call(index, "spectra_paged_attention", cache._at, batch._at, _DT[q.dtype], heads, q.data_ptr(), q_ts, q_hs,
-          out.data_ptr(), o_ts, o_hs, scale, softcap, None if slopes is None else slopes.data_ptr(), causal, window,
-          ws, nbytes)
+          out.data_ptr(), o_ts, o_hs, scale, softcap, None if slopes is None else slopes.data_ptr(), causal,
+          min(window, 2**31 - 1), ws, nbytes)
     return out
