@@ -115,7 +115,7 @@ def attention(q: np.ndarray, k: np.ndarray, v: np.ndarray, held: np.ndarray, ste
         if causal:
             see &= idx <= pos[i]
         if window:
-            see &= idx > pos[i] - window
+            see &= idx > max(int(pos[i]) - int(window), -1)  # (any window: numpy's integers have 64 bits)
         if not see.any():
             continue
         for h in range(Hq):
