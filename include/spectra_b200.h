@@ -334,15 +334,18 @@ SPECTRA_API int spectra_paged_kv_read(const SpectraPagedCache* cache, const Spec
  * A row that sees no key is 0; rows >= cu_q[batch] are 0.
  *   q, out [total][q_heads][D], element strides, dtype F16 or BF16;
  *   slopes fp32 [q_heads] or NULL; scale > 0.
- *   workspace: spectra_paged_attention_workspace_bytes(head_dim) bytes, zeroed
- *          once before its first use, 16-byte aligned; calls that share one
- *          must not overlap in time.
+ *   workspace: spectra_paged_attention_workspace_bytes(head_dim) bytes, of which
+ *          the first SPECTRA_PAGED_COUNTER_BYTES are zero before its first use
+ *          (every call leaves them zero), 16-byte aligned; calls that share one,
+ *          replays of captured ones among them, must not overlap in time.
  */
 SPECTRA_API int spectra_paged_attention(
     const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
     const void* q, int64_t q_ts, int64_t q_hs, void* out, int64_t o_ts, int64_t o_hs,
     float scale, float softcap, const float* slopes, int causal, int64_t window,
     void* workspace, size_t workspace_bytes, void* stream);
+
+#define SPECTRA_PAGED_COUNTER_BYTES 4096
 
 SPECTRA_API size_t spectra_paged_attention_workspace_bytes(int64_t head_dim);
 
@@ -435,6 +438,14 @@ SPECTRA_API int spectra_p2p_allgather(const void* src, void* const* peer_buffers
  * must be discarded.
  */
 SPECTRA_API int spectra_device_timeouts(int64_t* count, int reset);
+
+/*
+ * Not a reference interface: a number of the CUDA graph capture that `stream`
+ * is part of, different from every other capture's in this process; 0 if it is
+ * not being captured.  What a host keeps between calls (a zeroed workspace) it
+ * must not make inside a capture.
+ */
+SPECTRA_API uint64_t spectra_stream_capture_id(void* stream);
 
 /*
  * Self-test of the bounded wait (not a reference interface): launches one

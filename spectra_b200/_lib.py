@@ -6,7 +6,7 @@ fallback: if it is missing, every kernel call raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("libspectra_b200.so")
@@ -18,6 +18,7 @@ OK = 0
 ERR_NULL_POINTER, ERR_SHAPE, ERR_STRIDE, ERR_ALIGNMENT, ERR_DTYPE, ERR_WORKSPACE, ERR_CUDA, ERR_UNSUPPORTED = range(1, 9)
 ABI_VERSION = 1
 P2P_STATE_INTS = 128  # SPECTRA_P2P_STATE_INTS
+PAGED_COUNTER_BYTES = 4096  # SPECTRA_PAGED_COUNTER_BYTES
 P2P_SIGNAL_BYTES = 8 * 128 * 4  # epoch flags [rank][cta] at the start of an exchange buffer
 
 
@@ -118,6 +119,7 @@ PROTOTYPES = {
                                       c_int64, c_void_p, c_int, c_int, c_int64, c_void_p]),
     "spectra_device_timeouts": (c_int, [c_void_p, c_int]),
     "spectra_selftest_wait_timeout": (c_int, [c_void_p]),
+    "spectra_stream_capture_id": (c_uint64, [c_void_p]),
     "spectra_w4a16_dequant": (c_int, [
         c_void_p, c_int64,
         c_void_p, c_int64, c_int64,

@@ -347,6 +347,17 @@ int spectra_p2p_allgather(const void* src, void* const* peer_buffers, int64_t bu
   return launch_p2p_allgather(a, static_cast<cudaStream_t>(stream));
 }
 
+uint64_t spectra_stream_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id);
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // (the legacy stream while another is being captured: it is not)
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 int spectra_selftest_wait_timeout(void* stream) { return launch_selftest_wait(static_cast<cudaStream_t>(stream)); }
 
 int spectra_quantize_group32(

@@ -74,7 +74,7 @@ struct PagedAttnArgs {
   void* workspace; size_t workspace_bytes;
 };
 // A workspace: kPagedCounterBytes of counters (zero between calls), then partial results.
-constexpr size_t kPagedCounterBytes = 4096;
+constexpr size_t kPagedCounterBytes = SPECTRA_PAGED_COUNTER_BYTES;
 // One or a few tokens per sequence (paged_attn.cu); many (paged_prompt.cu).
 // Sequences with more than max_rows (the first) or at most min_rows (the
 // second) rows per key/value head are left to the other.

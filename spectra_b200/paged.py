@@ -27,6 +27,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib as L
+from . import _workspace as W
 
 GROUP = 32
 TILE_TOKENS = 16
@@ -288,21 +289,24 @@ def paged_kv_read(cache: PagedKVCache, batch: TokenBatch, dtype: torch.dtype = t
     return k, v
 
 
-# Partial results of split sequences, one buffer per (device, stream, head_dim):
-# calls on one stream never overlap.  Zeroed once; every call leaves its
-# counters zero.  The size does not depend on the batch, so a buffer is never
-# replaced and a captured graph's address stays good (a graph holds the buffer
-# of the stream it was captured on: its replays must not overlap other calls of
-# that stream).
+# Partial results of split sequences, one buffer per (device, stream, head_dim),
+# kept for the process: calls on one stream never overlap.  Zeroed once; every
+# call leaves its counters zero.  The size does not depend on the batch, so a
+# buffer is never replaced and a captured graph's address stays good.  A capture
+# on a stream that has none gets its own (_workspace.py).
 _WORKSPACES: dict = {}
 
 
 def _workspace(index: int, head_dim: int) -> Tuple[int, int]:
-    key = (index, torch._C._cuda_getCurrentRawStream(index), head_dim)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    key = (index, stream, head_dim)
     ws = _WORKSPACES.get(key)
     if ws is None:
-        nbytes = L.lib().spectra_paged_attention_workspace_bytes(head_dim)
-        buf = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+        nbytes, dev = L.lib().spectra_paged_attention_workspace_bytes(head_dim), torch.device("cuda", index)
+        buf = W.captured(dev, stream, ("paged", head_dim), nbytes, L.PAGED_COUNTER_BYTES)
+        if buf is not None:
+            return buf.data_ptr(), nbytes
+        buf = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
         ws = _WORKSPACES[key] = (buf.data_ptr(), nbytes, buf)
     return ws[0], ws[1]
 
@@ -318,7 +322,13 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, *, 
     1 / sqrt(D)) times the products, then ``softcap * tanh(score / softcap)``,
     then plus ``alibi_slopes[h] * (n - p)`` (fp32 [q_heads]).  q_heads is a
     multiple of kv_heads; consecutive heads share one.  A row that sees no key
-    is 0.  Scores, softmax statistics and sums are fp32."""
+    is 0.  Scores, softmax statistics and sums are fp32.
+
+    Partial results lie in a workspace of the current stream (17 MB for heads of
+    128, kept for the process).  A graph captured on a stream that has called
+    this before holds that stream's: do not let its replays overlap other calls
+    of that stream, or replays of another graph captured there.  Captured on a
+    stream that has not, it holds its own."""
     index = cache._index
     if batch._index != index:
         _other_device()
