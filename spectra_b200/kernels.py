@@ -26,6 +26,7 @@ from typing import Optional
 import torch
 
 from . import _lib as L
+from . import _workspace as W
 
 _DT = {torch.float16: L.DT_F16, torch.bfloat16: L.DT_BF16, torch.float32: L.DT_F32,
        torch.int32: L.DT_I32, torch.int64: L.DT_I64}
@@ -151,7 +152,8 @@ def fused_w4a16_gemv_hdsq(
 # every GEMM call leaves its counters zero again.  A workspace that grows is
 # replaced, but the old buffer is kept alive: a CUDA graph captured earlier on
 # the same stream still holds its address, and replaying that graph must not
-# write into memory the caching allocator has handed to another tensor.
+# write into memory the caching allocator has handed to another tensor.  A
+# captured call that finds none large enough gets its capture's (_workspace.py).
 _WORKSPACES: dict = {}
 _RETIRED_WORKSPACES: list = []
 
@@ -160,6 +162,9 @@ def _workspace(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     key = (dev.index, stream)
     ws = _WORKSPACES.get(key)
     if ws is None or ws.numel() < nbytes:
+        own = W.captured(dev, stream, "gemm", max(nbytes, 1 << 20), max(nbytes, 1 << 20))
+        if own is not None:
+            return own
         if ws is not None:
             _RETIRED_WORKSPACES.append(ws)
         ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=dev)

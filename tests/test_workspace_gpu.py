@@ -4,7 +4,9 @@ import pytest
 import torch
 
 from spectra_b200 import _lib as L
+from spectra_b200 import kernels as SK
 from spectra_b200 import paged as PG
+from tests.helpers import act, random_format
 from tests.test_paged_gpu import DEV, Step, draw
 
 pytestmark = pytest.mark.gpu
@@ -85,3 +87,30 @@ def test_graphs_of_paged_attention_with_their_own_workspaces_may_overlap():
         torch.cuda.synchronize()
         for _, outs in graphs:
             assert all(torch.equal(o, want) for o in outs)
+
+
+def test_split_gemm_captured_on_a_stream_without_a_large_enough_workspace():
+    def problem(M, N, K, seed):
+        fmt = random_format(N, K, 0, seed=seed, ow_dtype="bf16")
+        w = [torch.from_numpy(fmt[n]).to(DEV) for n in ("packed", "scales", "zeros")]
+        a = act(M, K, seed=seed + 1, dtype="bf16").to(DEV)
+        assert L.lib().spectra_w4a16_gemm_workspace_bytes(M, N, K, 0) > 0
+        return lambda: SK.batched_w4a16_gemm(a, *w, marlin_layout=True)
+
+    small, large = problem(16, 256, 16384, 41), problem(256, 1024, 4096, 43)  # (over 1 MB of partials)
+    want = [small(), large()]
+    p = DirtyPool()
+    a, out_a = p.capture(lambda: [small()])
+    b, out_b = p.capture(lambda: [small(), large()])
+    with torch.cuda.stream(p.stream):
+        eager = small()  # before any replay
+    torch.cuda.synchronize()
+    assert torch.equal(eager, want[0])
+    c, out_c = p.capture(lambda: [large(), small()])  # the stream's own is too small for the first
+    torch.cuda.synchronize()
+    for graph, outs, wants in ((c, out_c, want[::-1]), (b, out_b, want), (a, out_a, want[:1]), (b, out_b, want)):
+        for o in outs:
+            o.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, wants))
