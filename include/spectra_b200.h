@@ -271,7 +271,8 @@ SPECTRA_API int spectra_kv_dequantize(const uint8_t* packed, const uint16_t* sca
  * The batch: sequence b holds seq_lens[b] tokens, its new ones included, in
  * pages block_tables[b * table_stride + position / page_size]; its new tokens
  * are rows cu_q[b] .. cu_q[b + 1] of the token tensors (cu_q NULL: q_len rows
- * each) and have its last positions.  `total` rows in all, at most max_q of one sequence.
+ * each) and have its last positions.  `total` rows in all; max_q bounds the
+ * rows of one sequence in cu_q (the attention's results of rows past it are 0).
  * max_len bounds seq_lens: positions from min(max_len, width * page_size) on
  * are not touched.  A new token of negative position is padding (a slot of the
  * batch that holds no sequence has seq_lens 0).  A page number outside

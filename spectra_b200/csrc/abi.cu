@@ -468,7 +468,7 @@ int paged_view(const SpectraPagedCache* c, const SpectraTokenBatch* b, PagedView
   v.batch = int(b->batch);
   v.total = b->total;
   v.q_len = b->cu_q ? 0 : int(std::min<int64_t>(b->q_len, b->total));
-  v.max_q = int(std::min<int64_t>(b->max_q, b->total));
+  v.max_q = b->cu_q ? int(std::min<int64_t>(b->max_q, b->total)) : v.q_len;
   v.limit = c->num_pages == 0 ? 0 : int(std::min<int64_t>(b->max_len, std::min<int64_t>(b->width, INT32_MAX / P) * P));
   return SPECTRA_OK;
 }
@@ -534,7 +534,8 @@ int spectra_paged_attention(const SpectraPagedCache* cache, const SpectraTokenBa
   if (st != SPECTRA_OK) return st;
   if (!is_half_dt(dtype)) return SPECTRA_ERR_DTYPE;
   if (q_heads <= 0 || q_heads > 65535 || q_heads % cache->kv_heads != 0 || window < 0) return SPECTRA_ERR_SHAPE;
-  if (batch->max_q > (INT32_MAX - 4096) / q_heads) return SPECTRA_ERR_SHAPE;  // rows of a sequence are counted in 32 bits
+  const int64_t most = batch->cu_q ? batch->max_q : std::min(batch->q_len, batch->total);
+  if (most > (INT32_MAX - 4096) / q_heads) return SPECTRA_ERR_SHAPE;  // rows of a sequence are counted in 32 bits
   if (!(scale > 0.f) || !std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap)) return SPECTRA_ERR_UNSUPPORTED;
   if (empty) return SPECTRA_OK;
   if (!q || !out || !workspace) return SPECTRA_ERR_NULL_POINTER;

@@ -36,7 +36,7 @@ struct PagedView {
   const int* cu_q;           // [batch + 1], or NULL: every sequence has q_len new tokens
   int batch, q_len;
   int64_t total;             // new tokens of the batch
-  int max_q;                 // most new tokens of one sequence
+  int max_q;                 // most new tokens of one sequence (the host's bound: the attention keeps to it)
   int limit;                 // positions past this are not touched: min(max_len, width * page)
 };
 

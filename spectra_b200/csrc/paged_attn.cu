@@ -72,7 +72,8 @@ struct AttnParams {
 // ------------------------------------------------------------ the batch
 struct Span {  // a sequence's rows and the keys its rows look at
   int64_t first;  // first new token
-  int count;      // new tokens
+  int count;      // new tokens, up to max_q
+  int extra;      // new tokens past max_q
   int len;        // keys (cut to the batch's limit)
   int pos0;       // position of the first new token
   int unit0;      // first unit that any row looks at
@@ -84,9 +85,9 @@ template <int ROWS>
 __device__ __forceinline__ Span span_of(const AttnParams& p, int b) {
   const PagedAttnArgs& a = p.a;
   Span s;
-  new_tokens(a.c, b, s.first, s.count);
+  new_rows(a.c, b, s.first, s.count, s.extra);
   const int len = a.c.seq_lens[b];
-  s.pos0 = len - s.count;
+  s.pos0 = len - s.count - s.extra;
   s.len = len < 0 ? 0 : (len < a.c.limit ? len : a.c.limit);
   s.tiles = s.count * a.group > p.max_rows ? 0 : (s.count * a.group + ROWS - 1) / ROWS;
   s.unit0 = first_key(s.pos0, a.window) / kUnit;
@@ -149,9 +150,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
   sm100::pdl_trigger();
 
   // ---- this CTA's share of the units
+  bool over = false;  // a sequence has more new tokens than max_q
   auto units_of = [&](int i) -> long long {
     if (i >= c.batch) return 0;
     const Span s = span_of<ROWS>(p, i);
+    over = over || s.extra > 0;
     return (long long)(s.units) * s.tiles * c.kv_heads;
   };
   const long long first_units = units_of(tid);  // (the only ones of a batch of up to kThreads)
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
 #pragma unroll
   for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) s_scan[warp] = total;
-  __syncthreads();
+  over = __syncthreads_or(over);
   total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) total += s_scan[w];
@@ -170,13 +173,21 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
   const long long begin = share * blockIdx.x;
   const long long end = begin + share < total ? begin + share : total;
 
-  // rows that belong to no sequence
+  // rows that belong to no sequence, or lie past max_q
   if (c.cu_q) {
-    const int held = c.cu_q[c.batch];
     const int64_t row_words = int64_t(a.q_heads) * D;
-    for (int64_t t = (held < 0 ? 0 : held) + int64_t(blockIdx.x); t < c.total; t += gridDim.x)
+    auto clear = [&](int64_t t) {
       for (int64_t i = tid; i < row_words; i += kThreads)
         reinterpret_cast<uint16_t*>(a.out)[t * a.o_ts + (i / D) * a.o_hs + i % D] = 0;
+    };
+    const int held = c.cu_q[c.batch];
+    for (int64_t t = (held < 0 ? 0 : held) + int64_t(blockIdx.x); t < c.total; t += gridDim.x) clear(t);
+    if (over) {
+      for (int i = blockIdx.x; i < c.batch; i += gridDim.x) {
+        const Span s = span_of<ROWS>(p, i);
+        for (int64_t t = s.first + s.count; t < s.first + s.count + s.extra; ++t) clear(t);
+      }
+    }
   }
   if (begin >= end) return;
 

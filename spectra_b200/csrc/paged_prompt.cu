@@ -100,14 +100,14 @@ __device__ __forceinline__ bool item_of(const PromptParams& p, int index, int sp
   const int bh = index % per;
   it.head = bh % c.kv_heads;
   it.b = bh / c.kv_heads;
-  int count;
-  new_tokens(c, it.b, it.first, count);
+  int count, extra;
+  new_rows(c, it.b, it.first, count, extra);
   const int all = count * p.a.group;
   it.row0 = tile * p.rows;
   if (all <= p.min_rows || it.row0 >= all) return false;
   it.rows = min(p.rows, all - it.row0);
   const int len = c.seq_lens[it.b];
-  it.pos0 = len - count;
+  it.pos0 = len - count - extra;
   it.len = len < 0 ? 0 : (len < c.limit ? len : c.limit);
   const int p0 = it.pos0 + it.row0 / p.a.group, p1 = it.pos0 + (it.row0 + it.rows - 1) / p.a.group;
   const int hi = p1 < 0 ? 0 : (p.a.causal ? min(it.len, p1 + 1) : it.len);

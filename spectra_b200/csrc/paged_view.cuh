@@ -20,6 +20,13 @@ __device__ __forceinline__ void new_tokens(const PagedView& c, int b, int64_t& f
   }
 }
 
+// The same with the attention's rows: only the first max_q tokens have any; `extra` is how many have none.
+__device__ __forceinline__ void new_rows(const PagedView& c, int b, int64_t& first, int& count, int& extra) {
+  new_tokens(c, b, first, count);
+  extra = count > c.max_q ? count - c.max_q : 0;
+  count -= extra;
+}
+
 // Sequence of new token t, or -1 where none holds it; the whole warp asks for one
 // token.  (A 32-way search: two loads that wait for each other up to 1024 sequences.)
 __device__ __forceinline__ int sequence_of(const PagedView& c, int64_t t) {

@@ -91,8 +91,9 @@ class TokenBatch:
     (0: a slot that holds none).  The new tokens are a sequence's last ones;
     they are rows ``cu_q[b] .. cu_q[b + 1]`` of the token tensors (int32
     [B + 1]), or, without ``cu_q``, ``q_len`` rows each.  Host bounds:
-    ``total`` rows, at most ``max_q`` of one sequence, ``max_len`` over
-    seq_lens (default: what the tables can hold).
+    ``total`` rows, at most ``max_q`` of one sequence (the attention's results
+    of rows past it are 0), ``max_len`` over seq_lens (default: what the tables
+    can hold).
     """
 
     def __init__(self, block_tables: torch.Tensor, seq_lens: torch.Tensor, cu_q: Optional[torch.Tensor] = None,
