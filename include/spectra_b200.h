@@ -332,7 +332,9 @@ SPECTRA_API int spectra_paged_kv_read(const SpectraPagedCache* cache, const Spec
  *   t_n = scale q . k_n;  softcap > 0: t = softcap tanh(t / softcap);
  *   slopes: t += slopes[h] (n - p);  out = sum e^t_n v_n / sum e^t_n
  * over n < seq_lens[b], with `causal` n <= p, with window > 0 n > p - window.
- * A row that sees no key is 0; rows >= cu_q[batch] are 0.
+ * A row that sees no key is 0; rows >= cu_q[batch] are 0.  A capped score is off
+ * by at most 2^-20 of itself and, under caps up to 128, 2^-22 of the cap besides
+ * (its tanh; caps above 1e30 are taken as 1e30).
  *   q, out [total][q_heads][D], element strides, dtype F16 or BF16;
  *   slopes fp32 [q_heads] or NULL; scale > 0.
  *   workspace: spectra_paged_attention_workspace_bytes(head_dim) bytes, of which

@@ -546,7 +546,7 @@ int spectra_paged_attention(const SpectraPagedCache* cache, const SpectraTokenBa
   a.q = q; a.q_ts = q_ts; a.q_hs = q_hs;
   a.out = out; a.o_ts = o_ts; a.o_hs = o_hs;
   a.dtype = dtype; a.q_heads = int(q_heads); a.group = int(q_heads / cache->kv_heads);
-  a.scale = scale; a.softcap = softcap; a.slopes = slopes; a.causal = causal != 0;
+  a.scale = scale; a.softcap = std::min(softcap, 1e30f); a.slopes = slopes; a.causal = causal != 0;
   a.window = int(std::min<int64_t>(window, INT32_MAX));
   a.vec = head_rows_vec(q, q_ts, q_hs) && head_rows_vec(out, o_ts, o_hs);
   a.workspace = workspace; a.workspace_bytes = workspace_bytes;

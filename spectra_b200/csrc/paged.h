@@ -67,7 +67,7 @@ struct PagedAttnArgs {
   const void* q; int64_t q_ts, q_hs;       // [total, q_heads, D]
   void* out; int64_t o_ts, o_hs;
   int dtype, q_heads, group;               // group = q_heads / kv_heads
-  float scale, softcap;                    // softcap 0: none
+  float scale, softcap;                    // softcap 0: none (1e30 at most, which no score feels)
   const float* slopes;                     // [q_heads] or NULL
   int causal, window;                      // window 0: none
   int vec;                                 // rows of q and out on 16-byte boundaries

@@ -127,7 +127,8 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// MOD: 0 plain scores, 1 capped, 2 with a bias (and capped where softcap > 0)
+// MOD: 0 plain scores, 1 with a cap of up to kLowCap, 2 with a bias (and a cap where softcap > 0) or a
+// higher cap (whose code in MOD 1 took 490 us where 450 are taken without it)
 template <bool BF16, int G, int MOD>
 __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams p) {
   using C = Cfg<G>;
@@ -283,13 +284,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         hi = pos < 0 ? 0 : (a.causal ? min(it.len, pos + 1) : it.len);
         lo = first_key(pos, a.window);
       }
-      const float slope = MOD == 2 ? a.slopes[h] * kLog2e : 0.f;
-      const float inv = MOD != 0 && a.softcap > 0.f ? c_row / a.softcap : 0.f;
+      const float slope = MOD == 2 && a.slopes ? a.slopes[h] * kLog2e : 0.f;
+      const float inv = MOD != 0 && a.softcap > 0.f ? cap_factor(c_row, a.softcap) : 0.f;
       const float k_exp = MOD ? 1.f : c_row * kLog2e;
       // how a capped score's tanh is computed: four terms unless one of the last steps has shown
-      // that six are needed (or the factors, powers of inv, would vanish)
-      const bool tiny = MOD == 1 && __any_sync(0xffffffffu, fabsf(inv) < 2e-5f);
-      int wide = tiny ? 1 : 0;  // steps to go with six
+      // that six are needed (or the factors of the four, powers of inv, would vanish or pass fp32)
+      const bool apart = MOD == 1 && __any_sync(0xffffffffu, !(inv >= 1e-4f && inv <= 1e3f));
+      int wide = apart ? 1 : 0;  // steps to go with six
       const uint32_t quarter = uint32_t((warp & 3) * 32) << 16;
       const uint32_t to = tmem + quarter + 256 + t * 128;
       float m = kNone, l = 0.f;
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           const float c1 = TERMS == 0 ? (MOD == 0 ? k_exp : c_row * kLog2e) : inv, c2 = inv * inv;
           const uint64_t first = f2(c1, c1);
           if constexpr (TERMS == 4) {
-            float pw = a.softcap * kLog2e * inv;  // in the scores themselves: inv's powers go into the factors
+            float pw = c_row * kLog2e;  // in the products themselves: inv's powers go into the factors
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
               fit[d] = f2(pw * kTanhFit4[d], pw * kTanhFit4[d]);
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           s0 += s1;
           if constexpr (TERMS == 4) far *= c2;
           const bool out = __any_sync(0xffffffffu, s0 > kMost || (TERMS != 0 && far > (TERMS == 4 ? kTanhRange4 : kTanhRange6)));
-          if constexpr (MOD == 1) wide = __any_sync(0xffffffffu, far > kTanhRange4) ? 8 : max(wide - 1, int(tiny));
+          if constexpr (MOD == 1) wide = __any_sync(0xffffffffu, far > kTanhRange4) ? 8 : max(wide - 1, int(apart));
           if (out) return false;
           l += s0;
 #pragma unroll
@@ -398,13 +399,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           tmem_ld_x32_nowait(ts + 32, buf[1]);
           tmem_ld_wait32(buf[0]);
           tmem_ld_wait32(buf[1]);
+          if (MOD == 2 && a.softcap > kLowCap) {
+            const float back = 1.f / inv;
+#pragma unroll
+            for (int k = 0; k < 64; ++k) {
+              uint32_t& w = buf[k >> 5][k & 31];
+              w = __float_as_uint(high_cap(__uint_as_float(w), inv, back));
+            }
+          }
+          const bool low_cap = MOD == 1 || (a.softcap > 0.f && a.softcap <= kLowCap);
           float top = -INFINITY;
 #pragma unroll
           for (int k = 0; k < 64; ++k) {
             uint32_t& w = buf[k >> 5][k & 31];
             float x = __uint_as_float(w);
             if constexpr (MOD != 0) {
-              x = a.softcap > 0.f ? a.softcap * tanh_exp(x * inv) : x * c_row;
+              x = low_cap ? a.softcap * tanh_exp(x * inv) : x * c_row;
               x = fmaf(slope, float(n0 + k - pos), x * kLog2e);
             }
             if (masked) x = n0 + k >= hi || n0 + k < lo || !((held >> (k / 16)) & 1) ? -INFINITY : x;
@@ -811,7 +821,7 @@ int launch_one(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
 
 template <bool BF16, int G>
 int launch_mod(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
-  if (a.slopes) return launch_one<BF16, G, 2>(a, min_rows, st);
+  if (a.slopes || a.softcap > kLowCap) return launch_one<BF16, G, 2>(a, min_rows, st);
   return a.softcap > 0.f ? launch_one<BF16, G, 1>(a, min_rows, st) : launch_one<BF16, G, 0>(a, min_rows, st);
 }
 

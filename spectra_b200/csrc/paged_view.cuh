@@ -166,14 +166,14 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // tanh(x) = x P(x^2), on the FMA pipe where tanh_exp takes two of the special-function
-// unit's turns: fits of tanh(x) / x in powers of x^2 for the least maximum of the
-// absolute error (own computation: iteratively reweighted least squares on Chebyshev
-// nodes).  Six terms for |x| <= 1.25, error 2.4e-6; four for |x| <= 0.6, error 6.3e-7.
-constexpr float kTanhRange6 = 1.25f * 1.25f, kTanhRange4 = 0.6f * 0.6f;
-__device__ constexpr float kTanhFit6[6] = {0.9999746680259705f,  -0.3328392803668976f, 0.13053609430789948f,
-                                           -0.04692651331424713f, 0.01253186073154211f, -0.001682034693658352f};
-__device__ constexpr float kTanhFit4[4] = {0.9999909996986389f, -0.33298975229263306f, 0.1297455132007599f,
-                                           -0.03961124271154404f};
+// unit's turns: fits of tanh(x) / x in powers of x^2 with P(0) = 1, for the least maximum
+// of the relative error (own computation: iteratively reweighted least squares on Chebyshev
+// nodes), so that a score is off by a share of itself whatever its cap.  Six terms for
+// |x| <= 0.95, error 4.1e-7 (4.9e-7 with fp32's roundings); four for |x| <= 0.5, 6.5e-7 (7.2e-7).
+constexpr float kTanhRange6 = 0.95f * 0.95f, kTanhRange4 = 0.5f * 0.5f;
+__device__ constexpr float kTanhFit6[6] = {1.f, -0.3333132863044739f, 0.13300810754299164f, -0.05221107602119446f,
+                                           0.017525605857372284f, -0.003422057954594493f};
+__device__ constexpr float kTanhFit4[4] = {1.f, -0.33328160643577576f, 0.13205359876155853f, -0.0447506383061409f};
 // Larger magnitude of both halves (bf16 or fp16; a NaN is passed over), as bits.
 template <bool BF16>
 __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
@@ -195,11 +195,25 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// tanh by its exponential: absolute error a few 2^-24 over the whole range.
+// tanh by its exponential: absolute error a few 2^-24 over the whole range, so not for small |x|.
 __device__ __forceinline__ float tanh_exp(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(2.f * kLog2e * x)));
   return fmaf(-2.f, r, 1.f);
+}
+// A product's factor for the cap's argument; finite, so that 0 stays 0 under the smallest caps.
+__device__ __forceinline__ float cap_factor(float factor, float cap) { return fminf(factor / cap, 1e37f); }
+// Up to this cap tanh_exp's absolute error is less than 2^-15 of a score (in powers of e), and serves as
+// it is (high_cap in its place: capped prompts 490 us, 450 without).
+constexpr float kLowCap = 128.f;
+// Under a higher one: the product that, uncapped, has the capped score of v, to 2^-20 of itself.
+// back = 1 / inv (an infinity where inv vanishes, which is not used: then x does too).
+__device__ __forceinline__ float high_cap(float v, float inv, float back) {
+  const float x = v * inv, u = x * x;
+  float r = kTanhFit4[3];
+#pragma unroll
+  for (int d = 2; d >= 0; --d) r = fmaf(r, u, kTanhFit4[d]);
+  return u <= kTanhRange4 ? v * r : tanh_exp(x) * back;
 }
 
 }  // namespace spectra
