@@ -306,7 +306,7 @@ typedef struct {
  * (1 / s rounded once, then multiplied).  A group of key or value that holds a
  * NaN or infinity or spans more than 65472: its key group reads NaN, its value
  * group 0.  Padding: nothing is stored, the query row becomes 0.
- *   q [total][q_heads][D] or NULL, q_out the same shape, not overlapping q;
+ *   q [total][q_heads][D] or NULL, q_out the same shape, not overlapping q, k or v;
  *   k, v [total][kv_heads][D]; element (t, h, d) at t*_ts + h*_hs + d; dtype
  *   F16 or BF16 for all four.  rotary 0: cos, sin NULL.  rotary a multiple of
  *   16 (8 if interleaved), <= D.
@@ -335,7 +335,8 @@ SPECTRA_API int spectra_paged_kv_read(const SpectraPagedCache* cache, const Spec
  * A row that sees no key is 0; rows >= cu_q[batch] are 0.  A capped score is off
  * by at most 2^-20 of itself and, under caps up to 128, 2^-22 of the cap besides
  * (its tanh; caps above 1e30 are taken as 1e30).
- *   q, out [total][q_heads][D], element strides, dtype F16 or BF16;
+ *   q, out [total][q_heads][D], element strides, dtype F16 or BF16; out may be q
+ *   (the same strides), otherwise they do not overlap;
  *   slopes fp32 [q_heads] or NULL; scale > 0.
  *   workspace: spectra_paged_attention_workspace_bytes(head_dim) bytes, of which
  *          the first SPECTRA_PAGED_COUNTER_BYTES are zero before its first use

@@ -202,7 +202,8 @@ def paged_kv_append(cache: PagedKVCache, batch: TokenBatch, k: torch.Tensor, v: 
     queries rounded once, the keys quantised without rounding in between.
     Groups that hold a NaN or infinity make their token's key NaN, so every row
     that looks at it is NaN and no other.  Token tensors may be views (any
-    token and head strides), of a fused projection for example."""
+    token and head strides), of a fused projection for example.  ``out``, for the
+    rotated queries, shares no element with q, k or v."""
     index = cache._index
     if batch._index != index:
         _other_device()
@@ -230,10 +231,9 @@ def paged_kv_append(cache: PagedKVCache, batch: TokenBatch, k: torch.Tensor, v: 
             given, o_ts, o_hs = _strided("out", out, cache, batch, heads)
             if given is not out:
                 raise ValueError("out must have unit stride along a head")
-            lo, hi = _extent(q)
-            olo, ohi = _extent(out)
-            if lo < ohi and olo < hi:
-                raise ValueError("out must not overlap q")
+            _own_elements(out)
+            if _overlap(out, q) or _overlap(out, k) or _overlap(out, v):
+                raise ValueError("out must not overlap q, k or v")
         if q.dtype != dt or out.dtype != dt:
             raise TypeError("q, k, v and out must have one dtype")
         qp, op = q.data_ptr(), out.data_ptr()
@@ -270,6 +270,34 @@ def _angles(cos, sin, cache: PagedKVCache, batch: TokenBatch, interleaved: bool)
 def _extent(t: torch.Tensor) -> Tuple[int, int]:
     span = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
     return t.data_ptr(), t.data_ptr() + span * t.element_size()
+
+
+def _runs(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """Where the tensor's runs of consecutive elements start (addresses in order), and their bytes."""
+    (T, H, D), (ts, hs, _), size = t.shape, t.stride(), t.element_size()
+    if hs == D or H == 1:
+        return t.data_ptr() + torch.arange(T if ts else 1) * (ts * size), H * D * size
+    starts = torch.arange(T if ts else 1)[:, None] * ts + torch.arange(H) * hs
+    return t.data_ptr() + torch.unique(starts) * size, D * size
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether [tokens, heads, D] tensors of unit stride along a head share an element.  Views of one
+    buffer that lie between each other's rows do not."""
+    lo, hi = _extent(a)
+    blo, bhi = _extent(b)
+    if lo >= bhi or blo >= hi:
+        return False
+    (sa, la), (sb, lb) = _runs(a), _runs(b)
+    i = torch.searchsorted(sa, sb, right=True)  # the first run of a that starts past b's; one of either side touches it
+    first = torch.cat([sb[:1] - la, sa])[i]
+    after = torch.cat([sa, sb[-1:] + lb])[i]
+    return bool((first + la > sb).any() or (sb + lb > after).any())
+
+
+def _own_elements(out: torch.Tensor) -> None:
+    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        raise ValueError("out must not be an expanded tensor")
 
 
 def paged_kv_read(cache: PagedKVCache, batch: TokenBatch, dtype: torch.dtype = torch.bfloat16):
@@ -323,7 +351,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, *, 
     1 / sqrt(D)) times the products, then ``softcap * tanh(score / softcap)``,
     then plus ``alibi_slopes[h] * (n - p)`` (fp32 [q_heads]).  q_heads is a
     multiple of kv_heads; consecutive heads share one.  A row that sees no key
-    is 0.  Scores, softmax statistics and sums are fp32.
+    is 0.  Scores, softmax statistics and sums are fp32.  ``out`` may be q
+    itself (the same strides); otherwise they share no element.
 
     Partial results lie in a workspace of the current stream (17 MB for heads of
     128, kept for the process).  A graph captured on a stream that has called
@@ -359,6 +388,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, *, 
         given, o_ts, o_hs = _strided("out", out, cache, batch, heads)
         if given is not out or out.dtype != q.dtype:
             raise ValueError("out must have q's dtype and unit stride along a head")
+        _own_elements(out)
+        if (out.data_ptr() != q.data_ptr() or o_ts != q_ts or o_hs != q_hs) and _overlap(out, q):
+            raise ValueError("out must not overlap q, unless it is q")
     ws, nbytes = _workspace(index, cache.head_dim)
     _call(index, "spectra_paged_attention", cache._at, batch._at, _DT[q.dtype], heads, q.data_ptr(), q_ts, q_hs,
           out.data_ptr(), o_ts, o_hs, scale, softcap, None if slopes is None else slopes.data_ptr(), causal,
