@@ -92,7 +92,18 @@ class PagedLlama:
     def generate(self, prompts: List[List[int]], tokens: int, graph: bool = True):
         """Greedy continuations [B, tokens], and the logits each was chosen from [B, tokens, vocab]."""
         lens = [len(p) for p in prompts]
+        if not lens or min(lens) < 1 or tokens < 1:
+            raise ValueError("prompts of one token at least, and one token to generate")
+        # positions from max_len on have no angles and are not kept (the last token generated is not appended)
+        if max(lens) + tokens - 1 > self.max_len:
+            raise ValueError(f"a prompt of {max(lens)} and {tokens} tokens pass max_len={self.max_len}")
         tables = self.tables([n + tokens for n in lens])
+        try:
+            return self._generate(prompts, lens, tables, tokens, graph)
+        finally:
+            self.release(tables)
+
+    def _generate(self, prompts, lens, tables, tokens, graph):
         seq_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
         cu = torch.tensor([0] + lens, dtype=torch.int32, device="cuda").cumsum(0, dtype=torch.int32)
         ids = torch.tensor([t for p in prompts for t in p], device="cuda")
@@ -126,7 +137,6 @@ class PagedLlama:
             replay()
             out.append(last.clone())
             chosen_from.append(logits.clone())
-        self.release(tables)
         return torch.stack(out, 1), torch.stack(chosen_from, 1)
 
 
