@@ -396,7 +396,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) c_exp[nt][j] = MOD ? 1.f : factor[nt * 8 + 2 * cc + j] * kLog2e;
+      for (int j = 0; j < 2; ++j)  // (not 0, which a masked score of -infinity must not meet)
+        c_exp[nt][j] = MOD ? 1.f : fmaxf(factor[nt * 8 + 2 * cc + j] * kLog2e, 1e-37f);
+    bool loud = false;  // a maximum past kLoud
 
     auto arrived = [&](int stage, uint32_t parity) {  // (the vote makes the lanes agree)
       const bool ok = __all_sync(0xffffffffu, sm100::mbar_wait(bars + warp * kStages + stage, parity, &s_never));
@@ -518,6 +520,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
                 o[grp][h][nt][2 + j] *= f;
               }
           }
+        if constexpr (MOD == 0) {
+          bool any = false;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) any = any || fabsf(m[nt][0]) > kLoud || fabsf(m[nt][1]) > kLoud;
+          loud = __any_sync(0xffffffffu, any);
+        }
+      }
+      float to_exp[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) to_exp[nt][j] = loud ? 1.f : c_exp[nt][j];
+      if (loud) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sc[i >> 2][nt][i & 3] *= c_exp[nt][i & 1];
       }
       uint32_t pb[2][NT][2];  // P^T fragments: rows as columns
 #pragma unroll
@@ -527,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
           float e[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i]) : "f"(fmaf(sc[tile][nt][i], c_exp[nt][i & 1], kShift - m[nt][i & 1])));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i]) : "f"(fmaf(sc[tile][nt][i], to_exp[nt][i & 1], kShift - m[nt][i & 1])));
             l[nt][i & 1] += e[i];
           }
           pb[tile][nt][0] = transpose8x8(h2_pack(e[0], e[1]));

@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       }
       const float slope = MOD == 2 && a.slopes ? a.slopes[h] * kLog2e : 0.f;
       const float inv = MOD != 0 && a.softcap > 0.f ? cap_factor(c_row, a.softcap) : 0.f;
-      const float k_exp = MOD ? 1.f : c_row * kLog2e;
+      const float k_exp = c_row * kLog2e;
       // how a capped score's tanh is computed: four terms unless one of the last steps has shown
       // that six are needed (or the factors of the four, powers of inv, would vanish or pass fp32)
       const bool apart = MOD == 1 && __any_sync(0xffffffffu, !(inv >= 1e-4f && inv <= 1e3f));
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       const uint32_t quarter = uint32_t((warp & 3) * 32) << 16;
       const uint32_t to = tmem + quarter + 256 + t * 128;
       float m = kNone, l = 0.f;
-      bool ok = true;
+      bool ok = true, loud = false;  // loud: a maximum past kLoud
 
       for (int i = 0; i < n; ++i) {
         const uint32_t ts = tmem + quarter + t * 128 + (i & 1) * 64;
@@ -315,10 +315,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           uint64_t sums[2] = {0, 0}, fit[TERMS + 1];
           float far = 0.f;
           const uint64_t m2 = f2(kShift - m, kShift - m);
-          const float c1 = TERMS == 0 ? (MOD == 0 ? k_exp : c_row * kLog2e) : inv, c2 = inv * inv;
+          const float c1 = TERMS == 0 ? k_exp : inv, c2 = inv * inv;
           const uint64_t first = f2(c1, c1);
           if constexpr (TERMS == 4) {
-            float pw = c_row * kLog2e;  // in the products themselves: inv's powers go into the factors
+            float pw = k_exp;  // in the products themselves: inv's powers go into the factors
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
               fit[d] = f2(pw * kTanhFit4[d], pw * kTanhFit4[d]);
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           return true;
         };
         bool done = false;
-        if (i > 0 && !masked) {
+        if (i > 0 && !masked && !loud) {
           if constexpr (MOD == 0)
             done = fast(std::integral_constant<int, 0>{});
           else if (MOD == 2 && !(a.softcap > 0.f))
@@ -413,7 +413,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           for (int k = 0; k < 64; ++k) {
             uint32_t& w = buf[k >> 5][k & 31];
             float x = __uint_as_float(w);
-            if constexpr (MOD != 0) {
+            if constexpr (MOD == 0) {
+              x *= k_exp;
+            } else {
               x = low_cap ? a.softcap * tanh_exp(x * inv) : x * c_row;
               x = fmaf(slope, float(n0 + k - pos), x * kLog2e);
             }
@@ -422,9 +424,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
             top = fmaxf(top, x);
           }
           // (after this no weight of this step passes 2^(3 + kShift): sums like it stay in fast's bound)
-          if (__any_sync(0xffffffffu, top * k_exp > m + 3.f)) {
-            const float up = fmaxf(m, top * k_exp), f = exp2f(m - up);
+          if (__any_sync(0xffffffffu, top > m + 3.f)) {
+            const float up = fmaxf(m, top), f = exp2f(m - up);
             m = up;
+            loud = __any_sync(0xffffffffu, fabsf(m) > kLoud);
             l *= f;
             if (i > 0) {  // O, once the last step's product has been added
               ok = wait(o_full + t, (i - 1) & 1);
@@ -450,8 +453,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
             uint32_t u[16];
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
-              const float e0 = ex2(fmaf(__uint_as_float(buf[q][k]), k_exp, kShift - m));
-              const float e1 = ex2(fmaf(__uint_as_float(buf[q][k + 1]), k_exp, kShift - m));
+              const float e0 = ex2(__uint_as_float(buf[q][k]) + (kShift - m));
+              const float e1 = ex2(__uint_as_float(buf[q][k + 1]) + (kShift - m));
               sum[k & 2] += e0;
               sum[(k & 2) + 1] += e1;
               u[4 * ((k >> 1) & 3) + (k >> 3)] = h2_pack(e0, e1);

@@ -69,7 +69,11 @@ constexpr float kLazy = 8.f;
 // (More would raise it more often: prompts with a cap took 461 us with 5, 420
 // with 3, 408 with 1.)
 constexpr float kShift = 3.f;
-constexpr float kNone = -1e30f;  // below every score that is seen
+constexpr float kNone = -3e38f;  // below every score that is seen, as far as fp32 holds scores
+// A weight's exponent is one fma of the product, its factor and the maximum.  That leaves what the
+// maximum was rounded by, a share 2^-24 of it: under kLoud less than 2^-4 and the same for every key,
+// above it the product is rounded first (a maximum near 2^31 would give exponents past fp32's).
+constexpr float kLoud = 1048576.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // BYTES of shared memory into registers, as wide as their alignment allows.
