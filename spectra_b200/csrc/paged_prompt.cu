@@ -287,10 +287,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       const float slope = MOD == 2 && a.slopes ? a.slopes[h] * kLog2e : 0.f;
       const float inv = MOD != 0 && a.softcap > 0.f ? cap_factor(c_row, a.softcap) : 0.f;
       const float k_exp = c_row * kLog2e;
-      // how a capped score's tanh is computed: four terms unless one of the last steps has shown
-      // that six are needed (or the factors of the four, powers of inv, would vanish or pass fp32)
-      const bool apart = MOD == 1 && __any_sync(0xffffffffu, !(inv >= 1e-4f && inv <= 1e3f));
-      int wide = apart ? 1 : 0;  // steps to go with six
       const uint32_t quarter = uint32_t((warp & 3) * 32) << 16;
       const uint32_t to = tmem + quarter + 256 + t * 128;
       float m = kNone, l = 0.f;
@@ -307,24 +303,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
 
         // Most steps: no mask, no new maximum.  The weights are computed with the old maximum and
         // stored if their sum is small enough to say that no score passed it by much (then each
-        // weight fits fp16 too); TERMS: of the cap's tanh, which may be out of their range as well.
-        auto fast = [&](auto terms) -> bool {
-          constexpr int TERMS = decltype(terms)::value;
+        // weight fits fp16 too) and no score is out of the range of the cap's tanh.  (A second copy with
+        // four of its six terms, for steps of low scores, cost more in instruction fetches than it saved:
+        // heads of 64, 6 ragged prompts, 477 us against 426; heads of 128, 234 against 238.)
+        auto fast = [&](auto cap) -> bool {
+          constexpr bool CAP = decltype(cap)::value;
           constexpr float kMost = 61440.f;  // fits fp16, with 6 % for the sum's own error
           uint32_t buf[2][32], pk[32];
-          uint64_t sums[2] = {0, 0}, fit[TERMS + 1];
+          uint64_t sums[2] = {0, 0}, fit[6];
           float far = 0.f;
           const uint64_t m2 = f2(kShift - m, kShift - m);
-          const float c1 = TERMS == 0 ? k_exp : inv, c2 = inv * inv;
+          const float c1 = CAP ? inv : k_exp;
           const uint64_t first = f2(c1, c1);
-          if constexpr (TERMS == 4) {
-            float pw = k_exp;  // in the products themselves: inv's powers go into the factors
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              fit[d] = f2(pw * kTanhFit4[d], pw * kTanhFit4[d]);
-              pw *= c2;
-            }
-          } else if constexpr (TERMS == 6) {
+          if constexpr (CAP) {
 #pragma unroll
             for (int d = 0; d < 6; ++d) {
               const float x = a.softcap * kLog2e * kTanhFit6[d];
@@ -344,16 +335,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
               const uint64_t raw2 = f2(__uint_as_float(v[k]), __uint_as_float(v[k + 1]));
               uint64_t y = m2;
               if constexpr (MOD == 2) y = f2_fma(f2(slope, slope), f2(float(k), float(k + 1)), f2(bias, bias));
-              if constexpr (TERMS == 0) {
+              if constexpr (!CAP) {
                 y = f2_fma(raw2, first, y);
               } else {
-                const uint64_t x = TERMS == 6 ? f2_mul(raw2, first) : raw2, u = f2_mul(x, x);
+                const uint64_t x = f2_mul(raw2, first), u = f2_mul(x, x);
                 float u0, u1;
                 f2_split(u, u0, u1);
                 far = max3(far, u0, u1);
-                uint64_t r = fit[TERMS - 1];
+                uint64_t r = fit[5];
 #pragma unroll
-                for (int d = TERMS - 2; d >= 0; --d) r = f2_fma(r, u, fit[d]);
+                for (int d = 4; d >= 0; --d) r = f2_fma(r, u, fit[d]);
                 y = f2_fma(x, r, y);
               }
               float e0, e1;  // exponents: scores in powers of two, less the maximum
@@ -368,10 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
           float s0, s1;
           f2_split(f2_add(sums[0], sums[1]), s0, s1);
           s0 += s1;
-          if constexpr (TERMS == 4) far *= c2;
-          const bool out = __any_sync(0xffffffffu, s0 > kMost || (TERMS != 0 && far > (TERMS == 4 ? kTanhRange4 : kTanhRange6)));
-          if constexpr (MOD == 1) wide = __any_sync(0xffffffffu, far > kTanhRange4) ? 8 : max(wide - 1, int(apart));
-          if (out) return false;
+          if (__any_sync(0xffffffffu, s0 > kMost || (CAP && far > kTanhRange6))) return false;
           l += s0;
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
@@ -385,13 +373,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
         bool done = false;
         if (i > 0 && !masked && !loud) {
           if constexpr (MOD == 0)
-            done = fast(std::integral_constant<int, 0>{});
+            done = fast(std::false_type{});
           else if (MOD == 2 && !(a.softcap > 0.f))
-            done = fast(std::integral_constant<int, 0>{});
-          else {
-            if (MOD == 1 && wide == 0) done = fast(std::integral_constant<int, 4>{});
-            if (!done && (MOD == 2 || wide > 0)) done = fast(std::integral_constant<int, 6>{});
-          }
+            done = fast(std::false_type{});
+          else
+            done = fast(std::true_type{});
         }
         if (!done) {
           uint32_t buf[2][32];

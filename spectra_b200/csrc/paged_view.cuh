@@ -66,8 +66,8 @@ constexpr float kLazy = 8.f;
 // Weights are kept times 2^kShift (their sums too, so nothing else changes): the
 // smallest that fp16 holds as normal numbers lie 2^-17 below the maximum's, and
 // above it fp16 has 12 bits for scores that pass a maximum that was not raised.
-// (More would raise it more often: prompts with a cap took 461 us with 5, 420
-// with 3, 408 with 1.)
+// (More would raise it more often: prompts with a cap take 417 us with 5, 408
+// with 3, 401 with 1.)
 constexpr float kShift = 3.f;
 constexpr float kNone = -3e38f;  // below every score that is seen, as far as fp32 holds scores
 // A weight's exponent is one fma of the product, its factor and the maximum.  That leaves what the
@@ -173,7 +173,8 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 // unit's turns: fits of tanh(x) / x in powers of x^2 with P(0) = 1, for the least maximum
 // of the relative error (own computation: iteratively reweighted least squares on Chebyshev
 // nodes), so that a score is off by a share of itself whatever its cap.  Six terms for
-// |x| <= 0.95, error 4.1e-7 (4.9e-7 with fp32's roundings); four for |x| <= 0.5, 6.5e-7 (7.2e-7).
+// |x| <= 0.95 (prompts' usual steps), error 4.1e-7 (4.9e-7 with fp32's roundings); four for
+// |x| <= 0.5 (high_cap), 6.5e-7 (7.2e-7).
 constexpr float kTanhRange6 = 0.95f * 0.95f, kTanhRange4 = 0.5f * 0.5f;
 __device__ constexpr float kTanhFit6[6] = {1.f, -0.3333132863044739f, 0.13300810754299164f, -0.05221107602119446f,
                                            0.017525605857372284f, -0.003422057954594493f};
@@ -208,7 +209,7 @@ __device__ __forceinline__ float tanh_exp(float x) {
 // A product's factor for the cap's argument; finite, so that 0 stays 0 under the smallest caps.
 __device__ __forceinline__ float cap_factor(float factor, float cap) { return fminf(factor / cap, 1e37f); }
 // Up to this cap tanh_exp's absolute error is less than 2^-15 of a score (in powers of e), and serves as
-// it is (high_cap in its place: capped prompts 490 us, 450 without).
+// it is (high_cap in its place cost 40 us of the 450 that capped prompts took).
 constexpr float kLowCap = 128.f;
 // Under a higher one: the product that, uncapped, has the capped score of v, to 2^-20 of itself.
 // back = 1 / inv (an infinity where inv vanishes, which is not used: then x does too).
