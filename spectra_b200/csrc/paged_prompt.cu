@@ -56,6 +56,7 @@ using namespace sm100;
 
 constexpr int kRows = 256;   // rows of a CTA, at most
 constexpr int kKeys = 64;    // keys of a step
+constexpr uint32_t kUpper = 0xFFF0FFF0u;  // of two fp16 numbers: sign, exponent, 7 bits
 constexpr int kThreads = 512;  // warps 14 and 15 only give their registers away
 
 struct PromptParams {
@@ -67,7 +68,13 @@ struct PromptParams {
   float* partials; // [item][split][rows][D + 2]
 };
 
-template <int G>
+// Keys and values in one operand are rounded to 11 bits, which alone puts results 7e-4 off (keys of
+// loud features) where an fp16 result's own rounding is 2.0e-4.  fp16 queries of heads up to 64 take
+// them as two, (q - z) s_hi + (q - z) s_lo with the scale's upper 7 bits and the rest: exact in fp16.
+// That is twice the products, for which the tensor pipe has room there (6 capped prompts, heads of 64,
+// 448 us against 408, plain ones 162 against 145) and no longer with heads of 128 (258 us against 180;
+// a chunk of 4096 over 16384 1800 against 1033) or 256; a bf16 result has 1.6e-3 of its own.
+template <int G, bool BF16>
 struct Cfg {
   static constexpr int D = 32 * G;
   static constexpr int kAtoms = (D + 63) / 64;                 // 128-byte column blocks of Q and K
@@ -77,10 +84,11 @@ struct Cfg {
   // Heads of 256: O takes 256 columns of TMEM and a step's operands 64 KB, so one tile, two stages of
   // keys and one of values.
   static constexpr int kTiles = G == 8 ? 1 : 2;
-  static constexpr int kKStages = G == 8 ? 2 : 4, kVStages = G == 8 ? 1 : 4;
+  static constexpr int kParts = !BF16 && G <= 2 ? 2 : 1;       // operands
+  static constexpr int kKStages = (G == 8 ? 2 : 4) / kParts, kVStages = G == 8 ? 1 : 4 / kParts;
   static constexpr int kQ = kTiles * kAtoms * kQAtom;
-  static constexpr int kK = kAtoms * kKAtom;                   // one stage
-  static constexpr int kV = D * 128;                           // one stage
+  static constexpr int kKPart = kAtoms * kKAtom, kVPart = D * 128;
+  static constexpr int kK = kParts * kKPart, kV = kParts * kVPart;  // one stage
   static constexpr int kRaw = 4 * 2 * kTile;
   static constexpr int kSmem = 1024 + kQ + kKStages * kK + kVStages * kV + kRaw;
 };
@@ -131,7 +139,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 // higher cap (whose code in MOD 1 took 490 us where 450 are taken without it)
 template <bool BF16, int G, int MOD>
 __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams p) {
-  using C = Cfg<G>;
+  using C = Cfg<G, BF16>;
   constexpr int D = C::D;
   constexpr TileLayout L{G};
   const PagedAttnArgs& a = p.a;
@@ -611,13 +619,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
             const uint32_t b = q & 3, z2 = __byte_perm(kz[x][y][q >> 2], 0x64646464u, b | 0x40u | (b << 8) | 0x4000u);
             const uint32_t c2 = h2_sub(0x63806380u, z2);  // 960 - (1024 + z)
             const uint32_t w = kw[x][y][q];
-            uint4 o;
-            o.x = h2_mul(h2_sub(code_low(w, magic), z2), s2);
-            o.y = h2_mul(h2_fma(code_high(w, magic), 0x2C002C00u, c2), s2);
-            o.z = h2_mul(h2_sub(code_low(w >> 8, magic), z2), s2);
-            o.w = h2_mul(h2_fma(code_high(w >> 8, magic), 0x2C002C00u, c2), s2);
+            const uint32_t d0 = h2_sub(code_low(w, magic), z2), d1 = h2_fma(code_high(w, magic), 0x2C002C00u, c2),
+                           d2 = h2_sub(code_low(w >> 8, magic), z2), d3 = h2_fma(code_high(w >> 8, magic), 0x2C002C00u, c2);
             const int row = 32 * half + 16 * x + 8 * y + g;
-            *reinterpret_cast<uint4*>(kd + (q >> 1) * C::kKAtom + row * 128 + ((((q & 1) * 4 + cc) ^ g) << 4)) = o;
+            uint8_t* at = kd + (q >> 1) * C::kKAtom + row * 128 + ((((q & 1) * 4 + cc) ^ g) << 4);
+            const uint32_t hi = C::kParts == 2 ? s2 & kUpper : s2;
+            *reinterpret_cast<uint4*>(at) = make_uint4(h2_mul(d0, hi), h2_mul(d1, hi), h2_mul(d2, hi), h2_mul(d3, hi));
+            if constexpr (C::kParts == 2) {
+              const uint32_t lo = h2_sub(s2, hi);
+              *reinterpret_cast<uint4*>(at + C::kKPart) = make_uint4(h2_mul(d0, lo), h2_mul(d1, lo), h2_mul(d2, lo), h2_mul(d3, lo));
+            }
           }
       fence_proxy_async_smem();
       __syncwarp();
@@ -631,22 +642,29 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
 #pragma unroll
       for (int q = 0; q < G; ++q) {
         uint32_t o[4][4];
+        [[maybe_unused]] uint32_t rest[4][4];
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             const uint32_t z2 = byte_pair(vz[x][y][q >> 1], q & 1), c2 = h2_sub(0x63806380u, z2);
             const uint32_t w = vw[x][y][q], s2 = vs[x][y][q];
-            o[0][2 * x + y] = h2_mul(h2_sub(code_low(w, magic), z2), s2);
-            o[1][2 * x + y] = h2_mul(h2_fma(code_high(w, magic), 0x2C002C00u, c2), s2);
-            o[2][2 * x + y] = h2_mul(h2_sub(code_low(w >> 8, magic), z2), s2);
-            o[3][2 * x + y] = h2_mul(h2_fma(code_high(w >> 8, magic), 0x2C002C00u, c2), s2);
+            const uint32_t d[4] = {h2_sub(code_low(w, magic), z2), h2_fma(code_high(w, magic), 0x2C002C00u, c2),
+                                   h2_sub(code_low(w >> 8, magic), z2), h2_fma(code_high(w >> 8, magic), 0x2C002C00u, c2)};
+            const uint32_t hi = C::kParts == 2 ? s2 & kUpper : s2;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              o[j][2 * x + y] = h2_mul(d[j], hi);
+              if constexpr (C::kParts == 2) rest[j][2 * x + y] = h2_mul(d[j], h2_sub(s2, hi));
+            }
           }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int row = 32 * q + 4 * g + j;
-          *reinterpret_cast<uint4*>(vd + row * 128 + (((half * 4 + cc) ^ (row & 7)) << 4)) =
-              make_uint4(o[j][0], o[j][1], o[j][2], o[j][3]);
+          uint8_t* at = vd + row * 128 + (((half * 4 + cc) ^ (row & 7)) << 4);
+          *reinterpret_cast<uint4*>(at) = make_uint4(o[j][0], o[j][1], o[j][2], o[j][3]);
+          if constexpr (C::kParts == 2)
+            *reinterpret_cast<uint4*>(at + C::kVPart) = make_uint4(rest[j][0], rest[j][1], rest[j][2], rest[j][3]);
         }
       }
       fence_proxy_async_smem();
@@ -668,9 +686,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
     // (descriptors count in 16 bytes)
     auto scores = [&](int i) {
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k)
-        mma_ss_one(ts + (i & 1) * 64, dq + (((k / 4) * C::kQAtom + (k % 4) * 32) >> 4),
-                   dk + (((i % SK) * C::kK + (k / 4) * C::kKAtom + (k % 4) * 32) >> 4), id_s, k > 0, one);
+      for (int part = 0; part < C::kParts; ++part)
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_ss_one(ts + (i & 1) * 64, dq + (((k / 4) * C::kQAtom + (k % 4) * 32) >> 4),
+                     dk + (((i % SK) * C::kK + part * C::kKPart + (k / 4) * C::kKAtom + (k % 4) * 32) >> 4), id_s,
+                     part > 0 || k > 0, one);
       mma_commit_one(&s_full[t][i & 1], one);
       mma_commit_one(k_empty + i % SK, one);
     };
@@ -685,8 +706,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PromptParams 
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
-      for (int k = 0; k < kKeys / 16; ++k)
-        mma_ts_one(to, ts + (i & 1) * 64 + k * 8, dv + (((i % SV) * C::kV + k * 32) >> 4), id_o, i > 0 || k > 0, one);
+      for (int part = 0; part < C::kParts; ++part)
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k)
+          mma_ts_one(to, ts + (i & 1) * 64 + k * 8, dv + (((i % SV) * C::kV + part * C::kVPart + k * 32) >> 4), id_o,
+                     i > 0 || part > 0 || k > 0, one);
       mma_commit_one(o_full + t, one);
       mma_commit_one(v_empty + i % SE, one);
       if (i + 1 == n) mma_commit_one(o_done + t, one);
@@ -781,7 +805,7 @@ int launch_dep(K kernel, dim3 grid, int threads, int smem, const PromptParams& p
 
 template <bool BF16, int G, int MOD>
 int launch_one(const PagedAttnArgs& a, int min_rows, cudaStream_t st) {
-  using C = Cfg<G>;
+  using C = Cfg<G, BF16>;
   static PerContextOnce once;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
