@@ -333,7 +333,7 @@ SPECTRA_API int spectra_paged_kv_read(const SpectraPagedCache* cache, const Spec
  *   slopes: t += slopes[h] (n - p);  out = sum e^t_n v_n / sum e^t_n
  * over n < seq_lens[b], with `causal` n <= p, with window > 0 n > p - window.
  * A row that sees no key is 0; rows >= cu_q[batch] are 0.  A capped score is off
- * by at most 2^-20 of itself and, under caps up to 128, 2^-22 of the cap besides
+ * by at most 2^-20 of itself and, under caps up to 128, 2^-21 of the cap besides
  * (its tanh; caps above 1e30 are taken as 1e30).
  *   q, out [total][q_heads][D], element strides, dtype F16 or BF16; out may be q
  *   (the same strides), otherwise they do not overlap;

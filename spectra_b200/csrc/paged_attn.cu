@@ -14,15 +14,17 @@
 // and by unpacking instructions, not by the tensor pipe):
 //   S^T = K Q^T: A = raw key codes, 16 tokens x 16 features.  A nibble under
 //     fp16's 0x6400 is 1024 + q where it lies in bits 0-3 and 1024 + 16 q in
-//     bits 4-7 (no shift; those queries are divided by 16 and see 64 + q).  Per
-//     group of 32 features, X = sum of q over the group, the accumulator starts
-//     at the offsets' share of the sum less 1024 X, and t = s (D - (1024 + z)
-//     X) + 1024 X s in fp32, with 1024 + z again a nibble under 0x6400: the keys
-//     are never rounded.
+//     bits 4-7 (no shift; those queries are divided by 16 and see 64 + q).  With X
+//     a group's sum of queries and Y that of its divided ones, the accumulator
+//     starts at 960 Y and ends at D = (sum of code times query) + 1024 X; the
+//     group's share of t is s (D - (1024 + z) X) in fp32, with 1024 + z again a
+//     nibble under 0x6400: the keys are never rounded.
 //   O^T = V^T P^T: A = values (q - z) s in fp16 (exact difference, one
 //     rounding of the product, 11 bits), B = P in fp16, transposed in
 //     registers (movmatrix).  P <= 2^(kLazy + kShift), so fp16 holds it; its rounding
-//     (2^-12) averages over the keys.
+//     (2^-12) averages over the keys, and weights below 2^-28 of the largest are
+//     lost from O (not from their sum).  fp16 results are 3.2e-4 off, 2.1e-4 of it
+//     their own rounding; values as two exact operands took 18 % longer.
 // Queries of both types are scaled per row by a power of two to fp16's upper
 // range (exact down to 2^-24 of the row's largest entry).
 // The running maximum is only raised when a score passes it by more than
@@ -35,11 +37,11 @@
 // of the sequences; a segment that several CTAs share is put together by the
 // last of them to finish, always in the same order.
 //
-// Measured: one token over 131072, 32 query heads on 8, heads of 128, 48.6
-// us (3.3 TB/s); one token of 64 ragged sequences up to 8192, 64 on 8, 97.6 us
-// (3.8 TB/s); one over 1024 9 us, nearly all of it launch and latency.  Long
-// caches are bound by the unpacking instructions (about 390 a tile of 16 tokens,
-// a third of them for scales and zero points).
+// Measured: one token over 131072, 32 query heads on 8, heads of 128, 49.6
+// us (3.2 TB/s); one token of 64 ragged sequences up to 8192, 64 on 8, 102 us
+// (3.6 TB/s); one over 1024 9.2 us, nearly all of it launch and latency.  Long
+// caches are bound by the unpacking instructions (396 a tile of 16 tokens, a
+// third of them for scales and zero points; issue slots 62 % taken, ALU 44 %).
 #include <math.h>
 
 #include <algorithm>

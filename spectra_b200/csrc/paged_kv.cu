@@ -25,8 +25,8 @@
 // their sequences, positions and pages and brings their angles first.
 // Bound by HBM: 2 bytes in and out per query value, 2 in and 0.59 out per key
 // or value.  Measured: append and read back of 16384 tokens, 64 query heads on
-// 8, heads of 128, 163 us together (4.4 TB/s, 69 % of the copy rate); one token
-// of 128 sequences 20.6 us, which is the two calls on the host.
+// 8, heads of 128, 162 us together (4.4 TB/s, 69 % of the copy rate); one token
+// of 128 sequences 20.7 us, which is the two calls on the host.
 #include <math.h>
 
 #include <algorithm>

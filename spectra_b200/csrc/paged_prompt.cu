@@ -10,7 +10,8 @@
 //   warps 8-11  bring the raw tiles in by bulk copies and write them to shared
 //               memory as fp16 operands: K [token][feature] and V^T
 //               [feature][token], K-major, 128-byte swizzle; two warps a step,
-//               in turn.  (q - z) s is an exact difference and one rounding (11 bits).
+//               in turn.  (q - z) s is an exact difference and one rounding (11 bits),
+//               or two exact operands (Cfg).
 //   warps 12, 13  S_t = Q_t K^T (Q in shared memory) and O_t += P_t V (P in
 //               TMEM), t = 0, 1.  Each tile has two S buffers, so the scores of
 //               the next step are there when a softmax ends.
@@ -28,15 +29,17 @@
 // whose partial results a second small kernel puts together.
 //
 // Rounded to fp16's 11 bits: queries (fp16: not at all, bf16: only as said),
-// keys and values, because fp16 operands run at the full tensor rate and the
-// codes carry 4 bits; weights, kept times 2^kShift so that small ones are not
-// subnormal.  Scores, maxima, sums and outputs stay in fp32.
+// keys and values (except where Cfg has two operands), because fp16 operands run
+// at the full tensor rate and the codes carry 4 bits; weights, kept times 2^kShift
+// so that small ones are not subnormal (below 2^-28 of the largest they are lost
+// from O, not from their sum).  Scores, maxima, sums and outputs stay in fp32.
 //
-// Measured: 4096 tokens over 16384, 32 query heads on 8, heads of 128, 1097 us
-// (877 TFLOP/s over the visible pairs); a prompt of 1024 tokens 31 us; 6 ragged
-// prompts up to 2501 with a cap, 64 query heads on 8, heads of 64, 443 us.
+// Measured: 4096 tokens over 16384, 32 query heads on 8, heads of 128, 1101 us
+// (874 TFLOP/s over the visible pairs); a prompt of 1024 tokens 31 us; 6 ragged
+// prompts up to 2501 with a cap, 64 query heads on 8, heads of 64, fp16, 448 us.
 // Bound by the softmax warps (one exponential a score on the special-function
-// unit, and their issue slots) with the tensor pipe close behind.
+// unit, and their issue slots) with the tensor pipe close behind; short prompts
+// and small heads also by what a step waits for and by instruction fetches.
 #include <math.h>
 
 #include <algorithm>
