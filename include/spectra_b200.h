@@ -319,6 +319,23 @@ SPECTRA_API int spectra_paged_kv_append(
     void* stream);
 
 /*
+ * The same for tokens whose position has several axes (time, height and width
+ * of an image's or a video's patch, say): pair i is turned by row
+ * positions[pair_axes[i]][t] of cos and sin, whatever the token's place in its
+ * sequence.  A row outside [0, cs_rows) turns the pair into NaN.
+ *   positions device int32, element (axis, t) at axis * pos_row_stride + t;
+ *   axes 1..SPECTRA_MAX_POSITION_AXES; pair_axes host memory, rotary / 2 bytes
+ *   below axes, read before the call returns; cos, sin any cs_rows >= 1 rows.
+ */
+#define SPECTRA_MAX_POSITION_AXES 4
+SPECTRA_API int spectra_paged_kv_append_axes(
+    const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
+    const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int64_t qo_ts, int64_t qo_hs,
+    const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
+    const float* cos, const float* sin, int64_t cs_rows, int64_t cs_row_stride, int64_t rotary, int interleaved,
+    const int32_t* positions, int64_t pos_row_stride, int64_t axes, const uint8_t* pair_axes, void* stream);
+
+/*
  * What the cache holds of the batch's new tokens: k, v [total][kv_heads][D]
  * contiguous on 16-byte boundaries, (q - z) s rounded once to out_dtype (F16, BF16, F32);
  * 0 for padding and for tokens that no page holds.
@@ -349,9 +366,74 @@ SPECTRA_API int spectra_paged_attention(
     float scale, float softcap, const float* slopes, int causal, int64_t window,
     void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * The same over some blocks of the keys: row (token t, head h) sees, of the
+ * keys above, those in the blocks that are listed for t and h's key/value
+ * head.  Block j of a sequence is its tokens j * block_size .. (j + 1) *
+ * block_size - 1.  A list is read from its start; an entry that is not above
+ * every entry before it (a repeated one, a negative one) is passed over, and
+ * so is a block past the sequence's end.
+ *   blocks device int32, entry i of (t, kv head) at t * b_ts + head * b_hs + i;
+ *   0 < count <= SPECTRA_MAX_LISTED_BLOCKS; block_size a power of two, 32..65536.
+ */
+#define SPECTRA_MAX_LISTED_BLOCKS 1024
+SPECTRA_API int spectra_paged_attention_blocks(
+    const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
+    const void* q, int64_t q_ts, int64_t q_hs, void* out, int64_t o_ts, int64_t o_hs,
+    float scale, float softcap, const float* slopes, int causal, int64_t window,
+    const int32_t* blocks, int64_t b_ts, int64_t b_hs, int64_t count, int64_t block_size,
+    void* workspace, size_t workspace_bytes, void* stream);
+
 #define SPECTRA_PAGED_COUNTER_BYTES 4096
 
 SPECTRA_API size_t spectra_paged_attention_workspace_bytes(int64_t head_dim);
+
+/*
+ * A block index: of every block of block_size tokens of a page and every head,
+ * the range of its keys, feature by feature, as integers of 8 bits and one
+ * power of two:
+ *   hi_d, lo_d = the largest and smallest (q - z) s of feature d in the block
+ *   S = the least 2^e with max(|hi|, |lo|) <= 127 S  (1 where all are 0)
+ *   codes[0][d] = ceil(hi_d / S), codes[1][d] = floor(lo_d / S), scale = S
+ * (exact, so equal keys give equal bits).  A block with a NaN or infinite key
+ * has codes 0 and an infinite scale.
+ *   codes int8 [num_pages][kv_heads][page_size / block_size][2][head_dim], on a
+ *   16-byte boundary; scales fp32 [num_pages][kv_heads][page_size / block_size];
+ *   block_size a power of two, 32..page_size.
+ */
+typedef struct {
+  int8_t* codes;
+  float* scales;
+  int64_t block_size;
+} SpectraBlockIndex;
+
+/* Writes the index of every block whose last token is one of the batch's new
+ * tokens (append them first).  No other block of the index is written. */
+SPECTRA_API int spectra_paged_index_update(const SpectraPagedCache* cache, const SpectraTokenBatch* batch,
+                                           const SpectraBlockIndex* index, void* stream);
+
+/*
+ * The blocks that each new token looks at.  For the token at position p and a
+ * key/value head, of the blocks 0 .. p / block_size the first `first` and the
+ * last `last` (the token's own among them, whose index is never read), then
+ * those of the highest score, the lowest number first among equal ones, until
+ * there are `count`:
+ *   score(j) = S_j max_h sum_d (c_hd > 0 ? c_hd hi_jd : c_hd lo_jd)
+ * over the head's query heads h, with the codes hi, lo and the scale S of the
+ * index and c_hd = rint(q_hd / s_h), s_h the least 2^e, e >= -126, with
+ * max |q_h| <= 127 s_h (halves to even; a head that holds a NaN or infinity has
+ * c 0).  The sums are integers, so the choice is exact.  An infinite S scores
+ * above all; a block whose page the table does not name is never taken.
+ *   blocks device int32, entry i of (t, head) at t * b_ts + head * b_hs + i:
+ *   the numbers in ascending order, then -1 up to `count`; padding rows -1.
+ *   first >= 0, last >= 1, first + last <= count <= SPECTRA_MAX_LISTED_BLOCKS;
+ *   min(max_len, width * page_size) <= SPECTRA_MAX_INDEXED_BLOCKS * block_size.
+ */
+#define SPECTRA_MAX_INDEXED_BLOCKS 32768
+SPECTRA_API int spectra_paged_select_blocks(
+    const SpectraPagedCache* cache, const SpectraTokenBatch* batch, const SpectraBlockIndex* index, int dtype,
+    int64_t q_heads, const void* q, int64_t q_ts, int64_t q_hs, int64_t count, int64_t first, int64_t last,
+    int32_t* blocks, int64_t b_ts, int64_t b_hs, void* stream);
 
 /*
  * Quantised token-embedding gather (replaces SpectraFusedEmbedding.forward,
@@ -384,6 +466,57 @@ SPECTRA_API int spectra_w4a16_embedding(
  */
 SPECTRA_API int spectra_argmax(const void* x, int x_dtype, int64_t x_row_stride, int64_t M, int64_t N,
                                int64_t idx_offset, int64_t* idx, float* val, void* stream);
+
+/*
+ * Rules on the logits of a step: penalties for tokens that a sequence holds
+ * already, biases, and a mask of the tokens that may follow (the place of the
+ * engine's apply_sampling_penalties, spectra/engine.py:1626-1713; the formulas
+ * here are this library's own).  All of it device memory, one row per row of
+ * the logits; a NULL member leaves its rule out.
+ *   ids int32 [M][max_ids], row stride ids_stride: the tokens of the row's
+ *       sequence, the prompt first; lengths int32 [M] of them count (NULL:
+ *       max_ids); the first prompt_lengths int32 [M] are the prompt (NULL: 0)
+ *   repetition, frequency, presence fp32 [M]
+ *   bias_ids int32 [M][n_bias], bias fp32 [M][n_bias], row strides
+ *   allowed int32 [M][allowed_words], row stride: bit i % 32 of word i / 32 set:
+ *       token i may follow
+ * A negative id, or one past the vocabulary, names no token.
+ */
+typedef struct {
+  const int32_t* ids;
+  int64_t ids_stride, max_ids;
+  const int32_t* lengths;
+  const int32_t* prompt_lengths;
+  const float* repetition;
+  const float* frequency;
+  const float* presence;
+  const int32_t* bias_ids;
+  int64_t bias_ids_stride;
+  const float* bias;
+  int64_t bias_stride, n_bias;
+  const int32_t* allowed;
+  int64_t allowed_stride, allowed_words;
+} SpectraLogitRules;
+
+/*
+ * Row m of x [M, N] under the rules, token n + idx_offset at column n (an
+ * N-sharded head's slice).  In fp32, each step rounded by itself:
+ *   a token in ids[0 .. length): x = x > 0 ? x / repetition : x * repetition
+ *   n times in ids[prompt_length .. length), n > 0: x = x - frequency * n, then x = x - presence
+ *   x = x + bias (of an id that is listed more than once the last one)
+ *   not allowed: -infinity, whatever x was
+ * out (optional) is x rounded once to out_dtype; it may be x itself (the same
+ * dtype and stride), otherwise they do not overlap.  idx[m] (optional) =
+ * idx_offset + the first column of the maximum among the allowed, before the
+ * rounding (a NaN counts as the maximum), -1 where nothing is allowed; val[m]
+ * (optional, with idx) = that maximum, -infinity where there is none.
+ * max_ids <= SPECTRA_MAX_RULE_IDS, n_bias <= SPECTRA_MAX_RULE_BIASES.
+ */
+#define SPECTRA_MAX_RULE_IDS 524287
+#define SPECTRA_MAX_RULE_BIASES 4095
+SPECTRA_API int spectra_adjust_logits(const SpectraLogitRules* rules, const void* x, int x_dtype, int64_t x_row_stride,
+                                      int64_t M, int64_t N, int64_t idx_offset, void* out, int out_dtype,
+                                      int64_t out_row_stride, int64_t* idx, float* val, void* stream);
 
 /*
  * Walsh-Hadamard rotation of activation rows, the optional GEMV prologue

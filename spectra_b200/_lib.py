@@ -19,6 +19,9 @@ ERR_NULL_POINTER, ERR_SHAPE, ERR_STRIDE, ERR_ALIGNMENT, ERR_DTYPE, ERR_WORKSPACE
 ABI_VERSION = 1
 P2P_STATE_INTS = 128  # SPECTRA_P2P_STATE_INTS
 PAGED_COUNTER_BYTES = 4096  # SPECTRA_PAGED_COUNTER_BYTES
+MAX_POSITION_AXES = 4  # SPECTRA_MAX_POSITION_AXES
+MAX_LISTED_BLOCKS, MAX_INDEXED_BLOCKS = 1024, 32768  # SPECTRA_MAX_LISTED_BLOCKS, SPECTRA_MAX_INDEXED_BLOCKS
+MAX_RULE_IDS, MAX_RULE_BIASES = 524287, 4095  # SPECTRA_MAX_RULE_IDS, SPECTRA_MAX_RULE_BIASES
 P2P_SIGNAL_BYTES = 8 * 128 * 4  # epoch flags [rank][cta] at the start of an exchange buffer
 
 
@@ -32,6 +35,17 @@ class TokenBatch(ctypes.Structure):  # SpectraTokenBatch
     _fields_ = [("block_tables", c_void_p), ("table_stride", c_int64), ("width", c_int64),
                 ("seq_lens", c_void_p), ("cu_q", c_void_p), ("batch", c_int64), ("q_len", c_int64),
                 ("total", c_int64), ("max_q", c_int64), ("max_len", c_int64)]
+
+
+class BlockIndex(ctypes.Structure):  # SpectraBlockIndex
+    _fields_ = [("codes", c_void_p), ("scales", c_void_p), ("block_size", c_int64)]
+
+
+class LogitRules(ctypes.Structure):  # SpectraLogitRules
+    _fields_ = [("ids", c_void_p), ("ids_stride", c_int64), ("max_ids", c_int64), ("lengths", c_void_p),
+                ("prompt_lengths", c_void_p), ("repetition", c_void_p), ("frequency", c_void_p), ("presence", c_void_p),
+                ("bias_ids", c_void_p), ("bias_ids_stride", c_int64), ("bias", c_void_p), ("bias_stride", c_int64),
+                ("n_bias", c_int64), ("allowed", c_void_p), ("allowed_stride", c_int64), ("allowed_words", c_int64)]
 
 
 # name -> (restype, argtypes)
@@ -92,6 +106,15 @@ PROTOTYPES = {
         c_void_p, c_int64, c_int64,                    # v
         c_void_p, c_void_p, c_int64, c_int64,          # cos, sin, rows, row stride
         c_int64, c_int, c_void_p]),                    # rotary, interleaved, stream
+    "spectra_paged_kv_append_axes": (c_int, [
+        c_void_p, c_void_p, c_int, c_int64,            # cache, batch, dtype, q_heads
+        c_void_p, c_int64, c_int64,                    # q
+        c_void_p, c_int64, c_int64,                    # q_out
+        c_void_p, c_int64, c_int64,                    # k
+        c_void_p, c_int64, c_int64,                    # v
+        c_void_p, c_void_p, c_int64, c_int64,          # cos, sin, rows, row stride
+        c_int64, c_int,                                # rotary, interleaved
+        c_void_p, c_int64, c_int64, c_void_p, c_void_p]),  # positions, row stride, axes, pair_axes, stream
     "spectra_paged_kv_read": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
     "spectra_paged_attention": (c_int, [
         c_void_p, c_void_p, c_int, c_int64,            # cache, batch, dtype, q_heads
@@ -99,7 +122,20 @@ PROTOTYPES = {
         c_void_p, c_int64, c_int64,                    # out
         c_float, c_float, c_void_p, c_int, c_int64,    # scale, softcap, slopes, causal, window
         c_void_p, c_size_t, c_void_p]),                # workspace, workspace_bytes, stream
+    "spectra_paged_attention_blocks": (c_int, [
+        c_void_p, c_void_p, c_int, c_int64,            # cache, batch, dtype, q_heads
+        c_void_p, c_int64, c_int64,                    # q
+        c_void_p, c_int64, c_int64,                    # out
+        c_float, c_float, c_void_p, c_int, c_int64,    # scale, softcap, slopes, causal, window
+        c_void_p, c_int64, c_int64, c_int64, c_int64,  # blocks, token stride, head stride, count, block_size
+        c_void_p, c_size_t, c_void_p]),                # workspace, workspace_bytes, stream
     "spectra_paged_attention_workspace_bytes": (c_size_t, [c_int64]),
+    "spectra_paged_index_update": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
+    "spectra_paged_select_blocks": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_int, c_int64,  # cache, batch, index, dtype, q_heads
+        c_void_p, c_int64, c_int64,                    # q
+        c_int64, c_int64, c_int64,                     # count, first, last
+        c_void_p, c_int64, c_int64, c_void_p]),        # blocks, token stride, head stride, stream
     "spectra_w4a16_embedding": (c_int, [
         c_void_p, c_int, c_int64,                      # ids, ids_dtype, T
         c_void_p, c_int64, c_void_p, c_int64,          # packed, scales
@@ -109,6 +145,11 @@ PROTOTYPES = {
         c_void_p, c_int, c_int64,                      # out, out_dtype, out_row_stride
         c_int64, c_int64, c_int, c_void_p]),           # V, K, layout, stream
     "spectra_argmax": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "spectra_adjust_logits": (c_int, [
+        c_void_p, c_void_p, c_int, c_int64,            # rules, x, x_dtype, x_row_stride
+        c_int64, c_int64, c_int64,                     # M, N, idx_offset
+        c_void_p, c_int, c_int64,                      # out, out_dtype, out_row_stride
+        c_void_p, c_void_p, c_void_p]),                # idx, val, stream
     "spectra_fwht": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p]),
     "spectra_p2p_buffer_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
     "spectra_p2p_alloc": (c_int, [c_int64, c_void_p, c_void_p]),

@@ -13,6 +13,7 @@
 #include "format.h"
 #include "gemm.h"
 #include "gemv.h"
+#include "logits.h"
 #include "p2p.h"
 #include "paged.h"
 
@@ -479,11 +480,19 @@ bool head_rows_vec(const void* p, int64_t ts, int64_t hs) { return aligned(p, 16
 bool is_half_dt(int dt) { return dt == SPECTRA_DT_F16 || dt == SPECTRA_DT_BF16; }
 }  // namespace
 
-int spectra_paged_kv_append(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
-                            const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int64_t qo_ts, int64_t qo_hs,
-                            const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
-                            const float* cos, const float* sin, int64_t cs_rows, int64_t cs_row_stride, int64_t rotary,
-                            int interleaved, void* stream) {
+namespace {
+// What rotate-and-append turns by besides a token's own position.
+struct AppendAxes {
+  const int32_t* positions;
+  int64_t pos_row_stride, axes;
+  const uint8_t* pair_axes;  // host, [rotary / 2]
+};
+
+int append_checked(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads, const void* q,
+                   int64_t q_ts, int64_t q_hs, void* q_out, int64_t qo_ts, int64_t qo_hs, const void* k, int64_t k_ts,
+                   int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs, const float* cos, const float* sin,
+                   int64_t cs_rows, int64_t cs_row_stride, int64_t rotary, int interleaved, const AppendAxes* by,
+                   void* stream) {
   PagedAppendArgs a = {};
   bool empty = false;
   const int st = paged_view(cache, batch, a.c, empty);
@@ -491,23 +500,59 @@ int spectra_paged_kv_append(const SpectraPagedCache* cache, const SpectraTokenBa
   if (!is_half_dt(dtype)) return SPECTRA_ERR_DTYPE;
   if (rotary < 0 || rotary > cache->head_dim || rotary % (interleaved ? 8 : 16) != 0) return SPECTRA_ERR_SHAPE;
   if (q && (q_heads <= 0 || q_heads > 65535)) return SPECTRA_ERR_SHAPE;
+  if (by) {
+    if (by->axes < 1 || by->axes > SPECTRA_MAX_POSITION_AXES || rotary == 0) return SPECTRA_ERR_SHAPE;
+    if (!by->pair_axes) return SPECTRA_ERR_NULL_POINTER;
+    for (int64_t i = 0; i < rotary / 2; ++i) {
+      if (by->pair_axes[i] >= by->axes) return SPECTRA_ERR_SHAPE;
+      a.pair_axes[i / 16] |= uint32_t(by->pair_axes[i]) << (2 * (i % 16));
+    }
+  }
   if (empty) return SPECTRA_OK;
-  if (!k || !v || (q && !q_out) || (rotary > 0 && (!cos || !sin))) return SPECTRA_ERR_NULL_POINTER;
-  if (rotary > 0 && (cs_rows < a.c.limit || cs_row_stride < rotary / 2)) return SPECTRA_ERR_SHAPE;
-  if (!head_rows_ok(k_ts, k_hs) || !head_rows_ok(v_ts, v_hs) || (q && (!head_rows_ok(q_ts, q_hs) || !head_rows_ok(qo_ts, qo_hs))))
+  if (!k || !v || (q && !q_out) || (rotary > 0 && (!cos || !sin)) || (by && !by->positions)) return SPECTRA_ERR_NULL_POINTER;
+  if (rotary > 0 && (cs_rows < (by ? 1 : a.c.limit) || cs_row_stride < rotary / 2)) return SPECTRA_ERR_SHAPE;
+  if (!head_rows_ok(k_ts, k_hs) || !head_rows_ok(v_ts, v_hs) || (q && (!head_rows_ok(q_ts, q_hs) || !head_rows_ok(qo_ts, qo_hs))) ||
+      (by && by->axes > 1 && by->pos_row_stride < 0))
     return SPECTRA_ERR_STRIDE;
   if (!aligned(k, 2) || !aligned(v, 2) || (q && (!aligned(q, 2) || !aligned(q_out, 2))) ||
-      (rotary > 0 && (!aligned(cos, 4) || !aligned(sin, 4))))
+      (rotary > 0 && (!aligned(cos, 4) || !aligned(sin, 4))) || (by && !aligned(by->positions, 4)))
     return SPECTRA_ERR_ALIGNMENT;
   a.q = q; a.q_ts = q_ts; a.q_hs = q_hs;
   a.q_out = q_out; a.qo_ts = qo_ts; a.qo_hs = qo_hs;
   a.k = k; a.k_ts = k_ts; a.k_hs = k_hs;
   a.v = v; a.v_ts = v_ts; a.v_hs = v_hs;
   a.dtype = dtype; a.q_heads = q ? int(q_heads) : 0;
-  a.cos = cos; a.sin = sin; a.cs_rs = cs_row_stride; a.rotary = int(rotary); a.interleaved = interleaved != 0;
+  a.cos = cos; a.sin = sin; a.cs_rs = cs_row_stride; a.cs_rows = cs_rows;
+  a.rotary = int(rotary); a.interleaved = interleaved != 0;
+  if (by) {
+    a.positions = by->positions;
+    a.pos_rs = by->pos_row_stride;
+    a.axes = int(by->axes);
+  }
   a.vec = head_rows_vec(k, k_ts, k_hs) && head_rows_vec(v, v_ts, v_hs) &&
           (!q || (head_rows_vec(q, q_ts, q_hs) && head_rows_vec(q_out, qo_ts, qo_hs)));
   return launch_paged_append(a, static_cast<cudaStream_t>(stream));
+}
+}  // namespace
+
+int spectra_paged_kv_append(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
+                            const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int64_t qo_ts, int64_t qo_hs,
+                            const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
+                            const float* cos, const float* sin, int64_t cs_rows, int64_t cs_row_stride, int64_t rotary,
+                            int interleaved, void* stream) {
+  return append_checked(cache, batch, dtype, q_heads, q, q_ts, q_hs, q_out, qo_ts, qo_hs, k, k_ts, k_hs, v, v_ts, v_hs, cos,
+                        sin, cs_rows, cs_row_stride, rotary, interleaved, nullptr, stream);
+}
+
+int spectra_paged_kv_append_axes(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
+                                 const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int64_t qo_ts, int64_t qo_hs,
+                                 const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
+                                 const float* cos, const float* sin, int64_t cs_rows, int64_t cs_row_stride, int64_t rotary,
+                                 int interleaved, const int32_t* positions, int64_t pos_row_stride, int64_t axes,
+                                 const uint8_t* pair_axes, void* stream) {
+  const AppendAxes by = {positions, pos_row_stride, axes, pair_axes};
+  return append_checked(cache, batch, dtype, q_heads, q, q_ts, q_hs, q_out, qo_ts, qo_hs, k, k_ts, k_hs, v, v_ts, v_hs, cos,
+                        sin, cs_rows, cs_row_stride, rotary, interleaved, &by, stream);
 }
 
 int spectra_paged_kv_read(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, void* k, void* v, int out_dtype,
@@ -524,10 +569,22 @@ int spectra_paged_kv_read(const SpectraPagedCache* cache, const SpectraTokenBatc
   return launch_paged_read(a, static_cast<cudaStream_t>(stream));
 }
 
-int spectra_paged_attention(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
-                            const void* q, int64_t q_ts, int64_t q_hs, void* out, int64_t o_ts, int64_t o_hs, float scale,
-                            float softcap, const float* slopes, int causal, int64_t window, void* workspace,
-                            size_t workspace_bytes, void* stream) {
+namespace {
+struct BlockLists {
+  const int32_t* blocks;
+  int64_t b_ts, b_hs, count, block_size;
+};
+bool is_block_size(int64_t n) { return n >= 32 && n <= 65536 && (n & (n - 1)) == 0; }
+int log2_of(int64_t n) {
+  int l = 0;
+  while ((int64_t(1) << l) < n) ++l;
+  return l;
+}
+
+int attention_checked(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
+                      const void* q, int64_t q_ts, int64_t q_hs, void* out, int64_t o_ts, int64_t o_hs, float scale,
+                      float softcap, const float* slopes, int causal, int64_t window, const BlockLists* lists,
+                      void* workspace, size_t workspace_bytes, void* stream) {
   PagedAttnArgs a = {};
   bool empty = false;
   const int st = paged_view(cache, batch, a.c, empty);
@@ -537,10 +594,14 @@ int spectra_paged_attention(const SpectraPagedCache* cache, const SpectraTokenBa
   const int64_t most = batch->cu_q ? batch->max_q : std::min(batch->q_len, batch->total);
   if (most > (INT32_MAX - 4096) / q_heads) return SPECTRA_ERR_SHAPE;  // rows of a sequence are counted in 32 bits
   if (!(scale > 0.f) || !std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap)) return SPECTRA_ERR_UNSUPPORTED;
+  if (lists && !is_block_size(lists->block_size)) return SPECTRA_ERR_UNSUPPORTED;
+  if (lists && (lists->count <= 0 || lists->count > SPECTRA_MAX_LISTED_BLOCKS)) return SPECTRA_ERR_SHAPE;
   if (empty) return SPECTRA_OK;
-  if (!q || !out || !workspace) return SPECTRA_ERR_NULL_POINTER;
-  if (!head_rows_ok(q_ts, q_hs) || !head_rows_ok(o_ts, o_hs)) return SPECTRA_ERR_STRIDE;
-  if (!aligned(q, 2) || !aligned(out, 2) || (slopes && !aligned(slopes, 4)) || !aligned(workspace, 16))
+  if (!q || !out || !workspace || (lists && !lists->blocks)) return SPECTRA_ERR_NULL_POINTER;
+  if (!head_rows_ok(q_ts, q_hs) || !head_rows_ok(o_ts, o_hs) || (lists && !head_rows_ok(lists->b_ts, lists->b_hs)))
+    return SPECTRA_ERR_STRIDE;
+  if (!aligned(q, 2) || !aligned(out, 2) || (slopes && !aligned(slopes, 4)) || !aligned(workspace, 16) ||
+      (lists && !aligned(lists->blocks, 4)))
     return SPECTRA_ERR_ALIGNMENT;
   if (workspace_bytes < spectra_paged_attention_workspace_bytes(cache->head_dim)) return SPECTRA_ERR_WORKSPACE;
   a.q = q; a.q_ts = q_ts; a.q_hs = q_hs;
@@ -550,7 +611,85 @@ int spectra_paged_attention(const SpectraPagedCache* cache, const SpectraTokenBa
   a.window = int(std::min<int64_t>(window, INT32_MAX));
   a.vec = head_rows_vec(q, q_ts, q_hs) && head_rows_vec(out, o_ts, o_hs);
   a.workspace = workspace; a.workspace_bytes = workspace_bytes;
-  return launch_paged_attention(a, static_cast<cudaStream_t>(stream));
+  if (!lists) return launch_paged_attention(a, static_cast<cudaStream_t>(stream));
+  a.blocks = lists->blocks; a.b_ts = lists->b_ts; a.b_hs = lists->b_hs;
+  a.count = int(lists->count); a.block_log2 = log2_of(lists->block_size);
+  return launch_paged_attn_blocks(a, static_cast<cudaStream_t>(stream));
+}
+
+// Checks of an index beside its cache, which has been checked.
+int paged_index(const SpectraPagedCache* cache, const SpectraBlockIndex* index, PagedIndexArgs& a) {
+  if (!index) return SPECTRA_ERR_NULL_POINTER;
+  if (!is_block_size(index->block_size) || index->block_size > cache->page_size) return SPECTRA_ERR_UNSUPPORTED;
+  a.codes = index->codes;
+  a.scales = index->scales;
+  a.block_log2 = log2_of(index->block_size);
+  return SPECTRA_OK;
+}
+int index_memory(const PagedIndexArgs& a) {
+  if (a.c.num_pages > 0 && (!a.codes || !a.scales)) return SPECTRA_ERR_NULL_POINTER;
+  return aligned(a.codes, 16) && aligned(a.scales, 4) ? SPECTRA_OK : SPECTRA_ERR_ALIGNMENT;
+}
+}  // namespace
+
+int spectra_paged_attention(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
+                            const void* q, int64_t q_ts, int64_t q_hs, void* out, int64_t o_ts, int64_t o_hs, float scale,
+                            float softcap, const float* slopes, int causal, int64_t window, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  return attention_checked(cache, batch, dtype, q_heads, q, q_ts, q_hs, out, o_ts, o_hs, scale, softcap, slopes, causal, window,
+                           nullptr, workspace, workspace_bytes, stream);
+}
+
+int spectra_paged_attention_blocks(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, int dtype, int64_t q_heads,
+                                   const void* q, int64_t q_ts, int64_t q_hs, void* out, int64_t o_ts, int64_t o_hs,
+                                   float scale, float softcap, const float* slopes, int causal, int64_t window,
+                                   const int32_t* blocks, int64_t b_ts, int64_t b_hs, int64_t count, int64_t block_size,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  const BlockLists lists = {blocks, b_ts, b_hs, count, block_size};
+  return attention_checked(cache, batch, dtype, q_heads, q, q_ts, q_hs, out, o_ts, o_hs, scale, softcap, slopes, causal, window,
+                           &lists, workspace, workspace_bytes, stream);
+}
+
+int spectra_paged_index_update(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, const SpectraBlockIndex* index,
+                               void* stream) {
+  PagedIndexArgs a = {};
+  bool empty = false;
+  int st = paged_view(cache, batch, a.c, empty);
+  if (st == SPECTRA_OK) st = paged_index(cache, index, a);
+  if (st != SPECTRA_OK || empty) return st;
+  st = index_memory(a);
+  if (st != SPECTRA_OK || a.c.num_pages == 0) return st;
+  return launch_paged_index(a, static_cast<cudaStream_t>(stream));
+}
+
+int spectra_paged_select_blocks(const SpectraPagedCache* cache, const SpectraTokenBatch* batch, const SpectraBlockIndex* index,
+                                int dtype, int64_t q_heads, const void* q, int64_t q_ts, int64_t q_hs, int64_t count,
+                                int64_t first, int64_t last, int32_t* blocks, int64_t b_ts, int64_t b_hs, void* stream) {
+  PagedSelectArgs a = {};
+  bool empty = false;
+  int st = paged_view(cache, batch, a.i.c, empty);
+  if (st == SPECTRA_OK) st = paged_index(cache, index, a.i);
+  if (st != SPECTRA_OK) return st;
+  if (!is_half_dt(dtype)) return SPECTRA_ERR_DTYPE;
+  if (q_heads <= 0 || q_heads > 65535 || q_heads % cache->kv_heads != 0) return SPECTRA_ERR_SHAPE;
+  if (count <= 0 || count > SPECTRA_MAX_LISTED_BLOCKS || first < 0 || last < 1 || first > count || last > count - first)
+    return SPECTRA_ERR_SHAPE;
+  if (empty) return SPECTRA_OK;
+  const int64_t most = (int64_t(a.i.c.limit) + index->block_size - 1) / index->block_size;
+  if (most > SPECTRA_MAX_INDEXED_BLOCKS) return SPECTRA_ERR_SHAPE;
+  if (!q || !blocks) return SPECTRA_ERR_NULL_POINTER;
+  if (!head_rows_ok(q_ts, q_hs) || b_ts < (a.i.c.total > 1 ? count : 0) || b_hs < (cache->kv_heads > 1 ? count : 0))
+    return SPECTRA_ERR_STRIDE;
+  st = index_memory(a.i);
+  if (st != SPECTRA_OK) return st;
+  if (!aligned(q, 2) || !aligned(blocks, 4)) return SPECTRA_ERR_ALIGNMENT;
+  a.q = q; a.q_ts = q_ts; a.q_hs = q_hs;
+  a.dtype = dtype; a.q_heads = int(q_heads); a.group = int(q_heads / cache->kv_heads);
+  a.count = int(count); a.first = int(first); a.last = int(last);
+  a.max_blocks = int(most);
+  a.vec = head_rows_vec(q, q_ts, q_hs);
+  a.blocks = blocks; a.b_ts = b_ts; a.b_hs = b_hs;
+  return launch_paged_select(a, static_cast<cudaStream_t>(stream));
 }
 
 size_t spectra_paged_attention_workspace_bytes(int64_t head_dim) {
@@ -604,6 +743,40 @@ int spectra_argmax(const void* x, int x_dtype, int64_t x_row_stride, int64_t M, 
   a.x = x; a.x_dtype = x_dtype; a.x_rs = x_row_stride;
   a.idx = idx; a.val = val; a.M = M; a.N = N; a.idx_offset = idx_offset;
   return launch_argmax(a, static_cast<cudaStream_t>(stream));
+}
+
+int spectra_adjust_logits(const SpectraLogitRules* rules, const void* x, int x_dtype, int64_t x_row_stride, int64_t M, int64_t N,
+                          int64_t idx_offset, void* out, int out_dtype, int64_t out_row_stride, int64_t* idx, float* val,
+                          void* stream) {
+  if (!rules || !x || (!out && !idx) || (val && !idx)) return SPECTRA_ERR_NULL_POINTER;
+  if (M < 0 || N <= 0 || idx_offset < 0 || !fits_i32(N) || !fits_i32(idx_offset) || !fits_i32(idx_offset + N)) return SPECTRA_ERR_SHAPE;
+  if (!is_float_dt(x_dtype) || (out && !is_float_dt(out_dtype))) return SPECTRA_ERR_DTYPE;
+  if (M > 1 && (x_row_stride < N || (out && out_row_stride < N))) return SPECTRA_ERR_STRIDE;
+  LogitArgs a;
+  a.r = *rules;
+  SpectraLogitRules& r = a.r;
+  if (!r.ids || (!r.repetition && !r.frequency && !r.presence)) {
+    r.ids = nullptr;
+    r.max_ids = 0;
+  }
+  if (!r.bias_ids || !r.bias) r.n_bias = 0;
+  if (r.max_ids < 0 || r.max_ids > SPECTRA_MAX_RULE_IDS || r.n_bias < 0 || r.n_bias > SPECTRA_MAX_RULE_BIASES)
+    return SPECTRA_ERR_SHAPE;
+  if (r.allowed && r.allowed_words < (idx_offset + N + 31) / 32) return SPECTRA_ERR_SHAPE;
+  if (M > 1 && ((r.ids && r.ids_stride < 0) || (r.n_bias && (r.bias_ids_stride < 0 || r.bias_stride < 0)) ||
+                (r.allowed && r.allowed_stride < 0)))
+    return SPECTRA_ERR_STRIDE;
+  for (const void* p : {static_cast<const void*>(r.ids), static_cast<const void*>(r.lengths),
+                        static_cast<const void*>(r.prompt_lengths), static_cast<const void*>(r.repetition),
+                        static_cast<const void*>(r.frequency), static_cast<const void*>(r.presence),
+                        static_cast<const void*>(r.bias_ids), static_cast<const void*>(r.bias),
+                        static_cast<const void*>(r.allowed), static_cast<const void*>(val)})
+    if (!aligned(p, 4)) return SPECTRA_ERR_ALIGNMENT;
+  if (!aligned(x, dt_size(x_dtype)) || (out && !aligned(out, dt_size(out_dtype))) || !aligned(idx, 8)) return SPECTRA_ERR_ALIGNMENT;
+  a.x = x; a.x_dtype = x_dtype; a.x_rs = x_row_stride;
+  a.out = out; a.out_dtype = out_dtype; a.out_rs = out_row_stride;
+  a.idx = idx; a.val = val; a.M = M; a.N = N; a.idx_offset = idx_offset;
+  return launch_logits(a, static_cast<cudaStream_t>(stream));
 }
 
 int spectra_fwht(const void* x, int x_dtype, int64_t x_row_stride, void* y, int y_dtype, int64_t y_row_stride,

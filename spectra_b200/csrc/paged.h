@@ -47,8 +47,12 @@ struct PagedAppendArgs {
   const void* k; int64_t k_ts, k_hs;       // [total, kv_heads, D]
   const void* v; int64_t v_ts, v_hs;
   int dtype, q_heads;
-  const float* cos; const float* sin; int64_t cs_rs;  // [limit, rotary / 2] or NULL
+  const float* cos; const float* sin; int64_t cs_rs;  // [cs_rows, rotary / 2] or NULL
+  int64_t cs_rows;
   int rotary, interleaved;
+  const int* positions; int64_t pos_rs;    // [axes, total] rows of cos and sin, or NULL: a token's own position
+  int axes;
+  uint32_t pair_axes[8];                   // axis of pair i: bits 2 (i % 16).. of word i / 16
   int vec;                                 // every row starts on a 16-byte boundary
   int tokens;                              // of a block (set by the launcher)
 };
@@ -71,6 +75,8 @@ struct PagedAttnArgs {
   const float* slopes;                     // [q_heads] or NULL
   int causal, window;                      // window 0: none
   int vec;                                 // rows of q and out on 16-byte boundaries
+  const int* blocks; int64_t b_ts, b_hs;   // listed blocks of (token, kv head), or NULL: all keys
+  int count, block_log2;
   void* workspace; size_t workspace_bytes;
 };
 // A workspace: kPagedCounterBytes of counters (zero between calls), then partial results.
@@ -82,8 +88,30 @@ size_t paged_attn_workspace_bytes(int head_dim);
 size_t paged_prompt_workspace_bytes(int head_dim);
 int launch_paged_attn(const PagedAttnArgs& a, int max_rows, cudaStream_t st);
 int launch_paged_prompt(const PagedAttnArgs& a, int min_rows, cudaStream_t st);
+int launch_paged_attn_blocks(const PagedAttnArgs& a, cudaStream_t st);  // with a.blocks, any number of tokens
 int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st);  // the one or the other, or both
 int paged_attn_timeouts(long long* out, bool reset);
 int paged_prompt_timeouts(long long* out, bool reset);
+
+
+// A block index (paged_index.cu): what it holds is in the public header.
+struct PagedIndexArgs {
+  PagedView c;
+  int8_t* codes;                           // [pages][kv_heads][1 << page_log2 - block_log2][2][D]
+  float* scales;                           // the same without the last two
+  int block_log2;
+};
+int launch_paged_index(const PagedIndexArgs& a, cudaStream_t st);
+
+struct PagedSelectArgs {
+  PagedIndexArgs i;
+  const void* q; int64_t q_ts, q_hs;
+  int dtype, q_heads, group;
+  int count, first, last;
+  int max_blocks;                          // of a sequence: the host's bound
+  int vec;                                 // rows of q on 16-byte boundaries
+  int* blocks; int64_t b_ts, b_hs;
+};
+int launch_paged_select(const PagedSelectArgs& a, cudaStream_t st);
 
 }  // namespace spectra

@@ -59,7 +59,8 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kUnit = 32;          // tokens of a unit: two tiles
+constexpr int kUnitLog2 = 5;
+constexpr int kUnit = 1 << kUnitLog2;  // tokens of a unit: two tiles
 constexpr int kStages = 2;         // units in flight per warp
 constexpr int kMaxCtas = int(kPagedCounterBytes / sizeof(int));
 
@@ -83,7 +84,7 @@ struct Span {  // a sequence's rows and the keys its rows look at
   int tiles;      // row tiles
 };
 
-template <int ROWS>
+template <int ROWS, bool SEL>
 __device__ __forceinline__ Span span_of(const AttnParams& p, int b) {
   const PagedAttnArgs& a = p.a;
   Span s;
@@ -91,9 +92,16 @@ __device__ __forceinline__ Span span_of(const AttnParams& p, int b) {
   const int len = a.c.seq_lens[b];
   s.pos0 = len - s.count - s.extra;
   s.len = len < 0 ? 0 : (len < a.c.limit ? len : a.c.limit);
-  s.tiles = s.count * a.group > p.max_rows ? 0 : (s.count * a.group + ROWS - 1) / ROWS;
-  s.unit0 = first_key(s.pos0, a.window) / kUnit;
-  s.units = max(1, (s.len + kUnit - 1) / kUnit - s.unit0);
+  if constexpr (SEL) {  // a token's list holds each block once at most
+    const int blocks = s.len == 0 ? 0 : ((s.len - 1) >> a.block_log2) + 1;
+    s.tiles = s.count * ((a.group + ROWS - 1) / ROWS);
+    s.unit0 = 0;
+    s.units = max(1, min(a.count, blocks) << (a.block_log2 - kUnitLog2));
+  } else {
+    s.tiles = s.count * a.group > p.max_rows ? 0 : (s.count * a.group + ROWS - 1) / ROWS;
+    s.unit0 = first_key(s.pos0, a.window) / kUnit;
+    s.units = max(1, (s.len + kUnit - 1) / kUnit - s.unit0);
+  }
   return s;
 }
 
@@ -112,6 +120,7 @@ struct Cfg {
   static constexpr int kX = G * NT * 4 * 32;                  // {C, C', C, C'} and {X, X'} of a lane's two rows
   static constexpr int kMeta = ROWS * 16;                     // hi, lo, slope, position of a row
   static constexpr int kCtas = G * NT <= 4 ? 4 : 2;  // per SM: what the registers allow
+  static constexpr int kListCtas = kCtas == 4 ? 3 : kCtas;  // (lists take some more)
   static constexpr int kSmem = kBig + kQ + kX + kMeta + ROWS * 4 + kWarps * kStages * 8;
   static constexpr int kPartial = ROWS * (D + 2);             // floats of one CTA's partial result
 };
@@ -119,8 +128,9 @@ struct Cfg {
 // ------------------------------------------------------------ the kernel
 // MOD: 0 plain scores, 1 a bias or a cap of up to kLowCap, 2 a higher cap (in MOD 1 its code took
 // 35.4 us where 34.2 are taken without it: verification with a bias)
-template <int G, int NT, int MOD>
-__global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel(AttnParams p) {
+// SEL: a segment is one token and the blocks listed for it
+template <int G, int NT, int MOD, bool SEL>
+__global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G, NT>::kCtas) paged_attn_kernel(AttnParams p) {
   using C = Cfg<G, NT>;
   constexpr int D = C::D, ROWS = C::ROWS;
   constexpr TileLayout L{G};
@@ -140,6 +150,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
   __shared__ int s_seq, s_last;
   __shared__ volatile int s_stop;     // a copy did not arrive: the segments after this one load nothing
   __shared__ int s_held[kWarps * kStages];  // tiles of a stage that a page holds
+  __shared__ int s_list[SEL ? SPECTRA_MAX_LISTED_BLOCKS : 1];  // blocks that the segment's token sees
+  __shared__ int s_tops[2][kWarps], s_kepts[2][kWarps];  // by turns: a turn's are read while the next is under way
   __shared__ volatile int s_never;    // 0: each warp waits for its own copies, whatever the others saw
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, cc = lane & 3;
@@ -157,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
   bool over = false;  // a sequence has more new tokens than max_q
   auto units_of = [&](int i) -> long long {
     if (i >= c.batch) return 0;
-    const Span s = span_of<ROWS>(p, i);
+    const Span s = span_of<ROWS, SEL>(p, i);
     over = over || s.extra > 0;
     return (long long)(s.units) * s.tiles * c.kv_heads;
   };
@@ -188,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
     for (int64_t t = (held < 0 ? 0 : held) + int64_t(blockIdx.x); t < c.total; t += gridDim.x) clear(t);
     if (over) {
       for (int i = blockIdx.x; i < c.batch; i += gridDim.x) {
-        const Span s = span_of<ROWS>(p, i);
+        const Span s = span_of<ROWS, SEL>(p, i);
         for (int64_t t = s.first + s.count; t < s.first + s.count + s.extra; ++t) clear(t);
       }
     }
@@ -234,23 +246,82 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
 
   while (at < end) {
     // ---- the segment that holds unit `at`
-    Span s = span_of<ROWS>(p, b);
+    Span s = span_of<ROWS, SEL>(p, b);
     long long seq_units = (long long)(s.units) * s.tiles * c.kv_heads;
     while (at >= seq_base + seq_units) {
       seq_base += seq_units;
       ++b;
-      s = span_of<ROWS>(p, b);
+      s = span_of<ROWS, SEL>(p, b);
       seq_units = (long long)(s.units) * s.tiles * c.kv_heads;
     }
     const int seg = int(unsigned(at - seq_base) / unsigned(s.units));  // (the launch checks that a sequence's fit)
     const long long seg_begin = seq_base + (long long)(seg) * s.units, seg_end = seg_begin + s.units;
-    const int head = seg / s.tiles, row0 = (seg - head * s.tiles) * ROWS;
+    const int head = seg / s.tiles, of_token = (a.group + ROWS - 1) / ROWS;
+    const int only = SEL ? (seg - head * s.tiles) / of_token : 0;  // SEL: the segment's token
+    const int row0 = (seg - head * s.tiles - only * (SEL ? of_token : 0)) * ROWS;
     const int u_begin = s.unit0 + int(at - seg_begin);
     const int u_stop = s.unit0 + int((seg_end < end ? seg_end : end) - seg_begin);
     // nothing held, or a copy that did not arrive in an earlier segment: nothing to load.  (After a
     // loss the results are undefined, but every segment is counted, so that the counters end at zero.)
-    const int u_end = s.len > 0 && !s_stop ? u_stop : u_begin;
-    const int rows = min(ROWS, s.count * a.group - row0);
+    int u_end = s.len > 0 && !s_stop ? u_stop : u_begin;
+    const int rows = SEL ? min(ROWS, a.group - row0) : min(ROWS, s.count * a.group - row0);
+    auto place = [&](int row, int& tok, int& h) {  // token and query head of a row
+      if constexpr (SEL) {
+        tok = only;
+        h = head * a.group + row0 + row;
+      } else {
+        tok = (row0 + row) / a.group;
+        h = head * a.group + (row0 + row) - tok * a.group;
+      }
+    };
+    if constexpr (SEL) {
+      // ---- the token's list: entries above all before them that hold a key it sees
+      const int pos = s.pos0 + only, hi = pos < 0 ? 0 : (a.causal ? min(s.len, pos + 1) : s.len);
+      const int lo = first_key(pos, a.window);
+      const int* list = a.blocks + (s.first + only) * a.b_ts + head * a.b_hs;
+      int most = -1, kept = 0;  // of the entries before
+      for (int i0 = 0; i0 < a.count; i0 += kThreads) {
+        const int e = i0 + tid < a.count ? list[i0 + tid] : -1;
+        int* s_top = s_tops[i0 / kThreads & 1];
+        int* s_kept = s_kepts[i0 / kThreads & 1];
+        int top = e;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, top, o);
+          if (lane >= o) top = max(top, up);
+        }
+        if (lane == 31) s_top[warp] = top;
+        top = __shfl_up_sync(0xffffffffu, top, 1);
+        if (lane == 0) top = -1;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < warp) top = max(top, s_top[w]);
+        }
+        const bool ok = e > max(top, most) && e <= (hi - 1) >> a.block_log2 && e >= lo >> a.block_log2;
+        const uint32_t oks = __ballot_sync(0xffffffffu, ok);
+        if (lane == 0) s_kept[warp] = __popc(oks);
+        __syncthreads();
+        int slot = kept + __popc(oks & ((1u << lane) - 1));
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < warp) slot += s_kept[w];
+          kept += s_kept[w];
+          most = max(most, s_top[w]);
+        }
+        if (ok) s_list[slot] = e;
+      }
+      __syncthreads();
+      u_end = max(u_begin, min(u_end, kept << (a.block_log2 - kUnitLog2)));
+    }
+    auto unit_pos = [&](int u) {  // position of a unit's first token
+      if constexpr (SEL) {
+        const int of_block = a.block_log2 - kUnitLog2;
+        return (s_list[u >> of_block] << a.block_log2) + ((u & ((1 << of_block) - 1)) << kUnitLog2);
+      } else {
+        return u * kUnit;
+      }
+    };
 
     // ---- units to load: warp w takes u_end - 1 - w, - kWarps, ... (the last keys first: a
     // bias on distance only falls on the way).  Lane j knows where the j-th of the next 32
@@ -262,11 +333,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
     const bool small = c.page_log2 == 4;  // a page is one tile
     uint64_t here = 0, here1 = 0, ahead = 0, ahead1 = 0;
     auto look = [&](int from, uint64_t& w0, uint64_t& w1) {  // of the warp's units from `from` on
-      const int u = next - (from + lane) * kWarps, pos = u * kUnit;
+      const int u = next - (from + lane) * kWarps, pos = u >= u_begin ? unit_pos(u) : 0;
       const bool in = u >= u_begin && pos < s.len;
       const int p0 = in ? table[pos >> c.page_log2] : -1;
       const bool h0 = unsigned(p0) < unsigned(c.num_pages);
-      w0 = reinterpret_cast<uint64_t>(head_pool + (h0 ? p0 : 0) * c.page_stride + (u * 2 & (per_page - 1)) * C::kTile) + (h0 ? 3 : 0);
+      w0 = reinterpret_cast<uint64_t>(head_pool + (h0 ? p0 : 0) * c.page_stride + ((pos >> 4) & (per_page - 1)) * C::kTile) + (h0 ? 3 : 0);
       if (small) {
         const int p1 = in && pos + kTileTokens < s.len ? table[(pos >> 4) + 1] : -1;
         const bool h1 = unsigned(p1) < unsigned(c.num_pages);
@@ -308,7 +379,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
 #pragma unroll
         for (int j = 0; j < 4; ++j) raw[grp][j] = 0;
       if (row < rows) {
-        const int tok = (row0 + row) / a.group, h = head * a.group + (row0 + row) - tok * a.group;
+        int tok, h;
+        place(row, tok, h);
         const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (s.first + tok) * a.q_ts + h * a.q_hs + cc * 8;
 #pragma unroll
         for (int grp = 0; grp < G; ++grp) {
@@ -368,7 +440,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
       int hi = 0, lo = 0, pos = 0;
       float slope = 0.f;
       if (tid < rows) {
-        const int tok = (row0 + tid) / a.group, h = head * a.group + (row0 + tid) - tok * a.group;
+        int tok, h;
+        place(tid, tok, h);
         pos = s.pos0 + tok;
         if (pos >= 0) hi = a.causal ? min(s.len, pos + 1) : s.len;
         lo = first_key(pos, a.window);
@@ -460,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
       }
 
       // ---- cap, bias, mask
-      const int n0 = u * kUnit;
+      const int n0 = unit_pos(u);
       if constexpr (MOD != 0) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -618,7 +691,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
     const int cta1 = int(blockIdx.x) + (seg_end > end ? int(unsigned(seg_end - 1 - begin) / step) : 0);
     float* mine = p.partials + int64_t(2 * blockIdx.x + (seg_begin < begin ? 0 : 1)) * C::kPartial;
     auto put = [&](int row, int d, float4 v, float sum) {
-      const int tok = (row0 + row) / a.group, h = head * a.group + (row0 + row) - tok * a.group;
+      int tok, h;
+      place(row, tok, h);
       const float f = sum == 0.f ? 0.f : 1.f / sum;
       const int64_t at_out = (s.first + tok) * a.o_ts + h * a.o_hs + d;
       const float x[4] = {v.x, v.y, v.z, v.w};
@@ -760,7 +834,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<G, NT>::kCtas) paged_attn_kernel
   }
 }
 
-template <int G, int NT, int MOD>
+template <int G, int NT, int MOD, bool SEL>
 int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   using C = Cfg<G, NT>;
   static PerContextOnce once;
@@ -768,7 +842,7 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e);
-  auto kern = paged_attn_kernel<G, NT, MOD>;
+  auto kern = paged_attn_kernel<G, NT, MOD, SEL>;
   e = once.run(dev, [&] {
     cudaError_t r = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (r == cudaSuccess) r = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas_per_sm[dev], kern, kThreads, C::kSmem);
@@ -779,8 +853,13 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   p.a = a;
   p.min_share = kWarps;
   p.max_rows = max_rows;
-  const int64_t tiles = (std::min<int64_t>(int64_t(a.c.max_q) * a.group, max_rows) + C::ROWS - 1) / C::ROWS;
-  const int64_t of_one = int64_t(a.c.kv_heads) * tiles * ((a.c.limit + kUnit - 1) / kUnit + 1);
+  int64_t tiles = (std::min<int64_t>(int64_t(a.c.max_q) * a.group, max_rows) + C::ROWS - 1) / C::ROWS;
+  int64_t units = (a.c.limit + kUnit - 1) / kUnit + 1;
+  if (SEL) {
+    tiles = int64_t(a.c.max_q) * ((a.group + C::ROWS - 1) / C::ROWS);
+    units = std::min<int64_t>(a.count, (int64_t(a.c.limit) >> a.block_log2) + 1) << (a.block_log2 - kUnitLog2);
+  }
+  const int64_t of_one = int64_t(a.c.kv_heads) * tiles * units;
   if (of_one >= (int64_t(1) << 30)) return SPECTRA_ERR_SHAPE;
   const int64_t most = a.c.batch * of_one;
   const int64_t room = std::min<int64_t>(int64_t(device_sms(dev)) * std::max(1, ctas_per_sm[dev]), kMaxCtas);
@@ -802,33 +881,37 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
-template <int G, int NT>
+template <int G, int NT, bool SEL>
 int launch_mod(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
-  if (a.softcap > kLowCap) return launch_one<G, NT, 2>(a, max_rows, st);
-  return a.softcap > 0.f || a.slopes ? launch_one<G, NT, 1>(a, max_rows, st) : launch_one<G, NT, 0>(a, max_rows, st);
+  if (a.softcap > kLowCap) return launch_one<G, NT, 2, SEL>(a, max_rows, st);
+  return a.softcap > 0.f || a.slopes ? launch_one<G, NT, 1, SEL>(a, max_rows, st) : launch_one<G, NT, 0, SEL>(a, max_rows, st);
 }
 
-template <int G>
+template <int G, bool SEL>
 int launch_rows(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
-  // up to 8 rows per key/value head: one column tile (fewer registers, more CTAs per SM); heads of 256 have
-  // no registers for two
-  if (G == 8 || int64_t(a.c.max_q) * a.group <= 8)
-    return launch_mod<G, 1>(a, max_rows, st);
-  return launch_mod<G, G == 8 ? 1 : 2>(a, max_rows, st);
+  // up to 8 rows per key/value head (SEL: of one token): one column tile (fewer registers, more CTAs per SM);
+  // heads of 256 have no registers for two
+  if (G == 8 || (SEL ? 1 : int64_t(a.c.max_q)) * a.group <= 8)
+    return launch_mod<G, 1, SEL>(a, max_rows, st);
+  return launch_mod<G, G == 8 ? 1 : 2, SEL>(a, max_rows, st);
+}
+
+template <bool SEL>
+int launch_dim(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
+  switch (a.c.head_dim) {
+    case 32: return launch_rows<1, SEL>(a, max_rows, st);
+    case 64: return launch_rows<2, SEL>(a, max_rows, st);
+    case 96: return launch_rows<3, SEL>(a, max_rows, st);
+    case 128: return launch_rows<4, SEL>(a, max_rows, st);
+    case 256: return launch_rows<8, SEL>(a, max_rows, st);
+  }
+  return SPECTRA_ERR_UNSUPPORTED;
 }
 
 }  // namespace
 
-int launch_paged_attn(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
-  switch (a.c.head_dim) {
-    case 32: return launch_rows<1>(a, max_rows, st);
-    case 64: return launch_rows<2>(a, max_rows, st);
-    case 96: return launch_rows<3>(a, max_rows, st);
-    case 128: return launch_rows<4>(a, max_rows, st);
-    case 256: return launch_rows<8>(a, max_rows, st);
-  }
-  return SPECTRA_ERR_UNSUPPORTED;
-}
+int launch_paged_attn(const PagedAttnArgs& a, int max_rows, cudaStream_t st) { return launch_dim<false>(a, max_rows, st); }
+int launch_paged_attn_blocks(const PagedAttnArgs& a, cudaStream_t st) { return launch_dim<true>(a, INT32_MAX, st); }
 
 size_t paged_attn_workspace_bytes(int head_dim) {
   return kPagedCounterBytes + size_t(kMaxCtas) * 2 * 16 * (head_dim + 2) * sizeof(float);

@@ -22,7 +22,11 @@
 // One thread takes 8 features (16 bytes) of one head, four threads a group; where
 // a query head is turned as a whole by halves, the pair of 8 that turn into each
 // other, so that nothing is read twice.  A block takes 1 to 8 tokens; it looks up
-// their sequences, positions and pages and brings their angles first.
+// their sequences, positions and pages and brings their angles first.  With
+// positions of several axes (time, height and width of a patch, say) pair i is
+// turned by the row positions[axis of i][token] of the angles; they are loaded
+// before the look-ups, so they add no load to the chain.  A row outside the
+// table turns into NaN.
 // Bound by HBM: 2 bytes in and out per query value, 2 in and 0.59 out per key
 // or value.  Measured: append and read back of 16384 tokens, 64 query heads on
 // 8, heads of 128, 162 us together (4.4 TB/s, 69 % of the copy rate); one token
@@ -42,6 +46,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kMaxSpan = 65472.f;
 constexpr int kTokens = kThreads / 32;  // tokens of a block, at most: a warp looks each of them up
+constexpr int kAxes = 4;                // axes of a token's position, at most
 
 template <bool BF16>
 __device__ __forceinline__ float to_f(uint32_t bits16) {
@@ -245,6 +250,7 @@ __global__ void __launch_bounds__(kThreads, 5) paged_append_kernel(PagedAppendAr
   extern __shared__ float s_angles[];  // [tokens][rotary]
   __shared__ int s_pos[kTokens];
   __shared__ uint8_t* s_tile[kTokens];
+  __shared__ int s_axis[kAxes * kTokens];
   const PagedView& c = a.c;
   const int D = c.head_dim, half = D / 2;
   const int q_chunks = PAIR ? D / 16 : D / 8, kv_chunks = D / 8;
@@ -260,14 +266,21 @@ __global__ void __launch_bounds__(kThreads, 5) paged_append_kernel(PagedAppendAr
   const unsigned quad = 0xFu << (threadIdx.x & 28);
   for (int64_t t0 = int64_t(blockIdx.y) * a.tokens; t0 < c.total; t0 += int64_t(gridDim.y) * a.tokens) {
     const int n = int(c.total - t0 < a.tokens ? c.total - t0 : a.tokens);
+    if (a.positions && threadIdx.x < a.axes * kTokens) {
+      const int axis = threadIdx.x / kTokens, i = threadIdx.x % kTokens;
+      if (i < n) s_axis[threadIdx.x] = a.positions[axis * a.pos_rs + t0 + i];
+    }
     find_tokens(c, t0, n, s_pos, s_tile);
     __syncthreads();
     const int turns = a.rotary / 2;
     for (int i = threadIdx.x; i < n * turns; i += kThreads) {
       const int k = i / turns, j = i - k * turns, pos = s_pos[k];
       if (pos >= 0) {
-        s_angles[k * a.rotary + j] = a.cos[pos * a.cs_rs + j];
-        s_angles[k * a.rotary + turns + j] = a.sin[pos * a.cs_rs + j];
+        int row = pos;  // (the host has checked that the table reaches every position)
+        if (a.positions) row = s_axis[(a.pair_axes[j >> 4] >> (2 * (j & 15)) & 3) * kTokens + k];
+        const bool in = row >= 0 && row < a.cs_rows;
+        s_angles[k * a.rotary + j] = in ? a.cos[row * a.cs_rs + j] : NAN;
+        s_angles[k * a.rotary + turns + j] = in ? a.sin[row * a.cs_rs + j] : NAN;
       }
     }
     __syncthreads();

@@ -27,6 +27,7 @@ import torch
 
 from . import _lib as L
 from . import _workspace as W
+from .logits import LogitRules, _apply as _apply_rules, _rows as _rule_rows
 
 _DT = {torch.float16: L.DT_F16, torch.bfloat16: L.DT_BF16, torch.float32: L.DT_F32,
        torch.int32: L.DT_I32, torch.int64: L.DT_I64}
@@ -351,11 +352,13 @@ def embedding(input_ids: torch.Tensor, packed_w: torch.Tensor, scales: torch.Ten
     return out.reshape(tuple(input_ids.shape) + (K,))
 
 
-def argmax(logits: torch.Tensor, idx_offset: int = 0, with_values: bool = False):
+def argmax(logits: torch.Tensor, idx_offset: int = 0, with_values: bool = False, rules: Optional[LogitRules] = None):
     """Greedy choice over the last dimension of ``logits`` [..., N] (the
     engine's temperature-0 sample_token, spectra/engine.py:1690-1713): int64
     index of the first maximum (NaN counts as the maximum, as torch.argmax)
-    plus ``idx_offset``; with ``with_values`` also the maxima as fp32."""
+    plus ``idx_offset``; with ``with_values`` also the maxima as fp32.  With
+    ``rules`` the choice is made under them (spectra_b200.logits): -1, and
+    -infinity, where they allow no token."""
     _require_cuda("logits", logits, logits.device)
     N = logits.shape[-1]
     x2 = logits.reshape(-1, N)
@@ -364,10 +367,13 @@ def argmax(logits: torch.Tensor, idx_offset: int = 0, with_values: bool = False)
     M = x2.shape[0]
     idx = torch.empty(M, dtype=torch.int64, device=logits.device)
     val = torch.empty(M, dtype=torch.float32, device=logits.device) if with_values else None
-    with torch.cuda.device(logits.device):
-        st = L.lib().spectra_argmax(x2.data_ptr(), _dt(x2), x2.stride(0), M, N, int(idx_offset), idx.data_ptr(),
-                                    val.data_ptr() if val is not None else None, _stream(logits.device))
-    L.check("spectra_argmax", st)
+    if rules is not None:
+        _apply_rules(_rule_rows(x2), rules, int(idx_offset), None, idx, val)
+    else:
+        with torch.cuda.device(logits.device):
+            st = L.lib().spectra_argmax(x2.data_ptr(), _dt(x2), x2.stride(0), M, N, int(idx_offset), idx.data_ptr(),
+                                        val.data_ptr() if val is not None else None, _stream(logits.device))
+        L.check("spectra_argmax", st)
     shape = tuple(logits.shape[:-1])
     if with_values:
         return idx.reshape(shape), val.reshape(shape)
@@ -377,10 +383,11 @@ def argmax(logits: torch.Tensor, idx_offset: int = 0, with_values: bool = False)
 def lm_head_greedy(x: torch.Tensor, packed_w: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor,
                    bias: Optional[torch.Tensor] = None, outlier_idx: Optional[torch.Tensor] = None,
                    outlier_w: Optional[torch.Tensor] = None, marlin_layout: bool = False,
-                   out: Optional[torch.Tensor] = None):
+                   out: Optional[torch.Tensor] = None, rules: Optional[LogitRules] = None):
     """Greedy decode head at M=1: the lm_head GEMV (logits in x's dtype, as the
     engine's tied head computes them, spectra/engine.py:1124-1168) followed on
-    the same stream by the argmax kernel.  Returns (next_token int64 [1], logits)."""
+    the same stream by the argmax kernel, under ``rules`` where they are given.
+    Returns (next_token int64 [1], logits), the logits as the head gave them."""
     logits = fused_w4a16_gemv_hdsq(x, packed_w, scales, zeros, bias=bias, outlier_idx=outlier_idx,
                                    outlier_w=outlier_w, out=out, marlin_layout=marlin_layout)
-    return argmax(logits.reshape(1, -1)), logits
+    return argmax(logits.reshape(1, -1), rules=rules), logits

@@ -5,7 +5,7 @@ The reference keeps its INT4 cache as one dense tensor per layer
 all of it at every step for the model's own attention.  Here the cache stays
 in pages of 4-bit codes that sequences share out among themselves, the keys
 enter it with the position rotation applied, and the attention reads the codes
-(csrc/paged_kv.cu, csrc/paged_attn.cu, csrc/paged_prompt.cu):
+(csrc/paged_kv.cu, csrc/paged_attn.cu, csrc/paged_prompt.cu, csrc/paged_index.cu):
 
     cache = PagedKVCache(num_pages, kv_heads, head_dim, page_size=64)
     batch = TokenBatch(block_tables, seq_lens)              # one new token per sequence
@@ -13,6 +13,14 @@ enter it with the position rotation applied, and the attention reads the codes
     q = paged_kv_append(cache, batch, k, v, q=q, cos=cos, sin=sin)
     o = paged_attention(q, cache, batch)
     k_held, v_held = paged_kv_read(cache, batch)
+
+For long caches, attention over some blocks of keys that a cheap score chooses
+for every token and key/value head:
+
+    index = BlockIndex(cache, block_size=64)                # ranges of each block's keys, 8 bits
+    paged_index_update(index, batch)                        # after every append
+    blocks = paged_select_blocks(q, index, batch, count=32)
+    o = paged_attention(q, cache, batch, blocks=blocks, block_size=64)
 
 A batch's arrays live on the device and are read by the kernels alone, so a
 captured step can be replayed with other contents; ``max_len`` and ``max_q``
@@ -22,7 +30,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -81,6 +89,74 @@ class PagedKVCache:
         stride = pool.stride(0) if self.num_pages > 1 else heads * tiles * tile
         self._c = L.PagedCache(pool.data_ptr(), stride, self.num_pages, heads, head_dim, self.page_size)
         self._at = ctypes.addressof(self._c)
+
+
+class BlockIndex:
+    """What the choice of blocks knows of a cache: of every block of
+    ``block_size`` tokens of a page (a power of two, 32 to the page's size) and
+    every head, the range of the keys feature by feature.  ``codes`` int8
+    [num_pages, kv_heads, page_size / block_size, 2, head_dim]: the largest
+    values rounded up and the smallest rounded down, in steps of ``scales`` fp32
+    [num_pages, kv_heads, page_size / block_size] (powers of two; infinite where
+    a key is not finite).  ``codes * scales[..., None, None]`` are the bounds."""
+
+    def __init__(self, cache: PagedKVCache, block_size: int = 64):
+        _block_size(block_size, cache.page_size)
+        shape = (cache.num_pages, cache.kv_heads, cache.page_size // block_size)
+        self._bind(cache, torch.zeros(*shape, 2, cache.head_dim, dtype=torch.int8, device=cache.pool.device),
+                   torch.zeros(shape, dtype=torch.float32, device=cache.pool.device))
+
+    @classmethod
+    def from_buffers(cls, cache: PagedKVCache, codes: torch.Tensor, scales: torch.Tensor) -> "BlockIndex":
+        """An index on existing buffers; their third size says the block's."""
+        self = cls.__new__(cls)
+        self._bind(cache, codes, scales)
+        return self
+
+    def _bind(self, cache: PagedKVCache, codes: torch.Tensor, scales: torch.Tensor) -> None:
+        if codes.dtype != torch.int8 or scales.dtype != torch.float32:
+            raise TypeError(f"codes must be int8 and scales float32, got {codes.dtype} and {scales.dtype}")
+        if codes.dim() != 5 or codes.shape[2] < 1 or cache.page_size % codes.shape[2]:
+            raise ValueError("codes must be [num_pages, kv_heads, page_size / block_size, 2, head_dim], "
+                             f"got {tuple(codes.shape)}")
+        block_size = cache.page_size // codes.shape[2]
+        _block_size(block_size, cache.page_size)
+        shape = (cache.num_pages, cache.kv_heads, cache.page_size // block_size)
+        if codes.shape != (*shape, 2, cache.head_dim) or scales.shape != shape:
+            raise ValueError(f"codes and scales must be {(*shape, 2, cache.head_dim)} and {shape}, "
+                             f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
+        if not codes.is_contiguous() or not scales.is_contiguous():
+            raise ValueError("codes and scales must be contiguous")
+        if codes.get_device() != cache._index or scales.get_device() != cache._index:
+            raise RuntimeError("spectra_b200.paged: codes and scales must be on the cache's CUDA device (no CPU path)")
+        self.cache, self.codes, self.scales, self.block_size = cache, codes, scales, block_size
+        self._c = L.BlockIndex(codes.data_ptr(), scales.data_ptr(), block_size)
+        self._at = ctypes.addressof(self._c)
+
+
+def _block_size(n: int, most: int) -> None:
+    if n < 32 or n > most or n & (n - 1):
+        raise ValueError(f"block_size must be a power of two from 32 to {most}, got {n}")
+
+
+class RotaryAxes:
+    """Which axis of a token's position turns each pair of the rotated part:
+    ``pair_axes``, one axis number (up to 3) for each of the ``rotary / 2`` pairs."""
+
+    def __init__(self, pair_axes: Sequence[int]):
+        pair_axes = tuple(int(a) for a in pair_axes)
+        if not pair_axes or min(pair_axes) < 0 or max(pair_axes) >= L.MAX_POSITION_AXES:
+            raise ValueError(f"pair_axes must name axes 0 to {L.MAX_POSITION_AXES - 1}, got {pair_axes}")
+        self.pair_axes, self.axes = pair_axes, max(pair_axes) + 1
+        self._c = (ctypes.c_uint8 * len(pair_axes))(*pair_axes)
+        self._at = ctypes.addressof(self._c)
+
+    @classmethod
+    def sections(cls, *pairs: int) -> "RotaryAxes":
+        """The first ``pairs[0]`` pairs on axis 0, the next ``pairs[1]`` on axis 1, and so on."""
+        if any(n < 0 for n in pairs):
+            raise ValueError(f"sections must not be negative, got {pairs}")
+        return cls([axis for axis, n in enumerate(pairs) for _ in range(n)])
 
 
 class TokenBatch:
@@ -192,7 +268,8 @@ def _call(index: int, fn: str, *args) -> None:
 def paged_kv_append(cache: PagedKVCache, batch: TokenBatch, k: torch.Tensor, v: torch.Tensor,
                     q: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
                     sin: Optional[torch.Tensor] = None, interleaved: bool = False,
-                    out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+                    out: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                    axes: Optional[RotaryAxes] = None) -> Optional[torch.Tensor]:
     """Append the batch's new tokens ``k``, ``v`` [total, kv_heads, D] to the
     cache, and return ``q`` [total, q_heads, D] rotated (None without q).
 
@@ -203,7 +280,13 @@ def paged_kv_append(cache: PagedKVCache, batch: TokenBatch, k: torch.Tensor, v: 
     Groups that hold a NaN or infinity make their token's key NaN, so every row
     that looks at it is NaN and no other.  Token tensors may be views (any
     token and head strides), of a fused projection for example.  ``out``, for the
-    rotated queries, shares no element with q, k or v."""
+    rotated queries, shares no element with q, k or v.
+
+    ``positions`` int32 [axes, total] takes the place of the tokens' own
+    positions as rows of ``cos`` and ``sin``: pair i of token t is turned by row
+    ``positions[axes.pair_axes[i], t]`` (without ``axes``, [total]: one axis).  A
+    row outside the tables turns into NaN.  The place in the cache stays the
+    token's own."""
     index = cache._index
     if batch._index != index:
         _other_device()
@@ -213,9 +296,13 @@ def paged_kv_append(cache: PagedKVCache, batch: TokenBatch, k: torch.Tensor, v: 
     rotary = rows = cs = 0
     cp = sp = None
     if cos is not None or sin is not None:
-        cos, sin, rotary, rows, cs = _angles(cos, sin, cache, batch, interleaved)
+        cos, sin, rotary, rows, cs = _angles(cos, sin, cache, batch, interleaved, positions is not None)
         if rotary:
             cp, sp = cos.data_ptr(), sin.data_ptr()
+    by = None
+    if positions is not None or axes is not None:
+        positions, axes, ps = _axes(positions, axes, cache, batch, rotary)
+        by = positions.data_ptr(), ps, axes.axes, axes._at
     qp = op = None
     heads = q_ts = q_hs = o_ts = o_hs = 0
     if q is not None:
@@ -239,12 +326,44 @@ def paged_kv_append(cache: PagedKVCache, batch: TokenBatch, k: torch.Tensor, v: 
         qp, op = q.data_ptr(), out.data_ptr()
     if v.dtype != dt:
         raise TypeError("q, k, v and out must have one dtype")
-    _call(index, "spectra_paged_kv_append", cache._at, batch._at, _DT[dt], heads, qp, q_ts, q_hs, op, o_ts, o_hs,
-          k.data_ptr(), k_ts, k_hs, v.data_ptr(), v_ts, v_hs, cp, sp, rows, cs, rotary, interleaved)
+    args = (cache._at, batch._at, _DT[dt], heads, qp, q_ts, q_hs, op, o_ts, o_hs, k.data_ptr(), k_ts, k_hs, v.data_ptr(), v_ts,
+            v_hs, cp, sp, rows, cs, rotary, interleaved)
+    if by is None:
+        _call(index, "spectra_paged_kv_append", *args)
+    else:
+        _call(index, "spectra_paged_kv_append_axes", *args, *by)
     return out if q is not None else None
 
 
-def _angles(cos, sin, cache: PagedKVCache, batch: TokenBatch, interleaved: bool):
+_ONE_AXIS: dict = {}  # RotaryAxes of one axis, by number of pairs
+
+
+def _axes(positions, axes, cache: PagedKVCache, batch: TokenBatch, rotary: int):
+    if positions is None:
+        raise ValueError("axes come with positions")
+    if not rotary:
+        raise ValueError("positions need cos and sin")
+    if positions.dtype != torch.int32:
+        raise TypeError(f"positions must be int32, got {positions.dtype}")
+    if positions.get_device() != cache._index:
+        raise RuntimeError("spectra_b200.paged: positions must be on the cache's CUDA device (no CPU path), "
+                           f"got {positions.device}")
+    if axes is None:
+        axes = _ONE_AXIS.get(rotary) or _ONE_AXIS.setdefault(rotary, RotaryAxes([0] * (rotary // 2)))
+        if positions.dim() == 1:
+            positions = positions[None]
+    if len(axes.pair_axes) != rotary // 2:
+        raise ValueError(f"axes are of {len(axes.pair_axes)} pairs, cos and sin of {rotary // 2}")
+    if positions.dim() != 2 or positions.shape[0] < axes.axes or positions.shape[1] != batch.total:
+        raise ValueError(f"positions must be [{axes.axes}, {batch.total}], got {tuple(positions.shape)}")
+    ps, unit = positions.stride()
+    if unit != 1 and batch.total > 1:
+        positions = positions.contiguous()
+        ps = positions.stride(0)
+    return positions, axes, ps
+
+
+def _angles(cos, sin, cache: PagedKVCache, batch: TokenBatch, interleaved: bool, free: bool = False):
     if cos is None or sin is None:
         raise ValueError("cos and sin come together")
     if cos.dtype != torch.float32 or sin.dtype != torch.float32:
@@ -262,7 +381,10 @@ def _angles(cos, sin, cache: PagedKVCache, batch: TokenBatch, interleaved: bool)
     if rotary > cache.head_dim or rotary % (8 if interleaved else 16):
         raise ValueError(f"the rotated part must be a multiple of {8 if interleaved else 16} and at most "
                          f"{cache.head_dim}, got {rotary}")
-    if rows < batch._limit(cache):
+    if free:  # the rows are named by positions, and checked where they are read
+        if not rows:
+            raise ValueError("cos and sin have no positions")
+    elif rows < batch._limit(cache):
         raise ValueError(f"cos and sin have {rows} positions, the batch may hold {batch._limit(cache)}")
     return cos, sin, rotary, rows, strides[0]
 
@@ -342,7 +464,8 @@ def _workspace(index: int, head_dim: int) -> Tuple[int, int]:
 
 def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, *, scale: Optional[float] = None,
                     causal: bool = True, window: int = 0, softcap: float = 0.0,
-                    alibi_slopes: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    alibi_slopes: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                    blocks: Optional[torch.Tensor] = None, block_size: Optional[int] = None) -> torch.Tensor:
     """Attention of the batch's new tokens ``q`` [total, q_heads, D] over the
     cache (append them first); the result has q's shape and dtype.
 
@@ -353,6 +476,13 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, *, 
     multiple of kv_heads; consecutive heads share one.  A row that sees no key
     is 0.  Scores, softmax statistics and sums are fp32.  ``out`` may be q
     itself (the same strides); otherwise they share no element.
+
+    ``blocks`` int32 [total, kv_heads, count] (``paged_select_blocks``): of these
+    keys, the row sees those in the blocks of ``block_size`` tokens that are
+    listed for its token and key/value head.  A list is in ascending order; an
+    entry that is not above all before it (a repeated one, -1) and a block past
+    the sequence's end are passed over.  block_size is a power of two from 32 to
+    65536, count at most 1024.
 
     Partial results lie in a workspace of the current stream (17 MB for heads of
     128, kept for the process).  A graph captured on a stream that has called
@@ -391,8 +521,83 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, *, 
         _own_elements(out)
         if (out.data_ptr() != q.data_ptr() or o_ts != q_ts or o_hs != q_hs) and _overlap(out, q):
             raise ValueError("out must not overlap q, unless it is q")
+    lists = None
+    if blocks is not None or block_size is not None:
+        lists = _lists(blocks, block_size, cache, batch)
     ws, nbytes = _workspace(index, cache.head_dim)
-    _call(index, "spectra_paged_attention", cache._at, batch._at, _DT[q.dtype], heads, q.data_ptr(), q_ts, q_hs,
-          out.data_ptr(), o_ts, o_hs, scale, softcap, None if slopes is None else slopes.data_ptr(), causal,
-          min(window, 2**31 - 1), ws, nbytes)
+    args = (cache._at, batch._at, _DT[q.dtype], heads, q.data_ptr(), q_ts, q_hs, out.data_ptr(), o_ts, o_hs, scale, softcap,
+            None if slopes is None else slopes.data_ptr(), causal, min(window, 2**31 - 1))
+    if lists is None:
+        _call(index, "spectra_paged_attention", *args, ws, nbytes)
+    else:
+        _call(index, "spectra_paged_attention_blocks", *args, *lists, ws, nbytes)
+    return out
+
+
+def _lists(blocks, block_size, cache: PagedKVCache, batch: TokenBatch):
+    if blocks is None or block_size is None:
+        raise ValueError("blocks and block_size come together")
+    _block_size(block_size, 65536)
+    if blocks.dtype != torch.int32:
+        raise TypeError(f"blocks must be int32, got {blocks.dtype}")
+    if blocks.get_device() != cache._index:
+        raise RuntimeError(f"spectra_b200.paged: blocks must be on the cache's CUDA device (no CPU path), got {blocks.device}")
+    if blocks.dim() != 3 or blocks.shape[:2] != (batch.total, cache.kv_heads) or not 0 < blocks.shape[2] <= L.MAX_LISTED_BLOCKS:
+        raise ValueError(f"blocks must be [{batch.total}, {cache.kv_heads}, count], count 1 to {L.MAX_LISTED_BLOCKS}, "
+                         f"got {tuple(blocks.shape)}")
+    ts, hs, unit = blocks.stride()
+    if unit != 1 and blocks.shape[2] > 1:
+        raise ValueError("blocks must have unit stride along a list")
+    return blocks.data_ptr(), ts, hs, blocks.shape[2], block_size
+
+
+def paged_index_update(index: BlockIndex, batch: TokenBatch) -> None:
+    """Write the index of every block whose last token is among the batch's new
+    ones (append them first).  Exact: it depends on the cached keys alone.  A
+    block that is not full has no entry yet; the choice takes it unseen."""
+    if batch._index != index.cache._index:
+        _other_device()
+    _call(batch._index, "spectra_paged_index_update", index.cache._at, batch._at, index._at)
+
+
+def paged_select_blocks(q: torch.Tensor, index: BlockIndex, batch: TokenBatch, count: int, *, first: int = 1, last: int = 1,
+                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The ``count`` blocks that each of the batch's new tokens looks at, int32
+    [total, kv_heads, count]: their numbers in ascending order, then -1.
+
+    Of the blocks up to the token's own, the ``first`` first and the ``last``
+    last ones (the token's own among them) are always taken, then those of the
+    highest score, the lowest number first among equal ones.  The score bounds
+    q . k over the block's keys from above, for the best of the key/value head's
+    query heads: with H, L the block's codes, S its scale, and c the query
+    head's features rounded to 8 bits (each head in a power of two of its own,
+    so that no head outvotes another by its size),
+
+        score = S max_heads sum_d (c_d H_d if c_d > 0 else c_d L_d)
+
+    The sums are whole numbers, so equal inputs give equal lists.  A block with
+    a key that is not finite comes before all others; one whose page the table
+    does not name is never taken.  Tokens without a place in the cache get -1.
+    ``q`` [total, q_heads, D] are the queries as the attention gets them."""
+    cache = index.cache
+    dev = cache._index
+    if batch._index != dev:
+        _other_device()
+    q, q_ts, q_hs = _strided("q", q, cache, batch, None)
+    heads = q.shape[1]
+    if heads % cache.kv_heads or not heads:
+        raise ValueError(f"q has {heads} heads, not a multiple of the cache's {cache.kv_heads}")
+    if first < 0 or last < 1 or not first + last <= count <= L.MAX_LISTED_BLOCKS:
+        raise ValueError(f"count must be first + last to {L.MAX_LISTED_BLOCKS} and last positive, got count={count}, "
+                         f"first={first}, last={last}")
+    if batch._limit(cache) > L.MAX_INDEXED_BLOCKS * index.block_size:
+        raise ValueError(f"the choice is among {L.MAX_INDEXED_BLOCKS} blocks at most, the batch may hold "
+                         f"{-(-batch._limit(cache) // index.block_size)} (max_len bounds them)")
+    shape = (batch.total, cache.kv_heads, count)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.int32, device=q.device)
+    elif out.dtype != torch.int32 or out.shape != shape or not out.is_contiguous() or out.get_device() != dev:
+        raise ValueError(f"out must be contiguous int32 {shape} on the cache's device")
+    _call(dev, "spectra_paged_select_blocks", cache._at, batch._at, index._at, _DT[q.dtype], heads, q.data_ptr(), q_ts, q_hs,
+          count, first, last, out.data_ptr(), cache.kv_heads * count, count)
     return out

@@ -64,9 +64,9 @@ def _kernel_local(x2d, packed, scales, zeros, outlier_idx, outlier_w, bias, marl
         out += bias
 
 
-def _kernel_argmax(y: torch.Tensor, offset: int) -> Tuple[torch.Tensor, torch.Tensor]:
+def _kernel_argmax(y: torch.Tensor, offset: int, rules=None) -> Tuple[torch.Tensor, torch.Tensor]:
     from . import kernels as SK
-    idx, val = SK.argmax(y, idx_offset=offset, with_values=True)
+    idx, val = SK.argmax(y, idx_offset=offset, with_values=True, rules=rules)
     return val, idx
 
 
@@ -79,7 +79,7 @@ class ShardedW4A16Linear:
     ``device``.  ``local_fn(x2d, packed, scales, zeros, idx, ow, bias, marlin,
     out)`` writes one rank's slice into ``out``; it defaults to the CUDA kernels
     (tests on CPU pass a reference implementation instead), as does
-    ``argmax_fn(y, offset) -> (values, indices)``.
+    ``argmax_fn(y, offset) -> (values, indices)`` (and ``(y, offset, rules)``).
 
     ``exchange``: "auto" (the peer-memory exchange when the group's backend is
     NCCL on CUDA devices and SPECTRA_B200_P2P is not 0, else the group's
@@ -194,9 +194,11 @@ class ShardedW4A16Linear:
 
     __call__ = forward
 
-    def greedy(self, x: torch.Tensor) -> torch.Tensor:
+    def greedy(self, x: torch.Tensor, rules=None) -> torch.Tensor:
         """Index of the first maximum of each output row [..., N] (int64), from
-        this rank's slice and one all-gather of (value, index) pairs."""
+        this rank's slice and one all-gather of (value, index) pairs.  With
+        ``rules`` (spectra_b200.logits.LogitRules, the same on every rank) the
+        choice is made under them, -1 where they allow no token."""
         orig_shape = x.shape
         M = x.numel() // self.in_features
         x2d = x.reshape(M, self.in_features)
@@ -206,7 +208,8 @@ class ShardedW4A16Linear:
             ex = self._exchange(("pair", M), M, 2, 2 * self.world, torch.float64)
         pair = ex.src if ex is not None else torch.empty(M, 2, dtype=torch.float64, device=y_local.device)
         if self.rows > 0:
-            val, idx = self.argmax_fn(y_local[:, :self.rows], self.row0)
+            y_local = y_local[:, :self.rows]
+            val, idx = self.argmax_fn(y_local, self.row0) if rules is None else self.argmax_fn(y_local, self.row0, rules)
             torch.stack([val.to(torch.float64), idx.to(torch.float64)], dim=1, out=pair)  # [M, 2], exact
         else:  # an empty shard never wins
             pair[:, 0] = float("-inf")
@@ -221,6 +224,13 @@ class ShardedW4A16Linear:
             g = gathered.view(self.world, M, 2)
         # ranks hold increasing row ranges: the first maximum in rank order is the
         # first maximum of the row (torch.argmax: the first NaN counts as maximum)
-        r = torch.argmax(g[:, :, 0], dim=0)
+        if rules is None:
+            r = torch.argmax(g[:, :, 0], dim=0)
+        else:  # ranks with an allowed token come first, whatever its value
+            some = (g[:, :, 1] >= 0) & (g[:, :, 1] < 2 ** 53)
+            best, r = torch.where(some, g[:, :, 0], float("-inf")).max(dim=0)
+            r = torch.where(best == float("-inf"), some.to(torch.int8).argmax(dim=0), r)
         tok = g[:, :, 1].gather(0, r.view(1, M)).view(M)
+        if rules is not None:
+            tok = torch.where(some.any(dim=0), tok, -1.0)
         return tok.to(torch.int64).reshape(orig_shape[:-1])
