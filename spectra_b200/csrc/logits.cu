@@ -7,12 +7,20 @@
 //   v not allowed:  x = -inf
 // and the token: first maximum of x among the allowed (NaN above every number).
 //
-// A row belongs to a cluster of 8 CTAs, each a slice of the vocabulary in
-// chunks.  A chunk has a word of shared memory per token: 19 bits count the
-// token's ids, one says that the prompt holds it, 12 name its bias.  Whole
-// numbers are added up (atomics in shared memory), so their order does not
-// matter, and a list of any length costs one pass over it whatever the
-// vocabulary.  Most words stay 0: their logits go through untouched.
+// A row belongs to a cluster of 1 to 8 CTAs, which take its 128 bytes by turns
+// (the frequent tokens of a vocabulary lie together).  A CTA has a word of
+// shared memory per token, which counts: 19 bits the token's ids, one says that
+// the prompt holds it, 12 name its bias.  Whole numbers are added up (atomics in
+// shared memory), so their order does not matter, and a list costs one pass
+// over it whatever the vocabulary.  A bit per token says which were met.  Then
+//   1 a thread for each token met replaces its word by the new logit,
+//   2 a pass over the row writes what may follow and was not met as it is, and
+//     -infinity elsewhere, on pairs of 16 bits as they lie in memory,
+//   3 a thread for each token met writes its logit over it,
+// and the maximum is that of 2 and 3.  (Rules applied in the pass over the row
+// took 117 us for 333 rows of 50001, this 59: some lane of every warp has a rule.)
+// Logits move in units of 16 bytes cut at 16-byte addresses (rows of an odd
+// vocabulary start anywhere), four of a thread in flight while it counts.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -27,126 +35,323 @@ namespace spectra {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kCluster = 8;                     // CTAs per row (a portable cluster size)
-constexpr int kUnits = 4;                       // of 8 columns, that a thread takes in a chunk
-constexpr int kChunk = kThreads * kUnits * 8;   // columns
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;                  // CTAs per row, a power of two (8: a portable cluster size)
+constexpr int kUnits = 4;                       // 16-byte units that a thread takes in a chunk
+constexpr int kFlight = 4;                      // ids of a thread in flight
 constexpr uint32_t kCountBits = 19, kPrompt = 1u << kCountBits, kSlot = kCountBits + 1;
 constexpr uint32_t kCountMask = kPrompt - 1, kLow = (1u << kSlot) - 1;
 static_assert(SPECTRA_MAX_RULE_IDS <= kCountMask && SPECTRA_MAX_RULE_BIASES < (1 << (32 - kSlot)), "a word's fields");
 
-// Larger value first, a NaN above every number, the lower index among equals; index -1: none.
-__device__ __forceinline__ bool better(float v, int64_t i, float bv, int64_t bi) {
-  if (i < 0 || bi < 0) return i >= 0;
-  const bool vn = v != v, bn = bv != bv;
-  if (vn || bn) return vn && (!bn || i < bi);
-  return v > bv || (v == bv && i < bi);
-}
+template <int DT>
+constexpr int kPer = DT == SPECTRA_DT_F32 ? 4 : 8;  // logits of a unit
+template <int DT>
+constexpr int kChunk = kThreads * kUnits * kPer<DT>;  // columns that a CTA takes at once
+constexpr int kTurn = 3;                              // log2 of the units that a CTA takes before it is the next one's turn
 
 __device__ __forceinline__ int clamp_len(int v, int64_t most) { return v < 0 ? 0 : (v < most ? v : int(most)); }
 
-__global__ void __launch_bounds__(kThreads) logits_kernel(LogitArgs a) {
+// The order of a choice as whole numbers: larger value first, a NaN above every number; 0: none.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  if (v != v) return ~0u;
+  const uint32_t u = __float_as_uint(v + 0.f);  // (-0 as 0)
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t o) {
+  if (o == ~0u) return __uint_as_float(0x7FFFFFFFu);
+  return o == 0 ? -INFINITY : __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+}
+struct Choice {
+  uint32_t order;
+  int column;
+};
+// The best of the warp's, in every lane: the first of the highest.
+__device__ __forceinline__ Choice best_of_warp(const Choice& c) {
+  const uint32_t top = __reduce_max_sync(0xffffffffu, c.order);
+  return {top, __reduce_min_sync(0xffffffffu, c.order == top ? c.column : INT32_MAX)};
+}
+
+// The raw logits of a unit are pairs of 16 bits, or fp32.
+
+// -infinity where a bit of `keep` is not set.
+template <int DT>
+__device__ __forceinline__ void keep_only(uint32_t (&w)[4], uint32_t keep) {
+  constexpr uint32_t LOWEST = DT == SPECTRA_DT_F32 ? 0xFF800000u : DT == SPECTRA_DT_BF16 ? 0xFF80FF80u : 0xFC00FC00u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == SPECTRA_DT_F32) {
+      w[i] = keep >> i & 1u ? w[i] : LOWEST;
+    } else {
+      const uint32_t two = keep >> (2 * i) & 3u, mask = ((two | two << 15) & 0x10001u) * 0xFFFFu;
+      w[i] = (w[i] & mask) | (LOWEST & ~mask);
+    }
+  }
+}
+// The largest of both halves, a NaN where there is one.
+template <int DT>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (DT == SPECTRA_DT_BF16)
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else if constexpr (DT == SPECTRA_DT_F16)
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ float element(const uint32_t (&w)[4], int e) {
+  if constexpr (DT == SPECTRA_DT_F32) return __uint_as_float(w[e]);
+  return bits_to_float(w[e >> 1] >> (16 * (e & 1)) & 0xFFFFu, DT);
+}
+template <int DT>
+__device__ __forceinline__ float top_of(const uint32_t (&w)[4]) {
+  uint32_t t = max2<DT>(max2<DT>(w[0], w[1]), max2<DT>(w[2], w[3]));
+  if constexpr (DT != SPECTRA_DT_F32) t = max2<DT>(t, t >> 16) & 0xFFFFu;
+  return bits_to_float(t, DT);
+}
+
+struct Penalties {
+  float rep, freq, pres;
+  const float* bias;
+};
+__device__ __forceinline__ float ruled(float x, uint32_t w, const Penalties& p) {
+  const uint32_t times = w & kCountMask;
+  if (w & (kPrompt | kCountMask)) x = x > 0.f ? __fdiv_rn(x, p.rep) : __fmul_rn(x, p.rep);
+  if (times) x = __fsub_rn(__fsub_rn(x, __fmul_rn(p.freq, float(times))), p.pres);
+  if (w >> kSlot) x = __fadd_rn(x, p.bias[(w >> kSlot) - 1]);
+  return x;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads, 2) logits_kernel(LogitArgs a) {
   namespace cg = cooperative_groups;
+  constexpr int PER = kPer<DT>, ALL = (1 << PER) - 1, SIZE = DT == SPECTRA_DT_F32 ? 4 : 2;
   cg::cluster_group cluster = cg::this_cluster();
-  extern __shared__ __align__(16) uint32_t words[];  // [kChunk]
+  extern __shared__ __align__(16) uint32_t words[];  // [kChunk<DT>]
+  uint16_t* met = reinterpret_cast<uint16_t*>(words + kChunk<DT>);  // [kChunk<DT>] words of the tokens met
+  __shared__ uint32_t s_bits[kChunk<DT> / 32];                      // which were met
+  __shared__ int s_met;
+  __shared__ Choice s_best[kWarps];
   sm100::pdl_wait();
+  sm100::pdl_trigger();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t m = blockIdx.y;
   const SpectraLogitRules& r = a.r;
-  const int64_t lo = min(a.N, int64_t(cluster.block_rank()) * a.span), hi = min(a.N, lo + a.span);
+  const uint8_t* row = static_cast<const uint8_t*>(a.x) + m * a.x_rs * SIZE;
+  // unit u: columns u PER - shift ..: 16 bytes at a 16-byte address
+  const int shift = int(reinterpret_cast<uintptr_t>(row) % 16) / SIZE;
+  const int N = int(a.N), offset = int(a.idx_offset);
+  // local unit l of this CTA: unit ((l >> kTurn) * CTAs + rank) << kTurn | l % (1 << kTurn)
+  const int ctas = int(cluster.num_blocks()), rank = int(cluster.block_rank()), ctas_log2 = 31 - __clz(ctas);
+  const int turns = (((N + shift + PER - 1) / PER) + (1 << kTurn) - 1) >> kTurn;
+  const int mine = ((turns - rank + ctas - 1) >> ctas_log2) << kTurn;  // local units (a few past the row's end)
+  auto first_column = [&](int l) {
+    return (((((l >> kTurn) << ctas_log2) + rank) << kTurn) + (l & ((1 << kTurn) - 1))) * PER - shift;
+  };
+  uint8_t* out = static_cast<uint8_t*>(a.out) + m * a.out_rs * (a.out_dtype == SPECTRA_DT_F32 ? 4 : 2);
+  const bool as_units = a.out_dtype == DT && int(reinterpret_cast<uintptr_t>(out) % 16) / SIZE == shift;
   const int len = !r.ids ? 0 : (r.lengths ? clamp_len(r.lengths[m], r.max_ids) : int(r.max_ids));
   const int prompt = r.prompt_lengths ? clamp_len(r.prompt_lengths[m], len) : 0;
-  const float rep = r.repetition ? r.repetition[m] : 1.f;
-  const float freq = r.frequency ? r.frequency[m] : 0.f, pres = r.presence ? r.presence[m] : 0.f;
-  float bv = -INFINITY;
-  int64_t bi = -1;
-  for (int64_t c0 = lo; c0 < hi; c0 += kChunk) {
-    const int n = int(min(hi - c0, int64_t(kChunk)));
-    const int64_t token0 = c0 + a.idx_offset;
-    if (len > 0 || r.n_bias > 0) {
-      for (int i = threadIdx.x; i < n; i += kThreads) words[i] = 0;
-      __syncthreads();
-      for (int i = threadIdx.x; i < len; i += kThreads) {
-        const int64_t at = int64_t(r.ids[m * r.ids_stride + i]) - token0;
-        if (at < 0 || at >= n) continue;
-        if (i < prompt)
-          atomicOr(words + at, kPrompt);
-        else
-          atomicAdd(words + at, 1u);
-      }
-      __syncthreads();
-      for (int i = threadIdx.x; i < r.n_bias; i += kThreads) {
-        const int64_t id = r.bias_ids[m * r.bias_ids_stride + i], at = id - token0;
-        if (id < 0 || at < 0 || at >= n) continue;
-        // (the low bits are settled, so the larger word is the later entry)
-        atomicMax(words + at, (words[at] & kLow) | uint32_t(i + 1) << kSlot);
-      }
-      __syncthreads();
-    }
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      float x = load_as_float_cg(a.x, m * a.x_rs + c0 + i, a.x_dtype);
-      const uint32_t w = len > 0 || r.n_bias > 0 ? words[i] : 0;
-      const uint32_t times = w & kCountMask;
-      if (w & (kPrompt | kCountMask)) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-      if (times) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, float(times))), pres);
-      if (w >> kSlot) x = __fadd_rn(x, r.bias[m * r.bias_stride + (w >> kSlot) - 1]);
-      bool ok = true;
-      if (r.allowed) {
-        const int64_t t = token0 + i;
-        ok = (uint32_t(r.allowed[m * r.allowed_stride + (t >> 5)]) >> (t & 31)) & 1u;
-        if (!ok) x = -INFINITY;
-      }
-      if (a.out) store_from_float(a.out, m * a.out_rs + c0 + i, a.out_dtype, x);
-      if (ok && better(x, c0 + i, bv, bi)) {
-        bv = x;
-        bi = c0 + i;
+  const int* ids = r.ids + m * r.ids_stride;
+  const int* allowed = r.allowed ? r.allowed + m * r.allowed_stride : nullptr;
+  const int* bias_ids = r.bias_ids + m * r.bias_ids_stride;
+  const Penalties pen = {r.repetition ? r.repetition[m] : 1.f, r.frequency ? r.frequency[m] : 0.f,
+                         r.presence ? r.presence[m] : 0.f, r.bias + m * r.bias_stride};
+  const bool counted = len > 0 || r.n_bias > 0;
+  auto may_follow = [&](int n) { return !allowed || (uint32_t(__ldcg(allowed + ((n + offset) >> 5))) >> ((n + offset) & 31) & 1u); };
+  Choice best = {0, INT32_MAX};
+  auto consider = [&](float v, int n) {
+    const uint32_t o = order_of(v);
+    if (o > best.order || (o == best.order && n < best.column)) best = {o, n};
+  };
+  for (int c0 = 0; c0 < mine; c0 += kThreads * kUnits) {
+    const int c1 = min(mine, c0 + kThreads * kUnits), columns = (c1 - c0) * PER;
+    uint32_t raw[kUnits][4], word0[kUnits], word1[kUnits];
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      const int l = c0 + tid + k * kThreads, n0 = first_column(l);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[k][i] = 0;
+      word0[k] = word1[k] = ~0u;
+      if (l < c1 && n0 >= 0 && n0 + PER <= N) {  // (cut units, at a row's ends, are taken one by one)
+        const uint4 v = __ldcg(reinterpret_cast<const uint4*>(row + int64_t(n0) * SIZE));
+        raw[k][0] = v.x; raw[k][1] = v.y; raw[k][2] = v.z; raw[k][3] = v.w;
+        if (allowed) {
+          const int t = n0 + offset;
+          word0[k] = uint32_t(__ldcg(allowed + (t >> 5)));
+          if ((t & 31) > 32 - PER) word1[k] = uint32_t(__ldcg(allowed + (t >> 5) + 1));
+        }
       }
     }
-    __syncthreads();
+    uint32_t own = 0;  // which of the thread's columns were met
+    if (counted) {
+      for (int i = tid; i < columns / 4; i += kThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+      for (int i = tid; i < (columns + 31) / 32; i += kThreads) s_bits[i] = 0;
+      if (tid == 0) s_met = 0;
+      // a token's word, or -1: not of this CTA and chunk
+      auto word_of = [&](int id) {
+        const int n = id - offset;
+        if (id < 0 || unsigned(n) >= unsigned(N)) return -1;
+        const unsigned at = unsigned(n + shift), turn = at / (PER << kTurn);
+        if ((turn & unsigned(ctas - 1)) != unsigned(rank)) return -1;
+        const int w = int(turn >> ctas_log2) * (PER << kTurn) + int(at % (PER << kTurn)) - c0 * PER;
+        return w >= 0 && w < columns ? w : -1;
+      };
+      __syncthreads();
+      for (int i0 = tid; i0 < len; i0 += kFlight * kThreads) {
+        int id[kFlight];
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) id[k] = i0 + k * kThreads < len ? __ldcg(ids + i0 + k * kThreads) : -1;
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+          const int w = word_of(id[k]);
+          if (w < 0) continue;
+          atomicOr(s_bits + (w >> 5), 1u << (w & 31));
+          if (i0 + k * kThreads < prompt)
+            atomicOr(words + w, kPrompt);
+          else
+            atomicAdd(words + w, 1u);
+        }
+      }
+      __syncthreads();
+      if (r.n_bias > 0) {
+        for (int i = tid; i < r.n_bias; i += kThreads) {
+          const int w = word_of(__ldcg(bias_ids + i));
+          if (w < 0) continue;
+          atomicOr(s_bits + (w >> 5), 1u << (w & 31));
+          // (the low bits are settled, so the larger word is the later entry)
+          atomicMax(words + w, (words[w] & kLow) | uint32_t(i + 1) << kSlot);
+        }
+        __syncthreads();
+      }
+      // the tokens met, side by side
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k) {
+        const int w = (tid + k * kThreads) * PER;
+        if (w < columns) own |= (s_bits[w >> 5] >> (w & 31) & ALL) << (k * PER);
+      }
+      int before = __popc(own);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += up;
+      }
+      int base = 0;
+      if (lane == 31 && before) base = atomicAdd(&s_met, before);
+      int slot = __shfl_sync(0xffffffffu, base, 31) + before - __popc(own);
+      for (uint32_t left = own; left; left &= left - 1) {
+        const int i = __ffs(left) - 1;
+        met[slot++] = uint16_t((tid + i / PER * kThreads) * PER + i % PER);
+      }
+      __syncthreads();
+      for (int i = tid; i < s_met; i += kThreads) {
+        const int w = met[i], n = first_column(c0 + w / PER) + w % PER;
+        words[w] = __float_as_uint(ruled(load_as_float_cg(row, n, DT), words[w], pen));
+      }
+      __syncthreads();  // (the row is written from here on, and may be the logits themselves)
+    }
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      const int l = c0 + tid + k * kThreads, n0 = first_column(l);
+      if (l >= c1) break;
+      const uint32_t rest = ~(own >> (k * PER)) & ALL;  // not met
+      if (n0 >= 0 && n0 + PER <= N) {
+        const uint32_t keep = __funnelshift_r(word0[k], word1[k], (n0 + offset) & 31) & rest;
+        if (keep != ALL) keep_only<DT>(raw[k], keep);
+        if (a.out) {
+          if (as_units) {
+            *reinterpret_cast<uint4*>(out + int64_t(n0) * SIZE) = make_uint4(raw[k][0], raw[k][1], raw[k][2], raw[k][3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) store_from_float(out, n0 + e, a.out_dtype, element<DT>(raw[k], e));
+          }
+        }
+        if (a.idx && keep) {
+          const float top = top_of<DT>(raw[k]);
+          const uint32_t o = order_of(top);
+          if (o > best.order || (o == best.order && n0 < best.column)) {
+            // the first column that has it (where that is -infinity, among the kept)
+            int at = __ffs(keep) - 1;
+            if (top > -INFINITY) {
+#pragma unroll
+              for (int e = PER - 1; e >= 0; --e) at = element<DT>(raw[k], e) == top ? e : at;
+            } else if (top != top) {
+#pragma unroll
+              for (int e = PER - 1; e >= 0; --e) at = element<DT>(raw[k], e) != element<DT>(raw[k], e) ? e : at;
+            }
+            best = {o, n0 + at};
+          }
+        }
+      } else {
+        for (int e = max(0, -n0); e < PER && n0 + e < N; ++e) {
+          if (!(rest >> e & 1u)) continue;
+          const bool ok = may_follow(n0 + e);
+          const float y = ok ? load_as_float_cg(row, n0 + e, DT) : -INFINITY;
+          if (a.out) store_from_float(out, n0 + e, a.out_dtype, y);
+          if (ok) consider(y, n0 + e);
+        }
+      }
+    }
+    if (counted) {
+      __syncthreads();
+      for (int i = tid; i < s_met; i += kThreads) {
+        const int w = met[i], n = first_column(c0 + w / PER) + w % PER;
+        const bool ok = may_follow(n);
+        const float y = ok ? __uint_as_float(words[w]) : -INFINITY;
+        if (a.out) store_from_float(out, n, a.out_dtype, y);
+        if (ok) consider(y, n);
+      }
+      __syncthreads();  // before the next chunk clears the words
+    }
   }
   if (!a.idx) return;  // (the same for every CTA)
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
-    const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-    const int64_t oi = __shfl_xor_sync(0xffffffffu, bi, o);
-    if (better(ov, oi, bv, bi)) {
-      bv = ov;
-      bi = oi;
-    }
-  }
-  __shared__ float sv[kThreads / 32];
-  __shared__ int64_t si[kThreads / 32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) {
-    sv[warp] = bv;
-    si[warp] = bi;
-  }
+  best = best_of_warp(best);
+  if (lane == 0) s_best[warp] = best;
   cluster.sync();
-  if (cluster.block_rank() == 0 && warp == 0) {
-    bv = -INFINITY;
-    bi = -1;
-    for (int k = lane; k < kCluster * (kThreads / 32); k += 32) {
-      const int cta = k / (kThreads / 32), of = k % (kThreads / 32);
-      const float ov = *cluster.map_shared_rank(&sv[of], cta);
-      const int64_t oi = *cluster.map_shared_rank(&si[of], cta);
-      if (better(ov, oi, bv, bi)) {
-        bv = ov;
-        bi = oi;
-      }
+  if (rank == 0 && warp == 0) {
+    best = {0, INT32_MAX};
+    for (int k = lane; k < ctas * kWarps; k += 32) {
+      const Choice c = *cluster.map_shared_rank(&s_best[k % kWarps], k / kWarps);
+      if (c.order > best.order || (c.order == best.order && c.column < best.column)) best = c;
     }
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-      const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-      const int64_t oi = __shfl_xor_sync(0xffffffffu, bi, o);
-      if (better(ov, oi, bv, bi)) {
-        bv = ov;
-        bi = oi;
-      }
-    }
+    best = best_of_warp(best);
     if (lane == 0) {
-      a.idx[m] = bi < 0 ? -1 : bi + a.idx_offset;
-      if (a.val) a.val[m] = bv;
+      a.idx[m] = best.order ? best.column + a.idx_offset : -1;
+      if (a.val) a.val[m] = value_of(best.order);
     }
   }
   cluster.sync();  // no CTA leaves while the first may still read its shared memory
+}
+
+template <int DT>
+int launch_typed(const LogitArgs& a, cudaStream_t st) {
+  static PerContextOnce once;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e);
+  const int smem = kChunk<DT> * 6;
+  e = once.run(dev, [&] { return cudaFuncSetAttribute(logits_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+  if (e != cudaSuccess) return cuda_status(e);
+  // as few CTAs as hold the row at once (each reads the lists), more while there are SMs for them
+  const int64_t chunks = (a.N + kChunk<DT> - 1) / kChunk<DT>;
+  int ctas = 1;
+  while (ctas < kMaxCluster && (ctas < chunks || a.M * ctas < device_sms(dev))) ctas *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(ctas), unsigned(a.M));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(ctas);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cuda_status(cudaLaunchKernelEx(&cfg, logits_kernel<DT>, a));
 }
 
 }  // namespace
@@ -154,29 +359,8 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(LogitArgs a) {
 int launch_logits(LogitArgs a, cudaStream_t st) {
   if (a.M == 0) return SPECTRA_OK;
   if (a.M > 65535) return SPECTRA_ERR_SHAPE;  // grid y
-  static PerContextOnce once;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return cuda_status(e);
-  const int smem = kChunk * int(sizeof(uint32_t));
-  e = once.run(dev, [&] { return cudaFuncSetAttribute(logits_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
-  if (e != cudaSuccess) return cuda_status(e);
-  a.span = (a.N + kCluster - 1) / kCluster;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kCluster, unsigned(a.M));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kCluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cuda_status(cudaLaunchKernelEx(&cfg, logits_kernel, a));
+  if (a.x_dtype == SPECTRA_DT_BF16) return launch_typed<SPECTRA_DT_BF16>(a, st);
+  return a.x_dtype == SPECTRA_DT_F16 ? launch_typed<SPECTRA_DT_F16>(a, st) : launch_typed<SPECTRA_DT_F32>(a, st);
 }
 
 }  // namespace spectra

@@ -15,7 +15,6 @@ struct LogitArgs {
   void* out; int out_dtype; int64_t out_rs;       // [M, N] or NULL
   int64_t* idx; float* val;                       // [M] or NULL
   int64_t M, N, idx_offset;
-  int64_t span;                                   // columns of a CTA (set by the launcher)
 };
 int launch_logits(LogitArgs a, cudaStream_t st);
 

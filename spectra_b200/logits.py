@@ -112,7 +112,7 @@ def _apply(x: torch.Tensor, rules: LogitRules, idx_offset: int, out: Optional[to
         raise TypeError(f"logits must be bf16, fp16 or fp32, got {x.dtype}")
     if M != rules.rows or N < 1:
         raise ValueError(f"the rules are of {rules.rows} rows, the logits {tuple(x.shape)}")
-    if idx_offset < 0 or idx_offset + N > 2**31 - 1:
+    if idx_offset < 0 or idx_offset + N > 2**31 - 65:
         raise ValueError(f"idx_offset={idx_offset} and {N} logits pass 32 bits")
     if rules._c.allowed is not None and rules.words * 32 < idx_offset + N:
         raise ValueError(f"allowed has {rules.words} words a row, {-(-(idx_offset + N) // 32)} are needed")

@@ -31,7 +31,7 @@ def adjust(rules=None, **kw):
     ({}, dict(M=-1), L.ERR_SHAPE),
     ({}, dict(N=1 << 31, x_rs=1 << 31), L.ERR_SHAPE),
     ({}, dict(offset=-1), L.ERR_SHAPE),
-    ({}, dict(offset=2**31 - 100), L.ERR_SHAPE),
+    ({}, dict(offset=2**31 - 164), L.ERR_SHAPE),
     ({}, dict(offset=29), L.ERR_SHAPE),                       # 129 bits in 4 words
     (dict(allowed_words=3), {}, L.ERR_SHAPE),
     (dict(max_ids=L.MAX_RULE_IDS + 1), {}, L.ERR_SHAPE),
