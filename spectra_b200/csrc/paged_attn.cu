@@ -70,6 +70,7 @@ struct AttnParams {
   float* partials;
   int min_share;                   // units a CTA takes at least
   int max_rows;                    // a sequence with more rows per head is the other kernel's
+  int segments, pieces;            // lists: all segments, and CTAs per segment
 };
 
 // ------------------------------------------------------------ the batch
@@ -84,7 +85,7 @@ struct Span {  // a sequence's rows and the keys its rows look at
   int tiles;      // row tiles
 };
 
-template <int ROWS, bool SEL>
+template <int ROWS>
 __device__ __forceinline__ Span span_of(const AttnParams& p, int b) {
   const PagedAttnArgs& a = p.a;
   Span s;
@@ -92,16 +93,9 @@ __device__ __forceinline__ Span span_of(const AttnParams& p, int b) {
   const int len = a.c.seq_lens[b];
   s.pos0 = len - s.count - s.extra;
   s.len = len < 0 ? 0 : (len < a.c.limit ? len : a.c.limit);
-  if constexpr (SEL) {  // a token's list holds each block once at most
-    const int blocks = s.len == 0 ? 0 : ((s.len - 1) >> a.block_log2) + 1;
-    s.tiles = s.count * ((a.group + ROWS - 1) / ROWS);
-    s.unit0 = 0;
-    s.units = max(1, min(a.count, blocks) << (a.block_log2 - kUnitLog2));
-  } else {
-    s.tiles = s.count * a.group > p.max_rows ? 0 : (s.count * a.group + ROWS - 1) / ROWS;
-    s.unit0 = first_key(s.pos0, a.window) / kUnit;
-    s.units = max(1, (s.len + kUnit - 1) / kUnit - s.unit0);
-  }
+  s.tiles = s.count * a.group > p.max_rows ? 0 : (s.count * a.group + ROWS - 1) / ROWS;
+  s.unit0 = first_key(s.pos0, a.window) / kUnit;
+  s.units = max(1, (s.len + kUnit - 1) / kUnit - s.unit0);
   return s;
 }
 
@@ -120,7 +114,9 @@ struct Cfg {
   static constexpr int kX = G * NT * 4 * 32;                  // {C, C', C, C'} and {X, X'} of a lane's two rows
   static constexpr int kMeta = ROWS * 16;                     // hi, lo, slope, position of a row
   static constexpr int kCtas = G * NT <= 4 ? 4 : 2;  // per SM: what the registers allow
-  static constexpr int kListCtas = kCtas == 4 ? 3 : kCtas;  // (lists take some more)
+  // the same for lists (512 segments of heads of 128: 45.9 us with 4, 62.6 with 3; 384 of heads of 64, which fit
+  // at once either way: 18.4 with 4, 15.2 with 3)
+  static constexpr int kListCtas = kCtas == 4 && G < 3 ? 3 : kCtas;
   static constexpr int kSmem = kBig + kQ + kX + kMeta + ROWS * 4 + kWarps * kStages * 8;
   static constexpr int kPartial = ROWS * (D + 2);             // floats of one CTA's partial result
 };
@@ -165,11 +161,14 @@ __global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G,
   sm100::pdl_wait();
   sm100::pdl_trigger();
 
-  // ---- this CTA's share of the units
+  // ---- this CTA's share of the units (lists: of the segments)
+  long long share = 0, begin = 0, end = 0, seq_base = 0;
+  int b = -1;
+  if constexpr (!SEL) {
   bool over = false;  // a sequence has more new tokens than max_q
   auto units_of = [&](int i) -> long long {
     if (i >= c.batch) return 0;
-    const Span s = span_of<ROWS, SEL>(p, i);
+    const Span s = span_of<ROWS>(p, i);
     over = over || s.extra > 0;
     return (long long)(s.units) * s.tiles * c.kv_heads;
   };
@@ -184,10 +183,10 @@ __global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G,
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) total += s_scan[w];
   const long long up = total + gridDim.x - 1;
-  long long share = up < (1ll << 32) ? (long long)(unsigned(up) / gridDim.x) : up / gridDim.x;
+  share = up < (1ll << 32) ? (long long)(unsigned(up) / gridDim.x) : up / gridDim.x;
   if (share < p.min_share) share = p.min_share;
-  const long long begin = share * blockIdx.x;
-  const long long end = begin + share < total ? begin + share : total;
+  begin = share * blockIdx.x;
+  end = begin + share < total ? begin + share : total;
 
   // rows that belong to no sequence, or lie past max_q
   if (c.cu_q) {
@@ -200,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G,
     for (int64_t t = (held < 0 ? 0 : held) + int64_t(blockIdx.x); t < c.total; t += gridDim.x) clear(t);
     if (over) {
       for (int i = blockIdx.x; i < c.batch; i += gridDim.x) {
-        const Span s = span_of<ROWS, SEL>(p, i);
+        const Span s = span_of<ROWS>(p, i);
         for (int64_t t = s.first + s.count; t < s.first + s.count + s.extra; ++t) clear(t);
       }
     }
@@ -234,51 +233,46 @@ __global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G,
     if (base > begin) break;
   }
   __syncthreads();
-  int b = s_seq;
-  long long seq_base = s_base;
+  b = s_seq;
+  seq_base = s_base;
   if (b < 0) return;
+  }
 
   const bool bf16 = a.dtype == SPECTRA_DT_BF16;
   const int per_page = 1 << (c.page_log2 - 4);  // tiles
   CopyRing<kStages> ring_order;
   const uint32_t magic = fp16_1024();
   long long at = begin;
+  int work = int(blockIdx.x);  // lists: piece of a segment
 
-  while (at < end) {
-    // ---- the segment that holds unit `at`
-    Span s = span_of<ROWS, SEL>(p, b);
-    long long seq_units = (long long)(s.units) * s.tiles * c.kv_heads;
-    while (at >= seq_base + seq_units) {
-      seq_base += seq_units;
-      ++b;
-      s = span_of<ROWS, SEL>(p, b);
-      seq_units = (long long)(s.units) * s.tiles * c.kv_heads;
-    }
-    const int seg = int(unsigned(at - seq_base) / unsigned(s.units));  // (the launch checks that a sequence's fit)
-    const long long seg_begin = seq_base + (long long)(seg) * s.units, seg_end = seg_begin + s.units;
-    const int head = seg / s.tiles, of_token = (a.group + ROWS - 1) / ROWS;
-    const int only = SEL ? (seg - head * s.tiles) / of_token : 0;  // SEL: the segment's token
-    const int row0 = (seg - head * s.tiles - only * (SEL ? of_token : 0)) * ROWS;
-    const int u_begin = s.unit0 + int(at - seg_begin);
-    const int u_stop = s.unit0 + int((seg_end < end ? seg_end : end) - seg_begin);
-    // nothing held, or a copy that did not arrive in an earlier segment: nothing to load.  (After a
-    // loss the results are undefined, but every segment is counted, so that the counters end at zero.)
-    int u_end = s.len > 0 && !s_stop ? u_stop : u_begin;
-    const int rows = SEL ? min(ROWS, a.group - row0) : min(ROWS, s.count * a.group - row0);
-    auto place = [&](int row, int& tok, int& h) {  // token and query head of a row
-      if constexpr (SEL) {
-        tok = only;
-        h = head * a.group + row0 + row;
-      } else {
-        tok = (row0 + row) / a.group;
-        h = head * a.group + (row0 + row) - tok * a.group;
-      }
-    };
+  while (SEL ? work < p.segments * p.pieces : at < end) {
+    const int segment = SEL ? work / p.pieces : 0, piece = SEL ? work - segment * p.pieces : 0;
+    Span s;
+    long long seg_begin = 0, seg_end = 0;
+    int head, row0, u_begin, u_stop, u_end, rows;
+    const int of_token = (a.group + ROWS - 1) / ROWS;
     if constexpr (SEL) {
-      // ---- the token's list: entries above all before them that hold a key it sees
-      const int pos = s.pos0 + only, hi = pos < 0 ? 0 : (a.causal ? min(s.len, pos + 1) : s.len);
+      // ---- a segment: token, key/value head, row tile; neighbours share a token
+      const int t = segment / (c.kv_heads * of_token), rest = segment - t * (c.kv_heads * of_token);
+      head = rest / of_token;
+      row0 = (rest - head * of_token) * ROWS;
+      rows = min(ROWS, a.group - row0);
+      b = sequence_of(c, t);
+      s = Span{t, 1, 0, 0, -1, 0, 1, 1};  // a row of no sequence, or past max_q: no keys
+      if (b >= 0) {
+        int64_t first;
+        int count, extra;
+        new_rows(c, b, first, count, extra);
+        const int len = c.seq_lens[b], of_seq = int(t - first);
+        if (of_seq < count) {
+          s.pos0 = len - count - extra + of_seq;
+          s.len = len < 0 ? 0 : (len < c.limit ? len : c.limit);
+        }
+      }
+      // the token's list: entries above all before them that hold a key it sees
+      const int pos = s.pos0, hi = pos < 0 ? 0 : (a.causal ? min(s.len, pos + 1) : s.len);
       const int lo = first_key(pos, a.window);
-      const int* list = a.blocks + (s.first + only) * a.b_ts + head * a.b_hs;
+      const int* list = a.blocks + t * a.b_ts + head * a.b_hs;
       int most = -1, kept = 0;  // of the entries before
       for (int i0 = 0; i0 < a.count; i0 += kThreads) {
         const int e = i0 + tid < a.count ? list[i0 + tid] : -1;
@@ -312,8 +306,41 @@ __global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G,
         if (ok) s_list[slot] = e;
       }
       __syncthreads();
-      u_end = max(u_begin, min(u_end, kept << (a.block_log2 - kUnitLog2)));
+      s.units = kept << (a.block_log2 - kUnitLog2);
+      u_begin = int(int64_t(s.units) * piece / p.pieces);
+      u_stop = int(int64_t(s.units) * (piece + 1) / p.pieces);
+      u_end = s_stop ? u_begin : u_stop;
+    } else {
+      // ---- the segment that holds unit `at`
+      s = span_of<ROWS>(p, b);
+      long long seq_units = (long long)(s.units) * s.tiles * c.kv_heads;
+      while (at >= seq_base + seq_units) {
+        seq_base += seq_units;
+        ++b;
+        s = span_of<ROWS>(p, b);
+        seq_units = (long long)(s.units) * s.tiles * c.kv_heads;
+      }
+      const int seg = int(unsigned(at - seq_base) / unsigned(s.units));  // (the launch checks that a sequence's fit)
+      seg_begin = seq_base + (long long)(seg) * s.units;
+      seg_end = seg_begin + s.units;
+      head = seg / s.tiles;
+      row0 = (seg - head * s.tiles) * ROWS;
+      u_begin = s.unit0 + int(at - seg_begin);
+      u_stop = s.unit0 + int((seg_end < end ? seg_end : end) - seg_begin);
+      // nothing held, or a copy that did not arrive in an earlier segment: nothing to load.  (After a
+      // loss the results are undefined, but every segment is counted, so that the counters end at zero.)
+      u_end = s.len > 0 && !s_stop ? u_stop : u_begin;
+      rows = min(ROWS, s.count * a.group - row0);
     }
+    auto place = [&](int row, int& tok, int& h) {  // token and query head of a row
+      if constexpr (SEL) {
+        tok = 0;
+        h = head * a.group + row0 + row;
+      } else {
+        tok = (row0 + row) / a.group;
+        h = head * a.group + (row0 + row) - tok * a.group;
+      }
+    };
     auto unit_pos = [&](int u) {  // position of a unit's first token
       if constexpr (SEL) {
         const int of_block = a.block_log2 - kUnitLog2;
@@ -684,12 +711,17 @@ __global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G,
       }
     __syncthreads();
 
-    const bool whole = seg_begin >= begin && seg_end <= end;
+    const bool whole = SEL ? p.pieces == 1 : seg_begin >= begin && seg_end <= end;
     // the CTAs that share this segment
     const unsigned step = unsigned(share < (1ll << 30) ? share : (1ll << 30));
-    const int cta0 = seg_begin < begin ? int(blockIdx.x - (unsigned(begin - seg_begin) + step - 1) / step) : int(blockIdx.x);
-    const int cta1 = int(blockIdx.x) + (seg_end > end ? int(unsigned(seg_end - 1 - begin) / step) : 0);
+    int cta0 = seg_begin < begin ? int(blockIdx.x - (unsigned(begin - seg_begin) + step - 1) / step) : int(blockIdx.x);
+    int cta1 = int(blockIdx.x) + (seg_end > end ? int(unsigned(seg_end - 1 - begin) / step) : 0);
     float* mine = p.partials + int64_t(2 * blockIdx.x + (seg_begin < begin ? 0 : 1)) * C::kPartial;
+    if constexpr (SEL) {  // (a counter per segment, a part per piece)
+      cta0 = segment;
+      cta1 = segment + p.pieces - 1;
+      mine = p.partials + int64_t(work) * C::kPartial;
+    }
     auto put = [&](int row, int d, float4 v, float sum) {
       int tok, h;
       place(row, tok, h);
@@ -750,9 +782,9 @@ __global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G,
         // 64 parts at a time: a warp per row finds their weights, then every thread adds its
         // items up, 16 loads in flight (one after the other took 7 us of a 34 us call).  The first CTA's part is its last segment's (slot 1),
         // the others' their first's (slot 0).
-        const float* parts = p.partials + int64_t(2 * cta0) * C::kPartial;
+        const float* parts = p.partials + (SEL ? int64_t(segment) * p.pieces : int64_t(2 * cta0)) * C::kPartial;
         const int n = cta1 - cta0 + 1;
-        auto part_of = [&](int k) { return parts + int64_t(k == 0 ? 1 : 2 * k) * C::kPartial; };
+        auto part_of = [&](int k) { return parts + int64_t(SEL ? k : k == 0 ? 1 : 2 * k) * C::kPartial; };
         constexpr int kItems = (ROWS * D / 4 + kThreads - 1) / kThreads, kRowsOfWarp = ROWS / kWarps;
         constexpr int kFlight = kItems >= 4 ? 4 : 16 / kItems;  // parts whose loads are in flight
         float* weight = merge;                        // [ROWS][64] (every thread is past its reads of the slabs)
@@ -830,7 +862,10 @@ __global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G,
     }
     sm100::fence_proxy_async_smem();
     __syncthreads();  // before the ring, the fragments and the row table are written again
-    at = seg_begin + (u_stop - s.unit0);
+    if constexpr (SEL)
+      work += gridDim.x;
+    else
+      at = seg_begin + (u_stop - s.unit0);
   }
 }
 
@@ -853,20 +888,29 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   p.a = a;
   p.min_share = kWarps;
   p.max_rows = max_rows;
-  int64_t tiles = (std::min<int64_t>(int64_t(a.c.max_q) * a.group, max_rows) + C::ROWS - 1) / C::ROWS;
-  int64_t units = (a.c.limit + kUnit - 1) / kUnit + 1;
-  if (SEL) {
-    tiles = int64_t(a.c.max_q) * ((a.group + C::ROWS - 1) / C::ROWS);
-    units = std::min<int64_t>(a.count, (int64_t(a.c.limit) >> a.block_log2) + 1) << (a.block_log2 - kUnitLog2);
-  }
+  const int64_t tiles = (std::min<int64_t>(int64_t(a.c.max_q) * a.group, max_rows) + C::ROWS - 1) / C::ROWS;
+  const int64_t units = (a.c.limit + kUnit - 1) / kUnit + 1;
   const int64_t of_one = int64_t(a.c.kv_heads) * tiles * units;
-  if (of_one >= (int64_t(1) << 30)) return SPECTRA_ERR_SHAPE;
+  if (!SEL && of_one >= (int64_t(1) << 30)) return SPECTRA_ERR_SHAPE;
   const int64_t most = a.c.batch * of_one;
   const int64_t room = std::min<int64_t>(int64_t(device_sms(dev)) * std::max(1, ctas_per_sm[dev]), kMaxCtas);
-  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(room, (most + p.min_share - 1) / p.min_share));
+  int64_t parts = 0;
+  int64_t grid = std::max<int64_t>(1, std::min<int64_t>(room, (most + p.min_share - 1) / p.min_share));
+  if (SEL) {
+    const int64_t segments = a.c.total * a.c.kv_heads * ((a.group + C::ROWS - 1) / C::ROWS);
+    if (segments > INT32_MAX - kMaxCtas) return SPECTRA_ERR_SHAPE;
+    const int64_t list = std::min<int64_t>(a.count, (int64_t(a.c.limit) >> a.block_log2) + 1) << (a.block_log2 - kUnitLog2);
+    p.segments = int(segments);
+    // As many CTAs per segment as the GPU holds; whole ones by turns where there are more segments than CTAs
+    // (512 segments of 64 units in 3 pieces each on 444 CTAs: 72.7 us, whole 62.6)
+    p.pieces = int(std::max<int64_t>(1, std::min<int64_t>(room / segments, list / p.min_share)));
+    grid = std::min<int64_t>(room, segments * p.pieces);
+    if (p.pieces > 1) parts = segments * p.pieces;
+  }
   p.counters = static_cast<int*>(a.workspace);
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + kPagedCounterBytes);
-  if (a.workspace_bytes < kPagedCounterBytes + size_t(grid) * 2 * C::kPartial * sizeof(float)) return SPECTRA_ERR_WORKSPACE;
+  if (!SEL) parts = 2 * grid;
+  if (a.workspace_bytes < kPagedCounterBytes + size_t(parts) * C::kPartial * sizeof(float)) return SPECTRA_ERR_WORKSPACE;
 
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(grid));
