@@ -12,6 +12,7 @@
 // an upper bound of every c_h . k of the block, up to S's rounding.  The sum is
 // max(c, 0) . H + min(c, 0) . L, a product of integers below 2^22, so scores are
 // exact in fp32 and the choice does not depend on the order of the sums.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include <algorithm>
@@ -137,7 +138,8 @@ int launch_index(const PagedIndexArgs& a, cudaStream_t st) {
 // ------------------------------------------------------------ choice
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kHeads = 8;  // query heads whose codes are in shared memory at once
+constexpr int kTile = 16;      // blocks whose scores a warp finds at once
+constexpr int kMaxTokens = 32;  // of a CTA
 
 // A score's place in the order of unsigned numbers (finite or infinite; never 0).
 __device__ __forceinline__ uint32_t order_of(float s) {
@@ -146,30 +148,41 @@ __device__ __forceinline__ uint32_t order_of(float s) {
 }
 constexpr uint32_t kAlways = 0xFFFFFFFFu;
 
+struct TakeScratch {
+  int hist[256];
+  int digit, left, exact;
+  int above[kWarps], equal[kWarps];
+};
+
 // The `count` largest of keys[0 .. n) that are not 0, the lowest index first among
-// equal ones, in ascending order of index, then -1.
-__device__ __forceinline__ void take_best(const uint32_t* keys, int n, int count, int* out) {
-  __shared__ int s_hist[256];
-  __shared__ int s_digit, s_left, s_exact;
-  __shared__ int s_above[kWarps], s_equal[kWarps];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+// equal ones, in ascending order of index, then -1.  By the W threads of a warp or a CTA.
+template <int W>
+__device__ __forceinline__ void take_best(const uint32_t* keys, int n, int count, int* out, TakeScratch& s) {
+  constexpr int WARPS = W / 32;
+  const int tid = threadIdx.x % W, warp = tid >> 5, lane = tid & 31;
+  auto sync = [] {
+    if constexpr (W == 32)
+      __syncwarp();
+    else
+      __syncthreads();
+  };
   // digit by digit from the top: the prefix of the count-th largest key
   uint32_t prefix = 0, mask = 0;
   int left = count;  // to take among the keys of the prefix
   bool all = false;  // ... which is all of them
   for (int shift = 24; shift >= 0 && !all; shift -= 8) {
-    s_hist[tid] = 0;
-    __syncthreads();
-    for (int j = tid; j < n; j += kThreads) {
+    for (int i = tid; i < 256; i += W) s.hist[i] = 0;
+    sync();
+    for (int j = tid; j < n; j += W) {
       const uint32_t k = keys[j];
-      if (k && (k & mask) == prefix) atomicAdd(s_hist + (k >> shift & 255u), 1);
+      if (k && (k & mask) == prefix) atomicAdd(s.hist + (k >> shift & 255u), 1);
     }
-    __syncthreads();
+    sync();
     if (warp == 0) {  // lane l: digits 255 - 8 l .. 248 - 8 l
       int mine[8], sum = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        mine[i] = s_hist[255 - 8 * lane - i];
+        mine[i] = s.hist[255 - 8 * lane - i];
         sum += mine[i];
       }
       int before = sum;
@@ -180,59 +193,56 @@ __device__ __forceinline__ void take_best(const uint32_t* keys, int n, int count
       }
       const int total = __shfl_sync(0xffffffffu, before, 31);
       before -= sum;
-      if (lane == 0 && total <= left) {  // fewer than asked for: all of them
-        s_digit = 0;
-        s_left = 0;
-        s_exact = 2;
-      }
+      if (lane == 0 && total <= left) s.exact = 2;  // fewer than asked for: all of them
       if (total > left && before < left && left <= before + sum) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if (before < left && left <= before + mine[i]) {
-            s_digit = 255 - 8 * lane - i;
-            s_left = left - before;
-            s_exact = mine[i] == left - before;
+            s.digit = 255 - 8 * lane - i;
+            s.left = left - before;
+            s.exact = mine[i] == left - before;
           }
           before += mine[i];
         }
       }
     }
-    __syncthreads();
-    if (s_exact == 2) {
-      all = true;  // (only in the first round: later ones have enough keys)
+    sync();
+    if (s.exact == 2) {
+      all = true;  // (only in the first round: later ones have more keys than asked for)
     } else {
-      prefix |= uint32_t(s_digit) << shift;
+      prefix |= uint32_t(s.digit) << shift;
       mask |= 255u << shift;
-      left = s_left;
-      all = s_exact != 0;
+      left = s.left;
+      all = s.exact != 0;
     }
-    __syncthreads();
+    sync();
   }
   // taken: above the threshold, and `left` that equal it
   const uint32_t least = all ? max(prefix, 1u) : prefix;  // all: every key from here on is taken
   if (all) left = 0;
   auto above = [&](uint32_t k) { return all ? k >= least : k > least; };
-  const int span = (n + kThreads - 1) / kThreads * 32, from = warp * span, to = min(n, from + span);
-  int n_above = 0, n_equal = 0;
-  for (int j0 = from; j0 < to; j0 += 32) {
-    const uint32_t k = j0 + lane < to ? keys[j0 + lane] : 0;
-    n_above += __popc(__ballot_sync(0xffffffffu, k && above(k)));
-    n_equal += __popc(__ballot_sync(0xffffffffu, !all && k == least));
-  }
-  if (lane == 0) {
-    s_above[warp] = n_above;
-    s_equal[warp] = n_equal;
-  }
-  __syncthreads();
-  int taken = 0, equal = 0, whole = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) {
-      taken += s_above[w];
-      equal += s_equal[w];
+  const int span = (n + W - 1) / W * 32, from = warp * span, to = min(n, from + span);
+  int taken = 0, equal = 0, whole = left;
+  if constexpr (WARPS > 1) {
+    int n_above = 0, n_equal = 0;
+    for (int j0 = from; j0 < to; j0 += 32) {
+      const uint32_t k = j0 + lane < to ? keys[j0 + lane] : 0;
+      n_above += __popc(__ballot_sync(0xffffffffu, k && above(k)));
+      n_equal += __popc(__ballot_sync(0xffffffffu, !all && k == least));
     }
-    whole += s_above[w];
+    if (lane == 0) {
+      s.above[warp] = n_above;
+      s.equal[warp] = n_equal;
+    }
+    sync();
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) {
+        taken += s.above[w];
+        equal += s.equal[w];
+      }
+      whole += s.above[w];
+    }
   }
-  whole += left;
   for (int j0 = from; j0 < to; j0 += 32) {
     const uint32_t k = j0 + lane < to ? keys[j0 + lane] : 0;
     const uint32_t ups = __ballot_sync(0xffffffffu, k && above(k)), eqs = __ballot_sync(0xffffffffu, !all && k == least);
@@ -243,126 +253,253 @@ __device__ __forceinline__ void take_best(const uint32_t* keys, int n, int count
     taken += __popc(ups);
     equal += __popc(eqs);
   }
-  for (int i = whole + tid; i < count; i += kThreads) out[i] = -1;
+  if constexpr (WARPS == 1) whole += taken;
+  for (int i = whole + tid; i < count; i += W) out[i] = -1;
+  sync();
 }
 
-template <int G>
-__global__ void __launch_bounds__(kThreads) paged_select_kernel(PagedSelectArgs a) {
+// D += A B of mma.sync m16n8k32, s8 in, s32 out.
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+struct SelectParams {
+  PagedSelectArgs a;
+  int tokens;  // of a CTA
+  int pitch;   // keys of a token
+};
+
+// A cluster has one key/value head and `tokens` new tokens in a row, its CTAs every
+// n-th tile of 16 blocks; the first CTA keeps the keys and takes the best.  Columns of
+// the products: query heads of the tokens, 8 NT at a time.  Operand A, 16 blocks x 32
+// bytes of codes: lane (g, c) has bytes 16 c .. of a 64-byte piece of blocks g and g + 8
+// as they lie in memory, so the k index runs differently than the bytes, the same way in
+// operand B.
+template <int G, int NT>
+__global__ void __launch_bounds__(kThreads) paged_select_kernel(SelectParams p) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
   sm100::pdl_wait();
   sm100::pdl_trigger();
-  constexpr int D = 32 * G, D4 = 2 * D / 4;
-  extern __shared__ __align__(16) uint32_t keys[];  // [max_blocks]
-  __shared__ __align__(16) int8_t s_code[kHeads][2 * D];
+  constexpr int D = 32 * G, COLS = 8 * NT;
+  const PagedSelectArgs& a = p.a;
   const PagedView& c = a.i.c;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int h = blockIdx.x, bl = a.i.block_log2, per_page = 1 << (c.page_log2 - bl);
-  for (int64_t t = blockIdx.y; t < c.total; t += gridDim.y) {
-    int* out = a.blocks + t * a.b_ts + h * a.b_hs;
-    const int b = sequence_of(c, t);
-    int pos = -1;
-    if (b >= 0) {
-      int64_t first;
-      int count;
-      new_tokens(c, b, first, count);
-      pos = c.seq_lens[b] - count + int(t - first);
-      if (pos >= c.limit) pos = -1;
-    }
-    if (pos < 0) {
-      for (int i = tid; i < a.count; i += kThreads) out[i] = -1;
-      continue;
-    }
-    const int n = (pos >> bl) + 1;
-    const int* table = c.tables + b * c.table_stride;
-    const bool scored = n > a.count;
-    int* sums = reinterpret_cast<int*>(keys);
-    for (int j = tid; j < n; j += kThreads) sums[j] = INT32_MIN;
-    for (int g0 = 0; g0 < a.group && scored; g0 += kHeads) {
-      const int heads = min(kHeads, a.group - g0);
-      __syncthreads();
-      for (int i = warp; i < heads; i += kWarps) {
-        const int64_t at = t * a.q_ts + int64_t(h * a.group + g0 + i) * a.q_hs;
-        float x[G], top = 0.f;
-        bool bad = false;
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          x[g] = load_as_float_cg(a.q, at + g * 32 + lane, a.dtype);
-          bad = bad || !(fabsf(x[g]) < INFINITY);
-          top = fmaxf(top, fabsf(x[g]));
-        }
-        bad = __any_sync(0xffffffffu, bad);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float inv = inverse_step(range_step(bad ? 0.f : top));
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const int code = bad ? 0 : int(rintf(x[g] * inv));
-          s_code[i][g * 32 + lane] = int8_t(max(code, 0));
-          s_code[i][D + g * 32 + lane] = int8_t(min(code, 0));
-        }
+  extern __shared__ __align__(16) uint8_t smem[];
+  int8_t* frag = reinterpret_cast<int8_t*>(smem);                     // [G][NT][32 lanes][16 bytes]
+  uint32_t* keys = reinterpret_cast<uint32_t*>(smem + G * NT * 512);  // [tokens][pitch]
+  __shared__ TakeScratch s_take[kWarps];
+  __shared__ int s_pos[kMaxTokens], s_seq[kMaxTokens];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, cc = lane & 3;
+  const int ctas = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+  const int h = blockIdx.x / ctas, bl = a.i.block_log2, pl = c.page_log2 - bl, per_page = 1 << pl;
+  uint32_t* best = ctas > 1 ? cluster.map_shared_rank(keys, 0) : keys;
+
+  for (int64_t t0 = int64_t(blockIdx.y) * p.tokens; t0 < c.total; t0 += int64_t(gridDim.y) * p.tokens) {
+    const int tokens = int(c.total - t0 < p.tokens ? c.total - t0 : p.tokens);
+    // ---- sequences and positions (-1: no place in the cache)
+    for (int i = warp; i < tokens; i += kWarps) {
+      const int64_t t = t0 + i;
+      const int b = sequence_of(c, t);
+      int pos = -1;
+      if (b >= 0) {
+        int64_t first;
+        int count;
+        new_tokens(c, b, first, count);
+        pos = c.seq_lens[b] - count + int(t - first);
+        if (pos >= c.limit) pos = -1;
       }
-      __syncthreads();
-      for (int j = a.first + tid; j < n - a.last; j += kThreads) {
-        const int page = table[j >> (c.page_log2 - bl)];
-        if (unsigned(page) >= unsigned(c.num_pages)) continue;
-        const int64_t slot = (int64_t(page) * c.kv_heads + h) * per_page + (j & (per_page - 1));
-        const int4* codes = reinterpret_cast<const int4*>(a.i.codes + slot * 2 * D);
-        int sum[kHeads];
+      if (lane == 0) {
+        s_pos[i] = pos;
+        s_seq[i] = b;
+      }
+    }
+    __syncthreads();
+    if (rank == 0) {
+      for (int i = 0; i < tokens; ++i) {
+        const int n = s_pos[i] < 0 ? 0 : (s_pos[i] >> bl) + 1;
+        for (int j = tid; j < n; j += kThreads) keys[i * p.pitch + j] = 0;
+      }
+    }
+    if (ctas > 1) cluster.sync(); else __syncthreads();
+
+    // ---- scores, one run of tokens of the same sequence after the other
+    for (int i0 = 0, i1; i0 < tokens; i0 = i1) {
+      const int b = s_seq[i0];
+      int n = 0;  // blocks that a token of the run chooses among
+      for (i1 = i0; i1 < tokens && s_seq[i1] == b; ++i1) {
+        const int of = s_pos[i1] < 0 ? 0 : (s_pos[i1] >> bl) + 1;
+        if (of > a.count) n = max(n, of - a.last);
+      }
+      if (n == 0) continue;
+      const int* table = c.tables + b * c.table_stride;
+      const int columns = (i1 - i0) * a.group;
+      for (int col0 = 0; col0 < columns; col0 += COLS) {
+        __syncthreads();  // the fragments of the columns before have been used
+        for (int i = warp; i < COLS; i += kWarps) {
+          const int col = col0 + i;
+          float x[G], top = 0.f;
+          bool bad = false;
 #pragma unroll
-        for (int i = 0; i < kHeads; ++i) sum[i] = 0;
-        for (int w = 0; w < D4 / 4; ++w) {
-          const int4 k = codes[w];
+          for (int k = 0; k < G; ++k) x[k] = 0.f;
+          if (col < columns) {
+            const int tok = col / a.group, head = h * a.group + col - tok * a.group;
+            const int64_t at = (t0 + i0 + tok) * a.q_ts + head * a.q_hs;
 #pragma unroll
-          for (int i = 0; i < kHeads; ++i) {
-            const int4 q = reinterpret_cast<const int4*>(s_code[i])[w];
-            sum[i] = __dp4a(k.x, q.x, __dp4a(k.y, q.y, __dp4a(k.z, q.z, __dp4a(k.w, q.w, sum[i]))));
+            for (int k = 0; k < G; ++k) {
+              x[k] = load_as_float_cg(a.q, at + k * 32 + lane, a.dtype);
+              bad = bad || !(fabsf(x[k]) < INFINITY);
+              top = fmaxf(top, fabsf(x[k]));
+            }
+          }
+          bad = __any_sync(0xffffffffu, bad);
+          // (magnitudes, as whole numbers in the order of the values)
+          top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+          const float inv = inverse_step(range_step(bad ? 0.f : top));
+#pragma unroll
+          for (int k = 0; k < 2 * G; ++k) {  // feature d of the largest values, then of the smallest
+            const int code = bad ? 0 : int(rintf(x[k % G] * inv)), d = k * 32 + lane;
+            frag[(((d >> 6) * NT + (i >> 3)) * 32 + (i & 7) * 4 + (d >> 4 & 3)) * 16 + (d & 15)] =
+                int8_t(k < G ? max(code, 0) : min(code, 0));
           }
         }
-        int best = sums[j];
-        for (int i = 0; i < heads; ++i) best = max(best, sum[i]);
-        sums[j] = best;
-      }
-    }
-    __syncthreads();
-    for (int j = tid; j < n; j += kThreads) {
-      const int page = table[j >> (c.page_log2 - bl)];
-      uint32_t key = 0;
-      if (unsigned(page) < unsigned(c.num_pages)) {
-        key = kAlways;
-        if (scored && j >= a.first && j < n - a.last) {
-          const float s = a.i.scales[(int64_t(page) * c.kv_heads + h) * per_page + (j & (per_page - 1))];
-          key = order_of(s < INFINITY ? float(sums[j]) * s : INFINITY);
+        __syncthreads();
+        for (int j0 = (warp * ctas + rank) * kTile; j0 < n; j0 += kWarps * ctas * kTile) {
+          uint4 k0[G], k1[G];
+          float s0 = 0.f, s1 = 0.f;
+          bool in0 = false, in1 = false;
+          auto load = [&](int j, uint4 (&k)[G], float& s, bool& in) {
+            const int page = j < n && j >= a.first ? table[j >> pl] : -1;
+            in = unsigned(page) < unsigned(c.num_pages);
+            const int64_t slot = (int64_t(in ? page : 0) * c.kv_heads + h) * per_page + (j & (per_page - 1));
+            const uint4* from = reinterpret_cast<const uint4*>(a.i.codes + slot * 2 * D) + cc;
+#pragma unroll
+            for (int i = 0; i < G; ++i) k[i] = in ? __ldcg(from + 4 * i) : make_uint4(0, 0, 0, 0);
+            if (in) s = __ldcg(a.i.scales + slot);
+          };
+          load(j0 + g, k0, s0, in0);
+          load(j0 + g + 8, k1, s1, in1);
+          int d[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[nt][i] = 0;
+#pragma unroll
+          for (int i = 0; i < G; ++i) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint4 q = reinterpret_cast<const uint4*>(frag)[(i * NT + nt) * 32 + lane];
+              mma_s8(d[nt], k0[i].x, k1[i].x, k0[i].y, k1[i].y, q.x, q.y);
+              mma_s8(d[nt], k0[i].z, k1[i].z, k0[i].w, k1[i].w, q.z, q.w);
+            }
+          }
+          // the best head of each token: columns of a lane, of its neighbours, then in shared memory
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int j = j0 + g + 8 * half;
+              int v0 = d[nt][2 * half], v1 = d[nt][2 * half + 1];
+              int col = col0 + nt * 8 + 2 * cc;
+              bool two = true;  // columns v0 and v1 apart
+              if (a.group % 2 == 0) {
+                v0 = max(v0, v1);  // (columns past the last are of no token)
+                two = false;
+                if (a.group % 4 == 0) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 1));
+                if (a.group % 8 == 0) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 2));
+                if ((a.group % 4 == 0 && (cc & 1)) || (a.group % 8 == 0 && (cc & 2))) col = columns;
+              }
+              const float s = half ? s1 : s0;
+              if (half ? in1 : in0) {
+                auto put = [&](int of, int v) {
+                  if (of >= columns) return;
+                  const int tok = i0 + of / a.group, m = (s_pos[tok] >> bl) + 1;
+                  if (m > a.count && j < m - a.last)
+                    atomicMax(best + tok * p.pitch + j, order_of(s < INFINITY ? float(v) * s : INFINITY));
+                };
+                put(col, v0);
+                if (two) put(col + 1, v1);
+              }
+            }
+          }
         }
       }
-      keys[j] = key;
+    }
+    // ---- those that are always taken, and the best of the others
+    if (ctas > 1) cluster.sync(); else __syncthreads();
+    if (rank == 0) {
+      for (int i = 0; i < tokens; ++i) {
+        if (s_pos[i] < 0) continue;
+        const int* table = c.tables + s_seq[i] * c.table_stride;
+        const int n = (s_pos[i] >> bl) + 1, some = n > a.count ? a.first + a.last : n;
+        for (int k = tid; k < some; k += kThreads) {
+          const int j = n > a.count && k >= a.first ? n - some + k : k;
+          if (unsigned(table[j >> pl]) < unsigned(c.num_pages)) keys[i * p.pitch + j] = kAlways;
+        }
+      }
+      __syncthreads();
+      if (p.tokens == 1) {
+        take_best<kThreads>(keys, s_pos[0] < 0 ? 0 : (s_pos[0] >> bl) + 1, a.count, a.blocks + t0 * a.b_ts + h * a.b_hs, s_take[0]);
+      } else {
+        for (int i = warp; i < tokens; i += kWarps)
+          take_best<32>(keys + i * p.pitch, s_pos[i] < 0 ? 0 : (s_pos[i] >> bl) + 1, a.count,
+                        a.blocks + (t0 + i) * a.b_ts + h * a.b_hs, s_take[warp]);
+      }
     }
     __syncthreads();
-    take_best(keys, n, a.count, out);
-    __syncthreads();
+    if (ctas > 1) cluster.sync();  // before the keys are cleared
   }
 }
 
-template <int G>
-int launch_select(const PagedSelectArgs& a, cudaStream_t st) {
+template <int G, int NT>
+int launch_select_as(const PagedSelectArgs& a, int tokens, int ctas, cudaStream_t st) {
   static PerContextOnce once;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e);
-  auto kern = paged_select_kernel<G>;
+  auto kern = paged_select_kernel<G, NT>;
+  constexpr int kFrag = G * NT * 512;
   e = once.run(dev, [&] {
-    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SPECTRA_MAX_INDEXED_BLOCKS * 4);
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFrag + SPECTRA_MAX_INDEXED_BLOCKS * 4);
   });
   if (e != cudaSuccess) return cuda_status(e);
+  SelectParams p;
+  p.a = a;
+  p.tokens = tokens;
+  p.pitch = a.max_blocks;
+  const int64_t groups = (a.i.c.total + tokens - 1) / tokens;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(a.i.c.kv_heads), unsigned(std::min<int64_t>(a.i.c.total, 65535)));
+  cfg.gridDim = dim3(unsigned(a.i.c.kv_heads * ctas), unsigned(std::min<int64_t>(groups, 65535)));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = size_t(a.max_blocks) * 4;
+  cfg.dynamicSmemBytes = size_t(kFrag) + size_t(tokens) * p.pitch * 4;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(ctas);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, kern, a));
+  cfg.numAttrs = 2;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, p));
+}
+
+template <int G>
+int launch_select(const PagedSelectArgs& a, cudaStream_t st) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e);
+  const int64_t sms = device_sms(dev), lists = a.i.c.total * a.i.c.kv_heads;
+  // Prompts: several tokens a CTA, up to 32 columns, so that codes are read once for all of them.
+  int tokens = std::min({32 / a.group, kMaxTokens, a.i.c.max_q});
+  while (tokens > 1 && (int64_t(tokens) * a.max_blocks > 24 * 1024 || lists < 2 * sms * tokens)) tokens /= 2;
+  if (tokens > 1) return tokens * a.group <= 8 ? launch_select_as<G, 1>(a, tokens, 1, st) : launch_select_as<G, 4>(a, tokens, 1, st);
+  // Few lists: several CTAs each, while they have a tile for every warp.
+  int ctas = 1;
+  while (ctas < 8 && lists * ctas < sms && a.max_blocks > 2 * ctas * kWarps * kTile) ctas *= 2;
+  return a.group <= 8 ? launch_select_as<G, 1>(a, 1, ctas, st) : launch_select_as<G, 4>(a, 1, ctas, st);
 }
 
 }  // namespace
