@@ -152,6 +152,7 @@ struct TakeScratch {
   int hist[256];
   int digit, left, exact;
   int above[kWarps], equal[kWarps];
+  uint32_t any[kWarps], every[kWarps];
 };
 
 // The `count` largest of keys[0 .. n) that are not 0, the lowest index first among
@@ -166,16 +167,51 @@ __device__ __forceinline__ void take_best(const uint32_t* keys, int n, int count
     else
       __syncthreads();
   };
-  // digit by digit from the top: the prefix of the count-th largest key
-  uint32_t prefix = 0, mask = 0;
-  int left = count;  // to take among the keys of the prefix
-  bool all = false;  // ... which is all of them
-  for (int shift = 24; shift >= 0 && !all; shift -= 8) {
+  // the keys to rank: how many, and the bits that not all of them share
+  auto ranked = [](uint32_t k) { return k - 1u < kAlways - 1u; };
+  int always = 0, others = 0;
+  uint32_t any = 0, every = ~0u;
+  for (int j = tid; j < n; j += W) {
+    const uint32_t k = keys[j];
+    always += k == kAlways;
+    if (ranked(k)) {
+      ++others;
+      any |= k;
+      every &= k;
+    }
+  }
+  always = __reduce_add_sync(0xffffffffu, always);
+  others = __reduce_add_sync(0xffffffffu, others);
+  any = __reduce_or_sync(0xffffffffu, any);
+  every = __reduce_and_sync(0xffffffffu, every);
+  if constexpr (WARPS > 1) {
+    if (lane == 0) {
+      s.above[warp] = always;
+      s.equal[warp] = others;
+      s.any[warp] = any;
+      s.every[warp] = every;
+    }
+    sync();
+    always = others = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      always += s.above[w];
+      others += s.equal[w];
+      any |= s.any[w];
+      every &= s.every[w];
+    }
+  }
+  // digit by digit, from the first bit that differs: the prefix of the last key to take
+  int left = count - always;  // to take among the keys of the prefix
+  bool all = others <= left || left == 0;  // ... which is all of them, or none
+  const int top = 31 - __clz((any ^ every) | 1);
+  uint32_t mask = ~((2u << top) - 1u), prefix = left == 0 ? kAlways : all ? 0 : every & mask;
+  for (int shift = max(top - 7, 0), more = 1; more && !all; more = shift > 0, shift = max(shift - 8, 0)) {
     for (int i = tid; i < 256; i += W) s.hist[i] = 0;
     sync();
     for (int j = tid; j < n; j += W) {
       const uint32_t k = keys[j];
-      if (k && (k & mask) == prefix) atomicAdd(s.hist + (k >> shift & 255u), 1);
+      if (ranked(k) && (k & mask) == prefix) atomicAdd(s.hist + (k >> shift & 255u), 1);
     }
     sync();
     if (warp == 0) {  // lane l: digits 255 - 8 l .. 248 - 8 l
@@ -191,10 +227,8 @@ __device__ __forceinline__ void take_best(const uint32_t* keys, int n, int count
         const int up = __shfl_up_sync(0xffffffffu, before, o);
         if (lane >= o) before += up;
       }
-      const int total = __shfl_sync(0xffffffffu, before, 31);
       before -= sum;
-      if (lane == 0 && total <= left) s.exact = 2;  // fewer than asked for: all of them
-      if (total > left && before < left && left <= before + sum) {
+      if (before < left && left <= before + sum) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if (before < left && left <= before + mine[i]) {
@@ -207,16 +241,12 @@ __device__ __forceinline__ void take_best(const uint32_t* keys, int n, int count
       }
     }
     sync();
-    if (s.exact == 2) {
-      all = true;  // (only in the first round: later ones have more keys than asked for)
-    } else {
-      prefix |= uint32_t(s.digit) << shift;
-      mask |= 255u << shift;
-      left = s.left;
-      all = s.exact != 0;
-    }
-    sync();
+    prefix |= uint32_t(s.digit) << shift;  // (digits overlap where the last one is cut: the bits are the same)
+    mask |= 255u << shift;
+    left = s.left;
+    all = s.exact != 0;
   }
+  if constexpr (WARPS > 1) sync();
   // taken: above the threshold, and `left` that equal it
   const uint32_t least = all ? max(prefix, 1u) : prefix;  // all: every key from here on is taken
   if (all) left = 0;
@@ -278,7 +308,7 @@ struct SelectParams {
 // as they lie in memory, so the k index runs differently than the bytes, the same way in
 // operand B.
 template <int G, int NT>
-__global__ void __launch_bounds__(kThreads) paged_select_kernel(SelectParams p) {
+__global__ void __launch_bounds__(kThreads, G < 8 ? 3 : 2) paged_select_kernel(SelectParams p) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   sm100::pdl_wait();
@@ -319,7 +349,12 @@ __global__ void __launch_bounds__(kThreads) paged_select_kernel(SelectParams p) 
     if (rank == 0) {
       for (int i = 0; i < tokens; ++i) {
         const int n = s_pos[i] < 0 ? 0 : (s_pos[i] >> bl) + 1;
-        for (int j = tid; j < n; j += kThreads) keys[i * p.pitch + j] = 0;
+        for (int j = tid; j < n; j += kThreads) {
+          // those that are always taken (scores never touch their keys)
+          const bool always = n <= a.count || j < a.first || j >= n - a.last;
+          const int page = always ? c.tables[s_seq[i] * c.table_stride + (j >> pl)] : -1;
+          keys[i * p.pitch + j] = unsigned(page) < unsigned(c.num_pages) ? kAlways : 0;
+        }
       }
     }
     if (ctas > 1) cluster.sync(); else __syncthreads();
@@ -338,17 +373,31 @@ __global__ void __launch_bounds__(kThreads) paged_select_kernel(SelectParams p) 
       for (int col0 = 0; col0 < columns; col0 += COLS) {
         __syncthreads();  // the fragments of the columns before have been used
         for (int i = warp; i < COLS; i += kWarps) {
+          // four features a lane: d = 4 lane .. of every 128
+          constexpr int R = (G + 3) / 4;
           const int col = col0 + i;
-          float x[G], top = 0.f;
+          float x[4 * R], top = 0.f;
           bool bad = false;
 #pragma unroll
-          for (int k = 0; k < G; ++k) x[k] = 0.f;
+          for (int k = 0; k < 4 * R; ++k) x[k] = 0.f;
           if (col < columns) {
             const int tok = col / a.group, head = h * a.group + col - tok * a.group;
-            const int64_t at = (t0 + i0 + tok) * a.q_ts + head * a.q_hs;
+            const uint16_t* from = reinterpret_cast<const uint16_t*>(a.q) + (t0 + i0 + tok) * a.q_ts + head * a.q_hs + 4 * lane;
 #pragma unroll
-            for (int k = 0; k < G; ++k) {
-              x[k] = load_as_float_cg(a.q, at + k * 32 + lane, a.dtype);
+            for (int k = 0; k < R; ++k) {
+              if (k * 128 + 4 * lane >= D) continue;
+              uint2 w;
+              if (a.vec) {
+                w = __ldcg(reinterpret_cast<const uint2*>(from + k * 128));
+              } else {
+                w.x = uint32_t(__ldcg(from + k * 128)) | uint32_t(__ldcg(from + k * 128 + 1)) << 16;
+                w.y = uint32_t(__ldcg(from + k * 128 + 2)) | uint32_t(__ldcg(from + k * 128 + 3)) << 16;
+              }
+#pragma unroll
+              for (int z = 0; z < 4; ++z) x[4 * k + z] = bits_to_float((z < 2 ? w.x : w.y) >> (16 * (z & 1)) & 0xFFFFu, a.dtype);
+            }
+#pragma unroll
+            for (int k = 0; k < 4 * R; ++k) {
               bad = bad || !(fabsf(x[k]) < INFINITY);
               top = fmaxf(top, fabsf(x[k]));
             }
@@ -358,13 +407,37 @@ __global__ void __launch_bounds__(kThreads) paged_select_kernel(SelectParams p) 
           top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
           const float inv = inverse_step(range_step(bad ? 0.f : top));
 #pragma unroll
-          for (int k = 0; k < 2 * G; ++k) {  // feature d of the largest values, then of the smallest
-            const int code = bad ? 0 : int(rintf(x[k % G] * inv)), d = k * 32 + lane;
-            frag[(((d >> 6) * NT + (i >> 3)) * 32 + (i & 7) * 4 + (d >> 4 & 3)) * 16 + (d & 15)] =
-                int8_t(k < G ? max(code, 0) : min(code, 0));
+          for (int k = 0; k < R; ++k) {
+            if (k * 128 + 4 * lane >= D) continue;
+            uint32_t up = 0, down = 0;  // codes above 0 for the largest values, below 0 for the smallest
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              const int code = bad ? 0 : int(rintf(x[4 * k + z] * inv));
+              up |= uint32_t(max(code, 0)) << (8 * z);
+              down |= (uint32_t(min(code, 0)) & 255u) << (8 * z);
+            }
+            auto put = [&](int d, uint32_t w) {
+              *reinterpret_cast<uint32_t*>(frag + (((d >> 6) * NT + (i >> 3)) * 32 + (i & 7) * 4 + (d >> 4 & 3)) * 16 + (d & 15)) = w;
+            };
+            put(k * 128 + 4 * lane, up);
+            put(D + k * 128 + 4 * lane, down);
           }
         }
         __syncthreads();
+        // of a lane's columns (or of those it speaks for): where their token's keys are, and for how many blocks
+        constexpr int NV = 2 * NT;
+        int at[NV], below[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int col = col0 + (i >> 1) * 8 + 2 * cc + (i & 1);
+          const bool silent = (a.group % 2 == 0 && (i & 1)) || (a.group % 4 == 0 && (cc & 1)) || (a.group % 8 == 0 && (cc & 2));
+          at[i] = below[i] = 0;
+          if (col < columns && !silent) {
+            const int tok = i0 + col / a.group, m = (s_pos[tok] >> bl) + 1;
+            at[i] = tok * p.pitch;
+            if (m > a.count) below[i] = m - a.last;
+          }
+        }
         for (int j0 = (warp * ctas + rank) * kTile; j0 < n; j0 += kWarps * ctas * kTile) {
           uint4 k0[G], k1[G];
           float s0 = 0.f, s1 = 0.f;
@@ -400,45 +473,23 @@ __global__ void __launch_bounds__(kThreads) paged_select_kernel(SelectParams p) 
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               const int j = j0 + g + 8 * half;
-              int v0 = d[nt][2 * half], v1 = d[nt][2 * half + 1];
-              int col = col0 + nt * 8 + 2 * cc;
-              bool two = true;  // columns v0 and v1 apart
-              if (a.group % 2 == 0) {
-                v0 = max(v0, v1);  // (columns past the last are of no token)
-                two = false;
-                if (a.group % 4 == 0) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 1));
-                if (a.group % 8 == 0) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 2));
-                if ((a.group % 4 == 0 && (cc & 1)) || (a.group % 8 == 0 && (cc & 2))) col = columns;
-              }
+              int v0 = d[nt][2 * half];
+              const int v1 = d[nt][2 * half + 1];
+              if (a.group % 2 == 0) v0 = max(v0, v1);  // (a token's columns, or columns of none)
+              if (a.group % 4 == 0) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 1));
+              if (a.group % 8 == 0) v0 = max(v0, __shfl_xor_sync(0xffffffffu, v0, 2));
+              if (!(half ? in1 : in0)) continue;
               const float s = half ? s1 : s0;
-              if (half ? in1 : in0) {
-                auto put = [&](int of, int v) {
-                  if (of >= columns) return;
-                  const int tok = i0 + of / a.group, m = (s_pos[tok] >> bl) + 1;
-                  if (m > a.count && j < m - a.last)
-                    atomicMax(best + tok * p.pitch + j, order_of(s < INFINITY ? float(v) * s : INFINITY));
-                };
-                put(col, v0);
-                if (two) put(col + 1, v1);
-              }
+              if (j < below[2 * nt]) atomicMax(best + at[2 * nt] + j, order_of(s < INFINITY ? float(v0) * s : INFINITY));
+              if (j < below[2 * nt + 1]) atomicMax(best + at[2 * nt + 1] + j, order_of(s < INFINITY ? float(v1) * s : INFINITY));
             }
           }
         }
       }
     }
-    // ---- those that are always taken, and the best of the others
+    // ---- the best
     if (ctas > 1) cluster.sync(); else __syncthreads();
     if (rank == 0) {
-      for (int i = 0; i < tokens; ++i) {
-        if (s_pos[i] < 0) continue;
-        const int* table = c.tables + s_seq[i] * c.table_stride;
-        const int n = (s_pos[i] >> bl) + 1, some = n > a.count ? a.first + a.last : n;
-        for (int k = tid; k < some; k += kThreads) {
-          const int j = n > a.count && k >= a.first ? n - some + k : k;
-          if (unsigned(table[j >> pl]) < unsigned(c.num_pages)) keys[i * p.pitch + j] = kAlways;
-        }
-      }
-      __syncthreads();
       if (p.tokens == 1) {
         take_best<kThreads>(keys, s_pos[0] < 0 ? 0 : (s_pos[0] >> bl) + 1, a.count, a.blocks + t0 * a.b_ts + h * a.b_hs, s_take[0]);
       } else {
