@@ -12,7 +12,7 @@
 // shared memory per token, which counts: 19 bits the token's ids, one says that
 // the prompt holds it, 12 name its bias.  Whole numbers are added up (atomics in
 // shared memory), so their order does not matter, and a list costs one pass
-// over it whatever the vocabulary.  A bit per token says which were met.  Then
+// over it whatever the vocabulary.  The words that are not 0 are listed.  Then
 //   1 a thread for each token met replaces its word by the new logit,
 //   2 a pass over the row writes what may follow and was not met as it is, and
 //     -infinity elsewhere, on pairs of 16 bits as they lie in memory,
@@ -38,7 +38,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;                  // CTAs per row, a power of two (8: a portable cluster size)
 constexpr int kUnits = 4;                       // 16-byte units that a thread takes in a chunk
-constexpr int kFlight = 4;                      // ids of a thread in flight
+constexpr int kFlight = 8;                      // ids of a thread in flight
 constexpr uint32_t kCountBits = 19, kPrompt = 1u << kCountBits, kSlot = kCountBits + 1;
 constexpr uint32_t kCountMask = kPrompt - 1, kLow = (1u << kSlot) - 1;
 static_assert(SPECTRA_MAX_RULE_IDS <= kCountMask && SPECTRA_MAX_RULE_BIASES < (1 << (32 - kSlot)), "a word's fields");
@@ -111,6 +111,10 @@ __device__ __forceinline__ float top_of(const uint32_t (&w)[4]) {
   return bits_to_float(t, DT);
 }
 
+// The cluster's barrier in two halves (arriving releases, waiting acquires).
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
 struct Penalties {
   float rep, freq, pres;
   const float* bias;
@@ -130,17 +134,17 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(LogitArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) uint32_t words[];  // [kChunk<DT>]
   uint16_t* met = reinterpret_cast<uint16_t*>(words + kChunk<DT>);  // [kChunk<DT>] words of the tokens met
-  __shared__ uint32_t s_bits[kChunk<DT> / 32];                      // which were met
   __shared__ int s_met;
-  __shared__ Choice s_best[kWarps];
+  __shared__ Choice s_best[kWarps], s_rows_best[kMaxCluster];
   sm100::pdl_wait();
   sm100::pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t m = blockIdx.y;
   const SpectraLogitRules& r = a.r;
   const uint8_t* row = static_cast<const uint8_t*>(a.x) + m * a.x_rs * SIZE;
-  // unit u: columns u PER - shift ..: 16 bytes at a 16-byte address
-  const int shift = int(reinterpret_cast<uintptr_t>(row) % 16) / SIZE;
+  // unit u: columns u PER - shift ..: 16 bytes at a 16-byte address, the first at a multiple of a turn's 128 bytes,
+  // so that no two CTAs write into one sector
+  const int shift = int(reinterpret_cast<uintptr_t>(row) % (16 << kTurn)) / SIZE;
   const int N = int(a.N), offset = int(a.idx_offset);
   // local unit l of this CTA: unit ((l >> kTurn) * CTAs + rank) << kTurn | l % (1 << kTurn)
   const int ctas = int(cluster.num_blocks()), rank = int(cluster.block_rank()), ctas_log2 = 31 - __clz(ctas);
@@ -150,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(LogitArgs a) {
     return (((((l >> kTurn) << ctas_log2) + rank) << kTurn) + (l & ((1 << kTurn) - 1))) * PER - shift;
   };
   uint8_t* out = static_cast<uint8_t*>(a.out) + m * a.out_rs * (a.out_dtype == SPECTRA_DT_F32 ? 4 : 2);
-  const bool as_units = a.out_dtype == DT && int(reinterpret_cast<uintptr_t>(out) % 16) / SIZE == shift;
+  const bool as_units = a.out_dtype == DT && int(reinterpret_cast<uintptr_t>(out) % 16) / SIZE == shift % PER;
   const int len = !r.ids ? 0 : (r.lengths ? clamp_len(r.lengths[m], r.max_ids) : int(r.max_ids));
   const int prompt = r.prompt_lengths ? clamp_len(r.prompt_lengths[m], len) : 0;
   const int* ids = r.ids + m * r.ids_stride;
@@ -159,6 +163,7 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(LogitArgs a) {
   const Penalties pen = {r.repetition ? r.repetition[m] : 1.f, r.frequency ? r.frequency[m] : 0.f,
                          r.presence ? r.presence[m] : 0.f, r.bias + m * r.bias_stride};
   const bool counted = len > 0 || r.n_bias > 0;
+  if (a.idx) cluster_arrive();  // (waited for before the first CTA's memory is written)
   auto may_follow = [&](int n) { return !allowed || (uint32_t(__ldcg(allowed + ((n + offset) >> 5))) >> ((n + offset) & 31) & 1u); };
   Choice best = {0, INT32_MAX};
   auto consider = [&](float v, int n) {
@@ -167,14 +172,15 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(LogitArgs a) {
   };
   for (int c0 = 0; c0 < mine; c0 += kThreads * kUnits) {
     const int c1 = min(mine, c0 + kThreads * kUnits), columns = (c1 - c0) * PER;
+    const int column0 = first_column(c0 + tid), step = (kThreads * PER) << ctas_log2;
     uint32_t raw[kUnits][4], word0[kUnits], word1[kUnits];
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
-      const int l = c0 + tid + k * kThreads, n0 = first_column(l);
+      const int l = c0 + tid + k * kThreads, n0 = column0 + k * step;
 #pragma unroll
       for (int i = 0; i < 4; ++i) raw[k][i] = 0;
       word0[k] = word1[k] = ~0u;
-      if (l < c1 && n0 >= 0 && n0 + PER <= N) {  // (cut units, at a row's ends, are taken one by one)
+      if (l < c1 && n0 >= 0 && n0 + PER <= N) {
         const uint4 v = __ldcg(reinterpret_cast<const uint4*>(row + int64_t(n0) * SIZE));
         raw[k][0] = v.x; raw[k][1] = v.y; raw[k][2] = v.z; raw[k][3] = v.w;
         if (allowed) {
@@ -182,44 +188,57 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(LogitArgs a) {
           word0[k] = uint32_t(__ldcg(allowed + (t >> 5)));
           if ((t & 31) > 32 - PER) word1[k] = uint32_t(__ldcg(allowed + (t >> 5) + 1));
         }
+      } else if (l < c1) {  // cut at an end of the row: one by one, columns outside as if they were not allowed
+        uint32_t bits = 0;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          const int n = n0 + e;
+          if (n < 0 || n >= N) continue;
+          raw[k][DT == SPECTRA_DT_F32 ? e : e >> 1] |= load_bits_cg(row, n, DT) << (DT == SPECTRA_DT_F32 ? 0 : 16 * (e & 1));
+          bits |= uint32_t(may_follow(n)) << e;
+        }
+        const int at = (n0 + offset) & 31;
+        word0[k] = bits << at;
+        word1[k] = at > 32 - PER ? bits >> (32 - at) : 0;
       }
     }
+    // the first ids, before the row's length is known (a row of ids is max_ids long)
+    int early[kFlight], early_bias = -1;
+#pragma unroll
+    for (int k = 0; k < kFlight; ++k) early[k] = tid + k * kThreads < r.max_ids ? __ldcg(ids + tid + k * kThreads) : -1;
+    if (tid < r.n_bias) early_bias = __ldcg(bias_ids + tid);
     uint32_t own = 0;  // which of the thread's columns were met
     if (counted) {
       for (int i = tid; i < columns / 4; i += kThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
-      for (int i = tid; i < (columns + 31) / 32; i += kThreads) s_bits[i] = 0;
       if (tid == 0) s_met = 0;
       // a token's word, or -1: not of this CTA and chunk
       auto word_of = [&](int id) {
-        const int n = id - offset;
-        if (id < 0 || unsigned(n) >= unsigned(N)) return -1;
-        const unsigned at = unsigned(n + shift), turn = at / (PER << kTurn);
-        if ((turn & unsigned(ctas - 1)) != unsigned(rank)) return -1;
-        const int w = int(turn >> ctas_log2) * (PER << kTurn) + int(at % (PER << kTurn)) - c0 * PER;
-        return w >= 0 && w < columns ? w : -1;
+        const unsigned n = unsigned(id - offset), at = n + shift, turn = at / (PER << kTurn);  // (a negative id is past N)
+        const unsigned w = (turn >> ctas_log2) * (PER << kTurn) + at % (PER << kTurn) - c0 * PER;
+        return n < unsigned(N) && (turn & unsigned(ctas - 1)) == unsigned(rank) && w < unsigned(columns) ? int(w) : -1;
       };
       __syncthreads();
       for (int i0 = tid; i0 < len; i0 += kFlight * kThreads) {
-        int id[kFlight];
-#pragma unroll
-        for (int k = 0; k < kFlight; ++k) id[k] = i0 + k * kThreads < len ? __ldcg(ids + i0 + k * kThreads) : -1;
 #pragma unroll
         for (int k = 0; k < kFlight; ++k) {
-          const int w = word_of(id[k]);
+          const int w = i0 + k * kThreads < len ? word_of(early[k]) : -1;
           if (w < 0) continue;
-          atomicOr(s_bits + (w >> 5), 1u << (w & 31));
           if (i0 + k * kThreads < prompt)
             atomicOr(words + w, kPrompt);
           else
             atomicAdd(words + w, 1u);
         }
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+          const int i = i0 + (kFlight + k) * kThreads;
+          if (i < len) early[k] = __ldcg(ids + i);
+        }
       }
       __syncthreads();
       if (r.n_bias > 0) {
         for (int i = tid; i < r.n_bias; i += kThreads) {
-          const int w = word_of(__ldcg(bias_ids + i));
+          const int w = word_of(i == tid ? early_bias : __ldcg(bias_ids + i));
           if (w < 0) continue;
-          atomicOr(s_bits + (w >> 5), 1u << (w & 31));
           // (the low bits are settled, so the larger word is the later entry)
           atomicMax(words + w, (words[w] & kLow) | uint32_t(i + 1) << kSlot);
         }
@@ -229,7 +248,13 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(LogitArgs a) {
 #pragma unroll
       for (int k = 0; k < kUnits; ++k) {
         const int w = (tid + k * kThreads) * PER;
-        if (w < columns) own |= (s_bits[w >> 5] >> (w & 31) & ALL) << (k * PER);
+        if (w < columns) {
+#pragma unroll
+          for (int e = 0; e < PER; e += 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(words + w + e);
+            own |= uint32_t(min(v.x, 1u) | min(v.y, 1u) << 1 | min(v.z, 1u) << 2 | min(v.w, 1u) << 3) << (k * PER + e);
+          }
+        }
       }
       int before = __popc(own);
 #pragma unroll
@@ -251,47 +276,44 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(LogitArgs a) {
       }
       __syncthreads();  // (the row is written from here on, and may be the logits themselves)
     }
+    float top = -INFINITY;  // of the thread's units, the first that has it, and what it keeps
+    uint32_t top_keep = 0, top_raw[4] = {0, 0, 0, 0};
+    int top_column = 0;
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
-      const int l = c0 + tid + k * kThreads, n0 = first_column(l);
-      if (l >= c1) break;
-      const uint32_t rest = ~(own >> (k * PER)) & ALL;  // not met
-      if (n0 >= 0 && n0 + PER <= N) {
-        const uint32_t keep = __funnelshift_r(word0[k], word1[k], (n0 + offset) & 31) & rest;
-        if (keep != ALL) keep_only<DT>(raw[k], keep);
-        if (a.out) {
-          if (as_units) {
-            *reinterpret_cast<uint4*>(out + int64_t(n0) * SIZE) = make_uint4(raw[k][0], raw[k][1], raw[k][2], raw[k][3]);
-          } else {
+      const int n0 = column0 + k * step;
+      if (c0 + tid + k * kThreads >= c1) break;
+      const uint32_t keep = __funnelshift_r(word0[k], word1[k], (n0 + offset) & 31) & ~(own >> (k * PER)) & ALL;
+      if (keep != ALL) keep_only<DT>(raw[k], keep);
+      if (a.out) {
+        if (as_units && n0 >= 0 && n0 + PER <= N) {
+          *reinterpret_cast<uint4*>(out + int64_t(n0) * SIZE) = make_uint4(raw[k][0], raw[k][1], raw[k][2], raw[k][3]);
+        } else {
 #pragma unroll
-            for (int e = 0; e < PER; ++e) store_from_float(out, n0 + e, a.out_dtype, element<DT>(raw[k], e));
-          }
-        }
-        if (a.idx && keep) {
-          const float top = top_of<DT>(raw[k]);
-          const uint32_t o = order_of(top);
-          if (o > best.order || (o == best.order && n0 < best.column)) {
-            // the first column that has it (where that is -infinity, among the kept)
-            int at = __ffs(keep) - 1;
-            if (top > -INFINITY) {
-#pragma unroll
-              for (int e = PER - 1; e >= 0; --e) at = element<DT>(raw[k], e) == top ? e : at;
-            } else if (top != top) {
-#pragma unroll
-              for (int e = PER - 1; e >= 0; --e) at = element<DT>(raw[k], e) != element<DT>(raw[k], e) ? e : at;
-            }
-            best = {o, n0 + at};
-          }
-        }
-      } else {
-        for (int e = max(0, -n0); e < PER && n0 + e < N; ++e) {
-          if (!(rest >> e & 1u)) continue;
-          const bool ok = may_follow(n0 + e);
-          const float y = ok ? load_as_float_cg(row, n0 + e, DT) : -INFINITY;
-          if (a.out) store_from_float(out, n0 + e, a.out_dtype, y);
-          if (ok) consider(y, n0 + e);
+          for (int e = 0; e < PER; ++e)
+            if (n0 + e >= 0 && n0 + e < N) store_from_float(out, n0 + e, a.out_dtype, element<DT>(raw[k], e));
         }
       }
+      const float t = top_of<DT>(raw[k]);
+      if (keep && (!top_keep || t > top || (t != t && top == top))) {
+        top = t;
+        top_keep = keep;
+        top_column = n0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top_raw[i] = raw[k][i];
+      }
+    }
+    if (a.idx && top_keep) {
+      // the first column that has it (where that is -infinity, among the kept)
+      int at = __ffs(top_keep) - 1;
+      if (top > -INFINITY) {
+#pragma unroll
+        for (int e = PER - 1; e >= 0; --e) at = element<DT>(top_raw, e) == top ? e : at;
+      } else if (top != top) {
+#pragma unroll
+        for (int e = PER - 1; e >= 0; --e) at = element<DT>(top_raw, e) != element<DT>(top_raw, e) ? e : at;
+      }
+      consider(top, top_column + at);
     }
     if (counted) {
       __syncthreads();
@@ -308,20 +330,22 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(LogitArgs a) {
   if (!a.idx) return;  // (the same for every CTA)
   best = best_of_warp(best);
   if (lane == 0) s_best[warp] = best;
-  cluster.sync();
-  if (rank == 0 && warp == 0) {
-    best = {0, INT32_MAX};
-    for (int k = lane; k < ctas * kWarps; k += 32) {
-      const Choice c = *cluster.map_shared_rank(&s_best[k % kWarps], k / kWarps);
-      if (c.order > best.order || (c.order == best.order && c.column < best.column)) best = c;
-    }
+  __syncthreads();
+  if (warp == 0) {
+    best = lane < kWarps ? s_best[lane] : Choice{0, INT32_MAX};
     best = best_of_warp(best);
+  }
+  cluster_wait();  // every CTA of the cluster runs
+  if (tid == 0) *cluster.map_shared_rank(&s_rows_best[rank], 0) = best;
+  cluster_arrive();
+  cluster_wait();
+  if (rank == 0 && warp == 0) {
+    best = best_of_warp(lane < ctas ? s_rows_best[lane] : Choice{0, INT32_MAX});
     if (lane == 0) {
       a.idx[m] = best.order ? best.column + a.idx_offset : -1;
       if (a.val) a.val[m] = value_of(best.order);
     }
   }
-  cluster.sync();  // no CTA leaves while the first may still read its shared memory
 }
 
 template <int DT>

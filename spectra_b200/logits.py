@@ -86,7 +86,8 @@ class LogitRules:
             row[name] = t
         self._keep = (wide, row)
         self.words = 0 if allowed is None else allowed.shape[1]
-        self._index = some.get_device()
+        self._index, self._masked = some.get_device(), allowed is not None
+        self._like = torch.empty(1, dtype=torch.int64, device=self.device).expand(self.rows)  # a shape to allocate by
         at = lambda t: None if t is None or not t.numel() else t.data_ptr()  # noqa: E731
         step = lambda t: 0 if t is None else t.stride(0)  # noqa: E731
         self._c = L.LogitRules(
@@ -103,37 +104,46 @@ class LogitRules:
             raise RuntimeError(f"spectra_b200.logits: the rules must be on one CUDA device (no CPU path), got {name} on {t.device}")
 
 
+_FN = None  # the library's function, looked up once
+
+
 def _apply(x: torch.Tensor, rules: LogitRules, idx_offset: int, out: Optional[torch.Tensor], idx, val) -> None:
     """x, out [M, N] of unit stride along a row; idx int64, val fp32 [M] (each optional)."""
+    global _FN
     M, N = x.shape
-    if not x.is_cuda or x.get_device() != rules._index:
+    index = rules._index
+    if x.get_device() != index:
         raise RuntimeError(f"spectra_b200.logits: the logits must be on the rules' CUDA device (no CPU path), got {x.device}")
-    if x.dtype not in _DT:
+    dt = _DT.get(x.dtype)
+    if dt is None:
         raise TypeError(f"logits must be bf16, fp16 or fp32, got {x.dtype}")
     if M != rules.rows or N < 1:
         raise ValueError(f"the rules are of {rules.rows} rows, the logits {tuple(x.shape)}")
     if idx_offset < 0 or idx_offset + N > 2**31 - 65:
         raise ValueError(f"idx_offset={idx_offset} and {N} logits pass 32 bits")
-    if rules._c.allowed is not None and rules.words * 32 < idx_offset + N:
+    if rules.words * 32 < idx_offset + N and rules._masked:
         raise ValueError(f"allowed has {rules.words} words a row, {-(-(idx_offset + N) // 32)} are needed")
     if M == 0:
         return
-    args = (rules._at, x.data_ptr(), _DT[x.dtype], x.stride(0) if M > 1 else N, M, N, idx_offset,
+    if _FN is None:
+        _FN = L.lib().spectra_adjust_logits
+    args = (rules._at, x.data_ptr(), dt, x.stride(0) if M > 1 else N, M, N, idx_offset,
             None if out is None else out.data_ptr(), 0 if out is None else _DT[out.dtype],
             0 if out is None else (out.stride(0) if M > 1 else N), None if idx is None else idx.data_ptr(),
             None if val is None else val.data_ptr())
-    if torch._C._cuda_getDevice() == rules._index:
-        st = L.lib().spectra_adjust_logits(*args, torch._C._cuda_getCurrentRawStream(rules._index))
+    if torch._C._cuda_getDevice() == index:
+        st = _FN(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(rules._index):
-            st = L.lib().spectra_adjust_logits(*args, torch._C._cuda_getCurrentRawStream(rules._index))
+        with torch.cuda.device(index):
+            st = _FN(*args, torch._C._cuda_getCurrentRawStream(index))
     if st:
         L.check("spectra_adjust_logits", st)
 
 
 def _rows(logits: torch.Tensor) -> torch.Tensor:
     x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
-    return x if x.stride(1) == 1 and (x.shape[0] < 2 or x.stride(0) >= x.shape[1]) else x.contiguous()
+    step, unit = x.stride()
+    return x if unit == 1 and (step >= x.shape[1] or x.shape[0] < 2) else x.contiguous()
 
 
 def adjust_logits(logits: torch.Tensor, rules: LogitRules, *, out: Optional[torch.Tensor] = None,
@@ -147,30 +157,37 @@ def adjust_logits(logits: torch.Tensor, rules: LogitRules, *, out: Optional[torc
 
     ``out`` [..., N], unit stride along a row, may be the logits themselves;
     otherwise they share no element."""
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"logits must be [..., N], got {tuple(logits.shape)}")
-    x = _rows(logits)
     shape = logits.shape
+    flat = len(shape) == 2
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"logits must be [..., N], got {tuple(shape)}")
+    x = _rows(logits)
     if out is None:
-        y = res = torch.empty(x.shape, dtype=out_dtype or logits.dtype, device=x.device)
-        res = y if len(shape) == 2 else y.reshape(shape)
+        if out_dtype is None or out_dtype == x.dtype:
+            y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        elif out_dtype in _DT:
+            y = torch.empty_like(x, dtype=out_dtype, memory_format=torch.contiguous_format)
+        else:
+            raise TypeError(f"out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
+        res = y if flat else y.reshape(shape)
     else:
         if out.shape != shape or out.device != logits.device or (out_dtype or out.dtype) != out.dtype:
             raise ValueError(f"out must be {tuple(shape)} on the logits' device, of out_dtype where that is given")
-        y = out if out.dim() == 2 else out.view(-1, shape[-1])
+        if out.dtype not in _DT:
+            raise TypeError(f"out must be bf16, fp16 or fp32, got {out.dtype}")
+        y = out if flat else out.view(-1, shape[-1])
         if (y.shape[1] > 1 and y.stride(1) != 1) or (y.shape[0] > 1 and y.stride(0) < y.shape[1]):
             raise ValueError("out must have unit stride along a row, and rows that do not overlap")
         same = y.data_ptr() == x.data_ptr() and y.dtype == x.dtype and (y.shape[0] < 2 or y.stride(0) == x.stride(0))
         if not same and _overlap(x, y):
             raise ValueError("out must not overlap the logits, unless it is the logits")
         res = out
-    if y.dtype not in _DT:
-        raise TypeError(f"out_dtype must be bf16, fp16 or fp32, got {y.dtype}")
-    idx = torch.empty(x.shape[0], dtype=torch.int64, device=x.device) if with_tokens else None
-    _apply(x, rules, int(idx_offset), y, idx, None)
     if not with_tokens:
+        _apply(x, rules, idx_offset, y, None, None)
         return res
-    return res, idx if len(shape) == 2 else idx.reshape(shape[:-1])
+    idx = torch.empty_like(rules._like, memory_format=torch.contiguous_format)
+    _apply(x, rules, idx_offset, y, idx, None)
+    return res, idx if flat else idx.reshape(shape[:-1])
 
 
 def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:

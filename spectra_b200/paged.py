@@ -534,21 +534,26 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, *, 
     return out
 
 
+_LISTED = frozenset(1 << i for i in range(5, 17))  # sizes of listed blocks
+
+
 def _lists(blocks, block_size, cache: PagedKVCache, batch: TokenBatch):
     if blocks is None or block_size is None:
         raise ValueError("blocks and block_size come together")
-    _block_size(block_size, 65536)
+    if block_size not in _LISTED:
+        _block_size(block_size, 65536)
     if blocks.dtype != torch.int32:
         raise TypeError(f"blocks must be int32, got {blocks.dtype}")
     if blocks.get_device() != cache._index:
         raise RuntimeError(f"spectra_b200.paged: blocks must be on the cache's CUDA device (no CPU path), got {blocks.device}")
-    if blocks.dim() != 3 or blocks.shape[:2] != (batch.total, cache.kv_heads) or not 0 < blocks.shape[2] <= L.MAX_LISTED_BLOCKS:
+    total, heads, count = blocks.shape if blocks.dim() == 3 else (-1, -1, -1)
+    if total != batch.total or heads != cache.kv_heads or not 0 < count <= L.MAX_LISTED_BLOCKS:
         raise ValueError(f"blocks must be [{batch.total}, {cache.kv_heads}, count], count 1 to {L.MAX_LISTED_BLOCKS}, "
                          f"got {tuple(blocks.shape)}")
     ts, hs, unit = blocks.stride()
-    if unit != 1 and blocks.shape[2] > 1:
+    if unit != 1 and count > 1:
         raise ValueError("blocks must have unit stride along a list")
-    return blocks.data_ptr(), ts, hs, blocks.shape[2], block_size
+    return blocks.data_ptr(), ts, hs, count, block_size
 
 
 def paged_index_update(index: BlockIndex, batch: TokenBatch) -> None:
@@ -590,12 +595,16 @@ def paged_select_blocks(q: torch.Tensor, index: BlockIndex, batch: TokenBatch, c
     if first < 0 or last < 1 or not first + last <= count <= L.MAX_LISTED_BLOCKS:
         raise ValueError(f"count must be first + last to {L.MAX_LISTED_BLOCKS} and last positive, got count={count}, "
                          f"first={first}, last={last}")
-    if batch._limit(cache) > L.MAX_INDEXED_BLOCKS * index.block_size:
-        raise ValueError(f"the choice is among {L.MAX_INDEXED_BLOCKS} blocks at most, the batch may hold "
-                         f"{-(-batch._limit(cache) // index.block_size)} (max_len bounds them)")
     shape = (batch.total, cache.kv_heads, count)
     if out is None:
-        out = torch.empty(shape, dtype=torch.int32, device=q.device)
+        like = batch._like.get((index.block_size, shape))
+        if like is None:  # (the first call of its kind; later ones take few steps)
+            if batch._limit(cache) > L.MAX_INDEXED_BLOCKS * index.block_size:
+                raise ValueError(f"the choice is among {L.MAX_INDEXED_BLOCKS} blocks at most, the batch may hold "
+                                 f"{-(-batch._limit(cache) // index.block_size)} (max_len bounds them)")
+            like = torch.empty(1, 1, 1, dtype=torch.int32, device=q.device).expand(shape)
+            batch._like[index.block_size, shape] = like
+        out = torch.empty_like(like, memory_format=torch.contiguous_format)
     elif out.dtype != torch.int32 or out.shape != shape or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError(f"out must be contiguous int32 {shape} on the cache's device")
     _call(dev, "spectra_paged_select_blocks", cache._at, batch._at, index._at, _DT[q.dtype], heads, q.data_ptr(), q_ts, q_hs,
