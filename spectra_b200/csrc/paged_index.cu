@@ -37,83 +37,159 @@ __device__ __forceinline__ float range_step(float most) {
 __device__ __forceinline__ float inverse_step(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
 // ------------------------------------------------------------ index
-constexpr int kRowsAtOnce = 8;  // tokens that a CTA reads at once: half a tile
+// A warp has one block of one head.  A lane has one word of codes, 8 features, of every
+// ROWS-th token, so that little is left to put together.  A nibble under an exponent is
+// 2048 + q where it lies in bits 12-15 and 128 + q in bits 16-19, so one fma with
+// -(2048 + z) s or -(128 + z) s makes it (q - z) s: 23 and 19 bits, exact.  Bound by these
+// instructions.
+constexpr int kIndexWarps = 4;  // of a CTA
+constexpr int kIndexTokens = 16;
 
-template <int G>
-__global__ void __launch_bounds__(32 * G) paged_index_kernel(PagedIndexArgs a) {
+// 2048 + q of bits 12-15, 128 + q of bits 16-19 (the exponents in registers: mask-and-or is one instruction then).
+__device__ __forceinline__ float nibble_at_12(uint32_t w, uint32_t exponent) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x0000F000, %2, 0xEA;" : "=r"(r) : "r"(w), "r"(exponent));
+  return __uint_as_float(r);
+}
+__device__ __forceinline__ float nibble_at_16(uint32_t w, uint32_t exponent) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000F0000, %2, 0xEA;" : "=r"(r) : "r"(w), "r"(exponent));
+  return __uint_as_float(r);
+}
+__device__ __forceinline__ uint32_t in_register(uint32_t v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// SPLIT: warps that share a block (1, or all of the CTA).
+template <int G, int SPLIT>
+__global__ void __launch_bounds__(32 * kIndexWarps) paged_index_kernel(PagedIndexArgs a) {
   sm100::pdl_wait();
   sm100::pdl_trigger();
-  constexpr int D = 32 * G, W = 4 * G;
+  constexpr int D = 32 * G, W = 4 * G, ROWS = G == 8 ? 1 : G >= 3 ? 2 : 8 / G;
+  constexpr int AT_ONCE = SPLIT > 1 ? 8 : kIndexTokens;  // tokens of a warp whose loads are in flight
+  constexpr int FLIGHT = AT_ONCE / ROWS;
   constexpr TileLayout L{G};
-  __shared__ float4 s_hi[kRowsAtOnce * W * 2], s_lo[kRowsAtOnce * W * 2];
-  __shared__ float s_top[G];
   const PagedView& c = a.c;
-  const int tid = threadIdx.x, row = tid / W, word = tid - row * W, g = word % G;
-  const int h = blockIdx.x, per_page = 1 << (c.page_log2 - a.block_log2), tiles = 1 << (a.block_log2 - 4);
-  for (int b = blockIdx.z; b < c.batch; b += gridDim.z) {
+  __shared__ float2 s_part[SPLIT > 1 ? SPLIT : 1][8][SPLIT > 1 ? W : 1];  // [warp][feature of a word][word]: largest, smallest
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = min(lane / W, ROWS - 1), word = lane < ROWS * W ? lane % W : 0;
+  const int g = word % G, d0 = g * 32 + word / G * 8;  // its features d0 .. d0 + 7
+  const int to_word = (row * W + word) * 4, to_scale = (row * G + g) * 2, to_zero = row * G + g;
+  const uint32_t e12 = in_register(0x45000000u), e16 = in_register(0x43000000u);
+  const int pl = c.page_log2 - a.block_log2, per_page = 1 << pl, tiles = 1 << (a.block_log2 - 4);
+  for (int b = blockIdx.y; b < c.batch; b += gridDim.y) {
     int64_t first;
     int count;
     new_tokens(c, b, first, count);
     const int held = c.seq_lens[b], len = min(held, c.limit);
     if (len <= 0 || count == 0) continue;
-    const int end = len >> a.block_log2;
-    for (int j = (max(held - count, 0) >> a.block_log2) + int(blockIdx.y); j < end; j += gridDim.y) {
-      const int page = c.tables[b * c.table_stride + (j >> (c.page_log2 - a.block_log2))];
+    const int j0 = max(held - count, 0) >> a.block_log2, end = len >> a.block_log2;
+    constexpr int AT_A_TIME = kIndexWarps / SPLIT;  // blocks of a CTA
+    for (int64_t item = int64_t(blockIdx.x) * AT_A_TIME + warp / SPLIT; item < int64_t(end - j0) * c.kv_heads;
+         item += int64_t(gridDim.x) * AT_A_TIME) {
+      const int j = j0 + int(item / c.kv_heads), h = int(item % c.kv_heads);
+      const int page = c.tables[b * c.table_stride + (j >> pl)];
       if (unsigned(page) >= unsigned(c.num_pages)) continue;
       const int part = j & (per_page - 1);
       const uint8_t* t = c.pool + page * c.page_stride +
                          ((int64_t(h) << (c.page_log2 - 4)) + int64_t(part) * tiles) * L.bytes();
-      float hi[8], lo[8];
+      float hi[8], lo[8], finite = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         hi[i] = -INFINITY;
         lo[i] = INFINITY;
       }
-      bool bad = false;
-#pragma unroll 4
-      for (int k = 0; k < 2 * tiles; ++k) {
-        const uint8_t* tile = t + (k >> 1) * L.bytes();
-        const int tok = (k & 1) * 8 + row;
-        const uint32_t w = reinterpret_cast<const uint32_t*>(tile + L.k_codes() + (k & 1) * L.block())[tid];
-        const float s = __half2float(reinterpret_cast<const __half*>(tile + L.k_scales())[tok * G + g]);
-        const float z = float(tile[L.k_zeros() + tok * G + g]);
-        bad = bad || !(fabsf(s) <= 65504.f);
+      const int share = tiles * 16 / SPLIT, k_end = warp % SPLIT * share + share;
+      for (int k0 = k_end - share; k0 < k_end; k0 += AT_ONCE) {
+        // (a flight of 8 tokens is half a tile)
+        const uint8_t* from = t + (k0 >> 4) * L.bytes();
+        const int half = AT_ONCE == 8 ? k0 >> 3 & 1 : 0;
+        uint32_t w[FLIGHT];
+        __half s16[FLIGHT];
+        uint8_t z8[FLIGHT];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float v = (float((w >> (4 * i)) & 15u) - z) * s;
-          hi[i] = fmaxf(hi[i], v);
-          lo[i] = fminf(lo[i], v);
+        for (int k = 0; k < FLIGHT; ++k) {
+          const int tok = k * ROWS;  // (and row)
+          const uint8_t* tile = from + (tok >> 4) * L.bytes();
+          w[k] = __ldcg(reinterpret_cast<const uint32_t*>(tile + L.k_codes() + (half + (tok >> 3 & 1)) * L.block() + (tok & 7) * W * 4 + to_word));
+          s16[k] = __ldcg(reinterpret_cast<const __half*>(tile + L.k_scales() + (8 * half + (tok & 15)) * G * 2 + to_scale));
+          z8[k] = __ldcg(tile + L.k_zeros() + (8 * half + (tok & 15)) * G + to_zero);
+        }
+#pragma unroll
+        for (int k = 0; k < FLIGHT; k += 2) {
+          float v[2][8];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float s = __half2float(s16[k + x]), z = float(z8[k + x]);
+            const float c12 = -(2048.f + z) * s, c16 = -(128.f + z) * s;
+            finite = fmaf(s, 0.f, finite);
+            const uint32_t q[4] = {w[k + x] << 12, w[k + x] << 4, w[k + x] >> 4, w[k + x] >> 12};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              v[x][2 * i] = fmaf(nibble_at_12(q[i], e12), s, c12);
+              v[x][2 * i + 1] = fmaf(nibble_at_16(q[i], e16), s, c16);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            hi[i] = max3(hi[i], v[0][i], v[1][i]);
+            lo[i] = min3(lo[i], v[0][i], v[1][i]);
+          }
         }
       }
-      float4* out = s_hi + tid * 2;
-      out[0] = make_float4(hi[0], hi[1], hi[2], hi[3]);
-      out[1] = make_float4(hi[4], hi[5], hi[6], hi[7]);
-      out = s_lo + tid * 2;
-      out[0] = make_float4(lo[0], lo[1], lo[2], lo[3]);
-      out[1] = make_float4(lo[4], lo[5], lo[6], lo[7]);
-      bad = __syncthreads_or(bad);
-      // thread d: feature d = word (d % 32) / 8 of group d / 32, its d % 8-th
-      const int at = (((tid & 31) >> 3) * G + (tid >> 5)) * 8 + (tid & 7);
-      float up = -INFINITY, down = INFINITY;
+      // the rows: lanes of the same word, then every word's largest magnitude
 #pragma unroll
-      for (int i = 0; i < kRowsAtOnce; ++i) {
-        up = fmaxf(up, reinterpret_cast<const float*>(s_hi)[i * W * 8 + at]);
-        down = fminf(down, reinterpret_cast<const float*>(s_lo)[i * W * 8 + at]);
+      for (int o = W; o < ROWS * W; o *= 2) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          hi[i] = fmaxf(hi[i], __shfl_down_sync(0xffffffffu, hi[i], o));
+          lo[i] = fminf(lo[i], __shfl_down_sync(0xffffffffu, lo[i], o));
+        }
       }
-      float top = bad ? 0.f : fmaxf(fabsf(up), fabsf(down));
+      bool bad = __any_sync(0xffffffffu, !(finite == 0.f));
+      if constexpr (SPLIT > 1) {
+        if (lane < W) {
 #pragma unroll
-      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if ((tid & 31) == 0) s_top[tid >> 5] = top;
-      __syncthreads();
+          for (int i = 0; i < 8; ++i) s_part[warp][i][lane] = make_float2(hi[i], lo[i]);
+        }
+        bad = __syncthreads_or(bad);
+        if (warp == 0 && lane < W) {
 #pragma unroll
-      for (int i = 0; i < G; ++i) top = fmaxf(top, s_top[i]);
+          for (int x = 1; x < SPLIT; ++x)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              hi[i] = fmaxf(hi[i], s_part[x][i][lane].x);
+              lo[i] = fminf(lo[i], s_part[x][i][lane].y);
+            }
+        }
+        __syncthreads();  // before the next block's are written
+        if (warp > 0) continue;
+      }
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
+      // (magnitudes, as whole numbers in the order of the values; of the lanes that hold all rows)
+      top = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < W && !bad ? __float_as_uint(top) : 0u));
       const float step = range_step(top), inv = inverse_step(step);
       const int64_t slot = (int64_t(page) * c.kv_heads + h) * per_page + part;
-      int8_t* codes = a.codes + slot * 2 * D;
-      codes[tid] = bad ? 0 : int8_t(int(ceilf(up * inv)));
-      codes[D + tid] = bad ? 0 : int8_t(int(floorf(down * inv)));
-      if (tid == 0) a.scales[slot] = bad ? INFINITY : step;
-      __syncthreads();  // before the next block writes what this one still reads
+      if (lane < W) {
+        uint32_t up[2] = {0, 0}, down[2] = {0, 0};
+        if (!bad) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            up[i >> 2] |= (uint32_t(int(ceilf(hi[i] * inv))) & 255u) << (8 * (i & 3));
+            down[i >> 2] |= (uint32_t(int(floorf(lo[i] * inv))) & 255u) << (8 * (i & 3));
+          }
+        }
+        *reinterpret_cast<uint2*>(a.codes + slot * 2 * D + d0) = make_uint2(up[0], up[1]);
+        *reinterpret_cast<uint2*>(a.codes + slot * 2 * D + D + d0) = make_uint2(down[0], down[1]);
+      }
+      if (lane == 0) a.scales[slot] = bad ? INFINITY : step;
     }
   }
 }
@@ -122,17 +198,23 @@ template <int G>
 int launch_index(const PagedIndexArgs& a, cudaStream_t st) {
   // a sequence's new tokens fill at most this many blocks (more, where the host's bound does not hold: the kernel loops)
   const int64_t blocks = (int64_t(a.c.max_q) + (1 << a.block_log2) - 1) >> a.block_log2;
+  const int64_t items = blocks * a.c.kv_heads;
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e);
+  // few blocks: four warps each
+  const bool split = items * a.c.batch <= 16 * device_sms(dev);
+  const int64_t ctas = split ? items : (items + kIndexWarps - 1) / kIndexWarps;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(a.c.kv_heads), unsigned(std::min<int64_t>(blocks, 65535)),
-                     unsigned(std::min(a.c.batch, 65535)));
-  cfg.blockDim = dim3(32 * G);
+  cfg.gridDim = dim3(unsigned(std::min<int64_t>(ctas, INT32_MAX)), unsigned(std::min(a.c.batch, 65535)));
+  cfg.blockDim = dim3(32 * kIndexWarps);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, paged_index_kernel<G>, a));
+  return cuda_status(cudaLaunchKernelEx(&cfg, split ? paged_index_kernel<G, kIndexWarps> : paged_index_kernel<G, 1>, a));
 }
 
 // ------------------------------------------------------------ choice
