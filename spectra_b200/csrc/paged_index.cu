@@ -390,7 +390,7 @@ struct SelectParams {
 // as they lie in memory, so the k index runs differently than the bytes, the same way in
 // operand B.
 template <int G, int NT>
-__global__ void __launch_bounds__(kThreads, G < 8 ? 3 : 2) paged_select_kernel(SelectParams p) {
+__global__ void __launch_bounds__(kThreads, G < 8 ? (NT == 1 ? 4 : 2) : 2) paged_select_kernel(SelectParams p) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   sm100::pdl_wait();
