@@ -124,11 +124,14 @@ struct Cfg {
 // ------------------------------------------------------------ the kernel
 // MOD: 0 plain scores, 1 a bias or a cap of up to kLowCap, 2 a higher cap (in MOD 1 its code took
 // 35.4 us where 34.2 are taken without it: verification with a bias)
-// SEL: a segment is one token and the blocks listed for it
-template <int G, int NT, int MOD, bool SEL>
-__global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G, NT>::kCtas) paged_attn_kernel(AttnParams p) {
+// LISTS 1 and 2: a segment is one token and the blocks listed for it.  2 is for fp16 results: weights as two
+// operands, the second what the rounding of the first left (results 2.75e-4 off, 2.1e-4 of it their own rounding;
+// 3.2e-4 with one; 5 % longer, and as much for bf16 results where the kernel was the same).
+template <int G, int NT, int MOD, int LISTS>
+__global__ void __launch_bounds__(kThreads, LISTS ? Cfg<G, NT>::kListCtas : Cfg<G, NT>::kCtas) paged_attn_kernel(AttnParams p) {
   using C = Cfg<G, NT>;
   constexpr int D = C::D, ROWS = C::ROWS;
+  constexpr bool SEL = LISTS > 0;
   constexpr TileLayout L{G};
   const PagedAttnArgs& a = p.a;
   const PagedView& c = a.c;
@@ -641,6 +644,7 @@ __global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G,
           for (int i = 0; i < 8; ++i) sc[i >> 2][nt][i & 3] *= c_exp[nt][i & 1];
       }
       uint32_t pb[2][NT][2];  // P^T fragments: rows as columns
+      uint32_t pl[2][NT][2];  // what the rounding to pb left
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -651,8 +655,13 @@ __global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G,
             asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i]) : "f"(fmaf(sc[tile][nt][i], to_exp[nt][i & 1], kShift - m[nt][i & 1])));
             l[nt][i & 1] += e[i];
           }
-          pb[tile][nt][0] = transpose8x8(h2_pack(e[0], e[1]));
-          pb[tile][nt][1] = transpose8x8(h2_pack(e[2], e[3]));
+          const uint32_t p0 = h2_pack(e[0], e[1]), p1 = h2_pack(e[2], e[3]);
+          pb[tile][nt][0] = transpose8x8(p0);
+          pb[tile][nt][1] = transpose8x8(p1);
+          if constexpr (LISTS == 2) {
+            pl[tile][nt][0] = transpose8x8(h2_pack(e[0] - half_of(p0, 0), e[1] - half_of(p0, 1)));
+            pl[tile][nt][1] = transpose8x8(h2_pack(e[2] - half_of(p1, 0), e[3] - half_of(p1, 1)));
+          }
         }
 
       // ---- values
@@ -683,6 +692,10 @@ __global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G,
           for (int nt = 0; nt < NT; ++nt) {
             mma_f16(o[grp][0][nt], v0[0], v0[1], v1[0], v1[1], pb[tile][nt][0], pb[tile][nt][1]);
             mma_f16(o[grp][1][nt], v0[2], v0[3], v1[2], v1[3], pb[tile][nt][0], pb[tile][nt][1]);
+            if constexpr (LISTS == 2) {
+              mma_f16(o[grp][0][nt], v0[0], v0[1], v1[0], v1[1], pl[tile][nt][0], pl[tile][nt][1]);
+              mma_f16(o[grp][1][nt], v0[2], v0[3], v1[2], v1[3], pl[tile][nt][0], pl[tile][nt][1]);
+            }
           }
         }
       }
@@ -869,7 +882,7 @@ __global__ void __launch_bounds__(kThreads, SEL ? Cfg<G, NT>::kListCtas : Cfg<G,
   }
 }
 
-template <int G, int NT, int MOD, bool SEL>
+template <int G, int NT, int MOD, int LISTS>
 int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   using C = Cfg<G, NT>;
   static PerContextOnce once;
@@ -877,7 +890,7 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e);
-  auto kern = paged_attn_kernel<G, NT, MOD, SEL>;
+  auto kern = paged_attn_kernel<G, NT, MOD, LISTS>;
   e = once.run(dev, [&] {
     cudaError_t r = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (r == cudaSuccess) r = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas_per_sm[dev], kern, kThreads, C::kSmem);
@@ -891,12 +904,12 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   const int64_t tiles = (std::min<int64_t>(int64_t(a.c.max_q) * a.group, max_rows) + C::ROWS - 1) / C::ROWS;
   const int64_t units = (a.c.limit + kUnit - 1) / kUnit + 1;
   const int64_t of_one = int64_t(a.c.kv_heads) * tiles * units;
-  if (!SEL && of_one >= (int64_t(1) << 30)) return SPECTRA_ERR_SHAPE;
+  if (!LISTS && of_one >= (int64_t(1) << 30)) return SPECTRA_ERR_SHAPE;
   const int64_t most = a.c.batch * of_one;
   const int64_t room = std::min<int64_t>(int64_t(device_sms(dev)) * std::max(1, ctas_per_sm[dev]), kMaxCtas);
   int64_t parts = 0;
   int64_t grid = std::max<int64_t>(1, std::min<int64_t>(room, (most + p.min_share - 1) / p.min_share));
-  if (SEL) {
+  if (LISTS) {
     const int64_t segments = a.c.total * a.c.kv_heads * ((a.group + C::ROWS - 1) / C::ROWS);
     if (segments > INT32_MAX - kMaxCtas) return SPECTRA_ERR_SHAPE;
     const int64_t list = std::min<int64_t>(a.count, (int64_t(a.c.limit) >> a.block_log2) + 1) << (a.block_log2 - kUnitLog2);
@@ -909,7 +922,7 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   }
   p.counters = static_cast<int*>(a.workspace);
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + kPagedCounterBytes);
-  if (!SEL) parts = 2 * grid;
+  if (!LISTS) parts = 2 * grid;
   if (a.workspace_bytes < kPagedCounterBytes + size_t(parts) * C::kPartial * sizeof(float)) return SPECTRA_ERR_WORKSPACE;
 
   cudaLaunchConfig_t cfg = {};
@@ -925,37 +938,39 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
-template <int G, int NT, bool SEL>
+template <int G, int NT, int LISTS>
 int launch_mod(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
-  if (a.softcap > kLowCap) return launch_one<G, NT, 2, SEL>(a, max_rows, st);
-  return a.softcap > 0.f || a.slopes ? launch_one<G, NT, 1, SEL>(a, max_rows, st) : launch_one<G, NT, 0, SEL>(a, max_rows, st);
+  if (a.softcap > kLowCap) return launch_one<G, NT, 2, LISTS>(a, max_rows, st);
+  return a.softcap > 0.f || a.slopes ? launch_one<G, NT, 1, LISTS>(a, max_rows, st) : launch_one<G, NT, 0, LISTS>(a, max_rows, st);
 }
 
-template <int G, bool SEL>
+template <int G, int LISTS>
 int launch_rows(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
-  // up to 8 rows per key/value head (SEL: of one token): one column tile (fewer registers, more CTAs per SM);
+  // up to 8 rows per key/value head (lists: of one token): one column tile (fewer registers, more CTAs per SM);
   // heads of 256 have no registers for two
-  if (G == 8 || (SEL ? 1 : int64_t(a.c.max_q)) * a.group <= 8)
-    return launch_mod<G, 1, SEL>(a, max_rows, st);
-  return launch_mod<G, G == 8 ? 1 : 2, SEL>(a, max_rows, st);
+  if (G == 8 || (LISTS ? 1 : int64_t(a.c.max_q)) * a.group <= 8)
+    return launch_mod<G, 1, LISTS>(a, max_rows, st);
+  return launch_mod<G, G == 8 ? 1 : 2, LISTS>(a, max_rows, st);
 }
 
-template <bool SEL>
+template <int LISTS>
 int launch_dim(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   switch (a.c.head_dim) {
-    case 32: return launch_rows<1, SEL>(a, max_rows, st);
-    case 64: return launch_rows<2, SEL>(a, max_rows, st);
-    case 96: return launch_rows<3, SEL>(a, max_rows, st);
-    case 128: return launch_rows<4, SEL>(a, max_rows, st);
-    case 256: return launch_rows<8, SEL>(a, max_rows, st);
+    case 32: return launch_rows<1, LISTS>(a, max_rows, st);
+    case 64: return launch_rows<2, LISTS>(a, max_rows, st);
+    case 96: return launch_rows<3, LISTS>(a, max_rows, st);
+    case 128: return launch_rows<4, LISTS>(a, max_rows, st);
+    case 256: return launch_rows<8, LISTS>(a, max_rows, st);
   }
   return SPECTRA_ERR_UNSUPPORTED;
 }
 
 }  // namespace
 
-int launch_paged_attn(const PagedAttnArgs& a, int max_rows, cudaStream_t st) { return launch_dim<false>(a, max_rows, st); }
-int launch_paged_attn_blocks(const PagedAttnArgs& a, cudaStream_t st) { return launch_dim<true>(a, INT32_MAX, st); }
+int launch_paged_attn(const PagedAttnArgs& a, int max_rows, cudaStream_t st) { return launch_dim<0>(a, max_rows, st); }
+int launch_paged_attn_blocks(const PagedAttnArgs& a, cudaStream_t st) {
+  return a.dtype == SPECTRA_DT_BF16 ? launch_dim<1>(a, INT32_MAX, st) : launch_dim<2>(a, INT32_MAX, st);
+}
 
 size_t paged_attn_workspace_bytes(int head_dim) {
   return kPagedCounterBytes + size_t(kMaxCtas) * 2 * 16 * (head_dim + 2) * sizeof(float);
