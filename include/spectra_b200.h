@@ -511,12 +511,20 @@ typedef struct {
  * rounding (a NaN counts as the maximum), -1 where nothing is allowed; val[m]
  * (optional, with idx) = that maximum, -infinity where there is none.
  * max_ids <= SPECTRA_MAX_RULE_IDS, n_bias <= SPECTRA_MAX_RULE_BIASES.
+ * workspace: spectra_adjust_logits_workspace_bytes bytes, 8-byte aligned, of any
+ * contents; calls that may overlap in time do not share one.
  */
 #define SPECTRA_MAX_RULE_IDS 524287
 #define SPECTRA_MAX_RULE_BIASES 4095
 SPECTRA_API int spectra_adjust_logits(const SpectraLogitRules* rules, const void* x, int x_dtype, int64_t x_row_stride,
                                       int64_t M, int64_t N, int64_t idx_offset, void* out, int out_dtype,
-                                      int64_t out_row_stride, int64_t* idx, float* val, void* stream);
+                                      int64_t out_row_stride, int64_t* idx, float* val, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that such a call needs, 0 where it needs none (rules as in
+ * the call; tokens: whether idx is asked for). */
+SPECTRA_API size_t spectra_adjust_logits_workspace_bytes(const SpectraLogitRules* rules, int64_t M, int64_t N, int x_dtype,
+                                                         int tokens);
 
 /*
  * Walsh-Hadamard rotation of activation rows, the optional GEMV prologue

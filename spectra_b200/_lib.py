@@ -149,7 +149,9 @@ PROTOTYPES = {
         c_void_p, c_void_p, c_int, c_int64,            # rules, x, x_dtype, x_row_stride
         c_int64, c_int64, c_int64,                     # M, N, idx_offset
         c_void_p, c_int, c_int64,                      # out, out_dtype, out_row_stride
-        c_void_p, c_void_p, c_void_p]),                # idx, val, stream
+        c_void_p, c_void_p,                            # idx, val
+        c_void_p, c_size_t, c_void_p]),                # workspace, workspace_bytes, stream
+    "spectra_adjust_logits_workspace_bytes": (c_size_t, [c_void_p, c_int64, c_int64, c_int, c_int]),
     "spectra_fwht": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p]),
     "spectra_p2p_buffer_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
     "spectra_p2p_alloc": (c_int, [c_int64, c_void_p, c_void_p]),

@@ -745,9 +745,27 @@ int spectra_argmax(const void* x, int x_dtype, int64_t x_row_stride, int64_t M, 
   return launch_argmax(a, static_cast<cudaStream_t>(stream));
 }
 
+namespace {
+// The rules that have something to say.
+SpectraLogitRules live_rules(const SpectraLogitRules& rules) {
+  SpectraLogitRules r = rules;
+  if (!r.ids || (!r.repetition && !r.frequency && !r.presence)) {
+    r.ids = nullptr;
+    r.max_ids = 0;
+  }
+  if (!r.bias_ids || !r.bias) r.n_bias = 0;
+  return r;
+}
+}  // namespace
+
+size_t spectra_adjust_logits_workspace_bytes(const SpectraLogitRules* rules, int64_t M, int64_t N, int x_dtype, int tokens) {
+  if (!rules || M <= 0 || N <= 0 || !is_float_dt(x_dtype)) return 0;
+  return logits_workspace_bytes(live_rules(*rules), M, N, x_dtype, tokens != 0);
+}
+
 int spectra_adjust_logits(const SpectraLogitRules* rules, const void* x, int x_dtype, int64_t x_row_stride, int64_t M, int64_t N,
                           int64_t idx_offset, void* out, int out_dtype, int64_t out_row_stride, int64_t* idx, float* val,
-                          void* stream) {
+                          void* workspace, size_t workspace_bytes, void* stream) {
   if (!rules || !x || (!out && !idx) || (val && !idx)) return SPECTRA_ERR_NULL_POINTER;
   if (M < 0 || N <= 0 || idx_offset < 0 || !fits_i32(N) || !fits_i32(idx_offset) ||
       !fits_i32(idx_offset + N + 64))  // (columns are counted in 32 bits, to the end of the last 16 bytes)
@@ -755,13 +773,8 @@ int spectra_adjust_logits(const SpectraLogitRules* rules, const void* x, int x_d
   if (!is_float_dt(x_dtype) || (out && !is_float_dt(out_dtype))) return SPECTRA_ERR_DTYPE;
   if (M > 1 && (x_row_stride < N || (out && out_row_stride < N))) return SPECTRA_ERR_STRIDE;
   LogitArgs a;
-  a.r = *rules;
-  SpectraLogitRules& r = a.r;
-  if (!r.ids || (!r.repetition && !r.frequency && !r.presence)) {
-    r.ids = nullptr;
-    r.max_ids = 0;
-  }
-  if (!r.bias_ids || !r.bias) r.n_bias = 0;
+  a.r = live_rules(*rules);
+  const SpectraLogitRules& r = a.r;
   if (r.max_ids < 0 || r.max_ids > SPECTRA_MAX_RULE_IDS || r.n_bias < 0 || r.n_bias > SPECTRA_MAX_RULE_BIASES)
     return SPECTRA_ERR_SHAPE;
   if (r.allowed && r.allowed_words < (idx_offset + N + 31) / 32) return SPECTRA_ERR_SHAPE;
@@ -778,6 +791,10 @@ int spectra_adjust_logits(const SpectraLogitRules* rules, const void* x, int x_d
   a.x = x; a.x_dtype = x_dtype; a.x_rs = x_row_stride;
   a.out = out; a.out_dtype = out_dtype; a.out_rs = out_row_stride;
   a.idx = idx; a.val = val; a.M = M; a.N = N; a.idx_offset = idx_offset;
+  const size_t need = logits_workspace_bytes(r, M, N, x_dtype, idx != nullptr);
+  if (need && (!workspace || workspace_bytes < need)) return SPECTRA_ERR_WORKSPACE;
+  if (need && !aligned(workspace, 8)) return SPECTRA_ERR_ALIGNMENT;
+  a.tops = static_cast<uint2*>(workspace);
   return launch_logits(a, static_cast<cudaStream_t>(stream));
 }
 

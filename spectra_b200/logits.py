@@ -87,6 +87,7 @@ class LogitRules:
         self._keep = (wide, row)
         self.words = 0 if allowed is None else allowed.shape[1]
         self._index, self._masked = some.get_device(), allowed is not None
+        self._bytes: dict = {}  # of workspace, by what is asked for
         self._like = torch.empty(1, dtype=torch.int64, device=self.device).expand(self.rows)  # a shape to allocate by
         at = lambda t: None if t is None or not t.numel() else t.data_ptr()  # noqa: E731
         step = lambda t: 0 if t is None else t.stride(0)  # noqa: E731
@@ -127,10 +128,17 @@ def _apply(x: torch.Tensor, rules: LogitRules, idx_offset: int, out: Optional[to
         return
     if _FN is None:
         _FN = L.lib().spectra_adjust_logits
+    ws, nbytes = None, rules._bytes.get((N, dt, idx is None))
+    if nbytes is None:
+        nbytes = L.lib().spectra_adjust_logits_workspace_bytes(rules._at, M, N, dt, idx is not None)
+        rules._bytes[N, dt, idx is None] = nbytes
+    if nbytes:
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        ws = buf.data_ptr()
     args = (rules._at, x.data_ptr(), dt, x.stride(0) if M > 1 else N, M, N, idx_offset,
             None if out is None else out.data_ptr(), 0 if out is None else _DT[out.dtype],
             0 if out is None else (out.stride(0) if M > 1 else N), None if idx is None else idx.data_ptr(),
-            None if val is None else val.data_ptr())
+            None if val is None else val.data_ptr(), ws, nbytes)
     if torch._C._cuda_getDevice() == index:
         st = _FN(*args, torch._C._cuda_getCurrentRawStream(index))
     else:

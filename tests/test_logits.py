@@ -10,6 +10,7 @@ from oracle import logits as R
 from spectra_b200 import _lib as L
 from spectra_b200 import logits as LG
 
+MANY = dict(M=200, N=20000, x_rs=20000, out_rs=20000)  # two kernels, with a workspace
 P = 0x10000  # a fake device address: every call below fails its checks first
 
 
@@ -17,7 +18,8 @@ def adjust(rules=None, **kw):
     r = dict(ids=P, ids_stride=8, max_ids=8, lengths=P, prompt_lengths=P, repetition=P, frequency=P, presence=P, bias_ids=P,
              bias_ids_stride=4, bias=P, bias_stride=4, n_bias=4, allowed=P, allowed_stride=4, allowed_words=4)
     r.update(rules or {})
-    d = dict(x=P, x_dtype=L.DT_BF16, x_rs=100, M=2, N=100, offset=0, out=P, out_dtype=L.DT_BF16, out_rs=100, idx=P, val=P, stream=None)
+    d = dict(x=P, x_dtype=L.DT_BF16, x_rs=100, M=2, N=100, offset=0, out=P, out_dtype=L.DT_BF16, out_rs=100, idx=P, val=P, ws=P, ws_bytes=1 << 20,
+             stream=None)
     d.update(kw)
     c = L.LogitRules(*r.values())
     return L.lib().spectra_adjust_logits(ctypes.addressof(c) if rules != "null" else None, *d.values())
@@ -53,14 +55,28 @@ def adjust(rules=None, **kw):
     (dict(lengths=P + 1), {}, L.ERR_ALIGNMENT),
     (dict(bias=P + 2), {}, L.ERR_ALIGNMENT),
     (dict(allowed=P + 2), {}, L.ERR_ALIGNMENT),
+    (dict(allowed_words=700), dict(MANY, ws=None), L.ERR_WORKSPACE),
+    (dict(allowed_words=700), dict(MANY, ws_bytes=200 * 2 * 16 * 8 - 1), L.ERR_WORKSPACE),
+    (dict(allowed_words=700), dict(MANY, ws=P + 4), L.ERR_ALIGNMENT),
 ])
 def test_the_entry_point_refuses(rules, kw, code):
     assert adjust(rules, **kw) == code
 
 
+def test_workspace_bytes():
+    def need(M, N, tokens=1, ids=8, bias=4):
+        c = L.LogitRules(ids=P, max_ids=ids, repetition=P, bias_ids=P, bias=P, n_bias=bias)
+        return L.lib().spectra_adjust_logits_workspace_bytes(ctypes.addressof(c), M, N, L.DT_BF16, tokens)
+
+    assert need(200, 20000) == 200 * 2 * 16 * 8 and need(200, 20000, tokens=0) == 0
+    assert need(148, 20000) == 0 and need(149, 20000) > 0 and need(296, 100) == 0 and need(297, 100) > 0
+    assert need(200, 20000, ids=6000) == 0 and need(200, 300000) == 0  # lists and rows that one kernel takes
+    assert L.lib().spectra_adjust_logits_workspace_bytes(None, 200, 20000, L.DT_BF16, 1) == 0
+
+
 def test_no_rows_is_no_launch():
     assert adjust(M=0) == L.OK
-    assert L.lib().spectra_adjust_logits(None, P, 1, 9, 1, 9, 0, P, 1, 9, None, None, None) == L.ERR_NULL_POINTER
+    assert L.lib().spectra_adjust_logits(None, P, 1, 9, 1, 9, 0, P, 1, 9, None, None, None, 0, None) == L.ERR_NULL_POINTER
 
 
 def i32(*s):
