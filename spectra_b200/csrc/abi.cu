@@ -258,7 +258,7 @@ int spectra_w4a16_gemm_noalloc(
 
 int spectra_device_timeouts(int64_t* count, int reset) {
   if (!count) return SPECTRA_ERR_NULL_POINTER;
-  long long a = 0, b = 0, c = 0, d = 0, e = 0, f = 0, g = 0;
+  long long a = 0, b = 0, c = 0, d = 0, e = 0, f = 0, g = 0, h = 0;
   int st = gemv_timeouts(&a, reset != 0);
   if (st == SPECTRA_OK) st = gemv_pf_timeouts(&b, reset != 0);
   if (st == SPECTRA_OK) st = gemm_timeouts(&c, reset != 0);
@@ -266,8 +266,9 @@ int spectra_device_timeouts(int64_t* count, int reset) {
   if (st == SPECTRA_OK) st = gemv_mt_timeouts(&e, reset != 0);
   if (st == SPECTRA_OK) st = paged_attn_timeouts(&f, reset != 0);
   if (st == SPECTRA_OK) st = paged_prompt_timeouts(&g, reset != 0);
+  if (st == SPECTRA_OK) st = paged_index_timeouts(&h, reset != 0);
   if (st != SPECTRA_OK) return st;
-  *count = int64_t(a + b + c + d + e + f + g);
+  *count = int64_t(a + b + c + d + e + f + g + h);
   return SPECTRA_OK;
 }
 

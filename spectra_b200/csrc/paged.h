@@ -102,6 +102,7 @@ struct PagedIndexArgs {
   int block_log2;
 };
 int launch_paged_index(const PagedIndexArgs& a, cudaStream_t st);
+int paged_index_timeouts(long long* out, bool reset);
 
 struct PagedSelectArgs {
   PagedIndexArgs i;

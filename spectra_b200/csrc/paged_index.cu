@@ -17,11 +17,14 @@
 
 #include <algorithm>
 
+#include "copy_ring.h"
 #include "gemv_mma.cuh"
 #include "paged_view.cuh"
 #include "sm100_ptx.cuh"
 
 namespace spectra {
+
+__device__ int g_paged_index_timeouts = 0;
 
 namespace {
 
@@ -40,10 +43,12 @@ __device__ __forceinline__ float inverse_step(float s) { return __uint_as_float(
 // A warp has one block of one head.  A lane has one word of codes, 8 features, of every
 // ROWS-th token, so that little is left to put together.  A nibble under an exponent is
 // 2048 + q where it lies in bits 12-15 and 128 + q in bits 16-19, so one fma with
-// -(2048 + z) s or -(128 + z) s makes it (q - z) s: 23 and 19 bits, exact.  Bound by these
-// instructions.
+// -(2048 + z) s or -(128 + z) s makes it (q - z) s: 23 and 19 bits, exact.
+//
+// Bound by instructions, about 40 for a word of two tokens (issue slots 64 % taken, ALU 57 %).
+// Measured: 6 ragged prompts up to 16384, 8 heads of 128, blocks of 64: 20.3 us with the cache
+// in HBM (1.7 TB/s; loads straight from memory 25.7), one token of 128 sequences 3.9 us.
 constexpr int kIndexWarps = 4;  // of a CTA
-constexpr int kIndexTokens = 16;
 
 // 2048 + q of bits 12-15, 128 + q of bits 16-19 (the exponents in registers: mask-and-or is one instruction then).
 __device__ __forceinline__ float nibble_at_12(uint32_t w, uint32_t exponent) {
@@ -66,155 +71,324 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   return r;
 }
 
-// SPLIT: warps that share a block (1, or all of the CTA).
-template <int G, int SPLIT>
-__global__ void __launch_bounds__(32 * kIndexWarps) paged_index_kernel(PagedIndexArgs a) {
+// The range of a word's features over the tokens that a lane has seen.
+struct Range {
+  float hi[8], lo[8], finite;  // finite: 0, or NaN once a scale was not
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      hi[i] = -INFINITY;
+      lo[i] = INFINITY;
+    }
+    finite = 0.f;
+  }
+  // two tokens: words, scales, zero points
+  __device__ __forceinline__ void add(const uint32_t (&w)[2], const float (&scale)[2], const float (&zero)[2], uint32_t e12, uint32_t e16) {
+    float v[2][8];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float s = scale[x], c12 = -(2048.f + zero[x]) * s, c16 = -(128.f + zero[x]) * s;
+      finite = fmaf(s, 0.f, finite);
+      const uint32_t q[4] = {w[x] << 12, w[x] << 4, w[x] >> 4, w[x] >> 12};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[x][2 * i] = fmaf(nibble_at_12(q[i], e12), s, c12);
+        v[x][2 * i + 1] = fmaf(nibble_at_16(q[i], e16), s, c16);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      hi[i] = max3(hi[i], v[0][i], v[1][i]);
+      lo[i] = min3(lo[i], v[0][i], v[1][i]);
+    }
+  }
+};
+
+// A lane's word of a token and which of the tokens it takes.
+template <int G>
+struct LaneWord {
+  static constexpr int W = 4 * G, ROWS = G == 8 ? 1 : G >= 3 ? 2 : 8 / G;  // words of a token, tokens of a warp at once
+  int row, word, g;
+  __device__ __forceinline__ explicit LaneWord(int lane) {
+    row = min(lane / W, ROWS - 1);
+    word = lane < ROWS * W ? lane % W : 0;
+    g = word % G;
+  }
+  // lanes of the same word become one: lane word has it
+  __device__ __forceinline__ void join_rows(Range& r) const {
+#pragma unroll
+    for (int o = W; o < ROWS * W; o *= 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        r.hi[i] = fmaxf(r.hi[i], __shfl_down_sync(0xffffffffu, r.hi[i], o));
+        r.lo[i] = fminf(r.lo[i], __shfl_down_sync(0xffffffffu, r.lo[i], o));
+      }
+    }
+  }
+  // the index of a block, from the lanes that have a word's whole range
+  __device__ __forceinline__ void store(const PagedIndexArgs& a, int64_t slot, const Range& r, bool bad, int lane) const {
+    constexpr int D = 32 * G;
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(fabsf(r.hi[i]), fabsf(r.lo[i])));
+    // (magnitudes, as whole numbers in the order of the values)
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < W && !bad ? __float_as_uint(top) : 0u));
+    const float step = range_step(top), inv = inverse_step(step);
+    if (lane < W) {
+      uint32_t up[2] = {0, 0}, down[2] = {0, 0};
+      if (!bad) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          up[i >> 2] |= (uint32_t(int(ceilf(r.hi[i] * inv))) & 255u) << (8 * (i & 3));
+          down[i >> 2] |= (uint32_t(int(floorf(r.lo[i] * inv))) & 255u) << (8 * (i & 3));
+        }
+      }
+      const int d0 = g * 32 + word / G * 8;
+      *reinterpret_cast<uint2*>(a.codes + slot * 2 * D + d0) = make_uint2(up[0], up[1]);
+      *reinterpret_cast<uint2*>(a.codes + slot * 2 * D + D + d0) = make_uint2(down[0], down[1]);
+    }
+    if (lane == 0) a.scales[slot] = bad ? INFINITY : step;
+  }
+};
+
+// The blocks of sequence b that its new tokens filled: j0 .. end - 1.
+__device__ __forceinline__ void filled_blocks(const PagedIndexArgs& a, int b, int& j0, int& end) {
+  int64_t first;
+  int count;
+  new_tokens(a.c, b, first, count);
+  const int held = a.c.seq_lens[b], len = min(held, a.c.limit);
+  j0 = max(held - count, 0) >> a.block_log2;
+  end = len > 0 && count > 0 ? len >> a.block_log2 : j0;
+}
+
+// Few blocks: the four warps of a CTA share one, a quarter of its tokens each, straight from memory.
+template <int G>
+__global__ void __launch_bounds__(32 * kIndexWarps) paged_index_few_kernel(PagedIndexArgs a) {
   sm100::pdl_wait();
   sm100::pdl_trigger();
-  constexpr int D = 32 * G, W = 4 * G, ROWS = G == 8 ? 1 : G >= 3 ? 2 : 8 / G;
-  constexpr int AT_ONCE = SPLIT > 1 ? 8 : kIndexTokens;  // tokens of a warp whose loads are in flight
-  constexpr int FLIGHT = AT_ONCE / ROWS;
+  using Word = LaneWord<G>;
+  constexpr int W = Word::W, ROWS = Word::ROWS, FLIGHT = 8 / ROWS;  // 8 tokens of a warp are in flight: half a tile
   constexpr TileLayout L{G};
+  __shared__ float2 s_part[kIndexWarps][8][W];  // [warp][feature of a word][word]: largest, smallest
   const PagedView& c = a.c;
-  __shared__ float2 s_part[SPLIT > 1 ? SPLIT : 1][8][SPLIT > 1 ? W : 1];  // [warp][feature of a word][word]: largest, smallest
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = min(lane / W, ROWS - 1), word = lane < ROWS * W ? lane % W : 0;
-  const int g = word % G, d0 = g * 32 + word / G * 8;  // its features d0 .. d0 + 7
-  const int to_word = (row * W + word) * 4, to_scale = (row * G + g) * 2, to_zero = row * G + g;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Word at(lane);
   const uint32_t e12 = in_register(0x45000000u), e16 = in_register(0x43000000u);
   const int pl = c.page_log2 - a.block_log2, per_page = 1 << pl, tiles = 1 << (a.block_log2 - 4);
   for (int b = blockIdx.y; b < c.batch; b += gridDim.y) {
-    int64_t first;
-    int count;
-    new_tokens(c, b, first, count);
-    const int held = c.seq_lens[b], len = min(held, c.limit);
-    if (len <= 0 || count == 0) continue;
-    const int j0 = max(held - count, 0) >> a.block_log2, end = len >> a.block_log2;
-    constexpr int AT_A_TIME = kIndexWarps / SPLIT;  // blocks of a CTA
-    for (int64_t item = int64_t(blockIdx.x) * AT_A_TIME + warp / SPLIT; item < int64_t(end - j0) * c.kv_heads;
-         item += int64_t(gridDim.x) * AT_A_TIME) {
+    int j0, end;
+    filled_blocks(a, b, j0, end);
+    for (int64_t item = blockIdx.x; item < int64_t(end - j0) * c.kv_heads; item += gridDim.x) {
       const int j = j0 + int(item / c.kv_heads), h = int(item % c.kv_heads);
       const int page = c.tables[b * c.table_stride + (j >> pl)];
       if (unsigned(page) >= unsigned(c.num_pages)) continue;
       const int part = j & (per_page - 1);
-      const uint8_t* t = c.pool + page * c.page_stride +
-                         ((int64_t(h) << (c.page_log2 - 4)) + int64_t(part) * tiles) * L.bytes();
-      float hi[8], lo[8], finite = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        hi[i] = -INFINITY;
-        lo[i] = INFINITY;
-      }
-      const int share = tiles * 16 / SPLIT, k_end = warp % SPLIT * share + share;
-      for (int k0 = k_end - share; k0 < k_end; k0 += AT_ONCE) {
-        // (a flight of 8 tokens is half a tile)
-        const uint8_t* from = t + (k0 >> 4) * L.bytes();
-        const int half = AT_ONCE == 8 ? k0 >> 3 & 1 : 0;
+      const uint8_t* t = c.pool + page * c.page_stride + ((int64_t(h) << (c.page_log2 - 4)) + int64_t(part) * tiles) * L.bytes();
+      Range r;
+      r.clear();
+      const int share = tiles * 16 / kIndexWarps;
+      for (int k0 = warp * share; k0 < (warp + 1) * share; k0 += 8) {
+        const uint8_t* tile = t + (k0 >> 4) * L.bytes();
+        const int half = k0 >> 3 & 1;
         uint32_t w[FLIGHT];
-        __half s16[FLIGHT];
-        uint8_t z8[FLIGHT];
+        float s[FLIGHT], z[FLIGHT];
 #pragma unroll
         for (int k = 0; k < FLIGHT; ++k) {
-          const int tok = k * ROWS;  // (and row)
-          const uint8_t* tile = from + (tok >> 4) * L.bytes();
-          w[k] = __ldcg(reinterpret_cast<const uint32_t*>(tile + L.k_codes() + (half + (tok >> 3 & 1)) * L.block() + (tok & 7) * W * 4 + to_word));
-          s16[k] = __ldcg(reinterpret_cast<const __half*>(tile + L.k_scales() + (8 * half + (tok & 15)) * G * 2 + to_scale));
-          z8[k] = __ldcg(tile + L.k_zeros() + (8 * half + (tok & 15)) * G + to_zero);
+          const int tok = k * ROWS + at.row;
+          w[k] = __ldcg(reinterpret_cast<const uint32_t*>(tile + L.k_codes() + half * L.block()) + tok * W + at.word);
+          s[k] = __half2float(__ldcg(reinterpret_cast<const __half*>(tile + L.k_scales()) + (8 * half + tok) * G + at.g));
+          z[k] = float(__ldcg(tile + L.k_zeros() + (8 * half + tok) * G + at.g));
         }
 #pragma unroll
         for (int k = 0; k < FLIGHT; k += 2) {
-          float v[2][8];
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float s = __half2float(s16[k + x]), z = float(z8[k + x]);
-            const float c12 = -(2048.f + z) * s, c16 = -(128.f + z) * s;
-            finite = fmaf(s, 0.f, finite);
-            const uint32_t q[4] = {w[k + x] << 12, w[k + x] << 4, w[k + x] >> 4, w[k + x] >> 12};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              v[x][2 * i] = fmaf(nibble_at_12(q[i], e12), s, c12);
-              v[x][2 * i + 1] = fmaf(nibble_at_16(q[i], e16), s, c16);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            hi[i] = max3(hi[i], v[0][i], v[1][i]);
-            lo[i] = min3(lo[i], v[0][i], v[1][i]);
-          }
+          const int k1 = min(k + 1, FLIGHT - 1);  // (a flight of one token: the same again)
+          r.add({w[k], w[k1]}, {s[k], s[k1]}, {z[k], z[k1]}, e12, e16);
         }
       }
-      // the rows: lanes of the same word, then every word's largest magnitude
+      at.join_rows(r);
+      bool bad = __any_sync(0xffffffffu, !(r.finite == 0.f));
+      if (lane < W) {
 #pragma unroll
-      for (int o = W; o < ROWS * W; o *= 2) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          hi[i] = fmaxf(hi[i], __shfl_down_sync(0xffffffffu, hi[i], o));
-          lo[i] = fminf(lo[i], __shfl_down_sync(0xffffffffu, lo[i], o));
-        }
+        for (int i = 0; i < 8; ++i) s_part[warp][i][lane] = make_float2(r.hi[i], r.lo[i]);
       }
-      bool bad = __any_sync(0xffffffffu, !(finite == 0.f));
-      if constexpr (SPLIT > 1) {
+      bad = __syncthreads_or(bad);
+      if (warp == 0) {
         if (lane < W) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) s_part[warp][i][lane] = make_float2(hi[i], lo[i]);
-        }
-        bad = __syncthreads_or(bad);
-        if (warp == 0 && lane < W) {
-#pragma unroll
-          for (int x = 1; x < SPLIT; ++x)
+          for (int x = 1; x < kIndexWarps; ++x)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              hi[i] = fmaxf(hi[i], s_part[x][i][lane].x);
-              lo[i] = fminf(lo[i], s_part[x][i][lane].y);
+              r.hi[i] = fmaxf(r.hi[i], s_part[x][i][lane].x);
+              r.lo[i] = fminf(r.lo[i], s_part[x][i][lane].y);
             }
         }
-        __syncthreads();  // before the next block's are written
-        if (warp > 0) continue;
+        at.store(a, (int64_t(page) * c.kv_heads + h) * per_page + part, r, bad, lane);
       }
-      float top = 0.f;
+      __syncthreads();  // before the next block's are written
+    }
+  }
+}
+
+// Many blocks: a warp each, in pieces of 32 tokens that bulk copies bring into shared memory, the next piece
+// while one is looked at.  Of a tile the key codes, and what lies from the key scales to the key zero points.
+template <int G>
+struct Piece {
+  static constexpr int kTiles = 2, kCodes = 256 * G, kRest = 80 * G, kTile = kCodes + kRest, kBytes = kTiles * kTile;
+  static constexpr int kStages = 3;
+  static constexpr int kSmem = kIndexWarps * kStages * (kBytes + 8);
+  static constexpr int kCtas = 224 * 1024 / (kSmem + 1024) < 8 ? 224 * 1024 / (kSmem + 1024) : 8;  // per SM
+};
+
+template <int G>
+__global__ void __launch_bounds__(32 * kIndexWarps) paged_index_kernel(PagedIndexArgs a) {
+  using Word = LaneWord<G>;
+  using P = Piece<G>;
+  constexpr int W = Word::W, ROWS = Word::ROWS;
+  constexpr TileLayout L{G};
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ volatile int s_never;  // 0: each warp waits for its own copies
+  constexpr int kSeqs = 32 * kIndexWarps;
+  __shared__ int s_from[kSeqs], s_first[kSeqs], s_sum[kIndexWarps];
+  const PagedView& c = a.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint8_t* stages = smem + warp * P::kStages * P::kBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kIndexWarps * P::kStages * P::kBytes) + warp * P::kStages;
+  if (lane < P::kStages) sm100::mbar_init(bars + lane, 1);
+  if (threadIdx.x == 0) s_never = 0;
+  sm100::fence_mbar_init();
+  __syncthreads();
+  sm100::pdl_wait();
+  sm100::pdl_trigger();
+  const Word at(lane);
+  const uint32_t e12 = in_register(0x45000000u), e16 = in_register(0x43000000u);
+  const int pl = c.page_log2 - a.block_log2, per_page = 1 << pl;
+  const int pieces_log2 = a.block_log2 - 5;
+  const int h = blockIdx.y, block0 = int(blockIdx.x) * kIndexWarps + warp, stride = int(gridDim.x) * kIndexWarps;
+  CopyRing<P::kStages> ring;
+  for (int b0 = 0; b0 < c.batch; b0 += kSeqs) {
+    // ---- the blocks of some sequences, end to end
+    int j0 = 0, end = 0;
+    if (b0 + int(threadIdx.x) < c.batch) filled_blocks(a, b0 + int(threadIdx.x), j0, end);
+    int upto = end - j0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
-      // (magnitudes, as whole numbers in the order of the values; of the lanes that hold all rows)
-      top = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < W && !bad ? __float_as_uint(top) : 0u));
-      const float step = range_step(top), inv = inverse_step(step);
-      const int64_t slot = (int64_t(page) * c.kv_heads + h) * per_page + part;
-      if (lane < W) {
-        uint32_t up[2] = {0, 0}, down[2] = {0, 0};
-        if (!bad) {
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
+    }
+    __syncthreads();  // the sequences before have been read
+    if (lane == 31) s_sum[warp] = upto;
+    s_first[threadIdx.x] = j0;
+    __syncthreads();
+    int blocks = 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            up[i >> 2] |= (uint32_t(int(ceilf(hi[i] * inv))) & 255u) << (8 * (i & 3));
-            down[i >> 2] |= (uint32_t(int(floorf(lo[i] * inv))) & 255u) << (8 * (i & 3));
+    for (int w = 0; w < kIndexWarps; ++w) {
+      if (w < warp) upto += s_sum[w];
+      blocks += s_sum[w];
+    }
+    s_from[threadIdx.x] = upto - (end - j0);
+    __syncthreads();
+    int from[kSeqs / 32];
+#pragma unroll
+    for (int i = 0; i < kSeqs / 32; ++i) from[i] = s_from[i * 32 + lane];
+    // the warp's k-th piece: of block block0 + (k >> pieces_log2) * stride; its page, or one outside the pool
+    auto find = [&](int k, int& j) {
+      const int block = block0 + (k >> pieces_log2) * stride;
+      int of = -1;  // the last sequence that starts at or before it
+#pragma unroll
+      for (int i = 0; i < kSeqs / 32; ++i) of += __popc(__ballot_sync(0xffffffffu, from[i] <= block));
+      j = s_first[of] + block - s_from[of];
+      return c.tables[(b0 + of) * c.table_stride + (j >> pl)];
+    };
+    auto issue = [&](int k, int stage) {
+      int j;
+      const int page = find(k, j);
+      if (lane == 0) {
+        if (unsigned(page) < unsigned(c.num_pages))
+          sm100::mbar_arrive_expect_tx(bars + stage, P::kTiles * P::kTile);
+        else
+          sm100::mbar_arrive(bars + stage);
+      }
+      __syncwarp();
+      if (unsigned(page) < unsigned(c.num_pages) && lane < 2 * P::kTiles) {
+        const int tile = ((j & (per_page - 1)) << (a.block_log2 - 4)) + (k & ((1 << pieces_log2) - 1)) * P::kTiles + (lane >> 1);
+        const uint8_t* from = c.pool + page * c.page_stride + ((int64_t(h) << (c.page_log2 - 4)) + tile) * L.bytes();
+        uint8_t* to = stages + stage * P::kBytes + (lane >> 1) * P::kTile;
+        if (lane & 1)
+          bulk_g2s(to + P::kCodes, from + L.k_scales(), P::kRest, bars + stage);
+        else
+          bulk_g2s(to, from + L.k_codes(), P::kCodes, bars + stage);
+      }
+    };
+    auto arrived = [&](int stage, uint32_t parity) {  // (the vote makes the lanes agree)
+      const bool ok = __all_sync(0xffffffffu, sm100::mbar_wait(bars + stage, parity, &s_never));
+      if (!ok && lane == 0) atomicAdd(&g_paged_index_timeouts, 1);
+      return ok;
+    };
+    ring.start(block0 < blocks ? ((blocks - block0 + stride - 1) / stride) << pieces_log2 : 0, issue);
+    Range r;
+    for (int k = 0; ring.more(); ++k) {
+      if (!ring.take(arrived)) break;  // (a copy that did not arrive: counted, the index is undefined)
+      int j;
+      const int page = find(k, j);
+      const bool held = unsigned(page) < unsigned(c.num_pages);
+      if ((k & ((1 << pieces_log2) - 1)) == 0) r.clear();
+      if (held) {
+        const uint8_t* piece = stages + ring.stage * P::kBytes;
+#pragma unroll 1
+        for (int x = 0; x < P::kTiles; ++x, piece += P::kTile) {
+          const uint32_t* codes = reinterpret_cast<const uint32_t*>(piece) + at.row * W + at.word;
+          const __half* scales = reinterpret_cast<const __half*>(piece + P::kCodes) + at.row * G + at.g;
+          const uint8_t* zeros = piece + P::kCodes + (L.k_zeros() - L.k_scales()) + at.row * G + at.g;
+#pragma unroll
+          for (int t = 0; t < 16; t += 2 * ROWS) {
+            if constexpr (ROWS == 8) {  // one token a lane in half a tile: the two halves
+              r.add({codes[0], codes[8 * W]}, {__half2float(scales[0]), __half2float(scales[8 * G])},
+                    {float(zeros[0]), float(zeros[8 * G])}, e12, e16);
+            } else {
+              const int u = t + ROWS;
+              r.add({codes[t * W], codes[u * W]}, {__half2float(scales[t * G]), __half2float(scales[u * G])},
+                    {float(zeros[t * G]), float(zeros[u * G])}, e12, e16);
+            }
           }
         }
-        *reinterpret_cast<uint2*>(a.codes + slot * 2 * D + d0) = make_uint2(up[0], up[1]);
-        *reinterpret_cast<uint2*>(a.codes + slot * 2 * D + D + d0) = make_uint2(down[0], down[1]);
       }
-      if (lane == 0) a.scales[slot] = bad ? INFINITY : step;
+      __syncwarp();
+      ring.next(issue);
+      if (held && ((k + 1) & ((1 << pieces_log2) - 1)) == 0) {
+        at.join_rows(r);
+        at.store(a, (int64_t(page) * c.kv_heads + h) * per_page + (j & (per_page - 1)), r,
+                 __any_sync(0xffffffffu, !(r.finite == 0.f)), lane);
+      }
     }
   }
 }
 
 template <int G>
 int launch_index(const PagedIndexArgs& a, cudaStream_t st) {
-  // a sequence's new tokens fill at most this many blocks (more, where the host's bound does not hold: the kernel loops)
-  const int64_t blocks = (int64_t(a.c.max_q) + (1 << a.block_log2) - 1) >> a.block_log2;
-  const int64_t items = blocks * a.c.kv_heads;
+  static PerContextOnce once;
   int dev = 0;
-  const cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e);
-  // few blocks: four warps each
-  const bool split = items * a.c.batch <= 16 * device_sms(dev);
-  const int64_t ctas = split ? items : (items + kIndexWarps - 1) / kIndexWarps;
+  constexpr int kSmem = Piece<G>::kSmem;
+  e = once.run(dev, [&] { return cudaFuncSetAttribute(paged_index_kernel<G>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem); });
+  if (e != cudaSuccess) return cuda_status(e);
+  // a sequence's new tokens fill at most this many blocks (more, where the host's bound does not hold: the kernels loop)
+  const int64_t blocks = (int64_t(a.c.max_q) + (1 << a.block_log2) - 1) >> a.block_log2;
+  const int64_t items = blocks * a.c.kv_heads, sms = device_sms(dev);
+  const bool few = items * a.c.batch <= 16 * sms;
+  // enough warps to fill the GPU, some blocks each
+  const int64_t ctas = std::max<int64_t>(1, std::min<int64_t>(sms * Piece<G>::kCtas / a.c.kv_heads, blocks * a.c.batch / kIndexWarps));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(std::min<int64_t>(ctas, INT32_MAX)), unsigned(std::min(a.c.batch, 65535)));
+  cfg.gridDim = few ? dim3(unsigned(items), unsigned(std::min(a.c.batch, 65535))) : dim3(unsigned(ctas), unsigned(a.c.kv_heads));
   cfg.blockDim = dim3(32 * kIndexWarps);
+  cfg.dynamicSmemBytes = few ? 0 : kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, split ? paged_index_kernel<G, kIndexWarps> : paged_index_kernel<G, 1>, a));
+  return cuda_status(cudaLaunchKernelEx(&cfg, few ? paged_index_few_kernel<G> : paged_index_kernel<G>, a));
 }
 
 // ------------------------------------------------------------ choice
@@ -383,6 +557,11 @@ struct SelectParams {
   int pitch;   // keys of a token
 };
 
+// Measured: one token, 2048 blocks, 8 heads of 128 (a cluster of 8 CTAs a list) 10.5 to 11.4 us,
+// most of it a chain of look-ups, two cluster barriers and the ranking; 64 sequences 10.8 us
+// (33 MB of index: 3.1 TB/s); 512 tokens over 512 blocks (8 tokens a CTA) 46 us, where the
+// ranking by single warps takes as many instructions as the scores.
+//
 // A cluster has one key/value head and `tokens` new tokens in a row, its CTAs every
 // n-th tile of 16 blocks; the first CTA keeps the keys and takes the best.  Columns of
 // the products: query heads of the tokens, 8 NT at a time.  Operand A, 16 blocks x 32
@@ -647,6 +826,8 @@ int launch_paged_index(const PagedIndexArgs& a, cudaStream_t st) {
   }
   return SPECTRA_ERR_UNSUPPORTED;
 }
+
+int paged_index_timeouts(long long* out, bool reset) { return read_timeout_counter(g_paged_index_timeouts, out, reset); }
 
 int launch_paged_select(const PagedSelectArgs& a, cudaStream_t st) {
   switch (a.i.c.head_dim) {

@@ -97,6 +97,34 @@ def test_index_writes_the_blocks_that_the_new_tokens_filled_and_no_other(news):
     same(index, (codes, scales))
 
 
+@pytest.mark.parametrize("dim,kv_heads,page,block", [(32, 16, 64, 32), (64, 16, 256, 256), (96, 12, 128, 64), (128, 16, 64, 64),
+                                                      (256, 8, 128, 128), (128, 3, 512, 512)])
+def test_index_of_more_sequences_than_are_laid_out_at_once(dim, kv_heads, page, block):
+    lens = [block + (37 * i) % (3 * block) if i % 7 else 0 for i in range(150)]
+    news = [max(1, n - (11 * i) % 40) for i, n in enumerate(lens)]
+    st = Step(lens, news, kv_heads, kv_heads, dim, page, "bf16", seed=block)
+    st.tables[9, 0] = -1
+    st.t_tables.copy_(torch.from_numpy(st.tables))
+    rng = np.random.default_rng(3)  # (codes drawn as they are: filling 150 sequences takes long)
+    shape = st.ref.codes.shape
+    st.ref.codes[:] = rng.integers(0, 16, shape, np.uint8)
+    st.ref.scales[:] = rng.uniform(0.01, 3.0, st.ref.scales.shape).astype(np.float16)
+    st.ref.zeros[:] = rng.integers(0, 16, st.ref.zeros.shape, np.uint8)
+    st.upload()
+    index = PG.BlockIndex(st.cache, block)
+    PG.paged_index_update(index, st.batch)
+    codes, scales = np.zeros(index.codes.shape, np.int8), np.zeros(index.scales.shape, np.float32)
+    keys = ((st.ref.codes[:, :, :, 0].astype(np.float64).reshape(*shape[:3], -1, 32) - st.ref.zeros[:, :, :, 0, :, None])
+            * st.ref.scales[:, :, :, 0, :, None].astype(np.float64)).reshape(*shape[:3], dim)
+    for b, (n, new) in enumerate(zip(lens, news)):
+        for j in range(max(0, n - new) // block, n // block):
+            p, part = int(st.tables[b, j * block // page]), j % (page // block)
+            for h in range(kv_heads if p >= 0 else 0):
+                codes[p, h, part], scales[p, h, part] = B.bounds(keys[p, h, part * block:(part + 1) * block])
+    same(index, (codes, scales))
+    assert SK.device_timeouts() == 0
+
+
 def test_index_of_keys_that_are_not_finite_constant_or_zero():
     st = Step([192], [192], 2, 2, 64, 64, "bf16")
     k, v = draw((192, 2, 64), 1, "bf16"), draw((192, 2, 64), 2, "bf16")
