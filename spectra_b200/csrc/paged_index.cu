@@ -151,14 +151,15 @@ struct LaneWord {
   }
 };
 
-// The blocks of sequence b that its new tokens filled: j0 .. end - 1.
+// The blocks of sequence b that its new tokens filled: j0 .. end - 1 (end >= j0, also where the sequence goes on
+// past the bound: the counts are added up).
 __device__ __forceinline__ void filled_blocks(const PagedIndexArgs& a, int b, int& j0, int& end) {
   int64_t first;
   int count;
   new_tokens(a.c, b, first, count);
   const int held = a.c.seq_lens[b], len = min(held, a.c.limit);
   j0 = max(held - count, 0) >> a.block_log2;
-  end = len > 0 && count > 0 ? len >> a.block_log2 : j0;
+  end = len > 0 && count > 0 ? max(len >> a.block_log2, j0) : j0;
 }
 
 // Few blocks: the four warps of a CTA share one, a quarter of its tokens each, straight from memory.

@@ -153,6 +153,32 @@ def test_index_skips_bad_pages_and_positions_past_the_bound():
     same(index, want_index(st, 32, [70, 70]))
 
 
+def test_index_of_many_sequences_past_the_bound():
+    # every third one's new tokens all lie past the bound, and what it counts must not move the others' blocks
+    block, page, kv_heads, dim, limit = 32, 64, 16, 64, 96
+    lens = [300 if i % 3 == 0 else 33 + 5 * i for i in range(40)]
+    news = [40 if i % 3 == 0 else n for i, n in enumerate(lens)]
+    st = Step(lens, news, kv_heads, kv_heads, dim, page, "bf16", max_len=limit)
+    rng = np.random.default_rng(4)
+    shape = st.ref.codes.shape
+    st.ref.codes[:] = rng.integers(0, 16, shape, np.uint8)
+    st.ref.scales[:] = rng.uniform(0.01, 3.0, st.ref.scales.shape).astype(np.float16)
+    st.ref.zeros[:] = rng.integers(0, 16, st.ref.zeros.shape, np.uint8)
+    st.upload()
+    index = PG.BlockIndex(st.cache, block)
+    PG.paged_index_update(index, st.batch)
+    codes, scales = np.zeros(index.codes.shape, np.int8), np.zeros(index.scales.shape, np.float32)
+    for b, (n, new) in enumerate(zip(lens, news)):
+        keys = st.ref.values(st.tables[b], min(n, limit))[0][0]
+        for j in range((n - new) // block, min(n, limit) // block):
+            at = int(st.tables[b, j * block // page]), j % (page // block)
+            for h in range(kv_heads):
+                codes[at[0], h, at[1]], scales[at[0], h, at[1]] = B.bounds(keys[j * block:(j + 1) * block, h])
+    assert scales.any()
+    same(index, (codes, scales))
+    assert SK.device_timeouts() == 0
+
+
 def test_index_past_two_gigabytes_and_of_tokens_past_max_q():
     dim, page, heads = 128, 64, 8
     each = heads * (page // 16) * PG.tile_bytes(dim)
