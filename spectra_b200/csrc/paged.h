@@ -93,7 +93,6 @@ int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st);  // the one
 int paged_attn_timeouts(long long* out, bool reset);
 int paged_prompt_timeouts(long long* out, bool reset);
 
-
 // A block index (paged_index.cu): what it holds is in the public header.
 struct PagedIndexArgs {
   PagedView c;

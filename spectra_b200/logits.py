@@ -9,7 +9,8 @@ sample_token (spectra/engine.py:1626-1713); here one kernel does it in one pass:
     tokens = kernels.argmax(logits, rules=rules)            # the choice alone: no logits are written
 
 The rules' tensors stay on the device and are read by the kernel alone, so a
-captured step can be replayed with other contents.  There is no CPU path.
+captured step can be replayed with other contents.  There is no CPU path, and
+nothing here is differentiable.
 """
 from __future__ import annotations
 
