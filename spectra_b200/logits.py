@@ -79,7 +79,7 @@ class LogitRules:
             if t is not None and not isinstance(t, torch.Tensor):
                 if "lengths" in name:
                     raise TypeError(f"{name} must be an int32 tensor")
-                t = torch.full((self.rows,), float(t), device=self.device)
+                t = torch.full((self.rows,), float(t), dtype=torch.float32, device=self.device)
             if t is not None:
                 self._check(name, t, torch.int32 if "lengths" in name else torch.float32)
                 if t.shape != (self.rows,) or (self.rows > 1 and t.stride(0) != 1):

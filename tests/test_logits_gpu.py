@@ -119,6 +119,19 @@ def test_penalties_as_numbers_and_lists_of_full_length():
     assert chosen.tolist() == tokens.tolist()
 
 
+def test_penalties_as_numbers_whatever_torchs_default_type_is():
+    b = Batch(2, 500, ids=40, seed=6)
+    rows = {p: torch.full((2,), v) for p, v in (("repetition", 1.3), ("frequency", 0.3), ("presence", 0.7))}  # fp32
+    want, _ = LG.adjust_logits(b.x.to(DEV), b.rules(**rows), with_tokens=True)
+    try:
+        torch.set_default_dtype(torch.bfloat16)
+        rules = b.rules(repetition=1.3, frequency=0.3, presence=0.7)
+        got = LG.adjust_logits(b.x.to(DEV), rules)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert torch.equal(got, want)
+
+
 def test_lengths_past_their_lists_are_cut():
     b = Batch(6, 500, "f16", ids=30, seed=3)
     b.kw["lengths"] = torch.tensor([-1, -2**31, 0, 31, 2**31 - 1, 30], dtype=torch.int32)
