@@ -38,9 +38,10 @@
 // last of them to finish, always in the same order.
 //
 // Lists (attention over some blocks of the keys): a segment is one token of one
-// key/value head, its units are those of the blocks listed for it.  A CTA has a
-// segment, or a piece of one where there are few; it first brings the list into
-// order (entries above all before them, that hold a key the token sees).
+// key/value head, its units are those of the blocks listed for it, from the first
+// to the last key that the token sees (list_units.h).  A CTA has a segment, or a
+// piece of one where there are few; it first brings the list into order (entries
+// above all before them, that hold a key the token sees).
 // Measured: 512 segments of 2048 keys, 64 query heads on 8, heads of 128, 46 us
 // (3.5 TB/s); 4096 segments of 1024 keys (512 tokens of a prompt) 159 us; one
 // token, 2048 keys, 9.4 us.  Bound like the rest by unpacking: 430 instructions a
@@ -57,6 +58,7 @@
 
 #include "copy_ring.h"
 #include "gemv_mma.cuh"
+#include "list_units.h"
 #include "paged_view.cuh"
 #include "sm100_ptx.cuh"
 
@@ -318,9 +320,12 @@ __global__ void __launch_bounds__(kThreads, LISTS ? Cfg<G, NT>::kListCtas : Cfg<
         if (ok) s_list[slot] = e;
       }
       __syncthreads();
-      s.units = kept << (a.block_log2 - kUnitLog2);
-      u_begin = int(int64_t(s.units) * piece / p.pieces);
-      u_stop = int(int64_t(s.units) * (piece + 1) / p.pieces);
+      // (a block may be far larger than what the row sees of it: 512 segments of 100 keys in blocks of 65536
+      // took 1.27 ms as whole blocks, as long as in blocks of 128 this way)
+      const UnitRange seen = list_units(kept, s_list[0], s_list[kept > 0 ? kept - 1 : 0], lo, hi, a.block_log2, kUnitLog2);
+      const UnitRange mine = piece_of(seen, piece, p.pieces);
+      u_begin = mine.begin;
+      u_stop = mine.end;
       u_end = s_stop ? u_begin : u_stop;
     } else {
       // ---- the segment that holds unit `at`
@@ -921,7 +926,7 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   if (LISTS) {
     const int64_t segments = a.c.total * a.c.kv_heads * ((a.group + C::ROWS - 1) / C::ROWS);
     if (segments > INT32_MAX - kMaxCtas) return SPECTRA_ERR_SHAPE;
-    const int64_t list = std::min<int64_t>(a.count, (int64_t(a.c.limit) >> a.block_log2) + 1) << (a.block_log2 - kUnitLog2);
+    const int64_t list = most_list_units(a.count, a.c.limit, a.block_log2, kUnitLog2);
     p.segments = int(segments);
     // As many CTAs per segment as the GPU holds; whole ones by turns where there are more segments than CTAs
     // (512 segments of 64 units in 3 pieces each on 444 CTAs: 72.7 us, whole 62.6)
