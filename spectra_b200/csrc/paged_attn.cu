@@ -125,9 +125,8 @@ struct Cfg {
   static constexpr int kX = G * NT * 4 * 32;                  // {C, C', C, C'} and {X, X'} of a lane's two rows
   static constexpr int kMeta = ROWS * 16;                     // hi, lo, slope, position of a row
   static constexpr int kCtas = G * NT <= 4 ? 4 : 2;  // per SM: what the registers allow
-  // the same for lists (512 segments of heads of 128: 45.9 us with 4, 62.6 with 3; 384 of heads of 64, which fit
-  // at once either way: 18.4 with 4, 15.2 with 3)
-  static constexpr int kListCtas = kCtas == 4 && G < 3 ? 3 : kCtas;
+  // the same for lists where the GPU holds all segments at once so (heads of 128 gain nothing by it)
+  static constexpr int kFewListCtas = kCtas == 4 && G < 3 ? 3 : kCtas;
   static constexpr int kSmem = kBig + kQ + kX + kMeta + ROWS * 4 + kWarps * kStages * 8;
   static constexpr int kPartial = ROWS * (D + 2);             // floats of one CTA's partial result
 };
@@ -138,8 +137,8 @@ struct Cfg {
 // LISTS 1 and 2: a segment is one token and the blocks listed for it.  2 is for fp16 results: weights as two
 // operands, the second what the rounding of the first left (results 2.75e-4 off, 2.1e-4 of it their own rounding;
 // 3.2e-4 with one; 5 % longer, and as much for bf16 results where the kernel was the same).
-template <int G, int NT, int MOD, int LISTS>
-__global__ void __launch_bounds__(kThreads, LISTS ? Cfg<G, NT>::kListCtas : Cfg<G, NT>::kCtas) paged_attn_kernel(AttnParams p) {
+template <int G, int NT, int MOD, int LISTS, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS) paged_attn_kernel(AttnParams p) {
   using C = Cfg<G, NT>;
   constexpr int D = C::D, ROWS = C::ROWS;
   constexpr bool SEL = LISTS > 0;
@@ -896,7 +895,7 @@ __global__ void __launch_bounds__(kThreads, LISTS ? Cfg<G, NT>::kListCtas : Cfg<
   }
 }
 
-template <int G, int NT, int MOD, int LISTS>
+template <int G, int NT, int MOD, int LISTS, int CTAS>
 int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   using C = Cfg<G, NT>;
   static PerContextOnce once;
@@ -904,7 +903,7 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e);
-  auto kern = paged_attn_kernel<G, NT, MOD, LISTS>;
+  auto kern = paged_attn_kernel<G, NT, MOD, LISTS, CTAS>;
   e = once.run(dev, [&] {
     cudaError_t r = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (r == cudaSuccess) r = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas_per_sm[dev], kern, kThreads, C::kSmem);
@@ -952,10 +951,29 @@ int launch_one(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
-template <int G, int NT, int LISTS>
+template <int G, int NT, int LISTS, int CTAS>
 int launch_mod(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
-  if (a.softcap > kLowCap) return launch_one<G, NT, 2, LISTS>(a, max_rows, st);
-  return a.softcap > 0.f || a.slopes ? launch_one<G, NT, 1, LISTS>(a, max_rows, st) : launch_one<G, NT, 0, LISTS>(a, max_rows, st);
+  if (a.softcap > kLowCap) return launch_one<G, NT, 2, LISTS, CTAS>(a, max_rows, st);
+  return a.softcap > 0.f || a.slopes ? launch_one<G, NT, 1, LISTS, CTAS>(a, max_rows, st)
+                                     : launch_one<G, NT, 0, LISTS, CTAS>(a, max_rows, st);
+}
+
+// CTAs per SM.  Lists of heads of 32 and 64: three, with registers for more loads in flight, where the GPU holds all
+// segments at once that way, four above that.  Measured, 24 blocks of 32, 32 query heads on 8 of 64, with three and
+// with four: 128 segments 10.0 and 10.4 us, 384 11.5 and 13.3, 512 19.1 and 13.6, 768 (two turns either way) 21.4 and
+// 22.8, 1024 29.1 and 25.5, 4096 98.8 and 88.3; heads of 32: 384 9.5 and 10.6, 512 16.8 and 10.7, 768 17.3 and 18.1,
+// 4096 83.4 and 69.3.  (Heads of 128 with three: 512 segments 62.6, with four 45.9.)
+template <int G, int NT, int LISTS>
+int launch_ctas(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
+  using C = Cfg<G, NT>;
+  if constexpr (LISTS && C::kFewListCtas < C::kCtas) {
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return cuda_status(e);
+    const int64_t segments = a.c.total * a.c.kv_heads * ((a.group + C::ROWS - 1) / C::ROWS);
+    if (segments <= int64_t(device_sms(dev)) * C::kFewListCtas) return launch_mod<G, NT, LISTS, C::kFewListCtas>(a, max_rows, st);
+  }
+  return launch_mod<G, NT, LISTS, C::kCtas>(a, max_rows, st);
 }
 
 template <int G, int LISTS>
@@ -963,8 +981,8 @@ int launch_rows(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   // up to 8 rows per key/value head (lists: of one token): one column tile (fewer registers, more CTAs per SM);
   // heads of 256 have no registers for two
   if (G == 8 || (LISTS ? 1 : int64_t(a.c.max_q)) * a.group <= 8)
-    return launch_mod<G, 1, LISTS>(a, max_rows, st);
-  return launch_mod<G, G == 8 ? 1 : 2, LISTS>(a, max_rows, st);
+    return launch_ctas<G, 1, LISTS>(a, max_rows, st);
+  return launch_ctas<G, G == 8 ? 1 : 2, LISTS>(a, max_rows, st);
 }
 
 template <int LISTS>
