@@ -510,7 +510,7 @@ typedef struct {
  * idx_offset + the first column of the maximum among the allowed, before the
  * rounding (a NaN counts as the maximum), -1 where nothing is allowed; val[m]
  * (optional, with idx) = that maximum, -infinity where there is none.
- * max_ids <= SPECTRA_MAX_RULE_IDS, n_bias <= SPECTRA_MAX_RULE_BIASES.
+ * M <= 65535, max_ids <= SPECTRA_MAX_RULE_IDS, n_bias <= SPECTRA_MAX_RULE_BIASES.
  * workspace: spectra_adjust_logits_workspace_bytes bytes, 8-byte aligned, of any
  * contents; calls that may overlap in time do not share one.
  */

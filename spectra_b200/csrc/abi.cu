@@ -768,7 +768,7 @@ int spectra_adjust_logits(const SpectraLogitRules* rules, const void* x, int x_d
                           int64_t idx_offset, void* out, int out_dtype, int64_t out_row_stride, int64_t* idx, float* val,
                           void* workspace, size_t workspace_bytes, void* stream) {
   if (!rules || !x || (!out && !idx) || (val && !idx)) return SPECTRA_ERR_NULL_POINTER;
-  if (M < 0 || N <= 0 || idx_offset < 0 || !fits_i32(N) || !fits_i32(idx_offset) ||
+  if (M < 0 || M > 65535 /* grid y */ || N <= 0 || idx_offset < 0 || !fits_i32(N) || !fits_i32(idx_offset) ||
       !fits_i32(idx_offset + N + 64))  // (columns are counted in 32 bits, to the end of the last 16 bytes)
     return SPECTRA_ERR_SHAPE;
   if (!is_float_dt(x_dtype) || (out && !is_float_dt(out_dtype))) return SPECTRA_ERR_DTYPE;

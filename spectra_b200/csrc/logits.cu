@@ -738,7 +738,6 @@ size_t logits_workspace_bytes(const SpectraLogitRules& r, int64_t M, int64_t N, 
 
 int launch_logits(const LogitArgs& a, cudaStream_t st) {
   if (a.M == 0) return SPECTRA_OK;
-  if (a.M > 65535) return SPECTRA_ERR_SHAPE;  // grid y
   const bool many = many_rows(a.r, a.M, a.N, a.x_dtype);
   if (a.x_dtype == SPECTRA_DT_BF16) return many ? launch_many<SPECTRA_DT_BF16>(a, st) : launch_few<SPECTRA_DT_BF16>(a, st);
   if (a.x_dtype == SPECTRA_DT_F16) return many ? launch_many<SPECTRA_DT_F16>(a, st) : launch_few<SPECTRA_DT_F16>(a, st);

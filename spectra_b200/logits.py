@@ -25,7 +25,7 @@ _DT = {torch.float16: L.DT_F16, torch.bfloat16: L.DT_BF16, torch.float32: L.DT_F
 
 
 class LogitRules:
-    """The rules of a batch of rows, one row per row of the logits.
+    """The rules of a batch of rows, one row per row of the logits (65535 at most).
 
     ``ids`` int32 [rows, most]: the tokens that each sequence holds, its prompt
     first; the first ``lengths`` int32 [rows] of them count (default: all), the
@@ -57,6 +57,8 @@ class LogitRules:
         if some is None:
             raise ValueError("no rules: give ids, bias_ids and bias, or allowed")
         self.device, self.rows = some.device, some.shape[0] if some.dim() else -1
+        if self.rows > 65535:
+            raise ValueError(f"at most 65535 rows, got {self.rows}")
         for name, t in wide.items():
             if t is None:
                 continue
