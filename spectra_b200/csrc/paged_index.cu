@@ -9,7 +9,8 @@
 //
 // Choice, for a token and a key/value head whose query heads have codes c_h:
 //   score(j) = S_j max_h sum_d (c_hd > 0 ? c_hd H_jd : c_hd L_jd)
-// an upper bound of every c_h . k of the block, up to S's rounding.  The sum is
+// an upper bound of c_h . k for every key of the block and every head.  (Each head's
+// codes have a step of its own, which is left out: a ranking, no bound of q . k.)  The sum is
 // max(c, 0) . H + min(c, 0) . L, a product of integers below 2^22, so scores are
 // exact in fp32 and the choice does not depend on the order of the sums.
 #include <cooperative_groups.h>

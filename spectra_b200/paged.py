@@ -572,14 +572,16 @@ def paged_select_blocks(q: torch.Tensor, index: BlockIndex, batch: TokenBatch, c
 
     Of the blocks up to the token's own, the ``first`` first and the ``last``
     last ones (the token's own among them) are always taken, then those of the
-    highest score, the lowest number first among equal ones.  The score bounds
-    q . k over the block's keys from above, for the best of the key/value head's
-    query heads: with H, L the block's codes, S its scale, and c the query
-    head's features rounded to 8 bits (each head in a power of two of its own,
-    so that no head outvotes another by its size),
+    highest score, the lowest number first among equal ones.  With H, L the
+    block's codes, S its scale, and c the features of a query head rounded to 8
+    bits in a power of two of the head's own,
 
         score = S max_heads sum_d (c_d H_d if c_d > 0 else c_d L_d)
 
+    For every query head it is at least c . k of each key of the block.  It ranks
+    blocks and bounds no q . k: the heads' powers of two are left out, so that
+    no head outvotes another by the size of its queries (to a factor of two: a
+    head's largest code is 64 to 127), and c is rounded to the nearest.
     The sums are whole numbers, so equal inputs give equal lists.  A block with
     a key that is not finite comes before all others; one whose page the table
     does not name is never taken.  Tokens without a place in the cache get -1.
