@@ -378,8 +378,9 @@ int launch_index(const PagedIndexArgs& a, cudaStream_t st) {
   const int64_t blocks = (int64_t(a.c.max_q) + (1 << a.block_log2) - 1) >> a.block_log2;
   const int64_t items = blocks * a.c.kv_heads, sms = device_sms(dev);
   // (A token or a few of many sequences: most fill no block, and a CTA that finds that out leaves at once.  Measured, one
-  // token each, 8 heads of 128, a 64th of the sequences fill a block: 512 sequences 5.4 us, with the other kernel 15.9;
-  // 4096 sequences 35.0 and 122.7; 1024 with 32 heads 34.4 and 34.1.)
+  // token each, 8 heads of 128, a 64th of the sequences fill a block: 512 sequences 5.7 us, with the other kernel 15.9;
+  // 4096 sequences 35.2 and 122; 1024 with 32 heads 35.1 and 34.  Where every sequence brings a block of 64 tokens: 14.3
+  // and 31.6; 107 and 276; 106 and 120.)
   const bool few = blocks == 1 || items * a.c.batch <= 16 * sms;
   // enough warps to fill the GPU, some blocks each
   const int64_t ctas = std::max<int64_t>(1, std::min<int64_t>(sms * Piece<G>::kCtas / a.c.kv_heads, blocks * a.c.batch / kIndexWarps));
@@ -563,8 +564,8 @@ struct SelectParams {
 };
 
 // Measured: one token, 2048 blocks, 8 heads of 128 (a cluster of 8 CTAs a list) 10.5 to 11.4 us,
-// most of it a chain of look-ups, two cluster barriers and the ranking; 64 sequences 10.8 us
-// (33 MB of index: 3.1 TB/s); 512 tokens over 512 blocks (8 tokens a CTA) 46 us, where the
+// most of it a chain of look-ups, two cluster barriers and the ranking; 64 ragged sequences of up to 256
+// blocks 10.7 us (19.7 MB of index: 1.8 TB/s); 512 tokens over 512 blocks (8 tokens a CTA) 46 us, where the
 // ranking by single warps takes as many instructions as the scores.
 //
 // A cluster has one key/value head and `tokens` new tokens in a row, its CTAs every
@@ -809,9 +810,15 @@ int launch_select(const PagedSelectArgs& a, cudaStream_t st) {
   const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e);
   const int64_t sms = device_sms(dev), lists = a.i.c.total * a.i.c.kv_heads;
-  // Prompts: several tokens a CTA, up to 32 columns, so that codes are read once for all of them.
+  // Prompts: several tokens a CTA, up to 32 columns, so that codes are read once for all of them; fewer while their
+  // CTAs still run at once (four an SM with up to 8 columns, else two), and while two CTAs' keys do not fit an SM.
+  // Measured, heads of 128, 32 or 64 query heads on 8: 128 tokens over 32768 with 2 tokens a CTA 20.7 us, with 4 22.0
+  // (64 heads: 38.7, and with 4, at once, 23.8); 256 tokens with 4 39.9, with 8, at once, 25.9; 512 tokens with 8 47.9,
+  // with 4 76.8; 64 tokens of 64 heads with one 18.0, with 2 20.2 (32 heads: 17.9 and 15.9).  8 tokens with 2048 blocks
+  // each take 131 us for 512 tokens over 131072, 4 of them 219.
   int tokens = std::min({32 / a.group, kMaxTokens, a.i.c.max_q});
-  while (tokens > 1 && (int64_t(tokens) * a.max_blocks > 24 * 1024 || lists < 2 * sms * tokens)) tokens /= 2;
+  auto at_once = [&](int n) { return sms * (G < 8 && n * a.group <= 8 ? 4 : 2); };
+  while (tokens > 1 && (int64_t(tokens) * a.max_blocks > 24 * 1024 || lists <= at_once(tokens / 2) * (tokens / 2))) tokens /= 2;
   if (tokens > 1) return tokens * a.group <= 8 ? launch_select_as<G, 1>(a, tokens, 1, st) : launch_select_as<G, 4>(a, tokens, 1, st);
   // Few lists: several CTAs each, while they have a tile for every warp.
   int ctas = 1;
