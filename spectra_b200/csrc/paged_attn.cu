@@ -178,77 +178,77 @@ __global__ void __launch_bounds__(kThreads, CTAS) paged_attn_kernel(AttnParams p
   long long share = 0, begin = 0, end = 0, seq_base = 0;
   int b = -1;
   if constexpr (!SEL) {
-  bool over = false;  // a sequence has more new tokens than max_q
-  auto units_of = [&](int i) -> long long {
-    if (i >= c.batch) return 0;
-    const Span s = span_of<ROWS>(p, i);
-    over = over || s.extra > 0;
-    return (long long)(s.units) * s.tiles * c.kv_heads;
-  };
-  const long long first_units = units_of(tid);  // (the only ones of a batch of up to kThreads)
-  long long total = first_units;
-  for (int b0 = kThreads; b0 < c.batch; b0 += kThreads) total += units_of(b0 + tid);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) s_scan[warp] = total;
-  over = __syncthreads_or(over);
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) total += s_scan[w];
-  const long long up = total + gridDim.x - 1;
-  share = up < (1ll << 32) ? (long long)(unsigned(up) / gridDim.x) : up / gridDim.x;
-  if (share < p.min_share) share = p.min_share;
-  begin = share * blockIdx.x;
-  end = begin + share < total ? begin + share : total;
-
-  // rows that belong to no sequence, or lie past max_q
-  if (c.cu_q) {
-    const int64_t row_words = int64_t(a.q_heads) * D;
-    auto clear = [&](int64_t t) {
-      for (int64_t i = tid; i < row_words; i += kThreads)
-        reinterpret_cast<uint16_t*>(a.out)[t * a.o_ts + (i / D) * a.o_hs + i % D] = 0;
+    bool over = false;  // a sequence has more new tokens than max_q
+    auto units_of = [&](int i) -> long long {
+      if (i >= c.batch) return 0;
+      const Span s = span_of<ROWS>(p, i);
+      over = over || s.extra > 0;
+      return (long long)(s.units) * s.tiles * c.kv_heads;
     };
-    const int held = c.cu_q[c.batch];
-    for (int64_t t = (held < 0 ? 0 : held) + int64_t(blockIdx.x); t < c.total; t += gridDim.x) clear(t);
-    if (over) {
-      for (int i = blockIdx.x; i < c.batch; i += gridDim.x) {
-        const Span s = span_of<ROWS>(p, i);
-        for (int64_t t = s.first + s.count; t < s.first + s.count + s.extra; ++t) clear(t);
+    const long long first_units = units_of(tid);  // (the only ones of a batch of up to kThreads)
+    long long total = first_units;
+    for (int b0 = kThreads; b0 < c.batch; b0 += kThreads) total += units_of(b0 + tid);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (lane == 0) s_scan[warp] = total;
+    over = __syncthreads_or(over);
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) total += s_scan[w];
+    const long long up = total + gridDim.x - 1;
+    share = up < (1ll << 32) ? (long long)(unsigned(up) / gridDim.x) : up / gridDim.x;
+    if (share < p.min_share) share = p.min_share;
+    begin = share * blockIdx.x;
+    end = begin + share < total ? begin + share : total;
+
+    // rows that belong to no sequence, or lie past max_q
+    if (c.cu_q) {
+      const int64_t row_words = int64_t(a.q_heads) * D;
+      auto clear = [&](int64_t t) {
+        for (int64_t i = tid; i < row_words; i += kThreads)
+          reinterpret_cast<uint16_t*>(a.out)[t * a.o_ts + (i / D) * a.o_hs + i % D] = 0;
+      };
+      const int held = c.cu_q[c.batch];
+      for (int64_t t = (held < 0 ? 0 : held) + int64_t(blockIdx.x); t < c.total; t += gridDim.x) clear(t);
+      if (over) {
+        for (int i = blockIdx.x; i < c.batch; i += gridDim.x) {
+          const Span s = span_of<ROWS>(p, i);
+          for (int64_t t = s.first + s.count; t < s.first + s.count + s.extra; ++t) clear(t);
+        }
       }
     }
-  }
-  if (begin >= end) return;
+    if (begin >= end) return;
 
-  // ---- the sequence where the share begins
-  long long base = 0;
-  for (int b0 = 0; b0 < c.batch; b0 += kThreads) {
-    const long long mine = b0 == 0 ? first_units : units_of(b0 + tid);
-    long long sum = mine;
+    // ---- the sequence where the share begins
+    long long base = 0;
+    for (int b0 = 0; b0 < c.batch; b0 += kThreads) {
+      const long long mine = b0 == 0 ? first_units : units_of(b0 + tid);
+      long long sum = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += up;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+      }
+      __syncthreads();
+      if (lane == 31) s_scan[warp] = sum;
+      __syncthreads();
+      long long before = base + sum - mine, all = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += s_scan[w];
+        all += s_scan[w];
+      }
+      if (before <= begin && begin < before + mine) {
+        s_seq = b0 + tid;
+        s_base = before;
+      }
+      base += all;
+      if (base > begin) break;
     }
     __syncthreads();
-    if (lane == 31) s_scan[warp] = sum;
-    __syncthreads();
-    long long before = base + sum - mine, all = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += s_scan[w];
-      all += s_scan[w];
-    }
-    if (before <= begin && begin < before + mine) {
-      s_seq = b0 + tid;
-      s_base = before;
-    }
-    base += all;
-    if (base > begin) break;
-  }
-  __syncthreads();
-  b = s_seq;
-  seq_base = s_base;
-  if (b < 0) return;
+    b = s_seq;
+    seq_base = s_base;
+    if (b < 0) return;
   }
 
   const bool bf16 = a.dtype == SPECTRA_DT_BF16;
@@ -958,11 +958,11 @@ int launch_mod(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
                                      : launch_one<G, NT, 0, LISTS, CTAS>(a, max_rows, st);
 }
 
-// CTAs per SM.  Lists of heads of 32 and 64: three, with registers for more loads in flight, where the GPU holds all
-// segments at once that way, four above that.  Measured, 24 blocks of 32, 32 query heads on 8 of 64, with three and
-// with four: 128 segments 10.0 and 10.4 us, 384 11.5 and 13.3, 512 19.1 and 13.6, 768 (two turns either way) 21.4 and
-// 22.8, 1024 29.1 and 25.5, 4096 98.8 and 88.3; heads of 32: 384 9.5 and 10.6, 512 16.8 and 10.7, 768 17.3 and 18.1,
-// 4096 83.4 and 69.3.  (Heads of 128 with three: 512 segments 62.6, with four 45.9.)
+// CTAs per SM.  Lists of heads of 32 and 64: three, with more registers, where the GPU holds all segments at once that
+// way, four above that.  Measured, 24 blocks of 32, 32 query heads on 8 of 64, with three and with four: 128 segments
+// 10.0 and 10.4 us, 384 11.5 and 13.3, 512 19.1 and 13.6, 768 (two turns either way) 21.4 and 22.8, 1024 29.1 and 25.5,
+// 4096 98.8 and 88.3; heads of 32: 384 9.5 and 10.6, 512 16.8 and 10.7, 768 17.3 and 18.1, 4096 83.4 and 69.3.  (Heads
+// of 128 with three: 512 segments 62.6, with four 45.9.)
 template <int G, int NT, int LISTS>
 int launch_ctas(const PagedAttnArgs& a, int max_rows, cudaStream_t st) {
   using C = Cfg<G, NT>;

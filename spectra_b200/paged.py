@@ -479,9 +479,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: TokenBatch, *, 
 
     ``blocks`` int32 [total, kv_heads, count] (``paged_select_blocks``): of these
     keys, the row sees those in the blocks of ``block_size`` tokens that are
-    listed for its token and key/value head.  A list is in ascending order; an
-    entry that is not above all before it (a repeated one, -1) and a block past
-    the sequence's end are passed over.  block_size is a power of two from 32 to
+    listed for its token and key/value head.  A list is in ascending order (sort
+    a top-k's output first); an entry that is not above all before it (a
+    repeated one, -1) and a block past the sequence's end are passed over, and
+    nothing reports them.  block_size is a power of two from 32 to
     65536, count at most 1024.
 
     Partial results lie in a workspace of the current stream (17 MB for heads of
